@@ -15,8 +15,8 @@ Kinds of case:
 A query at position i sees the keys j <= i with i - j < window (window 0: all
 of them) or j < sinks.  Sequences of a padded batch end at their own length;
 rows past it give zeros.  The cache holds groups of 32 values along the head as
-e2m1 codes with one power-of-two scale: the least whose sevenfold reaches the
-group's largest magnitude.
+e2m1 codes with one power-of-two scale: the least, from 2^-126 to 2^125, whose
+sevenfold reaches the group's largest magnitude.
 """
 import math
 
@@ -200,7 +200,7 @@ def _quantise(x):
     # one more where m passes 7/8.
     m, e = torch.frexp(amax)
     s = e - 3 + (m > 0.875).int()
-    s = torch.where(amax == 0, torch.full_like(s, -126), s).clamp(-126, 127)
+    s = torch.where(amax == 0, torch.full_like(s, -126), s).clamp(-126, 125)
     a = torch.ldexp(x.abs(), -s.unsqueeze(-1))
     # Nearest level; a value midway goes to the level of even code.
     c = torch.zeros_like(a, dtype=torch.int32)
@@ -374,7 +374,7 @@ def _exact_values(x):
     x = x.double().unflatten(-1, (-1, GROUP))
     top = x.abs().amax(-1, keepdim=True)
     scale = torch.full_like(top, 2.0 ** -126)
-    for e in range(-125, 128):
+    for e in range(-125, 126):
         scale = torch.where(top > 7.0 * 2.0 ** (e - 1), torch.full_like(top, 2.0 ** e), scale)
     y = (x / scale).abs()
     # The step is 1/2 below 2, 1 below 4 and 2 above; torch.round is half to even.
