@@ -348,6 +348,103 @@ int prichs_attention_forward_rope_q(const void *q, size_t ldq, const void *k,
                                     const float *rope_sin, size_t cache_rows,
                                     size_t pos_offset, void *stream);
 
+/* Causal GQA attention with a sliding window and sinks: query i of a sequence
+ * sees the keys j <= i with i - j < window (window = 0: every earlier key) or
+ * j < sinks (the first tokens, which stay visible).  bf16 q/k/v/o, f32 softmax
+ * and accumulation; rows, heads and leading dimensions as in
+ * prichs_attention_forward; head_dim must be 128.  seq_lens (device int32
+ * [batch], may be NULL): sequence b has min(max(seq_lens[b], 0), seq_len) rows;
+ * its further rows of q/k/v are not used and get zeros in o.  lse (device f32
+ * [batch, n_heads, seq_len], may be NULL): log of the sum of exp(score) over the
+ * visible keys, for the backward (-inf past a sequence's length).  Keys that a
+ * query does not see do not reach it, whatever they hold.  The reference has no
+ * windowed attention. */
+int prichs_window_attention_forward(const void *q, size_t ldq, const void *k,
+                                    size_t ldk, const void *v, size_t ldv, void *o,
+                                    size_t ldo, float *lse, const int32_t *seq_lens,
+                                    size_t batch, size_t seq_len, size_t n_heads,
+                                    size_t n_kv_heads, size_t head_dim,
+                                    size_t window, size_t sinks, int dtype,
+                                    void *stream);
+/* Its gradients: d_q, d_k, d_v (bf16; past a sequence's length zeros) from d_o,
+ * the inputs, the output o and lse of the forward, for the same seq_lens, window
+ * and sinks.  With p = exp(s - lse), dP = d_o . v and D = d_o . o:
+ *   d_v[j] = sum p d_o[i],  dS = p (dP - D),
+ *   d_q[i] = scale sum dS k[j],  d_k[j] = scale sum dS q[i],
+ * the sums of d_k and d_v over the kv head's query heads too.  Outputs must not
+ * overlap inputs.  workspace: device memory, 16-byte aligned, of at least
+ * prichs_window_attention_backward_workspace bytes, used by this call alone until
+ * it has finished. */
+size_t prichs_window_attention_backward_workspace(size_t batch, size_t seq_len,
+                                                  size_t n_heads, size_t n_kv_heads);
+int prichs_window_attention_backward(const void *d_o, size_t ldd, const void *q,
+                                     size_t ldq, const void *k, size_t ldk,
+                                     const void *v, size_t ldv, const void *o,
+                                     size_t ldo, const float *lse,
+                                     const int32_t *seq_lens, void *d_q, size_t lddq,
+                                     void *d_k, size_t lddk, void *d_v, size_t lddv,
+                                     size_t batch, size_t seq_len, size_t n_heads,
+                                     size_t n_kv_heads, size_t head_dim,
+                                     size_t window, size_t sinks, int dtype,
+                                     void *workspace, size_t workspace_bytes,
+                                     void *stream);
+
+/* A paged KV cache in 4 bits.  The cache is device memory [n_pages][n_kv_heads]
+ * [PRICHS_KV_PAGE_BYTES], 16-byte aligned: a page holds PRICHS_KV_PAGE positions
+ * of every kv head.  page_table (device int32 [batch, max_pages]): position p of
+ * sequence b lives in slot p % PRICHS_KV_PAGE of page page_table[b][p /
+ * PRICHS_KV_PAGE]; sequences may share pages that none of them writes.
+ *
+ * Format: groups of 32 values along the head share a scale 2^(s - 127), one byte,
+ * the least (1 <= s <= 252) with max|x| <= 7 * scale; a value is a 4-bit float (0, .5, 1,
+ * 1.5, 2, 3, 4, 6 and a sign) times it, rounded to nearest, ties to the even code
+ * (magnitudes past the largest level become it).  A group that holds an infinity or NaN reads back as NaN.  136 bytes per
+ * position and kv head; what is read back is exact in bf16.
+ *
+ * write: rows b * n + i of k and v (bf16 or f32, leading dimensions ldk / ldv,
+ * multiples of 8, 16-byte aligned; kv head j at column j * 128) become position
+ * start[b] + i.  read: the reverse (dtype: of k and v).  start: device int32
+ * [batch]; counts (device int32 [batch], may be NULL): rows i >= counts[b] are
+ * skipped -- a read leaves them as they were.  Positions outside the table, and
+ * pages outside [0, n_pages), are not written and read as zeros.  A position must
+ * not be written twice in one call, nor read by a call that may run at the same
+ * time. */
+#define PRICHS_KV_PAGE 64
+#define PRICHS_KV_HEAD_DIM 128
+#define PRICHS_KV_PAGE_BYTES 8704 /* of one kv head */
+int prichs_kv_cache_write(void *cache, size_t n_pages, const int32_t *page_table,
+                          size_t max_pages, const int32_t *start,
+                          const int32_t *counts, const void *k, size_t ldk,
+                          const void *v, size_t ldv, size_t batch, size_t n,
+                          size_t n_kv_heads, size_t head_dim, int dtype,
+                          void *stream);
+int prichs_kv_cache_read(const void *cache, size_t n_pages,
+                         const int32_t *page_table, size_t max_pages,
+                         const int32_t *start, const int32_t *counts, void *k,
+                         size_t ldk, void *v, size_t ldv, size_t batch, size_t n,
+                         size_t n_kv_heads, size_t head_dim, int dtype,
+                         void *stream);
+/* Attention of each sequence's last n_q tokens over its cached keys and values:
+ * row b * n_q + i of q / o is the query at position lens[b] - n_q + i (lens:
+ * device int32 [batch], the positions the cache holds, the new tokens' own
+ * included; values past max_pages * PRICHS_KV_PAGE count as that).  It sees the
+ * keys of prichs_window_attention_forward's rule, except those on pages outside
+ * [0, n_pages); a query that sees none (also one at a negative position) gets
+ * zeros, and -inf in lse (f32 [batch, n_heads, n_q], may be NULL).  bf16 q / o.
+ * Nothing is read on the host, so a captured call replays with the lens and
+ * table of that time.  workspace as above, of at least
+ * prichs_kv_cache_attention_workspace bytes. */
+size_t prichs_kv_cache_attention_workspace(size_t batch, size_t n_q, size_t n_heads,
+                                           size_t n_kv_heads, size_t max_pages);
+int prichs_kv_cache_attention(const void *q, size_t ldq, const void *cache,
+                              size_t n_pages, const int32_t *page_table,
+                              size_t max_pages, const int32_t *lens, void *o,
+                              size_t ldo, float *lse, size_t batch, size_t n_q,
+                              size_t n_heads, size_t n_kv_heads, size_t head_dim,
+                              size_t window, size_t sinks, int dtype,
+                              void *workspace, size_t workspace_bytes,
+                              void *stream);
+
 /* f32 causal attention of one sequence with the probabilities kept: the
  * per-head computation of crates/prichs-model/src/attention.rs:96-149 (scores
  * (q . k) / sqrt(head_dim), sequential dot products; row max, expf, sum,

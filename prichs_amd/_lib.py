@@ -125,6 +125,19 @@ SIGNATURES = {
                                       _sz, _i, _vp]),
     "prichs_attention_forward_rope_q": (_i, [_vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _sz, _sz, _sz,
                                              _sz, _sz, _i, _vp, _vp, _sz, _sz, _vp]),
+    "prichs_window_attention_forward": (_i, [_vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp,
+                                             _sz, _sz, _sz, _sz, _sz, _sz, _sz, _i, _vp]),
+    "prichs_window_attention_backward_workspace": (_sz, [_sz, _sz, _sz, _sz]),
+    "prichs_window_attention_backward": (_i, [_vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz,
+                                              _vp, _vp, _vp, _sz, _vp, _sz, _vp, _sz, _sz, _sz,
+                                              _sz, _sz, _sz, _sz, _sz, _i, _vp, _sz, _vp]),
+    "prichs_kv_cache_write": (_i, [_vp, _sz, _vp, _sz, _vp, _vp, _vp, _sz, _vp, _sz, _sz, _sz, _sz,
+                                   _sz, _i, _vp]),
+    "prichs_kv_cache_read": (_i, [_vp, _sz, _vp, _sz, _vp, _vp, _vp, _sz, _vp, _sz, _sz, _sz, _sz,
+                                  _sz, _i, _vp]),
+    "prichs_kv_cache_attention_workspace": (_sz, [_sz, _sz, _sz, _sz, _sz]),
+    "prichs_kv_cache_attention": (_i, [_vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _sz, _vp, _sz, _sz,
+                                       _sz, _sz, _sz, _sz, _sz, _i, _vp, _sz, _vp]),
     "prichs_attention_probs_f32": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _vp]),
     "prichs_checkpoint_open": (_i, [C.c_char_p, C.POINTER(_vp)]),
     "prichs_checkpoint_close": (_i, [_vp]),
@@ -170,6 +183,8 @@ SIGNATURES = {
                                         _vp, _sz, _vp, _i, _vp]),
 }
 NOALLOC_SCRATCH_BYTES = 32 << 20
+KV_PAGE = 64
+KV_PAGE_BYTES = 8704
 MATMUL_AB = 0
 MATMUL_ATB = 1
 MATMUL_ABT = 2

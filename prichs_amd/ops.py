@@ -294,3 +294,210 @@ def attention(q, k, v, batch, seq_len, n_heads, n_kv_heads, head_dim=128, out=No
         L.check(lib.prichs_attention_forward_rope_q(*args, _p(cos), _p(sin), cache_rows,
                                                     pos_offset, _stream(stream)))
     return out
+
+
+# ---------------------------------------- window attention and KV cache ----
+def _rows(t, name, rows, cols, dtypes=(torch.bfloat16,)):
+    """A device operand of at least `rows` rows whose columns are contiguous."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != 2:
+        raise ValueError(f"{name}: expected a 2-D device tensor")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name}: unsupported dtype {t.dtype}")
+    if t.shape[0] < rows or t.shape[1] != cols:
+        raise ValueError(f"{name}: expected [{rows}, {cols}], got {list(t.shape)}")
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: operands need unit column stride")
+    return t
+
+
+def _ld(t):
+    """Row stride; of a single row its width, whatever stride torch keeps for it."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _i32(t, name, n, dim=1):
+    if not t.is_cuda or t.dtype != torch.int32 or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous int32 device tensor")
+    if t.dim() != dim or t.shape[0] != n:
+        raise ValueError(f"{name}: expected {n} rows, got {list(t.shape)}")
+    return t
+
+
+class _device_of:
+    """The device of the operands (all on one) made current, and its stream: the
+    given one, or torch's current one there.  Outputs and workspaces allocated
+    inside belong to that stream."""
+
+    def __init__(self, stream, *tensors):
+        dev = {t.device for t in tensors if t is not None}
+        if len(dev) != 1:
+            raise ValueError(f"operands on different devices: {sorted(map(str, dev))}")
+        self.device = dev.pop()
+        if stream is None:
+            stream = torch.cuda.current_stream(self.device)
+        elif stream.device != self.device:
+            raise ValueError(f"a stream of {stream.device} with operands on {self.device}")
+        self.stream = stream
+        self._ctx = torch.cuda.stream(stream)
+
+    def __enter__(self):
+        self._ctx.__enter__()
+        return C.c_void_p(self.stream.cuda_stream)
+
+    def __exit__(self, *exc):
+        return self._ctx.__exit__(*exc)
+
+
+def window_attention(q, k, v, batch, seq_len, n_heads, n_kv_heads, window, sinks=0,
+                     seq_lens=None, head_dim=128, out=None, want_lse=False, stream=None):
+    """prichs_window_attention_forward on 2-D row views, as ``attention``: each query
+    sees its last `window` keys, itself included (0: all earlier ones), and the
+    first `sinks` keys.  seq_lens: int32 device [batch], the rows of each sequence
+    of a padded batch.  -> (out, lse f32 [batch, n_heads, seq_len], or None)."""
+    lib = L.load()
+    rows, H, K = batch * seq_len, n_heads * head_dim, n_kv_heads * head_dim
+    for t, name, cols in ((q, "q", H), (k, "k", K), (v, "v", K)):
+        _rows(t, name, rows, cols)
+    if seq_lens is not None:
+        _i32(seq_lens, "seq_lens", batch)
+    if window < 0 or sinks < 0:
+        raise ValueError("window and sinks must not be negative")
+    with _device_of(stream, q, k, v, seq_lens, out) as s:
+        if out is None:
+            out = torch.empty((rows, H), dtype=q.dtype, device=q.device)
+        _rows(out, "out", rows, H)
+        lse = None
+        if want_lse:
+            lse = torch.empty((batch, n_heads, seq_len), dtype=torch.float32, device=q.device)
+        L.check(lib.prichs_window_attention_forward(
+            _p(q), _ld(q), _p(k), _ld(k), _p(v), _ld(v), _p(out), _ld(out), _p(lse), _p(seq_lens),
+            batch, seq_len, n_heads, n_kv_heads, head_dim, window, sinks, dtype_code(q), s))
+    return out, lse
+
+
+def window_attention_backward(d_out, q, k, v, out, lse, batch, seq_len, n_heads, n_kv_heads,
+                              window, sinks=0, seq_lens=None, head_dim=128, d_q=None, d_k=None,
+                              d_v=None, stream=None):
+    """prichs_window_attention_backward -> (d_q, d_k, d_v) bf16, from the operands,
+    the output and the lse of window_attention (want_lse=True).  d_q, d_k, d_v:
+    row views to write, e.g. column slices of one fused gradient; they must not
+    overlap the operands."""
+    lib = L.load()
+    rows, H, K = batch * seq_len, n_heads * head_dim, n_kv_heads * head_dim
+    for t, name, cols in ((d_out, "d_out", H), (q, "q", H), (k, "k", K), (v, "v", K),
+                          (out, "out", H)):
+        _rows(t, name, rows, cols)
+    if lse is None or lse.dtype != torch.float32 or not lse.is_contiguous() or \
+            lse.shape != (batch, n_heads, seq_len):
+        raise ValueError("lse: expected the contiguous f32 [batch, n_heads, seq_len] of "
+                         "window_attention(want_lse=True)")
+    if seq_lens is not None:
+        _i32(seq_lens, "seq_lens", batch)
+    if window < 0 or sinks < 0:
+        raise ValueError("window and sinks must not be negative")
+    with _device_of(stream, d_out, q, k, v, out, lse, seq_lens, d_q, d_k, d_v) as s:
+        grads = []
+        for t, name, cols in ((d_q, "d_q", H), (d_k, "d_k", K), (d_v, "d_v", K)):
+            if t is None:
+                t = torch.empty((rows, cols), dtype=q.dtype, device=q.device)
+            grads.append(_rows(t, name, rows, cols))
+        ws = torch.empty((lib.prichs_window_attention_backward_workspace(
+            batch, seq_len, n_heads, n_kv_heads),), dtype=torch.uint8, device=q.device)
+        args = [x for t in (d_out, q, k, v, out) for x in (_p(t), _ld(t))]
+        L.check(lib.prichs_window_attention_backward(
+            *args, _p(lse), _p(seq_lens), *[x for t in grads for x in (_p(t), _ld(t))], batch,
+            seq_len, n_heads, n_kv_heads, head_dim, window, sinks, dtype_code(q), _p(ws),
+            ws.numel(), s))
+    return tuple(grads)
+
+
+def kv_cache_pages(n_pages, n_kv_heads, device="cuda"):
+    """A 4-bit KV cache of n_pages pages, each of L.KV_PAGE positions of every kv
+    head: uint8 [n_pages, n_kv_heads, L.KV_PAGE_BYTES], not initialised."""
+    return torch.empty((n_pages, n_kv_heads, L.KV_PAGE_BYTES), dtype=torch.uint8, device=device)
+
+
+def _kv_cache(cache, page_table, batch, n_kv_heads):
+    if not cache.is_cuda or cache.dtype != torch.uint8 or not cache.is_contiguous() or \
+            cache.dim() != 3 or tuple(cache.shape[1:]) != (n_kv_heads, L.KV_PAGE_BYTES):
+        raise ValueError("cache: expected the pages of kv_cache_pages for these kv heads")
+    _i32(page_table, "page_table", batch, dim=2)
+
+
+def kv_cache_write(cache, page_table, start, k, v, batch, n, n_kv_heads, counts=None,
+                   stream=None):
+    """prichs_kv_cache_write: rows b * n + i of k and v (bf16 or f32, 2-D row views)
+    quantised into position start[b] + i of sequence b, whose pages page_table
+    (int32 device [batch, max_pages]) names; i < counts[b] where counts is given.
+    start, counts: int32 device [batch]."""
+    lib = L.load()
+    _kv_cache(cache, page_table, batch, n_kv_heads)
+    cols = n_kv_heads * 128
+    for t, name in ((k, "k"), (v, "v")):
+        _rows(t, name, batch * n, cols, (torch.bfloat16, torch.float32))
+    if k.dtype != v.dtype:
+        raise TypeError("k and v have different dtypes")
+    _i32(start, "start", batch)
+    if counts is not None:
+        _i32(counts, "counts", batch)
+    with _device_of(stream, cache, page_table, start, counts, k, v) as s:
+        L.check(lib.prichs_kv_cache_write(
+            _p(cache), cache.shape[0], _p(page_table), page_table.shape[1], _p(start), _p(counts),
+            _p(k), _ld(k), _p(v), _ld(v), batch, n, n_kv_heads, 128, dtype_code(k), s))
+
+
+def kv_cache_read(cache, page_table, start, batch, n, n_kv_heads, counts=None,
+                  out_dtype=torch.bfloat16, k=None, v=None, stream=None):
+    """prichs_kv_cache_read: positions start[b] .. start[b] + n - 1 of every sequence
+    -> (k, v) [batch * n, n_kv_heads * 128].  Rows past counts[b] keep what k and v
+    held (zeros where this call allocates them)."""
+    lib = L.load()
+    _kv_cache(cache, page_table, batch, n_kv_heads)
+    _i32(start, "start", batch)
+    if counts is not None:
+        _i32(counts, "counts", batch)
+    shape = (batch * n, n_kv_heads * 128)
+    with _device_of(stream, cache, page_table, start, counts, k, v) as s:
+        make = torch.empty if counts is None else torch.zeros
+        got = []
+        for t, name in ((k, "k"), (v, "v")):
+            if t is None:
+                t = make(shape, dtype=out_dtype, device=cache.device)
+            got.append(_rows(t, name, *shape, (torch.bfloat16, torch.float32)))
+        k, v = got
+        if k.dtype != v.dtype:
+            raise TypeError("k and v have different dtypes")
+        L.check(lib.prichs_kv_cache_read(
+            _p(cache), cache.shape[0], _p(page_table), page_table.shape[1], _p(start), _p(counts),
+            _p(k), _ld(k), _p(v), _ld(v), batch, n, n_kv_heads, 128, dtype_code(k), s))
+    return k, v
+
+
+def kv_cache_attention(q, cache, page_table, lens, batch, n_q, n_heads, n_kv_heads, window=0,
+                       sinks=0, head_dim=128, out=None, want_lse=False, stream=None):
+    """prichs_kv_cache_attention: row b * n_q + i of q is the query at position
+    lens[b] - n_q + i of sequence b, over the cached keys and values (its own
+    among them); lens: int32 device [batch].  -> (out, lse f32 [batch, n_heads,
+    n_q], or None)."""
+    lib = L.load()
+    _kv_cache(cache, page_table, batch, n_kv_heads)
+    rows, H = batch * n_q, n_heads * head_dim
+    _rows(q, "q", rows, H)
+    _i32(lens, "lens", batch)
+    if window < 0 or sinks < 0:
+        raise ValueError("window and sinks must not be negative")
+    with _device_of(stream, q, cache, page_table, lens, out) as s:
+        if out is None:
+            out = torch.empty((rows, H), dtype=q.dtype, device=q.device)
+        _rows(out, "out", rows, H)
+        lse = None
+        if want_lse:
+            lse = torch.empty((batch, n_heads, n_q), dtype=torch.float32, device=q.device)
+        max_pages = page_table.shape[1]
+        ws = torch.empty((lib.prichs_kv_cache_attention_workspace(
+            batch, n_q, n_heads, n_kv_heads, max_pages),), dtype=torch.uint8, device=q.device)
+        L.check(lib.prichs_kv_cache_attention(
+            _p(q), _ld(q), _p(cache), cache.shape[0], _p(page_table), max_pages, _p(lens), _p(out),
+            _ld(out), _p(lse), batch, n_q, n_heads, n_kv_heads, head_dim, window, sinks,
+            dtype_code(q), _p(ws), ws.numel(), s))
+    return out, lse
