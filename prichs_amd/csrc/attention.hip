@@ -55,6 +55,13 @@ constexpr int kThreads = 64 * kWaves;
 constexpr int kTileElems = kBKV * kHd;                   // one K or V tile [64][128]
 constexpr int kStageElems = 2 * kTileElems;              // K then V
 constexpr size_t kLdsBytes = 2 * (size_t)kStageElems * sizeof(bf16_t);  // two stages
+// Arguments of window attention alone (prichs_hip.h).
+struct WindowArgs {
+  float *lse;
+  const int32_t *seq_lens;
+  int window, sinks;
+};
+constexpr size_t kWinLdsBytes = kLdsBytes + 16;  // and a flag
 constexpr float kLazy = 8.0f;  // log2 headroom of the lazily raised softmax max
 
 __device__ __forceinline__ f32x4 mfma_bf16(bf16x8 a, bf16x8 b, f32x4 c) {
@@ -131,6 +138,13 @@ __device__ __forceinline__ void static_for(F &&f) {
   static_for_impl(f, std::make_integer_sequence<int, N>{});
 }
 
+// Two bf16 with an infinity or NaN replaced by 0.
+__device__ __forceinline__ uint32_t finite_bf16x2(uint32_t u) {
+  if ((u & 0x7f80u) == 0x7f80u) u &= 0xffff0000u;
+  if ((u & 0x7f800000u) == 0x7f800000u) u &= 0xffffu;
+  return u;
+}
+
 constexpr uint32_t kTileBytes = kTileElems * sizeof(bf16_t);
 constexpr uint32_t kStageBytes = kStageElems * sizeof(bf16_t);
 
@@ -156,13 +170,16 @@ __device__ __forceinline__ bf16x8 rope_frag(bf16x8 f, float4 c4, float4 s4) {
   return __builtin_bit_cast(bf16x8, u);
 }
 
-// NB: 16-row query blocks per wave.
-template <int HPW, int NB>
+// NB: 16-row query blocks per wave.  WIN: window attention -- a sliding window,
+// sinks, sequences of their own lengths, and the log-sum-exp written (the
+// arguments in wa); row i of a sequence then sees the keys j <= i with i - j <
+// window (0: all) or j < sinks.
+template <int HPW, int NB, bool WIN>
 __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
     const bf16_t *__restrict__ q, int ldq, const bf16_t *__restrict__ k, int ldk,
     const bf16_t *__restrict__ v, int ldv, bf16_t *__restrict__ o, int ldo, int S, int Hq,
     int group, float scale_log2, const float *__restrict__ rcos, const float *__restrict__ rsin,
-    int pos_offset) {
+    int pos_offset, WindowArgs wa) {
   static_assert(kWaves % HPW == 0, "whole row blocks per head");
   constexpr int kRowsWg = 16 * NB * kWaves / HPW;  // query rows per workgroup
   extern __shared__ __attribute__((aligned(16))) bf16_t lds[];
@@ -182,11 +199,28 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
   const int l16 = lane & 15;  // 0..15
 
   const size_t seq0 = (size_t)b * S;
+  // Rows of this sequence; those past them are padding.
+  int L = S;
+  if constexpr (WIN) {
+    if (wa.seq_lens != nullptr) L = min(max(wa.seq_lens[b], 0), S);
+  }
   const bf16_t *kbase = k + seq0 * ldk + (size_t)kvh * kHd;
   const bf16_t *vbase = v + seq0 * ldv + (size_t)kvh * kHd;
 
   // Query rows of this wave: q0 + 16*nb + l16 (nb < NB).
   const int q0 = qb * kRowsWg + (wave / HPW) * 16 * NB;
+  if constexpr (WIN) {
+    if (qb * kRowsWg >= L) {  // padding only
+      for (int nb = 0; nb < NB; ++nb) {
+        const int qrow = q0 + 16 * nb + l16;
+        if (qrow >= S) continue;
+        bf16_t *orow = o + (seq0 + qrow) * ldo + (size_t)h * kHd + 4 * g;
+        for (int jd = 0; jd < 8; ++jd) *reinterpret_cast<u32x2 *>(orow + 16 * jd) = u32x2{0, 0};
+        if (wa.lse != nullptr && g == 0) wa.lse[((size_t)b * Hq + h) * S + qrow] = -INFINITY;
+      }
+      return;
+    }
+  }
 
   // Q fragments (B operand of S^T = K Q^T): lane holds Q[q][32kk + 8g .. +8].
   bf16x8 qf[NB][4];
@@ -228,8 +262,23 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
                                                         0x3f803f80u});
 
   // kv blocks up to the last query row of the workgroup (causal).
-  const int q_last = min(S, (qb + 1) * kRowsWg) - 1;
-  const int n_kvb = q_last / kBKV + 1;
+  const int q_last = min(L, (qb + 1) * kRowsWg) - 1;
+  int n_kvb = q_last / kBKV + 1;
+  // With a window: the blocks that hold sinks (n_sink of them), then those from
+  // the first row's window on; block_of maps an iteration to its block.
+  int n_sink = 0, skip = 0;
+  if constexpr (WIN) {
+    const int first = wa.window == 0 ? 0 : max(0, qb * kRowsWg - wa.window + 1) / kBKV;
+    n_sink = min((wa.sinks + kBKV - 1) / kBKV, first);
+    skip = first - n_sink;
+    n_kvb -= skip;
+  }
+  // The last iteration (+ 1) whose V held an infinity or NaN (behind the tiles).
+  volatile int *scan_flag = reinterpret_cast<volatile int *>(lds + 2 * kStageElems);
+  if constexpr (WIN) {
+    if (tid == 0) *scan_flag = 0;
+  }
+  auto block_of = [&](int i) { return WIN && i >= n_sink ? i + skip : i; };
 
   // Loop-invariant LDS byte addresses of this lane's fragment reads within a
   // stage; rows 16c (K) and 32 ks2 / +16 (V) on share the chunk key and
@@ -257,6 +306,15 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
     dk[i] = 2u * ((uint32_t)row * (uint32_t)ldk + 8u * (uint32_t)(l16 ^ k_key(row)));
     dv[i] = 2u * ((uint32_t)row * (uint32_t)ldv + 8u * (uint32_t)(l16 ^ v_key(row)));
   }
+  // The window's masks need registers: there all but the first of each of these
+  // addresses are formed where they are used.  4 kk, 2 jd and 4 i (8 i) only reach
+  // bits of the chunk index that are exclusive-ored anyway.
+  auto k_at = [&](int kk) { return WIN ? k_addr[0] ^ (uint32_t)(64 * kk) : k_addr[kk]; };
+  auto v_at = [&](int jd, uint32_t stage) {
+    return WIN ? (v_addr[0] + stage) ^ (uint32_t)(32 * jd) : v_addr[jd] + stage;
+  };
+  const uint32_t xk = 16u * (uint32_t)(l16 ^ k_key(g)), rk = dk[0] - xk;
+  const uint32_t xv = 16u * (uint32_t)(l16 ^ v_key(g)), rv = dv[0] - xv;
 
   // Block kb's K tile lives in stage buffer kb & 1 of K, its V tile in stage
   // buffer kb & 1 of V.  K runs one block ahead of V: iteration kb computes
@@ -264,17 +322,22 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
   // its P.V product run, so the matrix and vector pipes overlap within a wave.
   // The buffer resources end after the sequence's last row, so rows past it
   // (last block only) load as zeros; their scores are masked.
-  auto issue_tile = [&](int kb, const bf16_t *src, int ld, const uint32_t (&off)[4],
-                        int tile) {
+  auto issue_tile = [&](int kb, const bf16_t *src, int ld, const uint32_t (&off)[4], uint32_t x,
+                        uint32_t row, int tile) {
     bf16_t *dst = lds + (kb & 1) * kStageElems + tile * kTileElems;
-    const uint64_t bytes = (uint64_t)(S - 1 - kb * kBKV) * 2 * (uint64_t)ld + 2 * kHd;
+    const int blk = block_of(kb);
+    const uint64_t bytes = (uint64_t)(L - 1 - blk * kBKV) * 2 * (uint64_t)ld + 2 * kHd;
     const __amdgpu_buffer_rsrc_t r = buffer_rsrc(
-        src + (size_t)kb * kBKV * ld, bytes > 0xffffffffull ? 0xffffffffu : (uint32_t)bytes);
+        src + (size_t)blk * kBKV * ld, bytes > 0xffffffffull ? 0xffffffffu : (uint32_t)bytes);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) dma_16b(r, off[i], dst + (16 * wave + 4 * i) * kHd);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t key = tile == 0 ? 64u * i : 128u * (i & 1);
+      dma_16b(r, WIN ? (x ^ key) + (row + 8u * i * (uint32_t)ld) : off[i],
+              dst + (16 * wave + 4 * i) * kHd);
+    }
   };
-  auto issue_k = [&](int kb) { issue_tile(kb, kbase, ldk, dk, 0); };
-  auto issue_v = [&](int kb) { issue_tile(kb, vbase, ldv, dv, 1); };
+  auto issue_k = [&](int kb) { issue_tile(kb, kbase, ldk, dk, xk, rk, 0); };
+  auto issue_v = [&](int kb) { issue_tile(kb, vbase, ldv, dv, xv, rv, 1); };
   // Every wave's DMAs issued so far have landed (each wave waits for its own,
   // the barrier for the others'), and every wave is past the reads before it.
   // s_waitcnt vmcnt(0) (gfx9 encoding: vmcnt[3:0] | expcnt 7 << 4 |
@@ -297,12 +360,36 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
       bf16x8 kf[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c)
-        kf[c] = *reinterpret_cast<const bf16x8 *>(kbytes + 16 * kHd * 2 * c + k_addr[kk]);
+        kf[c] = *reinterpret_cast<const bf16x8 *>(kbytes + 16 * kHd * 2 * c + k_at(kk));
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) sacc[c][nb] = mfma_bf16(kf[c], qf[nb][kk], sacc[c][nb]);
     }
+  };
+
+  // Masks block kv0's scores of query block nb.
+  auto hide = [&](int nb, int kv0, f32x4 (&scur)[4][NB]) {
+    // Valid iff kv <= query row and kv < L, i.e. 16c + r <= lim.
+    const int lim = min(q0 + 16 * nb + l16, L - 1) - kv0 - 4 * g;
+    // Behind the window: 16c + r <= old, unless a sink (16c + r < sink).
+    const int old = WIN && wa.window != 0 ? q0 + 16 * nb + l16 - wa.window - kv0 - 4 * g : -64;
+    const int sink = WIN ? wa.sinks - kv0 - 4 * g : 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        bool hidden = 16 * c + r > lim;
+        if constexpr (WIN) hidden |= (16 * c + r <= old) & (16 * c + r >= sink);
+        scur[c][nb][r] = hidden ? -INFINITY : scur[c][nb][r];
+      }
+  };
+  // Whether every row of the workgroup sees all of iteration i's block.
+  auto whole = [&](int i) {
+    const int kv0 = block_of(i) * kBKV;
+    return kv0 + kBKV <= min(qb * kRowsWg + 1, L) &&
+           (wa.window == 0 || (qb + 1) * kRowsWg - 1 - kv0 < wa.window ||
+            kv0 + kBKV <= wa.sinks);
   };
 
   // Iteration kb: S of block kb + 1 into snext (past the last block the
@@ -311,12 +398,44 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
   // (blocks reaching past this wave's first query row or the sequence end).
   auto run_iter = [&](int kb, auto masked_c, f32x4 (&scur)[4][NB], f32x4 (&snext)[4][NB]) {
     constexpr bool kMasked = decltype(masked_c)::value;
-    const int kv0 = kb * kBKV;
+    const int kv0 = block_of(kb) * kBKV;
     // K of block kb + 1 and V of block kb have landed; the buffers of K kb
     // and V kb - 1 are free for K kb + 2 and V kb + 1.
     sync_tiles();
     if (kb + 2 < n_kvb) issue_k(kb + 2);
     if (kb + 1 < n_kvb) issue_v(kb + 1);
+
+    // Window attention decides by block, in one body, whether it is masked (the
+    // waves of a workgroup agree: a masked block has one barrier more).
+    bool masked = kMasked;
+    if constexpr (WIN) masked = !whole(kb);
+    if (WIN && masked) {
+      // This block holds keys that some rows of the workgroup do not see.  Their p
+      // is 0, but 0 times an infinity or NaN of V is NaN: those elements are set to
+      // 0 in the tile, and added after the product to the rows that see them.  (A
+      // half of u has all exponent bits set where adding one to its exponent
+      // carries into the sign.)
+      char *vt = reinterpret_cast<char *>(lds) + (uint32_t)(kb & 1) * kStageBytes + kTileBytes;
+      uint32_t bad = 0;
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        const u32x4 u = *reinterpret_cast<const u32x4 *>(vt + 16 * (i * kThreads + tid));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bad |= (u[e] & 0x7f807f80u) + 0x00800080u;
+      }
+      if (bad & 0x80008000u) {
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          u32x4 u = *reinterpret_cast<const u32x4 *>(vt + 16 * (i * kThreads + tid));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) u[e] = finite_bf16x2(u[e]);
+          *reinterpret_cast<u32x4 *>(vt + 16 * (i * kThreads + tid)) = u;
+        }
+        *scan_flag = kb + 1;
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) hide(nb, kv0, scur);
+    }
 
     compute_s(kb + 1, snext);
 
@@ -328,15 +447,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
     bool raise[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      if constexpr (kMasked) {
-        // Valid iff kv <= query row and kv < S, i.e. 16c + r <= lim.
-        const int lim = min(q0 + 16 * nb + l16, S - 1) - kv0 - 4 * g;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (16 * c + r > lim) scur[c][nb][r] = -INFINITY;
-      }
+      if constexpr (kMasked && !WIN) hide(nb, kv0, scur);
       float mloc = -INFINITY;
 #pragma unroll
       for (int c = 0; c < 4; ++c)
@@ -352,7 +463,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
       float m_use = m_new;
       // Rows with no valid score yet keep m = -inf; exp2(-inf - -inf) would
       // be NaN.  Only a masked block can leave a row without one.
-      if constexpr (kMasked) m_use = m_new == -INFINITY ? 0.f : m_new;
+      if constexpr (kMasked || WIN) m_use = m_new == -INFINITY ? 0.f : m_new;
       const float neg_m = -m_use;
 #pragma unroll
       for (int ks2 = 0; ks2 < 2; ++ks2) {
@@ -386,6 +497,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
     // upper half), columns 16 jd + 4 (m % 4) .. + 3; four d blocks per batch
     // of transposing reads.
     const uint32_t v_stage = (uint32_t)(kb & 1) * kStageBytes;
+    if (WIN && masked) lds_write_barrier();  // the scan's zeros
     static_for<2>([&](auto ks2_c) {
       constexpr int ks2 = decltype(ks2_c)::value;
       constexpr int kLo = (int)kTileBytes + 2 * 32 * ks2 * kHd;  // rows 32 ks2 + ...
@@ -395,7 +507,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
         u32x2 lo[4], hi[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const uint32_t a = v_addr[j0 + t] + v_stage;
+          const uint32_t a = v_at(j0 + t, v_stage);
           lo[t] = ds_read_tr16<kLo>(a);
           hi[t] = ds_read_tr16<kHi>(a);
         }
@@ -413,6 +525,36 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
       for (int nb = 0; nb < NB; ++nb)
         lsum[nb] = mfma_bf16(ones, __builtin_bit_cast(bf16x8, pf[nb][ks2]), lsum[nb]);
     });
+    if (WIN && masked) {
+      // The infinities and NaN that the scan took out, for the rows that see
+      // them (p > 0 there: an infinity keeps its sign).
+      if (*scan_flag == kb + 1) {
+#pragma unroll 1
+        for (int j = 0; j < kBKV && kv0 + j < L; ++j) {
+          const int key = kv0 + j;
+          const bf16_t *vrow = vbase + (size_t)key * ldv + 4 * g;
+          bool sees[NB];
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            const int row = q0 + 16 * nb + l16;
+            sees[nb] = (key <= row) &
+                       ((wa.window == 0) | (row - key < wa.window) | (key < wa.sinks));
+          }
+#pragma unroll
+          for (int jd = 0; jd < 8; ++jd) {
+            const u32x2 raw = *reinterpret_cast<const u32x2 *>(vrow + 16 * jd);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const uint32_t x = r & 1 ? raw[r / 2] & 0xffff0000u : raw[r / 2] << 16;
+              const bool off = (x & 0x7f800000u) == 0x7f800000u;
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+                oacc[jd][nb][r] += (off & sees[nb]) ? __uint_as_float(x) : 0.f;
+            }
+          }
+        }
+      }
+    }
   };
 
   // Blocks whose kv rows all lie at or before this wave's first query row
@@ -427,32 +569,51 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
   if (n_kvb > 1) issue_k(1);
   compute_s(0, sa);
   int kb = 0;
-  for (; kb + 2 <= n_full; kb += 2) {
-    run_iter(kb, bool_c<false>{}, sa, sb);
-    run_iter(kb + 1, bool_c<false>{}, sb, sa);
-  }
   auto take_next = [&]() {
 #pragma unroll
     for (int c = 0; c < 4; ++c)
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) sa[c][nb] = sb[c][nb];
   };
-  if (kb < n_full) {
-    run_iter(kb, bool_c<false>{}, sa, sb);
-    take_next();
-    ++kb;
-  }
-  for (; kb < n_kvb; ++kb) {
-    run_iter(kb, bool_c<true>{}, sa, sb);
-    take_next();
+  if constexpr (WIN) {
+    for (; kb < n_kvb; kb += 2) {
+      run_iter(kb, bool_c<false>{}, sa, sb);
+      if (kb + 1 < n_kvb) run_iter(kb + 1, bool_c<false>{}, sb, sa);
+    }
+  } else {
+    for (; kb + 2 <= n_full; kb += 2) {
+      run_iter(kb, bool_c<false>{}, sa, sb);
+      run_iter(kb + 1, bool_c<false>{}, sb, sa);
+    }
+    if (kb < n_full) {
+      run_iter(kb, bool_c<false>{}, sa, sb);
+      take_next();
+      ++kb;
+    }
+    for (; kb < n_kvb; ++kb) {
+      run_iter(kb, bool_c<true>{}, sa, sb);
+      take_next();
+    }
   }
 
   // Normalise by the row sum and store: lane holds O[q][16 jd + 4g + r].
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    const float inv = 1.0f / fmaxf(lsum[nb][0], 1e-30f);
+    // (A row of window attention sees itself at least: a sum of 0 means that
+    // every score is -inf, and 0 / 0 is the softmax of that.)
+    const float inv = 1.0f / (WIN ? lsum[nb][0] : fmaxf(lsum[nb][0], 1e-30f));
     const int qrow = q0 + 16 * nb + l16;
-    if (qrow < S) {
+    if constexpr (WIN) {
+      if (wa.lse != nullptr && g == 0 && qrow < S)
+        wa.lse[((size_t)b * Hq + h) * S + qrow] =
+            qrow < L ? (m_ref[nb] + log2f(lsum[nb][0])) * 0.6931471805599453f : -INFINITY;
+      if (qrow >= L && qrow < S) {
+        bf16_t *orow = o + (seq0 + qrow) * ldo + (size_t)h * kHd + 4 * g;
+#pragma unroll
+        for (int jd = 0; jd < 8; ++jd) *reinterpret_cast<u32x2 *>(orow + 16 * jd) = u32x2{0, 0};
+      }
+    }
+    if (qrow < L) {
       bf16_t *orow = o + (seq0 + qrow) * ldo + (size_t)h * kHd + 4 * g;
 #pragma unroll
       for (int jd = 0; jd < 8; ++jd) {
@@ -520,18 +681,55 @@ int attention_forward_impl(const void *q, size_t ldq, const void *k, size_t ldk,
   const bool few = 2 * (n_heads / hpw) * batch * (size_t)n_qb <= 3 * (size_t)std::max(cus, 0);
   if (few) n_qb = (int)cdiv(seq_len, (size_t)(16 * kWaves / hpw));
   const dim3 grid((unsigned)(n_heads / hpw), (unsigned)batch, (unsigned)n_qb);
-  auto kern = few ? (hpw == 4   ? attn_fwd_kernel<4, 1>
-                     : hpw == 2 ? attn_fwd_kernel<2, 1>
-                                : attn_fwd_kernel<1, 1>)
-                  : (hpw == 4   ? attn_fwd_kernel<4, 2>
-                     : hpw == 2 ? attn_fwd_kernel<2, 2>
-                                : attn_fwd_kernel<1, 2>);
+  auto kern = few ? (hpw == 4   ? attn_fwd_kernel<4, 1, false>
+                     : hpw == 2 ? attn_fwd_kernel<2, 1, false>
+                                : attn_fwd_kernel<1, 1, false>)
+                  : (hpw == 4   ? attn_fwd_kernel<4, 2, false>
+                     : hpw == 2 ? attn_fwd_kernel<2, 2, false>
+                                : attn_fwd_kernel<1, 2, false>);
   hipLaunchKernelGGL(kern, grid, dim3(kThreads), kLdsBytes, as_stream(stream),
                      static_cast<const bf16_t *>(q), (int)ldq, static_cast<const bf16_t *>(k),
                      (int)ldk, static_cast<const bf16_t *>(v), (int)ldv,
                      static_cast<bf16_t *>(o), (int)ldo, (int)seq_len, (int)n_heads, group,
-                     scale_log2, rope_cos, rope_sin, (int)pos_offset);
+                     scale_log2, rope_cos, rope_sin, (int)pos_offset, WindowArgs{});
   PRICHS_LAUNCH_CHECK("attention launch");
+  return PRICHS_OK;
+}
+
+int window_attention_launch(const void *q, size_t ldq, const void *k, size_t ldk, const void *v,
+                            size_t ldv, void *o, size_t ldo, float *lse, const int32_t *seq_lens,
+                            size_t batch, size_t seq_len, size_t n_heads, size_t n_kv_heads,
+                            size_t window, size_t sinks, void *stream) {
+  const int group = (int)(n_heads / n_kv_heads);
+  const int hpw = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+  const size_t n_qb32 = cdiv(seq_len, (size_t)(32 * kWaves / hpw));
+  const int cus = device_cu_count();
+  const bool few = 2 * (n_heads / hpw) * batch * n_qb32 <= 3 * (size_t)std::max(cus, 0);
+  const size_t n_qb = few ? cdiv(seq_len, (size_t)(16 * kWaves / hpw)) : n_qb32;
+  PRICHS_REQUIRE(n_qb <= 65535, "window_attention: seq_len too large");
+  const float scale_log2 = (1.0f / sqrtf((float)kHd)) * 1.4426950408889634f;
+  const dim3 grid((unsigned)(n_heads / hpw), (unsigned)batch, (unsigned)n_qb);
+  static const struct {
+    decltype(&attn_fwd_kernel<4, 2, true>) kernel;
+    int hpw;
+    bool few;
+  } kinds[] = {{attn_fwd_kernel<4, 1, true>, 4, true},  {attn_fwd_kernel<2, 1, true>, 2, true},
+               {attn_fwd_kernel<1, 1, true>, 1, true},  {attn_fwd_kernel<4, 2, true>, 4, false},
+               {attn_fwd_kernel<2, 2, true>, 2, false}, {attn_fwd_kernel<1, 2, true>, 1, false}};
+  static LdsLimit limits[6];
+  int i = 0;
+  while (kinds[i].hpw != hpw || kinds[i].few != few) ++i;
+  const auto kern = kinds[i].kernel;
+  if (int rc = raise_lds_limit(limits[i], reinterpret_cast<const void *>(kern), kWinLdsBytes,
+                               "window_attention"))
+    return rc;
+  hipLaunchKernelGGL(kern, grid, dim3(kThreads), kWinLdsBytes, as_stream(stream),
+                     static_cast<const bf16_t *>(q), (int)ldq, static_cast<const bf16_t *>(k),
+                     (int)ldk, static_cast<const bf16_t *>(v), (int)ldv,
+                     static_cast<bf16_t *>(o), (int)ldo, (int)seq_len, (int)n_heads, group,
+                     scale_log2, nullptr, nullptr, 0,
+                     WindowArgs{lse, seq_lens, (int)window, (int)sinks});
+  PRICHS_LAUNCH_CHECK("window_attention launch");
   return PRICHS_OK;
 }
 }  // namespace prichs

@@ -252,6 +252,13 @@ int attention_forward_impl(const void *q, size_t ldq, const void *k, size_t ldk,
                            const float *rope_cos, const float *rope_sin, size_t cache_rows,
                            size_t pos_offset, void *stream);
 
+// prichs_window_attention_forward after its checks (attention.hip): window 0 or
+// below seq_len, sinks at most seq_len.
+int window_attention_launch(const void *q, size_t ldq, const void *k, size_t ldk, const void *v,
+                            size_t ldv, void *o, size_t ldo, float *lse, const int32_t *seq_lens,
+                            size_t batch, size_t seq_len, size_t n_heads, size_t n_kv_heads,
+                            size_t window, size_t sinks, void *stream);
+
 // prichs_router_topk then prichs_permute; when one router workgroup covers
 // the batch (decode-sized T) the router writes the permutation itself
 // (router.hip).  Same outputs either way.  w_lds (may be null): the router

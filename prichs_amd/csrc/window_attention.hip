@@ -27,41 +27,6 @@ struct Shape {
   float scale;
 };
 
-// One wave per (row, query head): an online softmax over the visible keys, the
-// lane holding dims 2 lane and 2 lane + 1.
-__global__ __launch_bounds__(64) void window_fwd_row_kernel(
-    const bf16_t *q, size_t ldq, const bf16_t *k, size_t ldk, const bf16_t *v, size_t ldv,
-    bf16_t *o, size_t ldo, float *lse, const int32_t *seq_lens, Shape sh) {
-  const int lane = threadIdx.x, h = blockIdx.y;
-  const int b = blockIdx.x / sh.S, i = blockIdx.x - b * sh.S;
-  const int kvh = h / (sh.Hq / sh.Hkv);
-  const size_t row0 = (size_t)b * sh.S;
-  bf16_t *orow = o + (row0 + i) * ldo + (size_t)h * kHd + 2 * lane;
-  float *ls = lse == nullptr ? nullptr : lse + ((size_t)b * sh.Hq + h) * sh.S + i;
-  if (i >= rows_of(seq_lens, b, sh.S)) {
-    store2(orow, 0.f, 0.f);
-    if (ls != nullptr && lane == 0) *ls = -INFINITY;
-    return;
-  }
-  const float2 qv = load2(q + (row0 + i) * ldq + (size_t)h * kHd + 2 * lane);
-  const int lo = sh.window == 0 ? 0 : max(0, i - sh.window + 1);
-  float m = -INFINITY, l = 0.f, a0 = 0.f, a1 = 0.f;
-  for (int j = 0; j <= i; ++j) {
-    if (j >= min(sh.sinks, lo) && j < lo) j = lo;
-    const size_t c = (size_t)kvh * kHd + 2 * lane;
-    const float2 kv = load2(k + (row0 + j) * ldk + c), vv = load2(v + (row0 + j) * ldv + c);
-    const float s = wave_sum(qv.x * kv.x + qv.y * kv.y) * sh.scale;
-    const float m2 = __builtin_elementwise_maximum(m, s);
-    const float r = m2 == m ? 1.f : expf(m - m2), p = m2 == -INFINITY ? 0.f : expf(s - m2);
-    l = l * r + p;
-    a0 = a0 * r + p * vv.x;
-    a1 = a1 * r + p * vv.y;
-    m = m2;
-  }
-  store2(orow, a0 / l, a1 / l);
-  if (ls != nullptr && lane == 0) *ls = m + logf(l);
-}
-
 // delta[b][h][i] = d_o . o, one wave per (row, query head).
 __global__ __launch_bounds__(64) void window_delta_kernel(const bf16_t *d_o, size_t ldd,
                                                           const bf16_t *o, size_t ldo,
@@ -204,12 +169,8 @@ extern "C" int prichs_window_attention_forward(
   WINDOW_TRY(check_rows(who, "k", k, ldk, K));
   WINDOW_TRY(check_rows(who, "v", v, ldv, K));
   WINDOW_TRY(check_rows(who, "o", o, ldo, H));
-  hipLaunchKernelGGL(window_fwd_row_kernel, dim3((unsigned)(batch * seq_len), (unsigned)n_heads),
-                     dim3(64), 0, as_stream(stream), static_cast<const bf16_t *>(q), ldq,
-                     static_cast<const bf16_t *>(k), ldk, static_cast<const bf16_t *>(v), ldv,
-                     static_cast<bf16_t *>(o), ldo, lse, seq_lens, sh);
-  PRICHS_LAUNCH_CHECK("window_attention launch");
-  return PRICHS_OK;
+  return window_attention_launch(q, ldq, k, ldk, v, ldv, o, ldo, lse, seq_lens, batch, seq_len,
+                                 n_heads, n_kv_heads, (size_t)sh.window, (size_t)sh.sinks, stream);
 }
 
 extern "C" size_t prichs_window_attention_backward_workspace(size_t batch, size_t seq_len,

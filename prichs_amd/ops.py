@@ -310,6 +310,10 @@ def _rows(t, name, rows, cols, dtypes=(torch.bfloat16,)):
     return t
 
 
+def _a(t):
+    return None if t is None else t.data_ptr()
+
+
 def _ld(t):
     """Row stride; of a single row its width, whatever stride torch keeps for it."""
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
@@ -324,28 +328,34 @@ def _i32(t, name, n, dim=1):
 
 
 class _device_of:
-    """The device of the operands (all on one) made current, and its stream: the
-    given one, or torch's current one there.  Outputs and workspaces allocated
-    inside belong to that stream."""
+    """The device of the operands (all on one) made current where it is not, and the
+    stream to launch on: the given one, or torch's current one there.  Outputs and
+    workspaces allocated inside belong to that stream."""
 
-    def __init__(self, stream, *tensors):
-        dev = {t.device for t in tensors if t is not None}
-        if len(dev) != 1:
-            raise ValueError(f"operands on different devices: {sorted(map(str, dev))}")
-        self.device = dev.pop()
+    def __init__(self, stream, first, *others):
+        dev = first.device
+        for t in others:
+            if t is not None and t.device != dev:
+                raise ValueError(f"operands on different devices: {dev} and {t.device}")
+        self._ctx = None
+        if stream is not None:
+            if stream.device != dev:
+                raise ValueError(f"a stream of {stream.device} with operands on {dev}")
+            self._ctx = torch.cuda.stream(stream)
+        elif torch.cuda.current_device() != dev.index:
+            self._ctx = torch.cuda.device(dev)
         if stream is None:
-            stream = torch.cuda.current_stream(self.device)
-        elif stream.device != self.device:
-            raise ValueError(f"a stream of {stream.device} with operands on {self.device}")
-        self.stream = stream
-        self._ctx = torch.cuda.stream(stream)
+            stream = torch.cuda.current_stream(dev)
+        self.raw = stream.cuda_stream
 
     def __enter__(self):
-        self._ctx.__enter__()
-        return C.c_void_p(self.stream.cuda_stream)
+        if self._ctx is not None:
+            self._ctx.__enter__()
+        return self.raw
 
     def __exit__(self, *exc):
-        return self._ctx.__exit__(*exc)
+        if self._ctx is not None:
+            self._ctx.__exit__(*exc)
 
 
 def window_attention(q, k, v, batch, seq_len, n_heads, n_kv_heads, window, sinks=0,
@@ -370,7 +380,7 @@ def window_attention(q, k, v, batch, seq_len, n_heads, n_kv_heads, window, sinks
         if want_lse:
             lse = torch.empty((batch, n_heads, seq_len), dtype=torch.float32, device=q.device)
         L.check(lib.prichs_window_attention_forward(
-            _p(q), _ld(q), _p(k), _ld(k), _p(v), _ld(v), _p(out), _ld(out), _p(lse), _p(seq_lens),
+            _a(q), _ld(q), _a(k), _ld(k), _a(v), _ld(v), _a(out), _ld(out), _a(lse), _a(seq_lens),
             batch, seq_len, n_heads, n_kv_heads, head_dim, window, sinks, dtype_code(q), s))
     return out, lse
 
@@ -403,10 +413,10 @@ def window_attention_backward(d_out, q, k, v, out, lse, batch, seq_len, n_heads,
             grads.append(_rows(t, name, rows, cols))
         ws = torch.empty((lib.prichs_window_attention_backward_workspace(
             batch, seq_len, n_heads, n_kv_heads),), dtype=torch.uint8, device=q.device)
-        args = [x for t in (d_out, q, k, v, out) for x in (_p(t), _ld(t))]
+        args = [x for t in (d_out, q, k, v, out) for x in (_a(t), _ld(t))]
         L.check(lib.prichs_window_attention_backward(
-            *args, _p(lse), _p(seq_lens), *[x for t in grads for x in (_p(t), _ld(t))], batch,
-            seq_len, n_heads, n_kv_heads, head_dim, window, sinks, dtype_code(q), _p(ws),
+            *args, _a(lse), _a(seq_lens), *[x for t in grads for x in (_a(t), _ld(t))], batch,
+            seq_len, n_heads, n_kv_heads, head_dim, window, sinks, dtype_code(q), _a(ws),
             ws.numel(), s))
     return tuple(grads)
 
@@ -442,8 +452,8 @@ def kv_cache_write(cache, page_table, start, k, v, batch, n, n_kv_heads, counts=
         _i32(counts, "counts", batch)
     with _device_of(stream, cache, page_table, start, counts, k, v) as s:
         L.check(lib.prichs_kv_cache_write(
-            _p(cache), cache.shape[0], _p(page_table), page_table.shape[1], _p(start), _p(counts),
-            _p(k), _ld(k), _p(v), _ld(v), batch, n, n_kv_heads, 128, dtype_code(k), s))
+            _a(cache), cache.shape[0], _a(page_table), page_table.shape[1], _a(start), _a(counts),
+            _a(k), _ld(k), _a(v), _ld(v), batch, n, n_kv_heads, 128, dtype_code(k), s))
 
 
 def kv_cache_read(cache, page_table, start, batch, n, n_kv_heads, counts=None,
@@ -468,8 +478,8 @@ def kv_cache_read(cache, page_table, start, batch, n, n_kv_heads, counts=None,
         if k.dtype != v.dtype:
             raise TypeError("k and v have different dtypes")
         L.check(lib.prichs_kv_cache_read(
-            _p(cache), cache.shape[0], _p(page_table), page_table.shape[1], _p(start), _p(counts),
-            _p(k), _ld(k), _p(v), _ld(v), batch, n, n_kv_heads, 128, dtype_code(k), s))
+            _a(cache), cache.shape[0], _a(page_table), page_table.shape[1], _a(start), _a(counts),
+            _a(k), _ld(k), _a(v), _ld(v), batch, n, n_kv_heads, 128, dtype_code(k), s))
     return k, v
 
 
@@ -497,7 +507,7 @@ def kv_cache_attention(q, cache, page_table, lens, batch, n_q, n_heads, n_kv_hea
         ws = torch.empty((lib.prichs_kv_cache_attention_workspace(
             batch, n_q, n_heads, n_kv_heads, max_pages),), dtype=torch.uint8, device=q.device)
         L.check(lib.prichs_kv_cache_attention(
-            _p(q), _ld(q), _p(cache), cache.shape[0], _p(page_table), max_pages, _p(lens), _p(out),
-            _ld(out), _p(lse), batch, n_q, n_heads, n_kv_heads, head_dim, window, sinks,
-            dtype_code(q), _p(ws), ws.numel(), s))
+            _a(q), _ld(q), _a(cache), cache.shape[0], _a(page_table), max_pages, _a(lens), _a(out),
+            _ld(out), _a(lse), batch, n_q, n_heads, n_kv_heads, head_dim, window, sinks,
+            dtype_code(q), _a(ws), ws.numel(), s))
     return out, lse
