@@ -1,57 +1,477 @@
 // kv_attention.hip -- GQA attention of a sequence's last tokens over its paged
 // 4-bit KV cache (kv_cache.hpp has the layout and the number format).
+//
+// All query rows that read one kv head (n_q tokens x G heads, row = token * G +
+// head) form tiles of 16 NB rows.  A wave takes whole pages of 64 keys:
+//   S^T = K Q^T     v_mfma_f32_16x16x32_bf16: a lane holds 32 head dims (16 bytes
+//                   of codes, one scale) of a key, converted two at a time with
+//                   their scale -- exact in bf16 -- straight into the operand; the
+//                   products' k index runs over dims 32 g + 8 kk .. + 7 (g = lane /
+//                   16) on both sides;
+//   O^T += V^T P^T  P comes from the softmax registers: a lane holds keys 16 c +
+//                   4 g .. + 3 of its query, two quads of each 32-key step, and
+//                   reads dword lane % 16 of the same quads of V.  A converted pair
+//                   holds two dims of one key; a byte permute of two keys' pairs
+//                   gives both dims' operands, and the product's row m of block jd
+//                   is dim 8 m + jd.
+// Nothing goes through LDS before the waves join, no lane exchange but the row
+// maximum, and a page is read once per row tile: 8704 bytes against 65 KB in f32 /
+// 32 KB in bf16.  Each wave reads its next page into registers while it computes one.
+//
+// The visible pages of a tile are dealt to 4 n_split waves in contiguous runs; the
+// waves of a workgroup join in LDS, workgroups through the workspace and a second
+// kernel (n_split > 1).  The order of both is fixed, so results are reproducible.
 #include "kv_cache.hpp"
+
+#include <algorithm>
+#include <type_traits>
 
 namespace prichs {
 namespace {
 
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr float kLazy = 8.0f;  // log2 headroom of the lazily raised softmax max
+
 struct AttendShape {
-  int n_pages, max_pages, n_q, Hq, Hkv, window, sinks;
-  float scale;
+  int n_pages, max_pages, n_q, Hq, Hkv, window, sinks, tiles, n_split;
+  float scale_log2;
 };
 
-// One wave per (query row, query head), the lane holding dims 2 lane, 2 lane + 1.
-__global__ __launch_bounds__(64) void kv_attend_row_kernel(
-    const bf16_t *q, size_t ldq, const uint8_t *cache, const int32_t *table, const int32_t *lens,
-    bf16_t *o, size_t ldo, float *lse, AttendShape sh) {
-  const int lane = threadIdx.x, h = blockIdx.y;
-  const int b = blockIdx.x / sh.n_q, iq = blockIdx.x - b * sh.n_q;
-  const int kvh = h / (sh.Hq / sh.Hkv);
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float vmax(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+// Max over the four 16-lane groups that share a query column (NaN propagates).
+__device__ __forceinline__ float max_across_groups(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  x = vmax(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const uint32_t w = __float_as_uint(x);
+  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return vmax(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// Values 2 BYTE and 2 BYTE + 1 of a dword of codes, in bf16.
+template <int BYTE>
+__device__ __forceinline__ uint32_t pair(uint32_t codes, float scale) {
+  return __builtin_bit_cast(uint32_t,
+                            __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, BYTE));
+}
+__device__ __forceinline__ u32x4 eight(uint32_t codes, float scale) {
+  return u32x4{pair<0>(codes, scale), pair<1>(codes, scale), pair<2>(codes, scale),
+               pair<3>(codes, scale)};
+}
+
+// A page of one kv head as a lane holds it.
+struct PageRegs {
+  u32x4 k[4];  // key 16 c + lane % 16, dims 32 g ..
+  u32x4 v[4];  // quad 4 q + g, dword lane % 16 of its four keys
+  uint32_t ks; // scales of k[0..3]
+  u32x4 vs;    // scales of v[0..3]
+};
+
+// NB: 16-row query blocks of a tile.
+template <int NB>
+__global__ __launch_bounds__(kThreads, NB == 1 ? 3 : 2) void kv_attend_kernel(
+    const bf16_t *__restrict__ q, size_t ldq, const uint8_t *__restrict__ cache,
+    const int32_t *__restrict__ table, const int32_t *__restrict__ lens, bf16_t *__restrict__ o,
+    size_t ldo, float *__restrict__ lse, float *__restrict__ part_o, float2 *__restrict__ part_ml,
+    AttendShape sh) {
+  constexpr int kRows = 16 * NB;
+  __shared__ float s_ml[2][kWaves][kRows];
+  __shared__ float s_o[kWaves][kRows * kKvHd];
+
+  const int split = blockIdx.x;
+  const int kvh = blockIdx.y / sh.tiles, tile = blockIdx.y - kvh * sh.tiles;
+  const int b = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, l16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = sh.Hq / sh.Hkv, rows = sh.n_q * G;
+
   const int L = min(max(lens[b], 0), sh.max_pages * kKvPage);
-  const int i = L - sh.n_q + iq;
-  const size_t c = (size_t)h * kKvHd + 2 * lane;
-  const float q0 = bf16_to_f32(q[(size_t)blockIdx.x * ldq + c]),
-              q1 = bf16_to_f32(q[(size_t)blockIdx.x * ldq + c + 1]);
-  const int lo = sh.window == 0 ? 0 : max(0, i - sh.window + 1);
-  float m = -INFINITY, l = 0.f, a0 = 0.f, a1 = 0.f;
-  bool any = false;
-  for (int j = 0; j <= i; ++j) {
-    if (j >= min(sh.sinks, lo) && j < lo) j = lo;
-    const int page = table[(size_t)b * sh.max_pages + j / kKvPage];
-    if (page < 0 || page >= sh.n_pages) continue;
-    any = true;
-    const uint8_t *part = cache + ((size_t)page * sh.Hkv + kvh) * kKvPart;
-    const int t = j % kKvPage;
-    const float ks = kv_scale(part[kKvKScale + 4 * t + lane / 16]),
-                vs = kv_scale(part[kKvVScale + 4 * t + lane / 16]);
-    const auto kk = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(
-        part[kKvK + t * (kKvHd / 2) + lane], 1.0f, 0);
-    const auto vv = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(
-        part[kv_v_off(t, lane >> 2) + (lane & 3)], 1.0f, 0);
-    float s = q0 * (kk[0] * ks) + q1 * (kk[1] * ks);
-    for (int x = 1; x < 64; x <<= 1) s += __shfl_xor(s, x);
-    s *= sh.scale;
-    const float m2 = __builtin_elementwise_maximum(m, s);
-    const float r = m2 == m ? 1.f : expf(m - m2), p = m2 == -INFINITY ? 0.f : expf(s - m2);
-    l = l * r + p;
-    a0 = a0 * r + p * (vv[0] * vs);
-    a1 = a1 * r + p * (vv[1] * vs);
+  // Positions of the tile's first and last row, and of this lane's rows.
+  const int r0 = tile * kRows, r1 = min(r0 + kRows, rows) - 1;
+  const int p0 = L - sh.n_q + r0 / G, p1 = L - sh.n_q + r1 / G;
+  int pos[NB];
+  u32x4 qf[NB][4];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int r = min(r0 + 16 * nb + l16, rows - 1);
+    const int iq = r / G;
+    pos[nb] = L - sh.n_q + iq;
+    const bf16_t *qrow = q + ((size_t)b * sh.n_q + iq) * ldq +
+                         (size_t)(kvh * G + r - iq * G) * kKvHd + 32 * g;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) qf[nb][kk] = *reinterpret_cast<const u32x4 *>(qrow + 8 * kk);
+  }
+
+  // The pages that some row sees: those of the sinks, then from the first row's
+  // window on.
+  const int first = sh.window == 0 ? 0 : max(0, p0 - sh.window + 1) / kKvPage;
+  const int n_sink = min((sh.sinks + kKvPage - 1) / kKvPage, first);
+  const int skip = first - n_sink;
+  const int n_vis = p1 < 0 ? 0 : p1 / kKvPage + 1 - skip;
+  const int per = (n_vis + kWaves * sh.n_split - 1) / (kWaves * sh.n_split);
+  const int begin = min((split * kWaves + wave) * per, n_vis), end = min(begin + per, n_vis);
+  auto block_of = [&](int i) { return i >= n_sink ? i + skip : i; };
+  const int32_t *row_table = table + (size_t)b * sh.max_pages;
+  // Page of the i-th visible block (-1: none); the same for the whole wave.
+  auto page_at = [&](int i) {
+    if (i >= end) return -1;
+    const int p = __builtin_amdgcn_readfirstlane(row_table[block_of(i)]);
+    return p >= 0 && p < sh.n_pages ? p : -1;
+  };
+
+  f32x4 oacc[8][NB], lsum[NB];
+  float m_ref[NB];
+  bool seen[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+    for (int jd = 0; jd < 8; ++jd) oacc[jd][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    lsum[nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m_ref[nb] = -INFINITY;
+    seen[nb] = false;
+  }
+  const u32x4 ones = u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+
+  auto part_of = [&](int page) { return cache + ((size_t)page * sh.Hkv + kvh) * kKvPart; };
+  // A lane's offsets within a page; the page's address is the wave's.
+  const uint32_t ko = kKvK + 64 * l16 + 16 * g, vo = kKvV + 256 * g + 16 * l16,
+                 kso = kKvKScale + kKvPage * g + 4 * l16,
+                 vso = kKvVScale + kKvPage * (l16 >> 2) + 16 * g;
+  auto load = [&](PageRegs &x, int page) {
+    if (page < 0) return;
+    const uint8_t *p = part_of(page);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      x.k[c] = *reinterpret_cast<const u32x4 *>(p + ko + 1024 * c);
+      x.v[c] = *reinterpret_cast<const u32x4 *>(p + vo + 1024 * c);
+    }
+    x.ks = *reinterpret_cast<const uint32_t *>(p + kso);
+    x.vs = *reinterpret_cast<const u32x4 *>(p + vso);
+  };
+
+  auto compute = [&](PageRegs &x, int i, int page) {
+    if (page < 0) return;
+    const int kv0 = block_of(i) * kKvPage;
+    f32x4 s[4][NB];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float sc = kv_scale((x.ks >> (8 * c)) & 255u);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) s[c][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        const u32x4 kf = eight(x.k[c][kk], sc);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) s[c][nb] = mfma_bf16(kf, qf[nb][kk], s[c][nb]);
+      }
+    }
+    // s[c][nb][r]: query row 16 nb + l16 of the tile, key kv0 + 16 c + 4 g + r.
+    const bool whole = kv0 + kKvPage - 1 <= p0 &&
+                       (sh.window == 0 || p1 - kv0 < sh.window || kv0 + kKvPage <= sh.sinks);
+    bool nans = false;  // a V group without finite values in a page that not all rows see
+    if (!whole) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const int lim = pos[nb] - kv0 - 4 * g;
+        const int old = sh.window == 0 ? -64 : lim - sh.window;
+        const int sink = sh.sinks - kv0 - 4 * g;
+        bool any = false;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int e = 16 * c + r;
+            const bool hidden = (e > lim) | ((e <= old) & (e >= sink));
+            any |= !hidden;
+            s[c][nb][r] = hidden ? -INFINITY : s[c][nb][r];
+          }
+        seen[nb] |= any;
+      }
+      // A key that a row does not see has p = 0 there, but 0 times an infinity or
+      // NaN of V is NaN: such groups (slots never written among them) count as
+      // zeros here, and as NaN after the product for the rows that see them.
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (((x.vs[c] >> (8 * j)) & 255u) > 252u) {
+            x.vs[c] &= ~(255u << (8 * j));
+            nans = true;
+          }
+    } else {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) seen[nb] = true;
+    }
+
+    u32x4 pf[NB][2];
+    float alpha[NB];
+    bool raised = false;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float mloc = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        mloc = vmax(vmax(vmax(mloc, s[c][nb][0]), s[c][nb][1]), vmax(s[c][nb][2], s[c][nb][3]));
+      mloc = max_across_groups(mloc);
+      // The reference max is raised only when a page's passes it by 2^8 in p.
+      const float m_blk = mloc * sh.scale_log2;
+      const bool raise = m_blk > m_ref[nb] + kLazy;
+      const float m_new = raise ? m_blk : m_ref[nb];
+      alpha[nb] = raise ? fast_exp2(m_ref[nb] - m_new) : 1.0f;
+      m_ref[nb] = m_new;
+      raised |= raise;
+      const float neg_m = m_new == -INFINITY ? 0.f : -m_new;
+#pragma unroll
+      for (int ks2 = 0; ks2 < 2; ++ks2) {
+        float p[8];
+#pragma unroll
+        for (int h2 = 0; h2 < 2; ++h2)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            p[4 * h2 + r] = fast_exp2(fmaf(s[2 * ks2 + h2][nb][r], sh.scale_log2, neg_m));
+        pf[nb][ks2] = u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]),
+                            pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])};
+      }
+    }
+    if (__any(raised)) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int jd = 0; jd < 8; ++jd) oacc[jd][nb] = oacc[jd][nb] * alpha[nb];
+        lsum[nb] = lsum[nb] * alpha[nb];
+      }
+    }
+    auto v_block = [&](auto byte_c, int ks2, const float (&sa)[4], const float (&sb)[4]) {
+      constexpr int BYTE = decltype(byte_c)::value;
+      uint32_t w[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        w[j] = pair<BYTE>(x.v[2 * ks2][j], sa[j]);
+        w[4 + j] = pair<BYTE>(x.v[2 * ks2 + 1][j], sb[j]);
+      }
+      u32x4 lo, hi;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        lo[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x05040100);
+        hi[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302);
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        oacc[2 * BYTE][nb] = mfma_bf16(lo, pf[nb][ks2], oacc[2 * BYTE][nb]);
+        oacc[2 * BYTE + 1][nb] = mfma_bf16(hi, pf[nb][ks2], oacc[2 * BYTE + 1][nb]);
+      }
+    };
+#pragma unroll
+    for (int ks2 = 0; ks2 < 2; ++ks2) {
+      float sa[4], sb[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sa[j] = kv_scale((x.vs[2 * ks2] >> (8 * j)) & 255u);
+        sb[j] = kv_scale((x.vs[2 * ks2 + 1] >> (8 * j)) & 255u);
+      }
+      v_block(std::integral_constant<int, 0>{}, ks2, sa, sb);
+      v_block(std::integral_constant<int, 1>{}, ks2, sa, sb);
+      v_block(std::integral_constant<int, 2>{}, ks2, sa, sb);
+      v_block(std::integral_constant<int, 3>{}, ks2, sa, sb);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) lsum[nb] = mfma_bf16(ones, pf[nb][ks2], lsum[nb]);
+    }
+    if (!whole && __any(nans)) {
+      // The lane's dims 8 (4 g + r) + jd are group g's.
+      const uint8_t *p = part_of(page);
+      bool hit[NB] = {};
+#pragma unroll 1
+      for (int t = 0; t < kKvPage; ++t) {
+        const bool off = p[kv_v_scale_off(t, g)] > 252;
+        const int key = kv0 + t;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+          hit[nb] |= off & (key <= pos[nb]) &
+                     ((sh.window == 0) | (pos[nb] - key < sh.window) | (key < sh.sinks));
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int jd = 0; jd < 8; ++jd)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            oacc[jd][nb][r] = hit[nb] ? __uint_as_float(0x7fc00000u) : oacc[jd][nb][r];
+    }
+  };
+
+#pragma unroll 1
+  for (int i = begin; i < end; ++i) {
+    const int page = page_at(i);
+    PageRegs x;
+    load(x, page);
+    compute(x, i, page);
+  }
+
+  // The waves join.
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    // A row that saw keys but no score above -inf has no softmax: NaN.
+    const bool lost = __any(seen[nb] && m_ref[nb] == -INFINITY) != 0 && seen[nb] &&
+                      m_ref[nb] == -INFINITY;
+    int flag = lost ? 1 : 0;
+    flag |= __shfl_xor(flag, 16);
+    flag |= __shfl_xor(flag, 32);
+    if (g == 0) {
+      s_ml[0][wave][16 * nb + l16] = m_ref[nb];
+      s_ml[1][wave][16 * nb + l16] = flag ? __uint_as_float(0x7fc00000u) : lsum[nb][0];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    float m = -INFINITY;
+    for (int w = 0; w < kWaves; ++w) m = vmax(m, s_ml[0][w][16 * nb + l16]);
+    const float f = m_ref[nb] == m ? 1.f : fast_exp2(m_ref[nb] - m);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j4 = 0; j4 < 2; ++j4) {
+        f32x4 t;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = oacc[4 * j4 + e][nb][r] * f;
+        *reinterpret_cast<f32x4 *>(
+            &s_o[wave][(16 * nb + l16) * kKvHd + 8 * (4 * g + r) + 4 * j4]) = t;
+      }
+  }
+  __syncthreads();
+  for (int x = tid; x < kRows * kKvHd / 4; x += kThreads) {
+    const int row = x / (kKvHd / 4), d = 4 * (x - row * (kKvHd / 4));
+    if (r0 + row > r1) break;
+    float m = -INFINITY, l = 0.f;
+    for (int w = 0; w < kWaves; ++w) m = vmax(m, s_ml[0][w][row]);
+    f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int w = 0; w < kWaves; ++w) {
+      const float mw = s_ml[0][w][row];
+      l += s_ml[1][w][row] * (mw == m ? 1.f : fast_exp2(mw - m));
+      t = t + *reinterpret_cast<const f32x4 *>(&s_o[w][row * kKvHd + d]);
+    }
+    if (sh.n_split > 1) {
+      const size_t at =
+          ((((size_t)b * sh.Hkv + kvh) * sh.tiles + tile) * sh.n_split + split) * kRows + row;
+      *reinterpret_cast<f32x4 *>(part_o + at * kKvHd + d) = t;
+      if (d == 0) part_ml[at] = make_float2(m, l);
+      continue;
+    }
+    const int r = r0 + row, iq = r / G, h = kvh * G + r - iq * G;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;  // l = 0: no key seen
+    uint2 u;
+    u.x = pack_bf16x2(t[0] * inv, t[1] * inv);
+    u.y = pack_bf16x2(t[2] * inv, t[3] * inv);
+    *reinterpret_cast<uint2 *>(o + ((size_t)b * sh.n_q + iq) * ldo + (size_t)h * kKvHd + d) = u;
+    if (lse != nullptr && d == 0)
+      lse[((size_t)b * sh.Hq + h) * sh.n_q + iq] = (m + log2f(l)) * 0.6931471805599453f;
+  }
+}
+
+// Joins the splits of a query row: KG groups of 32 threads, thread d4 of group k
+// taking dims 4 d4 .. + 3 of splits k, k + KG, ..; all loads of up to 8 splits are
+// in flight at once (the partial results come from other dies' caches).
+template <int KG>
+__global__ __launch_bounds__(256) void kv_join_kernel(const float *__restrict__ part_o,
+                                                      const float2 *__restrict__ part_ml,
+                                                      bf16_t *__restrict__ o, size_t ldo,
+                                                      float *__restrict__ lse, int tile_rows,
+                                                      AttendShape sh) {
+  __shared__ f32x4 s_o[8][32];
+  __shared__ float2 s_ml[8];
+  const int G = sh.Hq / sh.Hkv, rows = sh.n_q * G;
+  const int d4 = threadIdx.x & 31, slot = threadIdx.x >> 5, k = slot % KG;
+  const int r = blockIdx.x * (8 / KG) + slot / KG;
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  if (KG == 1 && r >= rows) return;  // with KG = 8 the grid is the rows
+  const int tile = r / tile_rows, row = r - tile * tile_rows;
+  const size_t base = (((size_t)b * sh.Hkv + kvh) * sh.tiles + tile) * sh.n_split * tile_rows + row;
+  float m = -INFINITY, l = 0.f;
+  f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s0 = k; s0 < sh.n_split; s0 += 8 * KG) {
+    f32x4 p[8];
+    float2 ml[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int s = s0 + j * KG;
+      ml[j] = make_float2(-INFINITY, 0.f);
+      p[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (s < sh.n_split) {
+        const size_t at = base + (size_t)s * tile_rows;
+        ml[j] = part_ml[at];
+        p[j] = *reinterpret_cast<const f32x4 *>(part_o + at * kKvHd + 4 * d4);
+      }
+    }
+    float m2 = m;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m2 = vmax(m2, ml[j].x);
+    const float f0 = m == m2 ? 1.f : fast_exp2(m - m2);
+    l *= f0;
+    t = t * f0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float f = ml[j].x == m2 ? 1.f : fast_exp2(ml[j].x - m2);
+      l += ml[j].y * f;
+      t = t + p[j] * f;
+    }
     m = m2;
   }
-  *reinterpret_cast<uint32_t *>(o + (size_t)blockIdx.x * ldo + c) =
-      any ? pack_bf16x2(a0 / l, a1 / l) : 0u;
-  if (lse != nullptr && lane == 0)
-    lse[((size_t)b * sh.Hq + h) * sh.n_q + iq] = any ? m + logf(l) : -INFINITY;
+  if (KG > 1) {
+    s_o[slot][d4] = t;
+    if (d4 == 0) s_ml[slot] = make_float2(m, l);
+    __syncthreads();
+    if (k != 0) return;
+    m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < KG; ++j) m = vmax(m, s_ml[j].x);
+    l = 0.f;
+    t = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < KG; ++j) {
+      const float f = s_ml[j].x == m ? 1.f : fast_exp2(s_ml[j].x - m);
+      l += s_ml[j].y * f;
+      t = t + s_o[j][d4] * f;
+    }
+  }
+  const int iq = r / G, h = kvh * G + r - iq * G;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;  // l = 0: no key seen
+  uint2 u;
+  u.x = pack_bf16x2(t[0] * inv, t[1] * inv);
+  u.y = pack_bf16x2(t[2] * inv, t[3] * inv);
+  *reinterpret_cast<uint2 *>(o + ((size_t)b * sh.n_q + iq) * ldo + (size_t)h * kKvHd + 4 * d4) = u;
+  if (lse != nullptr && d4 == 0)
+    lse[((size_t)b * sh.Hq + h) * sh.n_q + iq] = (m + log2f(l)) * 0.6931471805599453f;
+}
+
+// How a call is cut: 16 nb rows a tile, n_split workgroups over a tile's pages.
+struct Plan {
+  int nb;
+  size_t tiles, n_split;
+};
+Plan plan_of(size_t batch, size_t n_q, size_t n_heads, size_t n_kv_heads, size_t pages) {
+  const size_t rows = n_q * (n_heads / n_kv_heads);
+  Plan p;
+  p.nb = rows <= 16 ? 1 : 2;
+  p.tiles = cdiv(rows, 16 * (size_t)p.nb);
+  // As many workgroups as fit the chip at once (three a CU with 16 rows, two with
+  // 32), and a page for each wave of a workgroup.
+  const size_t wgs = std::max<size_t>(batch * n_kv_heads * p.tiles, 1);
+  const size_t fit = p.nb == 1 ? 768 : 512;
+  p.n_split = std::max<size_t>(std::min(fit / wgs, cdiv(pages, kWaves)), 1);
+  return p;
+}
+size_t workspace_of(const Plan &p, size_t batch, size_t n_kv_heads) {
+  if (p.n_split <= 1) return 0;
+  return batch * n_kv_heads * p.tiles * p.n_split * 16 * p.nb * (kKvHd + 2) * sizeof(float);
 }
 
 }  // namespace
@@ -61,8 +481,8 @@ using namespace prichs;
 
 extern "C" size_t prichs_kv_cache_attention_workspace(size_t batch, size_t n_q, size_t n_heads,
                                                       size_t n_kv_heads, size_t max_pages) {
-  (void)batch, (void)n_q, (void)n_heads, (void)n_kv_heads, (void)max_pages;
-  return 0;
+  if (n_kv_heads == 0 || n_heads < n_kv_heads || batch == 0 || n_q == 0) return 0;
+  return workspace_of(plan_of(batch, n_q, n_heads, n_kv_heads, max_pages), batch, n_kv_heads);
 }
 
 extern "C" int prichs_kv_cache_attention(const void *q, size_t ldq, const void *cache,
@@ -80,14 +500,14 @@ extern "C" int prichs_kv_cache_attention(const void *q, size_t ldq, const void *
   PRICHS_REQUIRE(n_heads >= 1 && n_kv_heads >= 1 && n_heads % n_kv_heads == 0,
                  "%s: n_heads=%zu must be a positive multiple of n_kv_heads=%zu", who, n_heads,
                  n_kv_heads);
-  PRICHS_REQUIRE(ldq >= n_heads * head_dim && ldo >= n_heads * head_dim && ldq % 8 == 0 &&
-                     ldo % 8 == 0,
-                 "%s: ldq and ldo must be multiples of 8 elements that hold all heads", who);
-  const size_t cap = max_pages * kKvPage;
   PRICHS_REQUIRE(n_heads <= 65535 && batch <= 65535 && n_q <= (size_t)1 << 21 &&
                      batch * n_q <= (size_t)INT32_MAX / 2 && n_pages <= (size_t)INT32_MAX &&
                      max_pages <= ((size_t)1 << 30) / kKvPage,
                  "%s: shape too large", who);
+  PRICHS_REQUIRE(ldq >= n_heads * head_dim && ldo >= n_heads * head_dim && ldq % 8 == 0 &&
+                     ldo % 8 == 0,
+                 "%s: ldq and ldo must be multiples of 8 elements that hold all heads", who);
+  const size_t cap = max_pages * kKvPage;
   if (batch == 0 || n_q == 0) return PRICHS_OK;
   PRICHS_REQUIRE(q && o && lens && (cap == 0 || (cache && page_table)),
                  "%s: null pointer argument", who);
@@ -102,18 +522,44 @@ extern "C" int prichs_kv_cache_attention(const void *q, size_t ldq, const void *
   PRICHS_REQUIRE(need == 0 ||
                      (workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                  "%s: the workspace must be 16-byte aligned device memory", who);
+  // Pages that a tile can see at most: those of the window and of the sinks (a
+  // window past the table hides nothing).
+  const size_t w = window >= cap ? 0 : window, sk = std::min(sinks, cap);
+  const size_t pages =
+      w == 0 ? max_pages
+             : std::min(max_pages, cdiv(w + n_q, kKvPage) + 1 + cdiv(sk, kKvPage));
+  const Plan p = plan_of(batch, n_q, n_heads, n_kv_heads, pages);
+  PRICHS_REQUIRE(n_kv_heads * p.tiles <= 65535, "%s: shape too large", who);
   const AttendShape sh{(int)n_pages,
                        (int)max_pages,
                        (int)n_q,
                        (int)n_heads,
                        (int)n_kv_heads,
-                       (int)(window >= cap ? 0 : window),
-                       (int)(sinks < cap ? sinks : cap),
-                       1.0f / sqrtf((float)head_dim)};
-  hipLaunchKernelGGL(kv_attend_row_kernel, dim3((unsigned)(batch * n_q), (unsigned)n_heads),
-                     dim3(64), 0, as_stream(stream), static_cast<const bf16_t *>(q), ldq,
-                     static_cast<const uint8_t *>(cache), page_table, lens,
-                     static_cast<bf16_t *>(o), ldo, lse, sh);
+                       (int)w,
+                       (int)sk,
+                       (int)p.tiles,
+                       (int)p.n_split,
+                       (1.0f / sqrtf((float)head_dim)) * 1.4426950408889634f};
+  const size_t part_rows = batch * n_kv_heads * p.tiles * p.n_split * 16 * p.nb;
+  float *part_o = static_cast<float *>(workspace);
+  float2 *part_ml = reinterpret_cast<float2 *>(part_o + (p.n_split > 1 ? part_rows * kKvHd : 0));
+  const dim3 grid((unsigned)p.n_split, (unsigned)(n_kv_heads * p.tiles), (unsigned)batch);
+  auto kern = p.nb == 1 ? kv_attend_kernel<1> : kv_attend_kernel<2>;
+  hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, as_stream(stream),
+                     static_cast<const bf16_t *>(q), ldq, static_cast<const uint8_t *>(cache),
+                     page_table, lens, static_cast<bf16_t *>(o), ldo, lse, part_o, part_ml, sh);
   PRICHS_LAUNCH_CHECK("kv_cache_attention launch");
+  if (p.n_split > 1) {
+    const size_t rows = n_q * (n_heads / n_kv_heads);
+    // Eight threads groups a row where a row has more splits than one can load at
+    // once.
+    const bool wide = p.n_split > 8;
+    const dim3 join((unsigned)(wide ? rows : cdiv(rows, 8)), (unsigned)n_kv_heads,
+                    (unsigned)batch);
+    auto join_kern = wide ? kv_join_kernel<8> : kv_join_kernel<1>;
+    hipLaunchKernelGGL(join_kern, join, dim3(256), 0, as_stream(stream), part_o, part_ml,
+                       static_cast<bf16_t *>(o), ldo, lse, 16 * p.nb, sh);
+    PRICHS_LAUNCH_CHECK("kv_cache_attention join launch");
+  }
   return PRICHS_OK;
 }

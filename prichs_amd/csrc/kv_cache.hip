@@ -5,77 +5,130 @@
 namespace prichs {
 namespace {
 
-// Page of position pos of sequence b, or -1 where the table has none.
-__device__ __forceinline__ int page_of(const int32_t *table, int max_pages, int n_pages, int b,
-                                       long long pos) {
-  if (pos < 0 || pos >= (long long)max_pages * kKvPage) return -1;
-  const int p = table[(long long)b * max_pages + (int)(pos / kKvPage)];
-  return p >= 0 && p < n_pages ? p : -1;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// Both kernels are bound by HBM (a read of 512 bytes and a write of 136 per
+// position and kv head in bf16, or the reverse).  16 lanes hold one (position, kv
+// head), 8 values each: one 16-byte access in bf16, one dword of codes.  Items run
+// over (sequence, head, row) with the row fastest, so that a wave's four items are
+// as a rule four positions of one head, whose V dwords are neighbours in the cache
+// -- and four heads where every sequence has one new token.
+constexpr int kItems = 16;  // items per workgroup of 256 threads
+constexpr size_t kMaxItems = ((size_t)1 << 28) - 1;  // 16 lanes each, below 2^32 in a launch
+
+struct Item {
+  int row, h, c, page, t;  // row of k / v; dword c; page (-1: none) and slot
+  bool live;               // not past its sequence's count
+};
+__device__ __forceinline__ bool item_of(Item &it, const int32_t *table, int max_pages, int n_pages,
+                                        const int32_t *start, const int32_t *counts, int n,
+                                        int kv_heads, uint32_t items) {
+  const uint32_t x = blockIdx.x * (uint32_t)kItems + threadIdx.x / 16;
+  if (x >= items) return false;
+  const uint32_t bh = x / (uint32_t)n;
+  const int i = (int)(x - bh * (uint32_t)n), b = (int)(bh / (uint32_t)kv_heads);
+  it.h = (int)(bh - (uint32_t)b * (uint32_t)kv_heads);
+  it.row = b * n + i;
+  it.c = threadIdx.x & 15;
+  it.live = counts == nullptr || i < counts[b];
+  const long long pos = (long long)start[b] + i;
+  it.page = kv_page_of(table, max_pages, n_pages, b, pos);
+  it.t = (int)(pos & (kKvPage - 1));
+  return true;
 }
 
-// One 64-thread workgroup per (row, kv head): lanes 0..31 quantise k, lanes
-// 32..63 v; a lane holds 4 values, 8 lanes a group of 32.
+__device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
+  const f32x4 a = *reinterpret_cast<const f32x4 *>(p), b = *reinterpret_cast<const f32x4 *>(p + 4);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
+}
+__device__ __forceinline__ void load8(const bf16_t *p, float (&x)[8]) {
+  const u32x4 u = *reinterpret_cast<const u32x4 *>(p);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[2 * e] = __uint_as_float(u[e] << 16);
+    x[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u);
+  }
+}
+
+// 8 values of a group of 32 that 4 neighbouring lanes hold: their codes, and the
+// group's scale byte.
+__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t *scale) {
+  uint32_t amax = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(x[e]) & 0x7fffffffu);
+  amax = max(amax, (uint32_t)__shfl_xor((int)amax, 1));
+  amax = max(amax, (uint32_t)__shfl_xor((int)amax, 2));
+  *scale = kv_scale_byte(amax);
+  if (*scale == 255) return 0;
+  const float sc = kv_scale(*scale);
+  uint32_t code = 0;
+  code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[0], x[1], sc, 0);
+  code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[2], x[3], sc, 1);
+  code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[4], x[5], sc, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[6], x[7], sc, 3);
+}
+
 template <typename T>
-__global__ __launch_bounds__(64) void kv_write_kernel(
+__global__ __launch_bounds__(256) void kv_write_kernel(
     const T *__restrict__ k, size_t ldk, const T *__restrict__ v, size_t ldv, uint8_t *cache,
     int n_pages, const int32_t *table, int max_pages, const int32_t *start, const int32_t *counts,
-    int n, int kv_heads) {
-  const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-  const int b = row / n, i = row - b * n;
-  if (counts != nullptr && i >= counts[b]) return;
-  const long long pos = (long long)start[b] + i;
-  const int page = page_of(table, max_pages, n_pages, b, pos);
-  if (page < 0) return;
-  const bool is_v = lane >= 32;
-  const int c = lane & 31;
-  const T *src = (is_v ? v + (size_t)row * ldv : k + (size_t)row * ldk) + (size_t)h * kKvHd + 4 * c;
-  float x[4];
-  uint32_t amax = 0;
-  for (int e = 0; e < 4; ++e) {
-    x[e] = Elem<T>::load(src + e);
-    amax = max(amax, __float_as_uint(x[e]) & 0x7fffffffu);
+    int n, int kv_heads, uint32_t items) {
+  Item it;
+  if (!item_of(it, table, max_pages, n_pages, start, counts, n, kv_heads, items)) return;
+  if (!it.live || it.page < 0) return;  // the 16 lanes of an item agree
+  const size_t col = (size_t)it.h * kKvHd + 8 * it.c;
+  float xk[8], xv[8];
+  load8(k + (size_t)it.row * ldk + col, xk);
+  load8(v + (size_t)it.row * ldv + col, xv);
+  uint32_t sk, sv;
+  const uint32_t ck = quantise8(xk, &sk), cv = quantise8(xv, &sv);
+  uint8_t *part = cache + ((size_t)it.page * kv_heads + it.h) * kKvPart;
+  *reinterpret_cast<uint32_t *>(part + kKvK + it.t * (kKvHd / 2) + 4 * it.c) = ck;
+  *reinterpret_cast<uint32_t *>(part + kv_v_off(it.t, it.c)) = cv;
+  if ((it.c & 3) == 0) {
+    part[kv_k_scale_off(it.t, it.c >> 2)] = (uint8_t)sk;
+    part[kv_v_scale_off(it.t, it.c >> 2)] = (uint8_t)sv;
   }
-  for (int m = 1; m < 8; m <<= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, m));
-  const uint32_t s = kv_scale_byte(amax);
-  uint32_t code = 0;
-  if (s != 255) {
-    const float sc = kv_scale(s);
-    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[0], x[1], sc, 0);
-    code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[2], x[3], sc, 1);
-  }
-  uint8_t *part = cache + ((size_t)page * kv_heads + h) * kKvPart;
-  const int t = (int)(pos % kKvPage);
-  const int off = is_v ? kv_v_off(t, c >> 1) + 2 * (c & 1) : kKvK + t * (kKvHd / 2) + 2 * c;
-  *reinterpret_cast<uint16_t *>(part + off) = (uint16_t)code;
-  if ((c & 7) == 0) part[(is_v ? kKvVScale : kKvKScale) + 4 * t + (c >> 3)] = (uint8_t)s;
+}
+
+__device__ __forceinline__ void store8(bf16_t *p, uint32_t code, float sc) {
+  u32x4 u;
+  u[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, sc, 0));
+  u[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, sc, 1));
+  u[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, sc, 2));
+  u[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, sc, 3));
+  *reinterpret_cast<u32x4 *>(p) = u;
+}
+__device__ __forceinline__ void store8(float *p, uint32_t code, float sc) {
+  const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, sc, 0);
+  const auto b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, sc, 1);
+  const auto c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, sc, 2);
+  const auto d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, sc, 3);
+  *reinterpret_cast<f32x4 *>(p) = f32x4{a[0], a[1], b[0], b[1]};
+  *reinterpret_cast<f32x4 *>(p + 4) = f32x4{c[0], c[1], d[0], d[1]};
 }
 
 template <typename T>
-__global__ __launch_bounds__(64) void kv_read_kernel(
+__global__ __launch_bounds__(256) void kv_read_kernel(
     T *__restrict__ k, size_t ldk, T *__restrict__ v, size_t ldv, const uint8_t *cache,
     int n_pages, const int32_t *table, int max_pages, const int32_t *start, const int32_t *counts,
-    int n, int kv_heads) {
-  const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-  const int b = row / n, i = row - b * n;
-  if (counts != nullptr && i >= counts[b]) return;
-  const long long pos = (long long)start[b] + i;
-  const int page = page_of(table, max_pages, n_pages, b, pos);
-  const bool is_v = lane >= 32;
-  const int c = lane & 31;
-  uint32_t code = 0, s = 127;
-  if (page >= 0) {
-    const uint8_t *part = cache + ((size_t)page * kv_heads + h) * kKvPart;
-    const int t = (int)(pos % kKvPage);
-    const int off = is_v ? kv_v_off(t, c >> 1) + 2 * (c & 1) : kKvK + t * (kKvHd / 2) + 2 * c;
-    code = *reinterpret_cast<const uint16_t *>(part + off);
-    s = part[(is_v ? kKvVScale : kKvKScale) + 4 * t + (c >> 3)];
+    int n, int kv_heads, uint32_t items) {
+  Item it;
+  if (!item_of(it, table, max_pages, n_pages, start, counts, n, kv_heads, items)) return;
+  if (!it.live) return;
+  uint32_t ck = 0, cv = 0, sk = 127, sv = 127;  // zeros where there is no page
+  if (it.page >= 0) {
+    const uint8_t *part = cache + ((size_t)it.page * kv_heads + it.h) * kKvPart;
+    ck = *reinterpret_cast<const uint32_t *>(part + kKvK + it.t * (kKvHd / 2) + 4 * it.c);
+    cv = *reinterpret_cast<const uint32_t *>(part + kv_v_off(it.t, it.c));
+    sk = part[kv_k_scale_off(it.t, it.c >> 2)];
+    sv = part[kv_v_scale_off(it.t, it.c >> 2)];
   }
-  const float sc = kv_scale(s);
-  const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, sc, 0);
-  const auto hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, sc, 1);
-  T *dst = (is_v ? v + (size_t)row * ldv : k + (size_t)row * ldk) + (size_t)h * kKvHd + 4 * c;
-  const float x[4] = {lo[0], lo[1], hi[0], hi[1]};
-  for (int e = 0; e < 4; ++e) Elem<T>::store(dst + e, s == 255 ? sc : x[e]);
+  const size_t col = (size_t)it.h * kKvHd + 8 * it.c;
+  store8(k + (size_t)it.row * ldk + col, ck, kv_scale(sk));
+  store8(v + (size_t)it.row * ldv + col, cv, kv_scale(sv));
 }
 
 // Checks shared by the write and the read entry point; PRICHS_OK with *work =
@@ -95,7 +148,7 @@ int kv_check(const char *who, const void *k, size_t ldk, const void *v, size_t l
   PRICHS_REQUIRE(ldk % 8 == 0 && ldv % 8 == 0,
                  "%s: leading dimensions must be multiples of 8 elements", who);
   PRICHS_REQUIRE(batch <= (size_t)INT32_MAX && n <= (size_t)INT32_MAX &&
-                     (n == 0 || batch <= (size_t)INT32_MAX / n) && n_pages <= (size_t)INT32_MAX &&
+                     (n == 0 || batch <= kMaxItems / n / n_kv_heads) && n_pages <= (size_t)INT32_MAX &&
                      max_pages <= (size_t)INT32_MAX / kKvPage,
                  "%s: shape too large", who);
   if (batch == 0 || n == 0) return PRICHS_OK;
@@ -122,17 +175,18 @@ extern "C" int prichs_kv_cache_write(void *cache, size_t n_pages, const int32_t 
   const int rc = kv_check("kv_cache_write", k, ldk, v, ldv, cache, n_pages, page_table, max_pages,
                           start, batch, n, n_kv_heads, head_dim, dtype, &work);
   if (rc != PRICHS_OK || !work) return rc;
-  const dim3 grid((unsigned)(batch * n), (unsigned)n_kv_heads);
+  const uint32_t items = (uint32_t)(batch * n * n_kv_heads);
+  const dim3 grid((unsigned)cdiv(items, kItems));
   if (dtype == PRICHS_DTYPE_BF16)
-    hipLaunchKernelGGL(kv_write_kernel<bf16_t>, grid, dim3(64), 0, as_stream(stream),
+    hipLaunchKernelGGL(kv_write_kernel<bf16_t>, grid, dim3(256), 0, as_stream(stream),
                        static_cast<const bf16_t *>(k), ldk, static_cast<const bf16_t *>(v), ldv,
                        static_cast<uint8_t *>(cache), (int)n_pages, page_table, (int)max_pages,
-                       start, counts, (int)n, (int)n_kv_heads);
+                       start, counts, (int)n, (int)n_kv_heads, items);
   else
-    hipLaunchKernelGGL(kv_write_kernel<float>, grid, dim3(64), 0, as_stream(stream),
+    hipLaunchKernelGGL(kv_write_kernel<float>, grid, dim3(256), 0, as_stream(stream),
                        static_cast<const float *>(k), ldk, static_cast<const float *>(v), ldv,
                        static_cast<uint8_t *>(cache), (int)n_pages, page_table, (int)max_pages,
-                       start, counts, (int)n, (int)n_kv_heads);
+                       start, counts, (int)n, (int)n_kv_heads, items);
   PRICHS_LAUNCH_CHECK("kv_cache_write launch");
   return PRICHS_OK;
 }
@@ -146,17 +200,18 @@ extern "C" int prichs_kv_cache_read(const void *cache, size_t n_pages, const int
   const int rc = kv_check("kv_cache_read", k, ldk, v, ldv, cache, n_pages, page_table, max_pages,
                           start, batch, n, n_kv_heads, head_dim, dtype, &work);
   if (rc != PRICHS_OK || !work) return rc;
-  const dim3 grid((unsigned)(batch * n), (unsigned)n_kv_heads);
+  const uint32_t items = (uint32_t)(batch * n * n_kv_heads);
+  const dim3 grid((unsigned)cdiv(items, kItems));
   if (dtype == PRICHS_DTYPE_BF16)
-    hipLaunchKernelGGL(kv_read_kernel<bf16_t>, grid, dim3(64), 0, as_stream(stream),
+    hipLaunchKernelGGL(kv_read_kernel<bf16_t>, grid, dim3(256), 0, as_stream(stream),
                        static_cast<bf16_t *>(k), ldk, static_cast<bf16_t *>(v), ldv,
                        static_cast<const uint8_t *>(cache), (int)n_pages, page_table,
-                       (int)max_pages, start, counts, (int)n, (int)n_kv_heads);
+                       (int)max_pages, start, counts, (int)n, (int)n_kv_heads, items);
   else
-    hipLaunchKernelGGL(kv_read_kernel<float>, grid, dim3(64), 0, as_stream(stream),
+    hipLaunchKernelGGL(kv_read_kernel<float>, grid, dim3(256), 0, as_stream(stream),
                        static_cast<float *>(k), ldk, static_cast<float *>(v), ldv,
                        static_cast<const uint8_t *>(cache), (int)n_pages, page_table,
-                       (int)max_pages, start, counts, (int)n, (int)n_kv_heads);
+                       (int)max_pages, start, counts, (int)n, (int)n_kv_heads, items);
   PRICHS_LAUNCH_CHECK("kv_cache_read launch");
   return PRICHS_OK;
 }

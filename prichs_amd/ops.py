@@ -5,6 +5,7 @@ runs in libprichs_hip.so.  Each wrapper names the C entry point it calls.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import numpy as np
@@ -299,13 +300,11 @@ def attention(q, k, v, batch, seq_len, n_heads, n_kv_heads, head_dim=128, out=No
 # ---------------------------------------- window attention and KV cache ----
 def _rows(t, name, rows, cols, dtypes=(torch.bfloat16,)):
     """A device operand of at least `rows` rows whose columns are contiguous."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != 2:
-        raise ValueError(f"{name}: expected a 2-D device tensor")
     if t.dtype not in dtypes:
         raise TypeError(f"{name}: unsupported dtype {t.dtype}")
-    if t.shape[0] < rows or t.shape[1] != cols:
+    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] != cols:
         raise ValueError(f"{name}: expected [{rows}, {cols}], got {list(t.shape)}")
-    if cols > 1 and t.stride(1) != 1:
+    if t.stride(1) != 1:
         raise ValueError(f"{name}: operands need unit column stride")
     return t
 
@@ -320,42 +319,28 @@ def _ld(t):
 
 
 def _i32(t, name, n, dim=1):
-    if not t.is_cuda or t.dtype != torch.int32 or not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous int32 device tensor")
-    if t.dim() != dim or t.shape[0] != n:
-        raise ValueError(f"{name}: expected {n} rows, got {list(t.shape)}")
-    return t
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != dim or t.shape[0] != n:
+        raise ValueError(f"{name}: expected contiguous int32 of {n} rows, got {t.dtype} "
+                         f"{list(t.shape)}")
 
 
-class _device_of:
-    """The device of the operands (all on one) made current where it is not, and the
-    stream to launch on: the given one, or torch's current one there.  Outputs and
-    workspaces allocated inside belong to that stream."""
+_HERE = contextlib.nullcontext()
 
-    def __init__(self, stream, first, *others):
-        dev = first.device
-        for t in others:
-            if t is not None and t.device != dev:
-                raise ValueError(f"operands on different devices: {dev} and {t.device}")
-        self._ctx = None
-        if stream is not None:
-            if stream.device != dev:
-                raise ValueError(f"a stream of {stream.device} with operands on {dev}")
-            self._ctx = torch.cuda.stream(stream)
-        elif torch.cuda.current_device() != dev.index:
-            self._ctx = torch.cuda.device(dev)
-        if stream is None:
-            stream = torch.cuda.current_stream(dev)
-        self.raw = stream.cuda_stream
 
-    def __enter__(self):
-        if self._ctx is not None:
-            self._ctx.__enter__()
-        return self.raw
-
-    def __exit__(self, *exc):
-        if self._ctx is not None:
-            self._ctx.__exit__(*exc)
+def _launch_on(stream, first, *others):
+    """(context, raw stream) of a launch on the operands' device, which must be one
+    for all: the given stream, or torch's current one there.  Outputs and
+    workspaces allocated in the context belong to that stream."""
+    dev = first.get_device()
+    for t in (first, *others):
+        if t is not None and t.get_device() != dev or dev < 0:
+            raise ValueError("expected device tensors, all on one device")
+    if stream is not None:
+        if stream.device_index != dev:
+            raise ValueError(f"a stream of {stream.device} with operands on cuda:{dev}")
+        return torch.cuda.stream(stream), stream.cuda_stream
+    raw = torch._C._cuda_getCurrentRawStream(dev)
+    return (_HERE if torch.cuda.current_device() == dev else torch.cuda.device(dev)), raw
 
 
 def window_attention(q, k, v, batch, seq_len, n_heads, n_kv_heads, window, sinks=0,
@@ -372,7 +357,8 @@ def window_attention(q, k, v, batch, seq_len, n_heads, n_kv_heads, window, sinks
         _i32(seq_lens, "seq_lens", batch)
     if window < 0 or sinks < 0:
         raise ValueError("window and sinks must not be negative")
-    with _device_of(stream, q, k, v, seq_lens, out) as s:
+    ctx, s = _launch_on(stream, q, k, v, seq_lens, out)
+    with ctx:
         if out is None:
             out = torch.empty((rows, H), dtype=q.dtype, device=q.device)
         _rows(out, "out", rows, H)
@@ -405,7 +391,8 @@ def window_attention_backward(d_out, q, k, v, out, lse, batch, seq_len, n_heads,
         _i32(seq_lens, "seq_lens", batch)
     if window < 0 or sinks < 0:
         raise ValueError("window and sinks must not be negative")
-    with _device_of(stream, d_out, q, k, v, out, lse, seq_lens, d_q, d_k, d_v) as s:
+    ctx, s = _launch_on(stream, d_out, q, k, v, out, lse, seq_lens, d_q, d_k, d_v)
+    with ctx:
         grads = []
         for t, name, cols in ((d_q, "d_q", H), (d_k, "d_k", K), (d_v, "d_v", K)):
             if t is None:
@@ -428,8 +415,8 @@ def kv_cache_pages(n_pages, n_kv_heads, device="cuda"):
 
 
 def _kv_cache(cache, page_table, batch, n_kv_heads):
-    if not cache.is_cuda or cache.dtype != torch.uint8 or not cache.is_contiguous() or \
-            cache.dim() != 3 or tuple(cache.shape[1:]) != (n_kv_heads, L.KV_PAGE_BYTES):
+    if cache.dtype != torch.uint8 or not cache.is_contiguous() or \
+            cache.shape != (cache.shape[0], n_kv_heads, L.KV_PAGE_BYTES):
         raise ValueError("cache: expected the pages of kv_cache_pages for these kv heads")
     _i32(page_table, "page_table", batch, dim=2)
 
@@ -450,7 +437,8 @@ def kv_cache_write(cache, page_table, start, k, v, batch, n, n_kv_heads, counts=
     _i32(start, "start", batch)
     if counts is not None:
         _i32(counts, "counts", batch)
-    with _device_of(stream, cache, page_table, start, counts, k, v) as s:
+    ctx, s = _launch_on(stream, cache, page_table, start, counts, k, v)
+    with ctx:
         L.check(lib.prichs_kv_cache_write(
             _a(cache), cache.shape[0], _a(page_table), page_table.shape[1], _a(start), _a(counts),
             _a(k), _ld(k), _a(v), _ld(v), batch, n, n_kv_heads, 128, dtype_code(k), s))
@@ -467,7 +455,8 @@ def kv_cache_read(cache, page_table, start, batch, n, n_kv_heads, counts=None,
     if counts is not None:
         _i32(counts, "counts", batch)
     shape = (batch * n, n_kv_heads * 128)
-    with _device_of(stream, cache, page_table, start, counts, k, v) as s:
+    ctx, s = _launch_on(stream, cache, page_table, start, counts, k, v)
+    with ctx:
         make = torch.empty if counts is None else torch.zeros
         got = []
         for t, name in ((k, "k"), (v, "v")):
@@ -496,7 +485,8 @@ def kv_cache_attention(q, cache, page_table, lens, batch, n_q, n_heads, n_kv_hea
     _i32(lens, "lens", batch)
     if window < 0 or sinks < 0:
         raise ValueError("window and sinks must not be negative")
-    with _device_of(stream, q, cache, page_table, lens, out) as s:
+    ctx, s = _launch_on(stream, q, cache, page_table, lens, out)
+    with ctx:
         if out is None:
             out = torch.empty((rows, H), dtype=q.dtype, device=q.device)
         _rows(out, "out", rows, H)

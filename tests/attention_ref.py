@@ -95,19 +95,17 @@ def cached_values(x):
     """What the cache holds of x [..., 128]: per group of 32 the least scale 2^s, -126
     <= s <= 125, with max|x| <= 7 * 2^s; nearest level, ties to the even code."""
     g = np.asarray(x, dtype=np.float64).reshape(-1, 32)
-    out = np.empty_like(g)
-    for r, row in enumerate(g):
-        if not np.isfinite(row).all():
-            out[r] = np.nan
-            continue
-        s = -126
-        while s < 125 and np.abs(row).max() > 7 * 2.0 ** s:
-            s += 1
-        y = np.abs(row) / 2.0 ** s
-        d = np.abs(y[:, None] - LEVELS[None])
-        near = d == d.min(1, keepdims=True)
-        # Of two levels equally near, the one of even code.
-        code = np.array([c[0] if len(c) == 1 or c[0] % 2 == 0 else c[1]
-                         for c in (np.flatnonzero(n) for n in near)])
-        out[r] = np.sign(row) * LEVELS[code] * 2.0 ** s
+    bad = ~np.isfinite(g).all(1)
+    top = np.abs(np.where(bad[:, None], 0, g)).max(1)
+    s = np.full(len(g), -126)
+    for e in range(-125, 126):
+        s[top > 7 * 2.0 ** (e - 1)] = e
+    y = np.abs(g) / 2.0 ** s[:, None]
+    # The nearest level; a value in the middle of two goes to the even code.
+    code = np.zeros(g.shape, dtype=int)
+    for c in range(7):
+        mid = (LEVELS[c] + LEVELS[c + 1]) / 2
+        code += (y > mid) | ((y == mid) & (c % 2 == 1))
+    out = np.sign(g) * LEVELS[code] * 2.0 ** s[:, None]
+    out[bad] = np.nan
     return out.reshape(np.shape(x))
