@@ -35,6 +35,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
+constexpr int kLdRow = kKvHd + 4;  // LDS row of joined outputs: 16 rows on distinct banks
 constexpr float kLazy = 8.0f;  // log2 headroom of the lazily raised softmax max
 
 struct AttendShape {
@@ -85,7 +86,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 3 : 2) void kv_attend_kernel(
     AttendShape sh) {
   constexpr int kRows = 16 * NB;
   __shared__ float s_ml[2][kWaves][kRows];
-  __shared__ float s_o[kWaves][kRows * kKvHd];
+  __shared__ float s_o[kWaves][kRows * kLdRow];
 
   const int split = blockIdx.x;
   const int kvh = blockIdx.y / sh.tiles, tile = blockIdx.y - kvh * sh.tiles;
@@ -117,8 +118,8 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 3 : 2) void kv_attend_kernel(
   const int n_sink = min((sh.sinks + kKvPage - 1) / kKvPage, first);
   const int skip = first - n_sink;
   const int n_vis = p1 < 0 ? 0 : p1 / kKvPage + 1 - skip;
-  const int per = (n_vis + kWaves * sh.n_split - 1) / (kWaves * sh.n_split);
-  const int begin = min((split * kWaves + wave) * per, n_vis), end = min(begin + per, n_vis);
+  const int64_t worker = split * kWaves + wave, workers = sh.n_split * kWaves;
+  const int begin = (int)(n_vis * worker / workers), end = (int)(n_vis * (worker + 1) / workers);
   auto block_of = [&](int i) { return i >= n_sink ? i + skip : i; };
   const int32_t *row_table = table + (size_t)b * sh.max_pages;
   // Page of the i-th visible block (-1: none); the same for the whole wave.
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 3 : 2) void kv_attend_kernel(
 #pragma unroll
         for (int e = 0; e < 4; ++e) t[e] = oacc[4 * j4 + e][nb][r] * f;
         *reinterpret_cast<f32x4 *>(
-            &s_o[wave][(16 * nb + l16) * kKvHd + 8 * (4 * g + r) + 4 * j4]) = t;
+            &s_o[wave][(16 * nb + l16) * kLdRow + 8 * (4 * g + r) + 4 * j4]) = t;
       }
   }
   __syncthreads();
@@ -357,7 +358,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 3 : 2) void kv_attend_kernel(
     for (int w = 0; w < kWaves; ++w) {
       const float mw = s_ml[0][w][row];
       l += s_ml[1][w][row] * (mw == m ? 1.f : fast_exp2(mw - m));
-      t = t + *reinterpret_cast<const f32x4 *>(&s_o[w][row * kKvHd + d]);
+      t = t + *reinterpret_cast<const f32x4 *>(&s_o[w][row * kLdRow + d]);
     }
     if (sh.n_split > 1) {
       const size_t at =
