@@ -376,7 +376,8 @@ int prichs_window_attention_forward(const void *q, size_t ldq, const void *k,
  * prichs_window_attention_backward_workspace bytes, used by this call alone until
  * it has finished. */
 size_t prichs_window_attention_backward_workspace(size_t batch, size_t seq_len,
-                                                  size_t n_heads, size_t n_kv_heads);
+                                                  size_t n_heads, size_t n_kv_heads,
+                                                  size_t window, size_t sinks);
 int prichs_window_attention_backward(const void *d_o, size_t ldd, const void *q,
                                      size_t ldq, const void *k, size_t ldk,
                                      const void *v, size_t ldv, const void *o,

@@ -127,7 +127,7 @@ SIGNATURES = {
                                              _sz, _sz, _i, _vp, _vp, _sz, _sz, _vp]),
     "prichs_window_attention_forward": (_i, [_vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp,
                                              _sz, _sz, _sz, _sz, _sz, _sz, _sz, _i, _vp]),
-    "prichs_window_attention_backward_workspace": (_sz, [_sz, _sz, _sz, _sz]),
+    "prichs_window_attention_backward_workspace": (_sz, [_sz, _sz, _sz, _sz, _sz, _sz]),
     "prichs_window_attention_backward": (_i, [_vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz,
                                               _vp, _vp, _vp, _sz, _vp, _sz, _vp, _sz, _sz, _sz,
                                               _sz, _sz, _sz, _sz, _sz, _i, _vp, _sz, _vp]),

@@ -1,0 +1,90 @@
+// attention_tile.hpp -- what the attention kernels share: matrix and transposing
+// reads, copies straight into LDS, exchanges between a query's lanes.
+#pragma once
+
+#include <type_traits>
+#include <utility>
+
+#include "common.hpp"
+
+namespace prichs {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ f32x4 mfma_bf16(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Buffer resource over `bytes` bytes from `base` (raw: stride 0, gfx9 word 3).
+// Loads at offsets at or past `bytes` return zeros instead of reading memory.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_rsrc(const void *base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), (short)0, (int)bytes,
+                                           0x00020000);
+}
+// 16 bytes per lane from buffer offset voff straight into LDS at lds_dst +
+// 16 * lane (lds_dst wave-uniform).
+__device__ __forceinline__ void dma_16b(__amdgpu_buffer_rsrc_t r, uint32_t voff, bf16_t *lds_dst) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      r, (__attribute__((address_space(3))) void *)lds_dst, 16, voff, 0, 0, 0);
+}
+// ds_read_b64_tr_b16 as inline asm: the builtin form makes the compiler wait
+// for every DMA in flight (it cannot tell the read from the DMA's target).
+// OFF is the instruction's immediate byte offset.  The result is pending
+// until lds_wait_tied() below, which takes the registers as operands so no
+// use can be scheduled before the wait.
+template <int OFF>
+__device__ __forceinline__ u32x2 ds_read_tr16(uint32_t lds_byte_addr) {
+  static_assert(OFF >= 0 && OFF < 65536, "ds offset is 16 bits");
+  u32x2 r;
+  asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(r) : "v"(lds_byte_addr), "n"(OFF));
+  return r;
+}
+__device__ __forceinline__ void lds_wait_tied(u32x2 &a, u32x2 &b, u32x2 &c, u32x2 &d, u32x2 &e,
+                                              u32x2 &f, u32x2 &g, u32x2 &h) {
+  asm volatile("s_waitcnt lgkmcnt(0)"
+               : "+v"(a), "+v"(b), "+v"(c), "+v"(d), "+v"(e), "+v"(f), "+v"(g), "+v"(h)
+               :
+               : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) { return pack_bf16x2(a, b); }
+
+// Max over lanes l, l ^ 16, l ^ 32, l ^ 48 (the four 16-lane groups
+// sharing a query column): v_permlane16_swap exchanges odd and even 16-lane
+// rows, v_permlane32_swap the two wave halves.
+// The maxima are IEEE 754-2019 maximum (v_maximum3_f32 on gfx950: NaN
+// propagates, so no operand needs the canonicalising pass that fmaxf's
+// maxNum semantics put before each raw MFMA result).
+__device__ __forceinline__ float vmax(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float max_across_groups(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  x = vmax(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const uint32_t w = __float_as_uint(x);
+  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return vmax(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+template <bool B> using bool_c = std::integral_constant<bool, B>;
+template <int I> using int_c = std::integral_constant<int, I>;
+template <typename F, int... I>
+__device__ __forceinline__ void static_for_impl(F &&f, std::integer_sequence<int, I...>) {
+  (f(int_c<I>{}), ...);
+}
+// f(int_c<0>), ..., f(int_c<N - 1>): loop indices usable as template arguments.
+template <int N, typename F>
+__device__ __forceinline__ void static_for(F &&f) {
+  static_for_impl(f, std::make_integer_sequence<int, N>{});
+}
+
+// Two bf16 with an infinity or NaN replaced by 0.
+__device__ __forceinline__ uint32_t finite_bf16x2(uint32_t u) {
+  if ((u & 0x7f80u) == 0x7f80u) u &= 0xffff0000u;
+  if ((u & 0x7f800000u) == 0x7f800000u) u &= 0xffffu;
+  return u;
+}
+
+}  // namespace prichs

@@ -21,17 +21,13 @@
 // The visible pages of a tile are dealt to 4 n_split waves in contiguous runs; the
 // waves of a workgroup join in LDS, workgroups through the workspace and a second
 // kernel (n_split > 1).  The order of both is fixed, so results are reproducible.
+#include "attention_tile.hpp"
 #include "kv_cache.hpp"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace prichs {
 namespace {
-
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
@@ -43,20 +39,8 @@ struct AttendShape {
   float scale_log2;
 };
 
-__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ __forceinline__ float vmax(float a, float b) { return __builtin_elementwise_maximum(a, b); }
-// Max over the four 16-lane groups that share a query column (NaN propagates).
-__device__ __forceinline__ float max_across_groups(float x) {
-  const uint32_t u = __float_as_uint(x);
-  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  x = vmax(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const uint32_t w = __float_as_uint(x);
-  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-  return vmax(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
-                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+__device__ __forceinline__ f32x4 mfma_u32(u32x4 a, u32x4 b, f32x4 c) {
+  return mfma_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c);
 }
 // Values 2 BYTE and 2 BYTE + 1 of a dword of codes, in bf16.
 template <int BYTE>
@@ -172,7 +156,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 3 : 2) void kv_attend_kernel(
       for (int kk = 0; kk < 4; ++kk) {
         const u32x4 kf = eight(x.k[c][kk], sc);
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) s[c][nb] = mfma_bf16(kf, qf[nb][kk], s[c][nb]);
+        for (int nb = 0; nb < NB; ++nb) s[c][nb] = mfma_u32(kf, qf[nb][kk], s[c][nb]);
       }
     }
     // s[c][nb][r]: query row 16 nb + l16 of the tile, key kv0 + 16 c + 4 g + r.
@@ -267,8 +251,8 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 3 : 2) void kv_attend_kernel(
       }
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        oacc[2 * BYTE][nb] = mfma_bf16(lo, pf[nb][ks2], oacc[2 * BYTE][nb]);
-        oacc[2 * BYTE + 1][nb] = mfma_bf16(hi, pf[nb][ks2], oacc[2 * BYTE + 1][nb]);
+        oacc[2 * BYTE][nb] = mfma_u32(lo, pf[nb][ks2], oacc[2 * BYTE][nb]);
+        oacc[2 * BYTE + 1][nb] = mfma_u32(hi, pf[nb][ks2], oacc[2 * BYTE + 1][nb]);
       }
     };
 #pragma unroll
@@ -284,7 +268,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 3 : 2) void kv_attend_kernel(
       v_block(std::integral_constant<int, 2>{}, ks2, sa, sb);
       v_block(std::integral_constant<int, 3>{}, ks2, sa, sb);
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) lsum[nb] = mfma_bf16(ones, pf[nb][ks2], lsum[nb]);
+      for (int nb = 0; nb < NB; ++nb) lsum[nb] = mfma_u32(ones, pf[nb][ks2], lsum[nb]);
     }
     if (!whole && __any(nans)) {
       // The lane's dims 8 (4 g + r) + jd are group g's.

@@ -1,6 +1,8 @@
 // window_attention.hip -- causal GQA attention with a sliding window and sinks,
 // and its backward.
-#include "common.hpp"
+#include "attention_tile.hpp"
+
+#include <algorithm>
 
 namespace prichs {
 namespace {
@@ -11,97 +13,729 @@ constexpr int kHd = 128;
 __device__ __forceinline__ int rows_of(const int32_t *seq_lens, int b, int S) {
   return seq_lens == nullptr ? S : min(max(seq_lens[b], 0), S);
 }
-__device__ __forceinline__ float wave_sum(float x) {
-  for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m);
-  return x;
-}
-__device__ __forceinline__ float2 load2(const bf16_t *p) {
-  return make_float2(bf16_to_f32(p[0]), bf16_to_f32(p[1]));
-}
-__device__ __forceinline__ void store2(bf16_t *p, float a, float b) {
-  *reinterpret_cast<uint32_t *>(p) = pack_bf16x2(a, b);
-}
-
 struct Shape {
   int S, Hq, Hkv, window, sinks;
-  float scale;
+  float scale, scale_log2;  // 1 / sqrt(128), and times log2(e)
 };
 
-// delta[b][h][i] = d_o . o, one wave per (row, query head).
-__global__ __launch_bounds__(64) void window_delta_kernel(const bf16_t *d_o, size_t ldd,
-                                                          const bf16_t *o, size_t ldo,
-                                                          const int32_t *seq_lens, float *delta,
-                                                          Shape sh) {
-  const int lane = threadIdx.x, h = blockIdx.y;
-  const int b = blockIdx.x / sh.S, i = blockIdx.x - b * sh.S;
-  if (i >= rows_of(seq_lens, b, sh.S)) return;
-  const size_t c = (size_t)h * kHd + 2 * lane;
-  const float2 x = load2(d_o + (size_t)blockIdx.x * ldd + c),
-               y = load2(o + (size_t)blockIdx.x * ldo + c);
-  const float s = wave_sum(x.x * y.x + x.y * y.y);
-  if (lane == 0) delta[((size_t)b * sh.Hq + h) * sh.S + i] = s;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Chunk key of a row of a [rows][128] tile in LDS: its 16-byte chunk c is stored at
+// c ^ tile_key(row).  The key is the row's low four bits rotated by one, so that
+// both a fragment read (16 rows, one chunk) and a transposing read (8 rows, two
+// neighbouring chunks each) meet every bank once.
+__device__ __forceinline__ int tile_key(int row) { return ((row << 1) | ((row >> 3) & 1)) & 15; }
+__device__ __forceinline__ int tile_off(int row, int c) { return row * kHd + ((c ^ tile_key(row)) << 3); }
+
+// Four transposing fragments (both halves of a 32-row step, column blocks jd0 ..
+// jd0 + 3), with their wait.  addr: the lane's byte address of column block 0; jd
+// only reaches bits of the chunk that are exclusive-ored anyway.
+template <int LO, int HI>
+__device__ __forceinline__ void read_tr4(uint32_t addr, int jd0, u32x4 (&f)[4]) {
+  u32x2 lo[4], hi[4];
+  const uint32_t a0 = addr ^ (uint32_t)(32 * jd0), a1 = addr ^ (uint32_t)(32 * (jd0 + 1)),
+                 a2 = addr ^ (uint32_t)(32 * (jd0 + 2)), a3 = addr ^ (uint32_t)(32 * (jd0 + 3));
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %2, %9 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %4, %10 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %6, %11 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2]),
+        "=&v"(lo[3]), "=&v"(hi[3])
+      : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(LO), "n"(HI)
+      : "memory");
+#pragma unroll
+  for (int t = 0; t < 4; ++t) f[t] = u32x4{lo[t][0], lo[t][1], hi[t][0], hi[t][1]};
+}
+__device__ __forceinline__ void finite_frags(u32x4 (&f)[4]) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[t][e] = finite_bf16x2(f[t][e]);
+}
+// 0 where every element is finite, NaN otherwise.
+__device__ __forceinline__ float not_finite(f32x4 x, float z) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) z = fmaf(x[r], 0.f, z);
+  return z;
 }
 
-// One wave per (row, query head): d_q.
-__global__ __launch_bounds__(64) void window_dq_row_kernel(
-    const bf16_t *d_o, size_t ldd, const bf16_t *q, size_t ldq, const bf16_t *k, size_t ldk,
-    const bf16_t *v, size_t ldv, const float *lse, const float *delta, const int32_t *seq_lens,
-    bf16_t *dq, size_t lddq, Shape sh) {
-  const int lane = threadIdx.x, h = blockIdx.y;
-  const int b = blockIdx.x / sh.S, i = blockIdx.x - b * sh.S;
-  const int kvh = h / (sh.Hq / sh.Hkv);
-  const size_t row0 = (size_t)b * sh.S, hc = (size_t)h * kHd + 2 * lane;
-  bf16_t *out = dq + (row0 + i) * lddq + hc;
-  if (i >= rows_of(seq_lens, b, sh.S)) {
-    store2(out, 0.f, 0.f);
+// The lane's number, formed anew where it is asked for: what a loop derives from
+// it then holds no register over the loop.
+__device__ __forceinline__ int lane_here() {
+  int x;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=&v"(x));
+  return x;
+}
+
+struct BwdArgs {
+  const bf16_t *d_o, *q, *k, *v, *o;
+  const float *lse;
+  const int32_t *seq_lens;
+  bf16_t *dq, *dk, *dv;
+  int ldd, ldq, ldk, ldv, ldo, lddq, lddk, lddv;
+  // Per (sequence, head), per 32 rows: lse * log2(e) of the rows, then delta =
+  // d_o . o of the rows; a row past the sequence has +inf and 0 (p = 0).
+  float *rows;
+  int row_tiles;  // 32-row tiles of a (sequence, head) there
+  float *part;    // f32 partial d_k, d_v (dkv_kernel)
+  int budget;     // steps of a workgroup (dkv_kernel)
+  Shape sh;
+};
+
+// ---------------------------------------------------------------- d_q --------
+// As the forward (attention.hip): a wave owns 32 query rows of one head, HPW heads
+// of a kv group share the K / V tiles that the workgroup streams through LDS (64
+// keys, two stages).
+//   S^T = K Q^T, dP^T = V d_o^T   both operands' rows straight from LDS / registers
+//   dS^T = exp2(S scale log2(e) - lse) (dP - delta)   in the accumulator layout,
+//                   which is the operand layout of
+//   dQ^T += K^T dS^T              K^T by transposing LDS reads
+// The kernel also forms delta of its rows and leaves it, with lse, to dkv_kernel.
+constexpr int kKeys = 64;
+constexpr int kQStage = 2 * kKeys * kHd;  // elements: K, then V
+constexpr size_t kQLds = 2 * (size_t)kQStage * sizeof(bf16_t);
+
+template <int HPW>
+__global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
+  constexpr int kRowsWg = 128 / HPW;
+  extern __shared__ __attribute__((aligned(16))) bf16_t lds[];
+  const Shape &sh = a.sh;
+  const int group = sh.Hq / sh.Hkv, sets = group / HPW;
+  const int kvh = blockIdx.x / sets, b = blockIdx.y;
+  const int n_qb = (sh.S + kRowsWg - 1) / kRowsWg;
+  const int qb = n_qb - 1 - (int)blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, l16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = kvh * group + (blockIdx.x - kvh * sets) * HPW + wave % HPW;
+  const int q0 = qb * kRowsWg + (wave / HPW) * 32;
+  const int L = rows_of(a.seq_lens, b, sh.S);
+  const size_t seq0 = (size_t)b * sh.S;
+
+  // This wave's rows: fragments of q and d_o, lse, delta.
+  bf16x8 qf[2][4], df[2][4];
+  float lse2[2], delta[2];
+  float *rows = a.rows + (((size_t)b * sh.Hq + h) * a.row_tiles + q0 / 32) * 64;
+#pragma unroll
+  for (int nb = 0; nb < 2; ++nb) {
+    const int row = q0 + 16 * nb + l16;
+    const size_t r = seq0 + min(row, sh.S - 1);
+    const size_t c = (size_t)h * kHd + 8 * g;
+    float s = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      qf[nb][kk] = *reinterpret_cast<const bf16x8 *>(a.q + r * a.ldq + c + 32 * kk);
+      df[nb][kk] = *reinterpret_cast<const bf16x8 *>(a.d_o + r * a.ldd + c + 32 * kk);
+      const u32x4 x = __builtin_bit_cast(u32x4, df[nb][kk]);
+      const u32x4 y = *reinterpret_cast<const u32x4 *>(a.o + r * a.ldo + c + 32 * kk);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s += __uint_as_float(x[e] << 16) * __uint_as_float(y[e] << 16);
+        s += __uint_as_float(x[e] & 0xffff0000u) * __uint_as_float(y[e] & 0xffff0000u);
+      }
+    }
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+    const bool live = row < L;
+    lse2[nb] = live ? a.lse[((size_t)b * sh.Hq + h) * sh.S + row] * kLog2e : INFINITY;
+    delta[nb] = live ? s : 0.f;
+    if (g == 0 && q0 < a.row_tiles * 32) {
+      rows[16 * nb + l16] = lse2[nb];
+      rows[32 + 16 * nb + l16] = delta[nb];
+    }
+  }
+  f32x4 acc[8][2];
+#pragma unroll
+  for (int jd = 0; jd < 8; ++jd)
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) acc[jd][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // Blocks of 64 keys: the sinks', then from the first row's window on.
+  const int q_last = min(L, (qb + 1) * kRowsWg) - 1;
+  const int first = sh.window == 0 ? 0 : max(0, qb * kRowsWg - sh.window + 1) / kKeys;
+  const int n_sink = min((sh.sinks + kKeys - 1) / kKeys, first), skip = first - n_sink;
+  const int n_blk = qb * kRowsWg >= L ? 0 : q_last / kKeys + 1 - skip;
+  auto block_of = [&](int i) { return i >= n_sink ? i + skip : i; };
+
+  const bf16_t *kbase = a.k + seq0 * a.ldk + (size_t)kvh * kHd;
+  const bf16_t *vbase = a.v + seq0 * a.ldv + (size_t)kvh * kHd;
+  auto issue_tile = [&](int i, const bf16_t *src, int ld, int tile) {
+    const int blk = block_of(i);
+    const uint64_t bytes = (uint64_t)(L - 1 - blk * kKeys) * 2 * (uint64_t)ld + 2 * kHd;
+    const __amdgpu_buffer_rsrc_t r = buffer_rsrc(
+        src + (size_t)blk * kKeys * ld, bytes > 0xffffffffull ? 0xffffffffu : (uint32_t)bytes);
+    bf16_t *dst = lds + (i & 1) * kQStage + tile * kKeys * kHd;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = 16 * wave + 4 * j + g;
+      dma_16b(r, 2u * ((uint32_t)row * (uint32_t)ld + 8u * (uint32_t)(l16 ^ tile_key(row))),
+              dst + (16 * wave + 4 * j) * kHd);
+    }
+  };
+  auto issue = [&](int i) {
+    issue_tile(i, kbase, a.ldk, 0);
+    issue_tile(i, vbase, a.ldv, 1);
+  };
+  const uint32_t lds_base =
+      (uint32_t)(size_t)(const __attribute__((address_space(3))) bf16_t *)lds;
+  const uint32_t row_addr = 2u * (uint32_t)tile_off(l16, g);
+  const uint32_t tr_addr =
+      lds_base + 2u * (uint32_t)(tile_off(4 * g + (l16 >> 2), (l16 & 3) >> 1) + 4 * (l16 & 1));
+
+  if (n_blk > 0) issue(0);
+#pragma unroll 1
+  for (int i = 0; i < n_blk; ++i) {
+    const int kv0 = block_of(i) * kKeys;
+    // Block i has landed for every wave, and every wave is done with block i - 1.
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    if (i + 1 < n_blk) issue(i + 1);
+    // Every row of the wave sees the whole block, or none of it.
+    const bool whole = kv0 + kKeys <= min(q0 + 1, L) &&
+                       (sh.window == 0 || q0 + 31 - kv0 < sh.window || kv0 + kKeys <= sh.sinks);
+    const bool none = kv0 > q0 + 31 || (sh.window != 0 && q0 - (kv0 + kKeys - 1) >= sh.window &&
+                                        kv0 >= sh.sinks);
+    if (none) continue;
+    const uint32_t stage = (uint32_t)(i & 1) * (uint32_t)(kQStage * sizeof(bf16_t));
+    const char *kt = reinterpret_cast<const char *>(lds) + stage;
+    static_for<2>([&](auto half_c) {
+      constexpr int half = decltype(half_c)::value;  // keys 32 half ..
+      f32x4 s[2][2], dp[2][2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) s[c][nb] = dp[c][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const char *p = kt + (row_addr ^ (uint32_t)(64 * kk)) + 2 * kHd * (32 * half + 16 * c);
+          const bf16x8 kf = *reinterpret_cast<const bf16x8 *>(p);
+          const bf16x8 vf = *reinterpret_cast<const bf16x8 *>(p + 2 * kKeys * kHd);
+#pragma unroll
+          for (int nb = 0; nb < 2; ++nb) {
+            s[c][nb] = mfma_bf16(kf, qf[nb][kk], s[c][nb]);
+            dp[c][nb] = mfma_bf16(vf, df[nb][kk], dp[c][nb]);
+          }
+        }
+      u32x4 ds[2];
+      bool rare = false;
+      if (!whole) {
+        // What a row does not see must not reach it: hidden elements become p = 0
+        // below, and an infinity or NaN in K^T, which 0 would turn into NaN, is
+        // taken out of the product (a row that sees such a key has NaN in dS).
+        float z = 0.f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int nb = 0; nb < 2; ++nb) {
+            z = not_finite(s[c][nb], z);
+            const int row = q0 + 16 * nb + l16, key = kv0 + 32 * half + 16 * c + 4 * g;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const bool seen = (key + r <= row) & (row < L) &
+                                ((sh.window == 0) | (row - key - r < sh.window) |
+                                 (key + r < sh.sinks));
+              s[c][nb][r] = seen ? s[c][nb][r] : -INFINITY;
+              dp[c][nb][r] = seen ? dp[c][nb][r] : 0.f;
+            }
+          }
+        rare = __any(!(z == 0.f)) != 0;
+      }
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) {
+        float e[8];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            e[4 * c + r] = fast_exp2(fmaf(s[c][nb][r], sh.scale_log2, -lse2[nb])) *
+                           (dp[c][nb][r] - delta[nb]);
+        // dS rounded to bf16 for the product.
+        ds[nb] = u32x4{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]),
+                       pack_bf16(e[6], e[7])};
+      }
+#pragma unroll
+      for (int j0 = 0; j0 < 8; j0 += 4) {
+        u32x4 f[4];
+        read_tr4<2 * 32 * half * kHd, 2 * (32 * half + 16) * kHd>(tr_addr + stage, j0, f);
+        if (rare) finite_frags(f);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+          for (int nb = 0; nb < 2; ++nb)
+            acc[j0 + t][nb] = mfma_bf16(__builtin_bit_cast(bf16x8, f[t]), __builtin_bit_cast(bf16x8, ds[nb]),
+                                       acc[j0 + t][nb]);
+        }
+      }
+    });
+  }
+
+#pragma unroll
+  for (int nb = 0; nb < 2; ++nb) {
+    const int row = q0 + 16 * nb + l16;
+    if (row >= sh.S) continue;
+    bf16_t *out = a.dq + (seq0 + row) * a.lddq + (size_t)h * kHd + 4 * g;
+    const bool live = row < L;
+#pragma unroll
+    for (int jd = 0; jd < 8; ++jd) {
+      const f32x4 t = acc[jd][nb] * sh.scale;
+      const u32x2 u = u32x2{pack_bf16(t[0], t[1]), pack_bf16(t[2], t[3])};
+      *reinterpret_cast<u32x2 *>(out + 16 * jd) = live ? u : u32x2{0, 0};
+    }
+  }
+}
+
+// ------------------------------------------------------------ d_k, d_v -------
+// A workgroup owns 128 keys of one kv head and runs over the (query head, 32-row
+// tile) steps that see them.  8 waves: 4 key groups of 32 keys, whose K and V
+// fragments and f32 gradients stay in registers, times 2 step groups, which take
+// every second step and join in LDS at the end.
+//   S = Q K^T, dP = d_o V^T       rows of the q and d_o tiles straight from LDS
+//   P, dS                         in the accumulator layout, which is the operand
+//                                 layout (a lane holds one key and 8 of 32 rows) of
+//   dV^T += d_o^T P, dK^T += Q^T dS   by transposing LDS reads
+// 64 products a step and wave against 32 KB of LDS reads: four waves a step group
+// take the LDS's whole bandwidth at the full rate of the matrix cores.
+// Steps are cut into items of at most `budget` (a block that holds sinks is seen by
+// every later row); the items of one block meet in f32 partial sums that
+// dkv_join_kernel adds in order.
+constexpr int kBlk = 128;                       // keys of a workgroup
+constexpr int kTr = 32;                         // rows of a step
+constexpr int kStages = 3;
+constexpr int kStepElems = 2 * kTr * kHd + 128; // q, d_o, then lse / delta (64 floats)
+constexpr size_t kKvLds = 2 * kStages * (size_t)kStepElems * sizeof(bf16_t);
+static_assert(kKvLds >= 4 * 64 * 64 * sizeof(float), "the join of the step groups fits");
+
+// Steps of key block j over sequences of S rows.
+__host__ __device__ inline int steps_of(const Shape &sh, int rows, int j) {
+  const int left = rows - j * kBlk;
+  const bool far = sh.window == 0 || j * kBlk < sh.sinks;
+  const int n = far || left < kBlk + sh.window - 1 ? left : kBlk + sh.window - 1;
+  return n <= 0 ? 0 : (n + kTr - 1) / kTr * (sh.Hq / sh.Hkv);
+}
+__host__ __device__ inline int splits_of(const Shape &sh, int budget, int j) {
+  const int n = (steps_of(sh, sh.S, j) + budget - 1) / budget;
+  return n < 1 ? 1 : n;
+}
+// The block and split of an item (the same in every lane).
+__device__ __forceinline__ void item_at(const Shape &sh, int budget, int item, int *block,
+                                        int *split) {
+  const int lane = threadIdx.x & 63, blocks = (sh.S + kBlk - 1) / kBlk;
+  for (int base = 0; base < blocks; base += 64) {
+    const int n = base + lane < blocks ? splits_of(sh, budget, base + lane) : 0;
+    int end = n;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int up = __shfl_up(end, d);
+      if (lane >= d) end += up;
+    }
+    const unsigned long long in = __ballot(item < end);
+    if (in != 0) {
+      const int at = __ffsll((long long)in) - 1;
+      *block = base + at;
+      *split = __builtin_amdgcn_readfirstlane(item - (__shfl(end, at) - __shfl(n, at)));
+      return;
+    }
+    item -= __shfl(end, 63);
+  }
+  *block = blocks - 1, *split = 0;  // not reached: the grid holds the items
+}
+
+__global__ __launch_bounds__(512, 2) void window_dkv_kernel(BwdArgs a) {
+  extern __shared__ __attribute__((aligned(16))) bf16_t lds[];
+  const Shape &sh = a.sh;
+  const int G = sh.Hq / sh.Hkv;
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  int blk, split;
+  item_at(sh, a.budget, blockIdx.x, &blk, &split);
+  blk = __builtin_amdgcn_readfirstlane(blk);
+  const int n_split = splits_of(sh, a.budget, blk);
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, l16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kg = wave & 3, sg = wave >> 2;
+  const int L = rows_of(a.seq_lens, b, sh.S);
+  const size_t seq0 = (size_t)b * sh.S;
+  const int k0 = blk * kBlk + 32 * kg;  // this wave's first key
+
+  bf16x8 kf[2][4], vf[2][4];
+  f32x4 dk[8][2], dv[8][2];
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb) {
+    const int key = k0 + 16 * kb + l16;
+    const size_t r = seq0 + min(key, sh.S - 1), c = (size_t)kvh * kHd + 8 * g;
+    const bool live = key < L;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      u32x4 x = *reinterpret_cast<const u32x4 *>(a.k + r * a.ldk + c + 32 * kk);
+      u32x4 y = *reinterpret_cast<const u32x4 *>(a.v + r * a.ldv + c + 32 * kk);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = live ? x[e] : 0u, y[e] = live ? y[e] : 0u;
+      kf[kb][kk] = __builtin_bit_cast(bf16x8, x);
+      vf[kb][kk] = __builtin_bit_cast(bf16x8, y);
+    }
+  }
+#pragma unroll
+  for (int jd = 0; jd < 8; ++jd)
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) dk[jd][kb] = dv[jd][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // This item's steps: step x is head x / tiles, row tile t_lo + x % tiles.
+  const int steps = steps_of(sh, L, blk), tiles = steps / G;
+  const int begin = (int)((int64_t)steps * split / n_split),
+            end = (int)((int64_t)steps * (split + 1) / n_split);
+  const int t_lo = blk * (kBlk / kTr);
+  const int n_it = (end - begin + 1) / 2;
+
+  // The step to fetch next, and the one to compute.
+  int fx = begin + sg, fh = tiles > 0 ? fx / tiles : 0, ft = fx - fh * tiles;
+  int cx = fx, ch = fh, ct = ft;
+  auto advance = [&](int &x, int &hh, int &t) {
+    x += 2;
+    t += 2;
+    while (t >= tiles && tiles > 0) {
+      t -= tiles;
+      ++hh;
+    }
+  };
+  // Every wave of a step group moves 8 of the step's rows of q and of d_o, and all
+  // of lse / delta (the same bytes): 5 copies.  A step past the end copies nothing
+  // (an empty buffer: zeros), so that the count of copies in flight stays known.
+  auto fetch = [&](int slot) {
+    bf16_t *dst = lds + (sg * kStages + slot) * kStepElems;
+    const bool on = fx < end;
+    const int h = kvh * G + fh, t0 = (t_lo + ft) * kTr;
+    const int ln = lane_here();
+    const size_t row = seq0 + t0;
+    auto rows = [&](const bf16_t *src, int ld, int at) {
+      const uint64_t bytes = (uint64_t)(L - 1 - t0) * 2 * (uint64_t)ld + 2 * kHd;
+      const __amdgpu_buffer_rsrc_t r =
+          buffer_rsrc(on ? src + row * ld + (size_t)h * kHd : src,
+                      !on ? 0u : bytes > 0xffffffffull ? 0xffffffffu : (uint32_t)bytes);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int x = 8 * kg + 4 * j + (ln >> 4);
+        dma_16b(r, 2u * ((uint32_t)x * (uint32_t)ld + 8u * (uint32_t)((ln & 15) ^ tile_key(x))),
+                dst + at + (8 * kg + 4 * j) * kHd);
+      }
+    };
+    rows(a.q, a.ldq, 0);
+    rows(a.d_o, a.ldd, kTr * kHd);
+    const __amdgpu_buffer_rsrc_t r = buffer_rsrc(
+        on ? a.rows + (((size_t)b * sh.Hq + h) * a.row_tiles + t_lo + ft) * 64 : a.rows,
+        on ? 256u : 0u);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        r, (__attribute__((address_space(3))) void *)(dst + 2 * kTr * kHd), 4, 4u * (uint32_t)ln,
+        0, 0, 0);
+    advance(fx, fh, ft);
+  };
+
+  const uint32_t lds_base =
+      (uint32_t)(size_t)(const __attribute__((address_space(3))) bf16_t *)lds;
+
+  auto compute = [&](int slot) {
+    const int t0 = (t_lo + ct) * kTr;
+    const bool none = cx >= end || k0 >= L || t0 + kTr - 1 < k0 ||
+                      (sh.window != 0 && t0 - (k0 + 31) >= sh.window && k0 >= sh.sinks);
+    if (none) return;
+    const bool whole = t0 >= k0 + 31 && (sh.window == 0 || t0 + kTr - 1 - k0 < sh.window ||
+                                         k0 + 32 <= sh.sinks);
+    const uint32_t at = (uint32_t)((sg * kStages + slot) * kStepElems) * 2u;
+    const char *tile = reinterpret_cast<const char *>(lds) + at;
+    const int ln = lane_here(), g = ln >> 4, l16 = ln & 15;
+    const uint32_t ra = at + 2u * (uint32_t)tile_off(l16, g);
+    const uint32_t ta = lds_base + at + 2u * (uint32_t)(tile_off(4 * g + (l16 >> 2), (l16 & 3) >> 1) +
+                                                        4 * (l16 & 1));
+    u32x4 pf[2], ds[2];  // P and dS rounded to bf16 for the products
+    float z = 0.f;
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      // One block of 16 rows after the other, S before dP: registers.
+      auto product = [&](f32x4 (&x)[2], const bf16x8 (&f)[2][4], int off) {
+        x[0] = x[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const bf16x8 rf = *reinterpret_cast<const bf16x8 *>(
+              reinterpret_cast<const char *>(lds) + (ra ^ (uint32_t)(64 * kk)) + off +
+              2 * kHd * 16 * qb);
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) x[kb] = mfma_bf16(rf, f[kb][kk], x[kb]);
+        }
+      };
+      // x is 0 where the key's row does not see it.
+      auto hide = [&](int kb, f32x4 &x) {
+        int row = t0 + 16 * qb + 4 * g;
+        asm volatile("" : "+v"(row));  // keeps this in the branches that call it
+        const int key = k0 + 16 * kb + l16;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool seen = (key <= row + r) & ((sh.window == 0) | (row + r - key < sh.window) |
+                                                (key < sh.sinks));
+          x[r] = seen ? x[r] : 0.f;
+        }
+      };
+      const float *st = reinterpret_cast<const float *>(tile + 4 * kTr * kHd) + 16 * qb + 4 * g;
+      f32x4 p[2], x[2];
+      product(x, kf, 0);
+      {
+        const f32x4 lse2 = *reinterpret_cast<const f32x4 *>(st);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) p[kb][r] = fast_exp2(fmaf(x[kb][r], sh.scale_log2, -lse2[r]));
+          // What a key's row does not see must not reach the key, whatever the row
+          // holds: p and dS are 0 there, and see rare below.
+          if (!whole) {
+            z = not_finite(x[kb], z);
+            hide(kb, p[kb]);
+          }
+          pf[kb][2 * qb] = pack_bf16(p[kb][0], p[kb][1]);
+          pf[kb][2 * qb + 1] = pack_bf16(p[kb][2], p[kb][3]);
+        }
+      }
+      product(x, vf, 2 * kTr * kHd);
+      const f32x4 delta = *reinterpret_cast<const f32x4 *>(st + kTr);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        f32x4 e;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) e[r] = p[kb][r] * (x[kb][r] - delta[r]);
+        if (!whole) {
+          z = not_finite(x[kb], z);
+          hide(kb, e);
+        }
+        ds[kb][2 * qb] = pack_bf16(e[0], e[1]);
+        ds[kb][2 * qb + 1] = pack_bf16(e[2], e[3]);
+      }
+    }
+    // An infinity or NaN of q or d_o, which 0 would turn into NaN, is taken out of
+    // the products of a step that not every key's row sees.
+    const bool rare = !whole && __any(!(z == 0.f)) != 0;
+    constexpr int kDo = 2 * kTr * kHd;  // bytes to the d_o tile
+#pragma unroll
+    for (int j0 = 0; j0 < 8; j0 += 4) {
+      u32x4 f[4];
+      read_tr4<kDo, kDo + 2 * 16 * kHd>(ta, j0, f);
+      if (rare) finite_frags(f);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+          dv[j0 + t][kb] = mfma_bf16(__builtin_bit_cast(bf16x8, f[t]), __builtin_bit_cast(bf16x8, pf[kb]),
+                                     dv[j0 + t][kb]);
+      }
+      read_tr4<0, 2 * 16 * kHd>(ta, j0, f);
+      if (rare) finite_frags(f);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+          dk[j0 + t][kb] = mfma_bf16(__builtin_bit_cast(bf16x8, f[t]), __builtin_bit_cast(bf16x8, ds[kb]),
+                                     dk[j0 + t][kb]);
+      }
+    }
+    if (rare) {
+      // The infinities and NaN of d_o that were taken out, for the keys that their
+      // rows see (p > 0: an infinity keeps its sign).  A row with such a q has NaN
+      // in P and dS already.
+#pragma unroll 1
+      for (int x = 0; x < kTr; ++x) {
+        const int row = t0 + x;
+#pragma unroll
+        for (int jd = 0; jd < 8; ++jd) {
+          asm volatile("" ::: "memory");  // one load after the other: registers
+          const u32x2 raw = *reinterpret_cast<const u32x2 *>(
+              tile + kDo + ((uint32_t)(2 * (tile_off(x, g >> 1) + 4 * (g & 1))) ^ (32u * jd)));
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            const int key = k0 + 16 * kb + l16;
+            const bool seen = (key <= row) & ((sh.window == 0) | (row - key < sh.window) |
+                                              (key < sh.sinks));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const uint32_t u = r & 1 ? raw[r / 2] & 0xffff0000u : raw[r / 2] << 16;
+              const bool off = (u & 0x7f800000u) == 0x7f800000u;
+              dv[jd][kb][r] += (off & seen) ? __uint_as_float(u) : 0.f;
+            }
+          }
+        }
+      }
+    }
+  };
+
+#pragma unroll
+  for (int x = 0; x < kStages - 1; ++x) fetch(x);
+  int slot = 0;
+#pragma unroll 1
+  for (int it = 0; it < n_it; ++it) {
+    // Of the copies in flight only the newest kStages - 2 steps' may be missing;
+    // every wave is done with the slot that is fetched into next.
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(5 * (kStages - 2)) : "memory");
+    fetch(slot == 0 ? kStages - 1 : slot - 1);
+    compute(slot);
+    advance(cx, ch, ct);
+    slot = slot + 1 == kStages ? 0 : slot + 1;
+  }
+  // The copies past the end write zeros: they must land before LDS is used again.
+  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+
+  // The second step group's sums join the first's, d_k then d_v.
+  const int le = lane_here(), ge = le >> 4, l16e = le & 15;
+  f32x4 *join = reinterpret_cast<f32x4 *>(lds);
+  auto joined = [&](f32x4 (&x)[8][2]) {
+    if (sg == 1) {
+#pragma unroll
+      for (int jd = 0; jd < 8; ++jd)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) join[((2 * jd + kb) * 4 + kg) * 64 + le] = x[jd][kb];
+    }
+    __syncthreads();
+    if (sg == 0) {
+#pragma unroll
+      for (int jd = 0; jd < 8; ++jd)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+          x[jd][kb] = x[jd][kb] + join[((2 * jd + kb) * 4 + kg) * 64 + le];
+    }
+    __syncthreads();
+  };
+  joined(dk);
+  joined(dv);
+  if (sg != 0) return;
+  if (n_split > 1) {
+    float *part = a.part + ((((size_t)b * sh.Hkv + kvh) * gridDim.x + blockIdx.x) * 2) * kBlk * kHd;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      float *row = part + (32 * kg + 16 * kb + l16e) * kHd + 4 * ge;
+#pragma unroll
+      for (int jd = 0; jd < 8; ++jd) {
+        *reinterpret_cast<f32x4 *>(row + 16 * jd) = dk[jd][kb];
+        *reinterpret_cast<f32x4 *>(row + kBlk * kHd + 16 * jd) = dv[jd][kb];
+      }
+    }
     return;
   }
-  const float2 qv = load2(q + (row0 + i) * ldq + hc), dv = load2(d_o + (row0 + i) * ldd + hc);
-  const size_t st = ((size_t)b * sh.Hq + h) * sh.S + i;
-  const int lo = sh.window == 0 ? 0 : max(0, i - sh.window + 1);
-  float a0 = 0.f, a1 = 0.f;
-  for (int j = 0; j <= i; ++j) {
-    if (j >= min(sh.sinks, lo) && j < lo) j = lo;
-    const size_t c = (size_t)kvh * kHd + 2 * lane;
-    const float2 kv = load2(k + (row0 + j) * ldk + c), vv = load2(v + (row0 + j) * ldv + c);
-    const float p = expf(wave_sum(qv.x * kv.x + qv.y * kv.y) * sh.scale - lse[st]);
-    const float ds = p * (wave_sum(dv.x * vv.x + dv.y * vv.y) - delta[st]) * sh.scale;
-    a0 += ds * kv.x;
-    a1 += ds * kv.y;
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb) {
+    const int key = k0 + 16 * kb + l16e;
+    if (key >= sh.S) continue;
+    bf16_t *ok = a.dk + (seq0 + key) * a.lddk + (size_t)kvh * kHd + 4 * ge;
+    bf16_t *ov = a.dv + (seq0 + key) * a.lddv + (size_t)kvh * kHd + 4 * ge;
+    const bool live = key < L;
+#pragma unroll
+    for (int jd = 0; jd < 8; ++jd) {
+      const f32x4 x = dk[jd][kb] * sh.scale, y = dv[jd][kb];
+      const u32x2 ux = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+      const u32x2 uy = u32x2{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])};
+      *reinterpret_cast<u32x2 *>(ok + 16 * jd) = live ? ux : u32x2{0, 0};
+      *reinterpret_cast<u32x2 *>(ov + 16 * jd) = live ? uy : u32x2{0, 0};
+    }
   }
-  store2(out, a0, a1);
 }
 
-// One wave per (key, kv head): d_k and d_v over the rows and query heads that
-// see the key.
-__global__ __launch_bounds__(64) void window_dkv_row_kernel(
-    const bf16_t *d_o, size_t ldd, const bf16_t *q, size_t ldq, const bf16_t *k, size_t ldk,
-    const bf16_t *v, size_t ldv, const float *lse, const float *delta, const int32_t *seq_lens,
-    bf16_t *dk, size_t lddk, bf16_t *dv, size_t lddv, Shape sh) {
-  const int lane = threadIdx.x, kvh = blockIdx.y;
-  const int b = blockIdx.x / sh.S, j = blockIdx.x - b * sh.S;
-  const int L = rows_of(seq_lens, b, sh.S), G = sh.Hq / sh.Hkv;
-  const size_t row0 = (size_t)b * sh.S, c = (size_t)kvh * kHd + 2 * lane;
-  float k0 = 0.f, k1 = 0.f, v0 = 0.f, v1 = 0.f;
-  if (j < L) {
-    const float2 kv = load2(k + (row0 + j) * ldk + c), vv = load2(v + (row0 + j) * ldv + c);
-    const bool far = sh.window == 0 || j < sh.sinks || sh.window > L - j;
-    const int end = far ? L : j + sh.window;
-    for (int h = kvh * G; h < (kvh + 1) * G; ++h)
-      for (int i = j; i < end; ++i) {
-        const size_t st = ((size_t)b * sh.Hq + h) * sh.S + i, hc = (size_t)h * kHd + 2 * lane;
-        const float2 qv = load2(q + (row0 + i) * ldq + hc),
-                     gv = load2(d_o + (row0 + i) * ldd + hc);
-        const float p = expf(wave_sum(qv.x * kv.x + qv.y * kv.y) * sh.scale - lse[st]);
-        const float ds = p * (wave_sum(gv.x * vv.x + gv.y * vv.y) - delta[st]) * sh.scale;
-        k0 += ds * qv.x;
-        k1 += ds * qv.y;
-        v0 += p * gv.x;
-        v1 += p * gv.y;
-      }
+// Adds the items of the blocks that were cut, in the items' order: a workgroup per
+// (block, kv head, sequence) and 16 of its keys.
+__global__ __launch_bounds__(256) void window_dkv_join_kernel(BwdArgs a, int items) {
+  const Shape &sh = a.sh;
+  const int blk = blockIdx.x / 8, kvh = blockIdx.y, b = blockIdx.z;
+  const int n_split = splits_of(sh, a.budget, blk);
+  if (n_split == 1) return;
+  int item = 0;  // the block's first
+  const int lane = threadIdx.x & 63;
+  for (int j = lane; j < blk; j += 64) item += splits_of(sh, a.budget, j);
+  for (int m = 1; m < 64; m <<= 1) item += __shfl_xor(item, m);
+  const int key = 16 * (blockIdx.x % 8) + (threadIdx.x >> 4), d = 8 * (threadIdx.x & 15);
+  const int row = blk * kBlk + key;
+  if (row >= sh.S) return;
+  const bool live = row < rows_of(a.seq_lens, b, sh.S);
+  const float *part =
+      a.part + ((((size_t)b * sh.Hkv + kvh) * items + item) * 2) * kBlk * kHd + key * kHd + d;
+  f32x4 t[2][2];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) t[w][0] = t[w][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < n_split; ++s)
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        t[w][e] = t[w][e] + *reinterpret_cast<const f32x4 *>(
+                                part + (size_t)(2 * s + w) * kBlk * kHd + 4 * e);
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    bf16_t *out = (w == 0 ? a.dk + ((size_t)b * sh.S + row) * a.lddk
+                          : a.dv + ((size_t)b * sh.S + row) * a.lddv) +
+                  (size_t)kvh * kHd + d;
+    const float f = w == 0 ? sh.scale : 1.0f;
+    u32x4 u;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      u[2 * e] = pack_bf16(t[w][e][0] * f, t[w][e][1] * f);
+      u[2 * e + 1] = pack_bf16(t[w][e][2] * f, t[w][e][3] * f);
+    }
+    *reinterpret_cast<u32x4 *>(out) = live ? u : u32x4{0, 0, 0, 0};
   }
-  store2(dk + (row0 + j) * lddk + c, k0, k1);
-  store2(dv + (row0 + j) * lddv + c, v0, v1);
+}
+
+// How the key blocks are cut: items of at most `budget` steps.
+struct BwdPlan {
+  int budget = 0;
+  size_t items = 0;
+  bool cut = false;
+};
+BwdPlan plan_bwd(const Shape &sh, size_t batch) {
+  const int blocks = (int)cdiv((size_t)sh.S, (size_t)kBlk);
+  int64_t total = 0, most = 1;
+  for (int j = 0; j < blocks; ++j) {
+    const int n = steps_of(sh, sh.S, j);
+    total += n;
+    most = std::max<int64_t>(most, n);
+  }
+  // One workgroup fits a CU.  The time is about that of the longest item where all
+  // items are resident, and the average load and half an item more beyond; an item
+  // of a cut block costs about 8 steps more (its sums go through memory).
+  const int64_t wgs = (int64_t)batch * sh.Hkv, cus = 256;
+  BwdPlan best;
+  double best_cost = 0;
+  for (int64_t n = 1; n <= 64; n += n < 8 ? 1 : n / 4) {
+    const int budget = (int)std::max<int64_t>((most + n - 1) / n, 8);
+    int64_t items = 0, extra = 0;
+    for (int j = 0; j < blocks; ++j) {
+      const int x = splits_of(sh, budget, j);
+      items += x;
+      if (x > 1) extra += x;
+    }
+    const double load = double(total + 8 * extra) * wgs / cus, item = budget + (extra ? 8 : 0);
+    const double cost = items * wgs <= cus ? item : std::max(load + item / 2, item);
+    if (best.budget == 0 || cost < best_cost) {
+      best_cost = cost;
+      best.budget = budget;
+      best.items = (size_t)items;
+      best.cut = extra != 0;
+    }
+    if (budget == 8) break;
+  }
+  return best;
+}
+// Bytes of the row statistics and of the partial sums.
+size_t stat_bytes(const Shape &sh, size_t batch) {
+  return roundup(batch * sh.Hq * cdiv((size_t)sh.S, (size_t)kTr) * 64 * sizeof(float), 256);
+}
+size_t part_bytes(const Shape &sh, size_t batch, const BwdPlan &p) {
+  return p.cut ? batch * sh.Hkv * p.items * 2 * kBlk * kHd * sizeof(float) : 0;
+}
+
+Shape shape_of(size_t seq_len, size_t n_heads, size_t n_kv_heads, size_t window, size_t sinks) {
+  // A window past the sequence hides nothing.
+  return Shape{(int)seq_len,
+               (int)n_heads,
+               (int)n_kv_heads,
+               (int)(window >= seq_len ? 0 : window),
+               (int)(sinks < seq_len ? sinks : seq_len),
+               1.0f / sqrtf((float)kHd),
+               1.0f / sqrtf((float)kHd) * kLog2e};
 }
 
 // Checks shared by both directions; PRICHS_OK with *work = false where there is
@@ -119,13 +753,7 @@ int check_shape(const char *who, size_t batch, size_t seq_len, size_t n_heads, s
   PRICHS_REQUIRE(n_heads <= 65535 && batch <= 65535 && seq_len <= (size_t)1 << 21 &&
                      batch * seq_len <= (size_t)INT32_MAX / 2,
                  "%s: shape too large", who);
-  // A window past the sequence hides nothing.
-  *sh = Shape{(int)seq_len,
-              (int)n_heads,
-              (int)n_kv_heads,
-              (int)(window >= seq_len ? 0 : window),
-              (int)(sinks < seq_len ? sinks : seq_len),
-              1.0f / sqrtf((float)head_dim)};
+  *sh = shape_of(seq_len, n_heads, n_kv_heads, window, sinks);
   *work = batch != 0 && seq_len != 0;
   return PRICHS_OK;
 }
@@ -174,9 +802,15 @@ extern "C" int prichs_window_attention_forward(
 }
 
 extern "C" size_t prichs_window_attention_backward_workspace(size_t batch, size_t seq_len,
-                                                             size_t n_heads, size_t n_kv_heads) {
-  (void)n_kv_heads;
-  return roundup(batch * seq_len * n_heads * sizeof(float), 256);
+                                                             size_t n_heads, size_t n_kv_heads,
+                                                             size_t window, size_t sinks) {
+  Shape sh;
+  bool work;
+  if (check_shape("window_attention_backward_workspace", batch, seq_len, n_heads, n_kv_heads, kHd,
+                  PRICHS_DTYPE_BF16, window, sinks, &sh, &work) != PRICHS_OK ||
+      !work)
+    return 0;
+  return stat_bytes(sh, batch) + part_bytes(sh, batch, plan_bwd(sh, batch));
 }
 
 extern "C" int prichs_window_attention_backward(
@@ -202,29 +836,39 @@ extern "C" int prichs_window_attention_backward(
   WINDOW_TRY(check_rows(who, "d_k", d_k, lddk, K));
   WINDOW_TRY(check_rows(who, "d_v", d_v, lddv, K));
   PRICHS_REQUIRE(lse != nullptr, "%s: null pointer argument lse", who);
-  const size_t need =
-      prichs_window_attention_backward_workspace(batch, seq_len, n_heads, n_kv_heads);
+  const BwdPlan plan = plan_bwd(sh, batch);
+  const size_t stats = stat_bytes(sh, batch), need = stats + part_bytes(sh, batch, plan);
   if (workspace_bytes < need)
     return fail(PRICHS_ERR_CAPACITY, "%s: workspace of %zu bytes, %zu needed", who,
                 workspace_bytes, need);
   PRICHS_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
                  "%s: the workspace must be 16-byte aligned device memory", who);
-  float *delta = static_cast<float *>(workspace);
-  const dim3 rows_q((unsigned)(batch * seq_len), (unsigned)n_heads),
-      rows_kv((unsigned)(batch * seq_len), (unsigned)n_kv_heads);
-  const auto *bd = static_cast<const bf16_t *>(d_o), *bq = static_cast<const bf16_t *>(q),
-             *bk = static_cast<const bf16_t *>(k), *bv = static_cast<const bf16_t *>(v),
-             *bo = static_cast<const bf16_t *>(o);
-  hipLaunchKernelGGL(window_delta_kernel, rows_q, dim3(64), 0, as_stream(stream), bd, ldd, bo, ldo,
-                     seq_lens, delta, sh);
-  PRICHS_LAUNCH_CHECK("window_attention_backward delta launch");
-  hipLaunchKernelGGL(window_dq_row_kernel, rows_q, dim3(64), 0, as_stream(stream), bd, ldd, bq,
-                     ldq, bk, ldk, bv, ldv, lse, delta, seq_lens, static_cast<bf16_t *>(d_q), lddq,
-                     sh);
+  const int group = (int)(n_heads / n_kv_heads);
+  const int hpw = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+  const size_t n_qb = cdiv(seq_len, (size_t)(128 / hpw)), blocks = cdiv(seq_len, (size_t)kBlk);
+  PRICHS_REQUIRE(n_qb <= 65535 && n_kv_heads <= 65535, "%s: shape too large", who);
+  const auto bf = [](const void *p) { return static_cast<const bf16_t *>(p); };
+  const auto out = [](void *p) { return static_cast<bf16_t *>(p); };
+  BwdArgs a{bf(d_o), bf(q), bf(k), bf(v), bf(o), lse, seq_lens, out(d_q), out(d_k), out(d_v),
+            (int)ldd, (int)ldq, (int)ldk, (int)ldv, (int)ldo, (int)lddq, (int)lddk, (int)lddv,
+            static_cast<float *>(workspace), (int)cdiv(seq_len, (size_t)kTr),
+            reinterpret_cast<float *>(static_cast<char *>(workspace) + stats), plan.budget, sh};
+  auto dq_kern = hpw == 4 ? window_dq_kernel<4> : hpw == 2 ? window_dq_kernel<2>
+                                                           : window_dq_kernel<1>;
+  hipLaunchKernelGGL(dq_kern, dim3((unsigned)(n_heads / hpw), (unsigned)batch, (unsigned)n_qb),
+                     dim3(256), kQLds, as_stream(stream), a);
   PRICHS_LAUNCH_CHECK("window_attention_backward d_q launch");
-  hipLaunchKernelGGL(window_dkv_row_kernel, rows_kv, dim3(64), 0, as_stream(stream), bd, ldd, bq,
-                     ldq, bk, ldk, bv, ldv, lse, delta, seq_lens, static_cast<bf16_t *>(d_k), lddk,
-                     static_cast<bf16_t *>(d_v), lddv, sh);
+  static LdsLimit limit;
+  WINDOW_TRY(raise_lds_limit(limit, reinterpret_cast<const void *>(window_dkv_kernel), kKvLds, who));
+  hipLaunchKernelGGL(window_dkv_kernel,
+                     dim3((unsigned)plan.items, (unsigned)n_kv_heads, (unsigned)batch), dim3(512),
+                     kKvLds, as_stream(stream), a);
   PRICHS_LAUNCH_CHECK("window_attention_backward d_k / d_v launch");
+  if (plan.cut) {
+    hipLaunchKernelGGL(window_dkv_join_kernel,
+                       dim3((unsigned)(8 * blocks), (unsigned)n_kv_heads, (unsigned)batch),
+                       dim3(256), 0, as_stream(stream), a, (int)plan.items);
+    PRICHS_LAUNCH_CHECK("window_attention_backward join launch");
+  }
   return PRICHS_OK;
 }

@@ -399,7 +399,8 @@ def window_attention_backward(d_out, q, k, v, out, lse, batch, seq_len, n_heads,
                 t = torch.empty((rows, cols), dtype=q.dtype, device=q.device)
             grads.append(_rows(t, name, rows, cols))
         ws = torch.empty((lib.prichs_window_attention_backward_workspace(
-            batch, seq_len, n_heads, n_kv_heads),), dtype=torch.uint8, device=q.device)
+            batch, seq_len, n_heads, n_kv_heads, window, sinks),), dtype=torch.uint8,
+            device=q.device)
         args = [x for t in (d_out, q, k, v, out) for x in (_a(t), _ld(t))]
         L.check(lib.prichs_window_attention_backward(
             *args, _a(lse), _a(seq_lens), *[x for t in grads for x in (_a(t), _ld(t))], batch,

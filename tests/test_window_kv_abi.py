@@ -80,7 +80,7 @@ def test_an_empty_batch_is_nothing_to_do(lib, name, base):
 
 
 def test_workspaces(lib):
-    need = lib.prichs_window_attention_backward_workspace(4, 2048, 12, 3)
+    need = lib.prichs_window_attention_backward_workspace(4, 2048, 12, 3, 4, 0)
     assert need >= 4 * 2048 * 12 * 4
     assert call(lib, "prichs_window_attention_backward",
                 {**BWD, "batch": 4, "seq_len": 2048, "n_heads": 12, "n_kv_heads": 3, "ldq": 1536,
