@@ -99,6 +99,7 @@ struct BwdArgs {
 // The kernel also forms delta of its rows and leaves it, with lse, to dkv_kernel.
 constexpr int kKeys = 64;
 constexpr int kQStage = 2 * kKeys * kHd;  // elements: K, then V
+constexpr int kExactBlocks = 4;  // delta in a sweep of its own up to so many blocks
 constexpr size_t kQLds = 2 * (size_t)kQStage * sizeof(bf16_t);
 
 template <int HPW>
@@ -144,10 +145,6 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
     const bool live = row < L;
     lse2[nb] = live ? a.lse[((size_t)b * sh.Hq + h) * sh.S + row] * kLog2e : INFINITY;
     delta[nb] = live ? s : 0.f;
-    if (g == 0 && q0 < a.row_tiles * 32) {
-      rows[16 * nb + l16] = lse2[nb];
-      rows[32 + 16 * nb + l16] = delta[nb];
-    }
   }
   f32x4 acc[8][2];
 #pragma unroll
@@ -187,93 +184,137 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
   const uint32_t tr_addr =
       lds_base + 2u * (uint32_t)(tile_off(4 * g + (l16 >> 2), (l16 & 3) >> 1) + 4 * (l16 & 1));
 
-  if (n_blk > 0) issue(0);
+  // One sweep over the blocks: f(half, S^T, dP^T, rare) for each half block that
+  // some row of the wave sees, hidden elements at -inf and 0.
+  auto sweep = [&](auto &&f) {
+    if (n_blk > 0) issue(0);
 #pragma unroll 1
-  for (int i = 0; i < n_blk; ++i) {
-    const int kv0 = block_of(i) * kKeys;
-    // Block i has landed for every wave, and every wave is done with block i - 1.
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    if (i + 1 < n_blk) issue(i + 1);
-    // Every row of the wave sees the whole block, or none of it.
-    const bool whole = kv0 + kKeys <= min(q0 + 1, L) &&
-                       (sh.window == 0 || q0 + 31 - kv0 < sh.window || kv0 + kKeys <= sh.sinks);
-    const bool none = kv0 > q0 + 31 || (sh.window != 0 && q0 - (kv0 + kKeys - 1) >= sh.window &&
-                                        kv0 >= sh.sinks);
-    if (none) continue;
-    const uint32_t stage = (uint32_t)(i & 1) * (uint32_t)(kQStage * sizeof(bf16_t));
-    const char *kt = reinterpret_cast<const char *>(lds) + stage;
-    static_for<2>([&](auto half_c) {
-      constexpr int half = decltype(half_c)::value;  // keys 32 half ..
-      f32x4 s[2][2], dp[2][2];
+    for (int i = 0; i < n_blk; ++i) {
+      const int kv0 = block_of(i) * kKeys;
+      // Block i has landed for every wave, and every wave is done with block i - 1.
+      asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+      if (i + 1 < n_blk) issue(i + 1);
+      // Every row of the wave sees the whole block, or none of it.
+      const bool whole = kv0 + kKeys <= min(q0 + 1, L) &&
+                         (sh.window == 0 || q0 + 31 - kv0 < sh.window || kv0 + kKeys <= sh.sinks);
+      const bool none = kv0 > q0 + 31 || (sh.window != 0 && q0 - (kv0 + kKeys - 1) >= sh.window &&
+                                          kv0 >= sh.sinks);
+      if (none) continue;
+      const uint32_t stage = (uint32_t)(i & 1) * (uint32_t)(kQStage * sizeof(bf16_t));
+      const char *kt = reinterpret_cast<const char *>(lds) + stage;
+      static_for<2>([&](auto half_c) {
+        constexpr int half = decltype(half_c)::value;  // keys 32 half ..
+        f32x4 s[2][2], dp[2][2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int nb = 0; nb < 2; ++nb) s[c][nb] = dp[c][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const char *p = kt + (row_addr ^ (uint32_t)(64 * kk)) + 2 * kHd * (32 * half + 16 * c);
+            const bf16x8 kf = *reinterpret_cast<const bf16x8 *>(p);
+            const bf16x8 vf = *reinterpret_cast<const bf16x8 *>(p + 2 * kKeys * kHd);
+#pragma unroll
+            for (int nb = 0; nb < 2; ++nb) {
+              s[c][nb] = mfma_bf16(kf, qf[nb][kk], s[c][nb]);
+              dp[c][nb] = mfma_bf16(vf, df[nb][kk], dp[c][nb]);
+            }
+          }
+        bool rare = false;
+        if (!whole) {
+          // What a row does not see must not reach it: hidden elements become p = 0,
+          // and an infinity or NaN in K^T, which 0 would turn into NaN, is taken out
+          // of the product (a row that sees such a key has NaN in dS).
+          float z = 0.f;
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int nb = 0; nb < 2; ++nb) {
+              z = not_finite(s[c][nb], z);
+              const int row = q0 + 16 * nb + l16, key = kv0 + 32 * half + 16 * c + 4 * g;
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const bool seen = (key + r <= row) & (row < L) &
+                                  ((sh.window == 0) | (row - key - r < sh.window) |
+                                   (key + r < sh.sinks));
+                s[c][nb][r] = seen ? s[c][nb][r] : -INFINITY;
+                dp[c][nb][r] = seen ? dp[c][nb][r] : 0.f;
+              }
+            }
+          rare = __any(!(z == 0.f)) != 0;
+        }
+        f(half_c, stage, s, dp, rare);
+      });
+    }
+  };
+
+  // delta = d_o . o, from an o that was rounded to bf16, is off by some 2^-9 of the
+  // terms' root sum of squares: little beside dP where a row sees many keys, but half
+  // again the error of d_q and d_k where it sees few (0.0038 instead of 0.0024 of
+  // their norm at 2 keys, 0.0027 at 8, 0.0025 at 64).  Rows of few blocks form it as
+  // sum p dP / sum p instead, in a sweep of their own (2 of the 3 products again).
+  if (n_blk > 0 && n_blk <= kExactBlocks) {
+    float num[2] = {0.f, 0.f}, den[2] = {0.f, 0.f};
+    sweep([&](auto, uint32_t, f32x4 (&s)[2][2], f32x4 (&dp)[2][2], bool) {
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float p = fast_exp2(fmaf(s[c][nb][r], sh.scale_log2, -lse2[nb]));
+            num[nb] = fmaf(p, dp[c][nb][r], num[nb]);
+            den[nb] += p;
+          }
+    });
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) {
+      num[nb] += __shfl_xor(num[nb], 16);
+      den[nb] += __shfl_xor(den[nb], 16);
+      num[nb] += __shfl_xor(num[nb], 32);
+      den[nb] += __shfl_xor(den[nb], 32);
+      if (q0 + 16 * nb + l16 < L) delta[nb] = num[nb] / den[nb];
+    }
+    asm volatile("s_barrier" ::: "memory");  // the last block's readers, before it is refilled
+  }
+#pragma unroll
+  for (int nb = 0; nb < 2; ++nb)
+    if (g == 0 && q0 < a.row_tiles * 32) {
+      rows[16 * nb + l16] = lse2[nb];
+      rows[32 + 16 * nb + l16] = delta[nb];
+    }
+
+  sweep([&](auto half_c, uint32_t stage, f32x4 (&s)[2][2], f32x4 (&dp)[2][2], bool rare) {
+    constexpr int half = decltype(half_c)::value;
+    u32x4 ds[2];
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) {
+      float e[8];
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int nb = 0; nb < 2; ++nb) s[c][nb] = dp[c][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int r = 0; r < 4; ++r)
+          e[4 * c + r] = fast_exp2(fmaf(s[c][nb][r], sh.scale_log2, -lse2[nb])) *
+                         (dp[c][nb][r] - delta[nb]);
+      // dS rounded to bf16 for the product.
+      ds[nb] = u32x4{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]),
+                     pack_bf16(e[6], e[7])};
+    }
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
+    for (int j0 = 0; j0 < 8; j0 += 4) {
+      u32x4 f[4];
+      read_tr4<2 * 32 * half * kHd, 2 * (32 * half + 16) * kHd>(tr_addr + stage, j0, f);
+      if (rare) finite_frags(f);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const char *p = kt + (row_addr ^ (uint32_t)(64 * kk)) + 2 * kHd * (32 * half + 16 * c);
-          const bf16x8 kf = *reinterpret_cast<const bf16x8 *>(p);
-          const bf16x8 vf = *reinterpret_cast<const bf16x8 *>(p + 2 * kKeys * kHd);
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int nb = 0; nb < 2; ++nb) {
-            s[c][nb] = mfma_bf16(kf, qf[nb][kk], s[c][nb]);
-            dp[c][nb] = mfma_bf16(vf, df[nb][kk], dp[c][nb]);
-          }
-        }
-      u32x4 ds[2];
-      bool rare = false;
-      if (!whole) {
-        // What a row does not see must not reach it: hidden elements become p = 0
-        // below, and an infinity or NaN in K^T, which 0 would turn into NaN, is
-        // taken out of the product (a row that sees such a key has NaN in dS).
-        float z = 0.f;
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int nb = 0; nb < 2; ++nb) {
-            z = not_finite(s[c][nb], z);
-            const int row = q0 + 16 * nb + l16, key = kv0 + 32 * half + 16 * c + 4 * g;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const bool seen = (key + r <= row) & (row < L) &
-                                ((sh.window == 0) | (row - key - r < sh.window) |
-                                 (key + r < sh.sinks));
-              s[c][nb][r] = seen ? s[c][nb][r] : -INFINITY;
-              dp[c][nb][r] = seen ? dp[c][nb][r] : 0.f;
-            }
-          }
-        rare = __any(!(z == 0.f)) != 0;
-      }
-#pragma unroll
-      for (int nb = 0; nb < 2; ++nb) {
-        float e[8];
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            e[4 * c + r] = fast_exp2(fmaf(s[c][nb][r], sh.scale_log2, -lse2[nb])) *
-                           (dp[c][nb][r] - delta[nb]);
-        // dS rounded to bf16 for the product.
-        ds[nb] = u32x4{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]),
-                       pack_bf16(e[6], e[7])};
-      }
-#pragma unroll
-      for (int j0 = 0; j0 < 8; j0 += 4) {
-        u32x4 f[4];
-        read_tr4<2 * 32 * half * kHd, 2 * (32 * half + 16) * kHd>(tr_addr + stage, j0, f);
-        if (rare) finite_frags(f);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-#pragma unroll
-          for (int nb = 0; nb < 2; ++nb)
-            acc[j0 + t][nb] = mfma_bf16(__builtin_bit_cast(bf16x8, f[t]), __builtin_bit_cast(bf16x8, ds[nb]),
-                                       acc[j0 + t][nb]);
-        }
-      }
-    });
-  }
+        for (int nb = 0; nb < 2; ++nb)
+          acc[j0 + t][nb] = mfma_bf16(__builtin_bit_cast(bf16x8, f[t]),
+                                      __builtin_bit_cast(bf16x8, ds[nb]), acc[j0 + t][nb]);
+    }
+  });
 
 #pragma unroll
   for (int nb = 0; nb < 2; ++nb) {
