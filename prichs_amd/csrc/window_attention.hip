@@ -21,37 +21,39 @@ struct Shape {
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Chunk key of a row of a [rows][128] tile in LDS: its 16-byte chunk c is stored at
-// c ^ tile_key(row).  The key is the row's low four bits rotated by one, so that
-// both a fragment read (16 rows, one chunk) and a transposing read (8 rows, two
-// neighbouring chunks each) meet every bank once.
-__device__ __forceinline__ int tile_key(int row) { return ((row << 1) | ((row >> 3) & 1)) & 15; }
+// c ^ tile_key(row).  One key serves both kinds of read without a bank conflict
+// (counted: SQ_LDS_BANK_CONFLICT 0; the row's bits rotated by one double every
+// fragment read): a transposing read takes two neighbouring chunks of 8 rows at a
+// time, whose keys differ above bit 0; a fragment read is served in quarters of 16
+// lanes that pair rows 0-3 and 12-15 of one chunk with rows 4-7 and 8-11 of the
+// next, and each of the two sets of keys is closed under exclusive or with 1.
+__device__ __forceinline__ int tile_key(int row) {
+  return (((row & 7) ^ ((row & 8) >> 1)) << 1) | ((row >> 3) & 1);
+}
 __device__ __forceinline__ int tile_off(int row, int c) { return row * kHd + ((c ^ tile_key(row)) << 3); }
 
-// Four transposing fragments (both halves of a 32-row step, column blocks jd0 ..
-// jd0 + 3), with their wait.  addr: the lane's byte address of column block 0; jd
-// only reaches bits of the chunk that are exclusive-ored anyway.
-template <int LO, int HI>
-__device__ __forceinline__ void read_tr4(uint32_t addr, int jd0, u32x4 (&f)[4]) {
-  u32x2 lo[4], hi[4];
-  const uint32_t a0 = addr ^ (uint32_t)(32 * jd0), a1 = addr ^ (uint32_t)(32 * (jd0 + 1)),
-                 a2 = addr ^ (uint32_t)(32 * (jd0 + 2)), a3 = addr ^ (uint32_t)(32 * (jd0 + 3));
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
-      "ds_read_b64_tr_b16 %2, %9 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
-      "ds_read_b64_tr_b16 %4, %10 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
-      "ds_read_b64_tr_b16 %6, %11 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2]),
-        "=&v"(lo[3]), "=&v"(hi[3])
-      : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(LO), "n"(HI)
-      : "memory");
-#pragma unroll
-  for (int t = 0; t < 4; ++t) f[t] = u32x4{lo[t][0], lo[t][1], hi[t][0], hi[t][1]};
+// A copy of 16 (or 4) bytes a lane to LDS, as dma_16b, in a form whose target the
+// compiler does not see: it would wait for all copies in flight before every
+// transposing read.  There are no result registers; callers wait by vmcnt.
+__device__ __forceinline__ void copy_16b(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t lds_at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds_at),
+               "v"(voff), "s"(r)
+               : "memory", "m0");
 }
+__device__ __forceinline__ void copy_4b(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t lds_at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds_at),
+               "v"(voff), "s"(r)
+               : "memory", "m0");
+}
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+// A transposing fragment: both halves of a 32-row step.
+__device__ __forceinline__ u32x4 read_tr(uint32_t lds_at) {
+  typedef __attribute__((address_space(3))) bf16x4 *at_t;
+  const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((at_t)(uintptr_t)lds_at);
+  const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((at_t)(uintptr_t)(lds_at + 2 * 16 * kHd));
+  return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
 __device__ __forceinline__ void finite_frags(u32x4 (&f)[4]) {
 #pragma unroll
   for (int t = 0; t < 4; ++t)
@@ -97,14 +99,16 @@ struct BwdArgs {
 //                   which is the operand layout of
 //   dQ^T += K^T dS^T              K^T by transposing LDS reads
 // The kernel also forms delta of its rows and leaves it, with lse, to dkv_kernel.
+constexpr int kTr = 32;  // rows of a step of dkv_kernel
 constexpr int kKeys = 64;
 constexpr int kQStage = 2 * kKeys * kHd;  // elements: K, then V
 constexpr int kExactBlocks = 4;  // delta in a sweep of its own up to so many blocks
 constexpr size_t kQLds = 2 * (size_t)kQStage * sizeof(bf16_t);
 
-template <int HPW>
+// NB: 16-row blocks of a wave.
+template <int HPW, int NB>
 __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
-  constexpr int kRowsWg = 128 / HPW;
+  constexpr int kRowsWg = 64 * NB / HPW;
   extern __shared__ __attribute__((aligned(16))) bf16_t lds[];
   const Shape &sh = a.sh;
   const int group = sh.Hq / sh.Hkv, sets = group / HPW;
@@ -114,16 +118,16 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = kvh * group + (blockIdx.x - kvh * sets) * HPW + wave % HPW;
-  const int q0 = qb * kRowsWg + (wave / HPW) * 32;
+  const int q0 = qb * kRowsWg + (wave / HPW) * 16 * NB;
   const int L = rows_of(a.seq_lens, b, sh.S);
   const size_t seq0 = (size_t)b * sh.S;
 
   // This wave's rows: fragments of q and d_o, lse, delta.
-  bf16x8 qf[2][4], df[2][4];
-  float lse2[2], delta[2];
-  float *rows = a.rows + (((size_t)b * sh.Hq + h) * a.row_tiles + q0 / 32) * 64;
+  bf16x8 qf[NB][4], df[NB][4];
+  float lse2[NB], delta[NB];
+  float *rows = a.rows + (((size_t)b * sh.Hq + h) * a.row_tiles + q0 / kTr) * 2 * kTr + q0 % kTr;
 #pragma unroll
-  for (int nb = 0; nb < 2; ++nb) {
+  for (int nb = 0; nb < NB; ++nb) {
     const int row = q0 + 16 * nb + l16;
     const size_t r = seq0 + min(row, sh.S - 1);
     const size_t c = (size_t)h * kHd + 8 * g;
@@ -146,11 +150,11 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
     lse2[nb] = live ? a.lse[((size_t)b * sh.Hq + h) * sh.S + row] * kLog2e : INFINITY;
     delta[nb] = live ? s : 0.f;
   }
-  f32x4 acc[8][2];
+  f32x4 acc[8][NB];
 #pragma unroll
   for (int jd = 0; jd < 8; ++jd)
 #pragma unroll
-    for (int nb = 0; nb < 2; ++nb) acc[jd][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int nb = 0; nb < NB; ++nb) acc[jd][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   // Blocks of 64 keys: the sinks', then from the first row's window on.
   const int q_last = min(L, (qb + 1) * kRowsWg) - 1;
@@ -161,25 +165,25 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
 
   const bf16_t *kbase = a.k + seq0 * a.ldk + (size_t)kvh * kHd;
   const bf16_t *vbase = a.v + seq0 * a.ldv + (size_t)kvh * kHd;
+  const uint32_t lds_base =
+      (uint32_t)(size_t)(const __attribute__((address_space(3))) bf16_t *)lds;
   auto issue_tile = [&](int i, const bf16_t *src, int ld, int tile) {
     const int blk = block_of(i);
     const uint64_t bytes = (uint64_t)(L - 1 - blk * kKeys) * 2 * (uint64_t)ld + 2 * kHd;
     const __amdgpu_buffer_rsrc_t r = buffer_rsrc(
         src + (size_t)blk * kKeys * ld, bytes > 0xffffffffull ? 0xffffffffu : (uint32_t)bytes);
-    bf16_t *dst = lds + (i & 1) * kQStage + tile * kKeys * kHd;
+    const uint32_t dst = lds_base + 2u * (uint32_t)((i & 1) * kQStage + tile * kKeys * kHd);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int row = 16 * wave + 4 * j + g;
-      dma_16b(r, 2u * ((uint32_t)row * (uint32_t)ld + 8u * (uint32_t)(l16 ^ tile_key(row))),
-              dst + (16 * wave + 4 * j) * kHd);
+      copy_16b(r, 2u * ((uint32_t)row * (uint32_t)ld + 8u * (uint32_t)(l16 ^ tile_key(row))),
+               dst + (uint32_t)(2 * (16 * wave + 4 * j) * kHd));
     }
   };
   auto issue = [&](int i) {
     issue_tile(i, kbase, a.ldk, 0);
     issue_tile(i, vbase, a.ldv, 1);
   };
-  const uint32_t lds_base =
-      (uint32_t)(size_t)(const __attribute__((address_space(3))) bf16_t *)lds;
   const uint32_t row_addr = 2u * (uint32_t)tile_off(l16, g);
   const uint32_t tr_addr =
       lds_base + 2u * (uint32_t)(tile_off(4 * g + (l16 >> 2), (l16 & 3) >> 1) + 4 * (l16 & 1));
@@ -196,19 +200,19 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
       if (i + 1 < n_blk) issue(i + 1);
       // Every row of the wave sees the whole block, or none of it.
       const bool whole = kv0 + kKeys <= min(q0 + 1, L) &&
-                         (sh.window == 0 || q0 + 31 - kv0 < sh.window || kv0 + kKeys <= sh.sinks);
-      const bool none = kv0 > q0 + 31 || (sh.window != 0 && q0 - (kv0 + kKeys - 1) >= sh.window &&
+                         (sh.window == 0 || q0 + 16 * NB - 1 - kv0 < sh.window || kv0 + kKeys <= sh.sinks);
+      const bool none = kv0 > q0 + 16 * NB - 1 || (sh.window != 0 && q0 - (kv0 + kKeys - 1) >= sh.window &&
                                           kv0 >= sh.sinks);
       if (none) continue;
       const uint32_t stage = (uint32_t)(i & 1) * (uint32_t)(kQStage * sizeof(bf16_t));
       const char *kt = reinterpret_cast<const char *>(lds) + stage;
       static_for<2>([&](auto half_c) {
         constexpr int half = decltype(half_c)::value;  // keys 32 half ..
-        f32x4 s[2][2], dp[2][2];
+        f32x4 s[2][NB], dp[2][NB];
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int nb = 0; nb < 2; ++nb) s[c][nb] = dp[c][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int nb = 0; nb < NB; ++nb) s[c][nb] = dp[c][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
@@ -217,7 +221,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
             const bf16x8 kf = *reinterpret_cast<const bf16x8 *>(p);
             const bf16x8 vf = *reinterpret_cast<const bf16x8 *>(p + 2 * kKeys * kHd);
 #pragma unroll
-            for (int nb = 0; nb < 2; ++nb) {
+            for (int nb = 0; nb < NB; ++nb) {
               s[c][nb] = mfma_bf16(kf, qf[nb][kk], s[c][nb]);
               dp[c][nb] = mfma_bf16(vf, df[nb][kk], dp[c][nb]);
             }
@@ -231,7 +235,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int nb = 0; nb < 2; ++nb) {
+            for (int nb = 0; nb < NB; ++nb) {
               z = not_finite(s[c][nb], z);
               const int row = q0 + 16 * nb + l16, key = kv0 + 32 * half + 16 * c + 4 * g;
 #pragma unroll
@@ -256,10 +260,10 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
   // their norm at 2 keys, 0.0027 at 8, 0.0025 at 64).  Rows of few blocks form it as
   // sum p dP / sum p instead, in a sweep of their own (2 of the 3 products again).
   if (n_blk > 0 && n_blk <= kExactBlocks) {
-    float num[2] = {0.f, 0.f}, den[2] = {0.f, 0.f};
-    sweep([&](auto, uint32_t, f32x4 (&s)[2][2], f32x4 (&dp)[2][2], bool) {
+    float num[NB] = {}, den[NB] = {};
+    sweep([&](auto, uint32_t, f32x4 (&s)[2][NB], f32x4 (&dp)[2][NB], bool) {
 #pragma unroll
-      for (int nb = 0; nb < 2; ++nb)
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -270,7 +274,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
           }
     });
 #pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
+    for (int nb = 0; nb < NB; ++nb) {
       num[nb] += __shfl_xor(num[nb], 16);
       den[nb] += __shfl_xor(den[nb], 16);
       num[nb] += __shfl_xor(num[nb], 32);
@@ -280,17 +284,17 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
     asm volatile("s_barrier" ::: "memory");  // the last block's readers, before it is refilled
   }
 #pragma unroll
-  for (int nb = 0; nb < 2; ++nb)
-    if (g == 0 && q0 < a.row_tiles * 32) {
+  for (int nb = 0; nb < NB; ++nb)
+    if (g == 0 && q0 < a.row_tiles * kTr) {
       rows[16 * nb + l16] = lse2[nb];
-      rows[32 + 16 * nb + l16] = delta[nb];
+      rows[kTr + 16 * nb + l16] = delta[nb];
     }
 
-  sweep([&](auto half_c, uint32_t stage, f32x4 (&s)[2][2], f32x4 (&dp)[2][2], bool rare) {
+  sweep([&](auto half_c, uint32_t stage, f32x4 (&s)[2][NB], f32x4 (&dp)[2][NB], bool rare) {
     constexpr int half = decltype(half_c)::value;
-    u32x4 ds[2];
+    u32x4 ds[NB];
 #pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
+    for (int nb = 0; nb < NB; ++nb) {
       float e[8];
 #pragma unroll
       for (int c = 0; c < 2; ++c)
@@ -305,19 +309,21 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
 #pragma unroll
     for (int j0 = 0; j0 < 8; j0 += 4) {
       u32x4 f[4];
-      read_tr4<2 * 32 * half * kHd, 2 * (32 * half + 16) * kHd>(tr_addr + stage, j0, f);
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        f[t] = read_tr(((tr_addr + stage) ^ (uint32_t)(32 * (j0 + t))) + 2 * 32 * half * kHd);
       if (rare) finite_frags(f);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int nb = 0; nb < 2; ++nb)
+        for (int nb = 0; nb < NB; ++nb)
           acc[j0 + t][nb] = mfma_bf16(__builtin_bit_cast(bf16x8, f[t]),
                                       __builtin_bit_cast(bf16x8, ds[nb]), acc[j0 + t][nb]);
     }
   });
 
 #pragma unroll
-  for (int nb = 0; nb < 2; ++nb) {
+  for (int nb = 0; nb < NB; ++nb) {
     const int row = q0 + 16 * nb + l16;
     if (row >= sh.S) continue;
     bf16_t *out = a.dq + (seq0 + row) * a.lddq + (size_t)h * kHd + 4 * g;
@@ -346,11 +352,12 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
 // every later row); the items of one block meet in f32 partial sums that
 // dkv_join_kernel adds in order.
 constexpr int kBlk = 128;                       // keys of a workgroup
-constexpr int kTr = 32;                         // rows of a step
+constexpr int kKb = 1;                          // 16-key blocks of a wave
+constexpr int kKg = kBlk / (16 * kKb);          // key groups
 constexpr int kStages = 3;
 constexpr int kStepElems = 2 * kTr * kHd + 128; // q, d_o, then lse / delta (64 floats)
-constexpr size_t kKvLds = 2 * kStages * (size_t)kStepElems * sizeof(bf16_t);
-static_assert(kKvLds >= 4 * 64 * 64 * sizeof(float), "the join of the step groups fits");
+constexpr size_t kKvLds = (2 * kStages * (size_t)kStepElems + kBlk * kHd) * sizeof(bf16_t);
+static_assert(kKvLds >= kKg * 8 * kKb * 64 * sizeof(f32x4), "the join of the step groups fits");
 
 // Steps of key block j over sequences of S rows.
 __host__ __device__ inline int steps_of(const Shape &sh, int rows, int j) {
@@ -386,7 +393,7 @@ __device__ __forceinline__ void item_at(const Shape &sh, int budget, int item, i
   *block = blocks - 1, *split = 0;  // not reached: the grid holds the items
 }
 
-__global__ __launch_bounds__(512, 2) void window_dkv_kernel(BwdArgs a) {
+__global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
   extern __shared__ __attribute__((aligned(16))) bf16_t lds[];
   const Shape &sh = a.sh;
   const int G = sh.Hq / sh.Hkv;
@@ -397,32 +404,28 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(BwdArgs a) {
   const int n_split = splits_of(sh, a.budget, blk);
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kg = wave & 3, sg = wave >> 2;
+  const int kg = wave % kKg, sg = wave / kKg;
   const int L = rows_of(a.seq_lens, b, sh.S);
   const size_t seq0 = (size_t)b * sh.S;
-  const int k0 = blk * kBlk + 32 * kg;  // this wave's first key
+  const int k0 = blk * kBlk + 16 * kg;  // this wave's first key
 
-  bf16x8 kf[2][4], vf[2][4];
-  f32x4 dk[8][2], dv[8][2];
-#pragma unroll
-  for (int kb = 0; kb < 2; ++kb) {
-    const int key = k0 + 16 * kb + l16;
+  bf16x8 kf[4];
+  f32x4 dk[8], dv[8];
+{
+    const int key = k0 + l16;
     const size_t r = seq0 + min(key, sh.S - 1), c = (size_t)kvh * kHd + 8 * g;
     const bool live = key < L;
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
       u32x4 x = *reinterpret_cast<const u32x4 *>(a.k + r * a.ldk + c + 32 * kk);
-      u32x4 y = *reinterpret_cast<const u32x4 *>(a.v + r * a.ldv + c + 32 * kk);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = live ? x[e] : 0u, y[e] = live ? y[e] : 0u;
-      kf[kb][kk] = __builtin_bit_cast(bf16x8, x);
-      vf[kb][kk] = __builtin_bit_cast(bf16x8, y);
+      for (int e = 0; e < 4; ++e) x[e] = live ? x[e] : 0u;
+      kf[kk] = __builtin_bit_cast(bf16x8, x);
     }
   }
 #pragma unroll
   for (int jd = 0; jd < 8; ++jd)
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) dk[jd][kb] = dv[jd][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    dk[jd] = dv[jd] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   // This item's steps: step x is head x / tiles, row tile t_lo + x % tiles.
   const int steps = steps_of(sh, L, blk), tiles = steps / G;
@@ -431,126 +434,153 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(BwdArgs a) {
   const int t_lo = blk * (kBlk / kTr);
   const int n_it = (end - begin + 1) / 2;
 
-  // The step to fetch next, and the one to compute.
-  int fx = begin + sg, fh = tiles > 0 ? fx / tiles : 0, ft = fx - fh * tiles;
-  int cx = fx, ch = fh, ct = ft;
-  auto advance = [&](int &x, int &hh, int &t) {
-    x += 2;
-    t += 2;
-    while (t >= tiles && tiles > 0) {
-      t -= tiles;
-      ++hh;
-    }
+  // The step to compute next: its number and row tile.
+  int cx = begin + sg, ct = tiles > 0 ? cx % tiles : 0;
+  // The step to fetch next: where its rows of q and d_o start, how many bytes the
+  // sequence has from there on (past them a copy gives zeros), and its statistics.
+  int fx = cx, ft = ct, fh = tiles > 0 ? cx / tiles : 0;
+  const char *pq, *pd;
+  const float *pr;
+  int64_t lq, ld;
+  auto seek = [&]() {
+    const int h = kvh * G + fh, t0 = (t_lo + ft) * kTr;
+    pq = reinterpret_cast<const char *>(a.q + (seq0 + t0) * a.ldq + (size_t)h * kHd);
+    pd = reinterpret_cast<const char *>(a.d_o + (seq0 + t0) * a.ldd + (size_t)h * kHd);
+    lq = (int64_t)(L - 1 - t0) * 2 * a.ldq + 2 * kHd;
+    ld = (int64_t)(L - 1 - t0) * 2 * a.ldd + 2 * kHd;
+    pr = a.rows + (((size_t)b * sh.Hq + h) * a.row_tiles + t_lo + ft) * 64;
   };
+  seek();
+  const uint32_t lds_base =
+      (uint32_t)(size_t)(const __attribute__((address_space(3))) bf16_t *)lds;
+  // V of the block, behind the steps' tiles.
+  const uint32_t v_tile = 2 * kStages * kStepElems * 2u;
+  {
+    const int left = L - blk * kBlk;
+    const uint64_t bytes = (uint64_t)(left - 1) * 2 * (uint64_t)a.ldv + 2 * kHd;
+    const __amdgpu_buffer_rsrc_t r = buffer_rsrc(
+        a.v + (seq0 + (left > 0 ? blk * kBlk : 0)) * a.ldv + (size_t)kvh * kHd,
+        left <= 0 ? 0u : bytes > 0xffffffffull ? 0xffffffffu : (uint32_t)bytes);
+#pragma unroll
+    for (int j = 0; j < kBlk / (8 * kKg); ++j) {
+      const int x = kBlk / (2 * kKg) * wave + 4 * j + g;
+      copy_16b(r, 2u * ((uint32_t)x * (uint32_t)a.ldv + 8u * (uint32_t)(l16 ^ tile_key(x))),
+               lds_base + v_tile + (uint32_t)(2 * (kBlk / (2 * kKg) * wave + 4 * j) * kHd));
+    }
+  }
   // Every wave of a step group moves 8 of the step's rows of q and of d_o, and all
   // of lse / delta (the same bytes): 5 copies.  A step past the end copies nothing
   // (an empty buffer: zeros), so that the count of copies in flight stays known.
+  constexpr int kRowsEach = kTr / kKg, kCopies = kRowsEach / 2 + 1;
   auto fetch = [&](int slot) {
-    bf16_t *dst = lds + (sg * kStages + slot) * kStepElems;
+    const uint32_t dst = lds_base + (uint32_t)((sg * kStages + slot) * kStepElems) * 2u;
     const bool on = fx < end;
-    const int h = kvh * G + fh, t0 = (t_lo + ft) * kTr;
     const int ln = lane_here();
-    const size_t row = seq0 + t0;
-    auto rows = [&](const bf16_t *src, int ld, int at) {
-      const uint64_t bytes = (uint64_t)(L - 1 - t0) * 2 * (uint64_t)ld + 2 * kHd;
+    auto rows = [&](const char *src, int64_t left, int pitch, int at) {
       const __amdgpu_buffer_rsrc_t r =
-          buffer_rsrc(on ? src + row * ld + (size_t)h * kHd : src,
-                      !on ? 0u : bytes > 0xffffffffull ? 0xffffffffu : (uint32_t)bytes);
+          buffer_rsrc(src, !on ? 0u : left > 0xffffffffll ? 0xffffffffu : (uint32_t)left);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int x = 8 * kg + 4 * j + (ln >> 4);
-        dma_16b(r, 2u * ((uint32_t)x * (uint32_t)ld + 8u * (uint32_t)((ln & 15) ^ tile_key(x))),
-                dst + at + (8 * kg + 4 * j) * kHd);
+      for (int j = 0; j < kRowsEach / 4; ++j) {
+        const int x = kRowsEach * kg + 4 * j + (ln >> 4);
+        copy_16b(r, 2u * ((uint32_t)x * (uint32_t)pitch + 8u * (uint32_t)((ln & 15) ^ tile_key(x))),
+                 dst + (uint32_t)(2 * (at + (kRowsEach * kg + 4 * j) * kHd)));
       }
     };
-    rows(a.q, a.ldq, 0);
-    rows(a.d_o, a.ldd, kTr * kHd);
-    const __amdgpu_buffer_rsrc_t r = buffer_rsrc(
-        on ? a.rows + (((size_t)b * sh.Hq + h) * a.row_tiles + t_lo + ft) * 64 : a.rows,
-        on ? 256u : 0u);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(
-        r, (__attribute__((address_space(3))) void *)(dst + 2 * kTr * kHd), 4, 4u * (uint32_t)ln,
-        0, 0, 0);
-    advance(fx, fh, ft);
+    rows(pq, lq, a.ldq, 0);
+    rows(pd, ld, a.ldd, kTr * kHd);
+    copy_4b(buffer_rsrc(pr, on ? 256u : 0u), 4u * (uint32_t)ln, dst + 4 * kTr * kHd);
+    fx += 2;
+    ft += 2;
+    if (ft < tiles) {
+      pq += 4 * kTr * (int64_t)a.ldq, lq -= 4 * kTr * (int64_t)a.ldq;
+      pd += 4 * kTr * (int64_t)a.ldd, ld -= 4 * kTr * (int64_t)a.ldd;
+      pr += 2 * 64;
+    } else if (tiles > 0) {
+      while (ft >= tiles) ft -= tiles, ++fh;
+      seek();
+    }
   };
 
-  const uint32_t lds_base =
-      (uint32_t)(size_t)(const __attribute__((address_space(3))) bf16_t *)lds;
-
+  const uint32_t ra0 = 2u * (uint32_t)tile_off(l16, g);
+  const uint32_t ta0 = 2u * (uint32_t)(tile_off(4 * g + (l16 >> 2), (l16 & 3) >> 1) + 4 * (l16 & 1));
   auto compute = [&](int slot) {
     const int t0 = (t_lo + ct) * kTr;
     const bool none = cx >= end || k0 >= L || t0 + kTr - 1 < k0 ||
-                      (sh.window != 0 && t0 - (k0 + 31) >= sh.window && k0 >= sh.sinks);
+                      (sh.window != 0 && t0 - (k0 + 16 - 1) >= sh.window && k0 >= sh.sinks);
     if (none) return;
-    const bool whole = t0 >= k0 + 31 && (sh.window == 0 || t0 + kTr - 1 - k0 < sh.window ||
-                                         k0 + 32 <= sh.sinks);
+    const bool whole = t0 >= k0 + 16 - 1 && (sh.window == 0 || t0 + kTr - 1 - k0 < sh.window ||
+                                         k0 + 16 <= sh.sinks);
     const uint32_t at = (uint32_t)((sg * kStages + slot) * kStepElems) * 2u;
     const char *tile = reinterpret_cast<const char *>(lds) + at;
-    const int ln = lane_here(), g = ln >> 4, l16 = ln & 15;
-    const uint32_t ra = at + 2u * (uint32_t)tile_off(l16, g);
-    const uint32_t ta = lds_base + at + 2u * (uint32_t)(tile_off(4 * g + (l16 >> 2), (l16 & 3) >> 1) +
-                                                        4 * (l16 & 1));
-    u32x4 pf[2], ds[2];  // P and dS rounded to bf16 for the products
+    const uint32_t ra = at + ra0, ta = lds_base + at + ta0;
+    auto frag_at = [&](uint32_t lane_at, int kk, uint32_t off) {
+      return *reinterpret_cast<const bf16x8 *>(reinterpret_cast<const char *>(lds) +
+                                               (lane_at ^ (uint32_t)(64 * kk)) + off);
+    };
+    // x is 0 where the key's row does not see it.
+    auto hide = [&](int qb, f32x4 &x) {
+      int row = t0 + 16 * qb + 4 * g;
+      asm volatile("" : "+v"(row));  // keeps this in the branches that call it
+      const int key = k0 + l16;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool seen = (key <= row + r) & ((sh.window == 0) | (row + r - key < sh.window) |
+                                              (key < sh.sinks));
+        x[r] = seen ? x[r] : 0.f;
+      }
+    };
+    u32x4 pf, ds;  // P and dS rounded to bf16 for the products
     float z = 0.f;
+    f32x4 p[2], x[2];  // of 16 rows each
+    x[0] = x[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb)
+        x[qb] = mfma_bf16(frag_at(ra, kk, 2 * kHd * 16 * qb), kf[kk], x[qb]);
+    const float *st = reinterpret_cast<const float *>(tile + 4 * kTr * kHd) + 4 * g;
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
-      // One block of 16 rows after the other, S before dP: registers.
-      auto product = [&](f32x4 (&x)[2], const bf16x8 (&f)[2][4], int off) {
-        x[0] = x[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const f32x4 lse2 = *reinterpret_cast<const f32x4 *>(st + 16 * qb);
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          const bf16x8 rf = *reinterpret_cast<const bf16x8 *>(
-              reinterpret_cast<const char *>(lds) + (ra ^ (uint32_t)(64 * kk)) + off +
-              2 * kHd * 16 * qb);
+      for (int r = 0; r < 4; ++r) p[qb][r] = fast_exp2(fmaf(x[qb][r], sh.scale_log2, -lse2[r]));
+    }
+    // What a key's row does not see must not reach the key, whatever the row holds: p
+    // and dS are 0 there, and see rare below.
+    if (!whole) {
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb) x[kb] = mfma_bf16(rf, f[kb][kk], x[kb]);
-        }
-      };
-      // x is 0 where the key's row does not see it.
-      auto hide = [&](int kb, f32x4 &x) {
-        int row = t0 + 16 * qb + 4 * g;
-        asm volatile("" : "+v"(row));  // keeps this in the branches that call it
-        const int key = k0 + 16 * kb + l16;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const bool seen = (key <= row + r) & ((sh.window == 0) | (row + r - key < sh.window) |
-                                                (key < sh.sinks));
-          x[r] = seen ? x[r] : 0.f;
-        }
-      };
-      const float *st = reinterpret_cast<const float *>(tile + 4 * kTr * kHd) + 16 * qb + 4 * g;
-      f32x4 p[2], x[2];
-      product(x, kf, 0);
-      {
-        const f32x4 lse2 = *reinterpret_cast<const f32x4 *>(st);
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) p[kb][r] = fast_exp2(fmaf(x[kb][r], sh.scale_log2, -lse2[r]));
-          // What a key's row does not see must not reach the key, whatever the row
-          // holds: p and dS are 0 there, and see rare below.
-          if (!whole) {
-            z = not_finite(x[kb], z);
-            hide(kb, p[kb]);
-          }
-          pf[kb][2 * qb] = pack_bf16(p[kb][0], p[kb][1]);
-          pf[kb][2 * qb + 1] = pack_bf16(p[kb][2], p[kb][3]);
-        }
+      for (int qb = 0; qb < 2; ++qb) {
+        z = not_finite(x[qb], z);
+        hide(qb, p[qb]);
       }
-      product(x, vf, 2 * kTr * kHd);
-      const f32x4 delta = *reinterpret_cast<const f32x4 *>(st + kTr);
+    }
+    x[0] = x[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const uint32_t va = ra0 + v_tile + 2 * kHd * 16 * kg;
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        f32x4 e;
+    for (int kk = 0; kk < 4; ++kk) {
+      const bf16x8 vf = frag_at(va, kk, 0);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) e[r] = p[kb][r] * (x[kb][r] - delta[r]);
-        if (!whole) {
-          z = not_finite(x[kb], z);
-          hide(kb, e);
-        }
-        ds[kb][2 * qb] = pack_bf16(e[0], e[1]);
-        ds[kb][2 * qb + 1] = pack_bf16(e[2], e[3]);
+      for (int qb = 0; qb < 2; ++qb)
+        x[qb] = mfma_bf16(frag_at(ra, kk, 2 * kTr * kHd + 2 * kHd * 16 * qb), vf, x[qb]);
+    }
+    f32x4 e[2];
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      const f32x4 delta = *reinterpret_cast<const f32x4 *>(st + kTr + 16 * qb);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) e[qb][r] = p[qb][r] * (x[qb][r] - delta[r]);
+    }
+    if (!whole) {
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) {
+        z = not_finite(x[qb], z);
+        hide(qb, e[qb]);
       }
+    }
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      pf[2 * qb] = pack_bf16(p[qb][0], p[qb][1]), pf[2 * qb + 1] = pack_bf16(p[qb][2], p[qb][3]);
+      ds[2 * qb] = pack_bf16(e[qb][0], e[qb][1]), ds[2 * qb + 1] = pack_bf16(e[qb][2], e[qb][3]);
     }
     // An infinity or NaN of q or d_o, which 0 would turn into NaN, is taken out of
     // the products of a step that not every key's row sees.
@@ -559,23 +589,21 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(BwdArgs a) {
 #pragma unroll
     for (int j0 = 0; j0 < 8; j0 += 4) {
       u32x4 f[4];
-      read_tr4<kDo, kDo + 2 * 16 * kHd>(ta, j0, f);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) f[t] = read_tr((ta ^ (uint32_t)(32 * (j0 + t))) + kDo);
       if (rare) finite_frags(f);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-          dv[j0 + t][kb] = mfma_bf16(__builtin_bit_cast(bf16x8, f[t]), __builtin_bit_cast(bf16x8, pf[kb]),
-                                     dv[j0 + t][kb]);
+          dv[j0 + t] = mfma_bf16(__builtin_bit_cast(bf16x8, f[t]), __builtin_bit_cast(bf16x8, pf),
+                                     dv[j0 + t]);
       }
-      read_tr4<0, 2 * 16 * kHd>(ta, j0, f);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) f[t] = read_tr(ta ^ (uint32_t)(32 * (j0 + t)));
       if (rare) finite_frags(f);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-          dk[j0 + t][kb] = mfma_bf16(__builtin_bit_cast(bf16x8, f[t]), __builtin_bit_cast(bf16x8, ds[kb]),
-                                     dk[j0 + t][kb]);
+          dk[j0 + t] = mfma_bf16(__builtin_bit_cast(bf16x8, f[t]), __builtin_bit_cast(bf16x8, ds),
+                                     dk[j0 + t]);
       }
     }
     if (rare) {
@@ -590,16 +618,15 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(BwdArgs a) {
           asm volatile("" ::: "memory");  // one load after the other: registers
           const u32x2 raw = *reinterpret_cast<const u32x2 *>(
               tile + kDo + ((uint32_t)(2 * (tile_off(x, g >> 1) + 4 * (g & 1))) ^ (32u * jd)));
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb) {
-            const int key = k0 + 16 * kb + l16;
+{
+            const int key = k0 + l16;
             const bool seen = (key <= row) & ((sh.window == 0) | (row - key < sh.window) |
                                               (key < sh.sinks));
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const uint32_t u = r & 1 ? raw[r / 2] & 0xffff0000u : raw[r / 2] << 16;
               const bool off = (u & 0x7f800000u) == 0x7f800000u;
-              dv[jd][kb][r] += (off & seen) ? __uint_as_float(u) : 0.f;
+              dv[jd][r] += (off & seen) ? __uint_as_float(u) : 0.f;
             }
           }
         }
@@ -614,10 +641,11 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(BwdArgs a) {
   for (int it = 0; it < n_it; ++it) {
     // Of the copies in flight only the newest kStages - 2 steps' may be missing;
     // every wave is done with the slot that is fetched into next.
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(5 * (kStages - 2)) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(kCopies * (kStages - 2)) : "memory");
     fetch(slot == 0 ? kStages - 1 : slot - 1);
     compute(slot);
-    advance(cx, ch, ct);
+    cx += 2, ct += 2;
+    while (ct >= tiles) ct -= tiles;
     slot = slot + 1 == kStages ? 0 : slot + 1;
   }
   // The copies past the end write zeros: they must land before LDS is used again.
@@ -626,20 +654,17 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(BwdArgs a) {
   // The second step group's sums join the first's, d_k then d_v.
   const int le = lane_here(), ge = le >> 4, l16e = le & 15;
   f32x4 *join = reinterpret_cast<f32x4 *>(lds);
-  auto joined = [&](f32x4 (&x)[8][2]) {
+  auto joined = [&](f32x4 (&x)[8]) {
     if (sg == 1) {
 #pragma unroll
       for (int jd = 0; jd < 8; ++jd)
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) join[((2 * jd + kb) * 4 + kg) * 64 + le] = x[jd][kb];
+join[((jd) * kKg + kg) * 64 + le] = x[jd];
     }
     __syncthreads();
     if (sg == 0) {
 #pragma unroll
       for (int jd = 0; jd < 8; ++jd)
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-          x[jd][kb] = x[jd][kb] + join[((2 * jd + kb) * 4 + kg) * 64 + le];
+          x[jd] = x[jd] + join[((jd) * kKg + kg) * 64 + le];
     }
     __syncthreads();
   };
@@ -648,27 +673,25 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(BwdArgs a) {
   if (sg != 0) return;
   if (n_split > 1) {
     float *part = a.part + ((((size_t)b * sh.Hkv + kvh) * gridDim.x + blockIdx.x) * 2) * kBlk * kHd;
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      float *row = part + (32 * kg + 16 * kb + l16e) * kHd + 4 * ge;
+{
+      float *row = part + (16 * kg + l16e) * kHd + 4 * ge;
 #pragma unroll
       for (int jd = 0; jd < 8; ++jd) {
-        *reinterpret_cast<f32x4 *>(row + 16 * jd) = dk[jd][kb];
-        *reinterpret_cast<f32x4 *>(row + kBlk * kHd + 16 * jd) = dv[jd][kb];
+        *reinterpret_cast<f32x4 *>(row + 16 * jd) = dk[jd];
+        *reinterpret_cast<f32x4 *>(row + kBlk * kHd + 16 * jd) = dv[jd];
       }
     }
     return;
   }
-#pragma unroll
-  for (int kb = 0; kb < 2; ++kb) {
-    const int key = k0 + 16 * kb + l16e;
-    if (key >= sh.S) continue;
+{
+    const int key = k0 + l16e;
+    if (key >= sh.S) return;
     bf16_t *ok = a.dk + (seq0 + key) * a.lddk + (size_t)kvh * kHd + 4 * ge;
     bf16_t *ov = a.dv + (seq0 + key) * a.lddv + (size_t)kvh * kHd + 4 * ge;
     const bool live = key < L;
 #pragma unroll
     for (int jd = 0; jd < 8; ++jd) {
-      const f32x4 x = dk[jd][kb] * sh.scale, y = dv[jd][kb];
+      const f32x4 x = dk[jd] * sh.scale, y = dv[jd];
       const u32x2 ux = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
       const u32x2 uy = u32x2{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])};
       *reinterpret_cast<u32x2 *>(ok + 16 * jd) = live ? ux : u32x2{0, 0};
@@ -681,14 +704,14 @@ __global__ __launch_bounds__(512, 2) void window_dkv_kernel(BwdArgs a) {
 // (block, kv head, sequence) and 16 of its keys.
 __global__ __launch_bounds__(256) void window_dkv_join_kernel(BwdArgs a, int items) {
   const Shape &sh = a.sh;
-  const int blk = blockIdx.x / 8, kvh = blockIdx.y, b = blockIdx.z;
+  const int blk = blockIdx.x / (kBlk / 16), kvh = blockIdx.y, b = blockIdx.z;
   const int n_split = splits_of(sh, a.budget, blk);
   if (n_split == 1) return;
   int item = 0;  // the block's first
   const int lane = threadIdx.x & 63;
   for (int j = lane; j < blk; j += 64) item += splits_of(sh, a.budget, j);
   for (int m = 1; m < 64; m <<= 1) item += __shfl_xor(item, m);
-  const int key = 16 * (blockIdx.x % 8) + (threadIdx.x >> 4), d = 8 * (threadIdx.x & 15);
+  const int key = 16 * (blockIdx.x % (kBlk / 16)) + (threadIdx.x >> 4), d = 8 * (threadIdx.x & 15);
   const int row = blk * kBlk + key;
   if (row >= sh.S) return;
   const bool live = row < rows_of(a.seq_lens, b, sh.S);
@@ -886,7 +909,9 @@ extern "C" int prichs_window_attention_backward(
                  "%s: the workspace must be 16-byte aligned device memory", who);
   const int group = (int)(n_heads / n_kv_heads);
   const int hpw = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
-  const size_t n_qb = cdiv(seq_len, (size_t)(128 / hpw)), blocks = cdiv(seq_len, (size_t)kBlk);
+  const size_t blocks = cdiv(seq_len, (size_t)kBlk), n_qb32 = cdiv(seq_len, (size_t)(128 / hpw));
+  const bool few = 2 * (n_heads / hpw) * batch * n_qb32 <= 3 * 256;
+  const size_t n_qb = few ? cdiv(seq_len, (size_t)(64 / hpw)) : n_qb32;
   PRICHS_REQUIRE(n_qb <= 65535 && n_kv_heads <= 65535, "%s: shape too large", who);
   const auto bf = [](const void *p) { return static_cast<const bf16_t *>(p); };
   const auto out = [](void *p) { return static_cast<bf16_t *>(p); };
@@ -894,20 +919,24 @@ extern "C" int prichs_window_attention_backward(
             (int)ldd, (int)ldq, (int)ldk, (int)ldv, (int)ldo, (int)lddq, (int)lddk, (int)lddv,
             static_cast<float *>(workspace), (int)cdiv(seq_len, (size_t)kTr),
             reinterpret_cast<float *>(static_cast<char *>(workspace) + stats), plan.budget, sh};
-  auto dq_kern = hpw == 4 ? window_dq_kernel<4> : hpw == 2 ? window_dq_kernel<2>
-                                                           : window_dq_kernel<1>;
+  auto dq_kern = few ? (hpw == 4   ? window_dq_kernel<4, 1>
+                        : hpw == 2 ? window_dq_kernel<2, 1>
+                                   : window_dq_kernel<1, 1>)
+                     : (hpw == 4   ? window_dq_kernel<4, 2>
+                        : hpw == 2 ? window_dq_kernel<2, 2>
+                                   : window_dq_kernel<1, 2>);
   hipLaunchKernelGGL(dq_kern, dim3((unsigned)(n_heads / hpw), (unsigned)batch, (unsigned)n_qb),
                      dim3(256), kQLds, as_stream(stream), a);
   PRICHS_LAUNCH_CHECK("window_attention_backward d_q launch");
   static LdsLimit limit;
   WINDOW_TRY(raise_lds_limit(limit, reinterpret_cast<const void *>(window_dkv_kernel), kKvLds, who));
   hipLaunchKernelGGL(window_dkv_kernel,
-                     dim3((unsigned)plan.items, (unsigned)n_kv_heads, (unsigned)batch), dim3(512),
+                     dim3((unsigned)plan.items, (unsigned)n_kv_heads, (unsigned)batch), dim3(128 * kKg),
                      kKvLds, as_stream(stream), a);
   PRICHS_LAUNCH_CHECK("window_attention_backward d_k / d_v launch");
   if (plan.cut) {
     hipLaunchKernelGGL(window_dkv_join_kernel,
-                       dim3((unsigned)(8 * blocks), (unsigned)n_kv_heads, (unsigned)batch),
+                       dim3((unsigned)(kBlk / 16 * blocks), (unsigned)n_kv_heads, (unsigned)batch),
                        dim3(256), 0, as_stream(stream), a, (int)plan.items);
     PRICHS_LAUNCH_CHECK("window_attention_backward join launch");
   }
