@@ -298,24 +298,26 @@ def attention(q, k, v, batch, seq_len, n_heads, n_kv_heads, head_dim=128, out=No
 
 
 # ---------------------------------------- window attention and KV cache ----
-def _rows(t, name, rows, cols, dtypes=(torch.bfloat16,)):
-    """A device operand of at least `rows` rows whose columns are contiguous."""
+_BF16 = (torch.bfloat16,)
+_FLOATS = (torch.bfloat16, torch.float32)
+
+
+def _rows(t, name, rows, cols, dtypes=_BF16):
+    """Checks an operand of at least `rows` rows whose columns are contiguous and
+    returns its row stride (of a single row its width, whatever torch keeps)."""
     if t.dtype not in dtypes:
         raise TypeError(f"{name}: unsupported dtype {t.dtype}")
-    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] != cols:
-        raise ValueError(f"{name}: expected [{rows}, {cols}], got {list(t.shape)}")
-    if t.stride(1) != 1:
+    shape = t.shape
+    if len(shape) != 2 or shape[0] < rows or shape[1] != cols:
+        raise ValueError(f"{name}: expected [{rows}, {cols}], got {list(shape)}")
+    ld, unit = t.stride()
+    if unit != 1:
         raise ValueError(f"{name}: operands need unit column stride")
-    return t
+    return ld if shape[0] > 1 else cols
 
 
 def _a(t):
     return None if t is None else t.data_ptr()
-
-
-def _ld(t):
-    """Row stride; of a single row its width, whatever stride torch keeps for it."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _i32(t, name, n, dim=1):
@@ -349,10 +351,8 @@ def window_attention(q, k, v, batch, seq_len, n_heads, n_kv_heads, window, sinks
     sees its last `window` keys, itself included (0: all earlier ones), and the
     first `sinks` keys.  seq_lens: int32 device [batch], the rows of each sequence
     of a padded batch.  -> (out, lse f32 [batch, n_heads, seq_len], or None)."""
-    lib = L.load()
     rows, H, K = batch * seq_len, n_heads * head_dim, n_kv_heads * head_dim
-    for t, name, cols in ((q, "q", H), (k, "k", K), (v, "v", K)):
-        _rows(t, name, rows, cols)
+    ldq, ldk, ldv = _rows(q, "q", rows, H), _rows(k, "k", rows, K), _rows(v, "v", rows, K)
     if seq_lens is not None:
         _i32(seq_lens, "seq_lens", batch)
     if window < 0 or sinks < 0:
@@ -361,13 +361,14 @@ def window_attention(q, k, v, batch, seq_len, n_heads, n_kv_heads, window, sinks
     with ctx:
         if out is None:
             out = torch.empty((rows, H), dtype=q.dtype, device=q.device)
-        _rows(out, "out", rows, H)
+        ldo = _rows(out, "out", rows, H)
         lse = None
         if want_lse:
             lse = torch.empty((batch, n_heads, seq_len), dtype=torch.float32, device=q.device)
-        L.check(lib.prichs_window_attention_forward(
-            _a(q), _ld(q), _a(k), _ld(k), _a(v), _ld(v), _a(out), _ld(out), _a(lse), _a(seq_lens),
-            batch, seq_len, n_heads, n_kv_heads, head_dim, window, sinks, dtype_code(q), s))
+        L.check(L.load().prichs_window_attention_forward(
+            q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo, _a(lse),
+            _a(seq_lens), batch, seq_len, n_heads, n_kv_heads, head_dim, window, sinks,
+            L.DTYPE_BF16, s))
     return out, lse
 
 
@@ -380,9 +381,11 @@ def window_attention_backward(d_out, q, k, v, out, lse, batch, seq_len, n_heads,
     overlap the operands."""
     lib = L.load()
     rows, H, K = batch * seq_len, n_heads * head_dim, n_kv_heads * head_dim
+    args = []
     for t, name, cols in ((d_out, "d_out", H), (q, "q", H), (k, "k", K), (v, "v", K),
                           (out, "out", H)):
-        _rows(t, name, rows, cols)
+        ld = _rows(t, name, rows, cols)
+        args += (t.data_ptr(), ld)
     if lse is None or lse.dtype != torch.float32 or not lse.is_contiguous() or \
             lse.shape != (batch, n_heads, seq_len):
         raise ValueError("lse: expected the contiguous f32 [batch, n_heads, seq_len] of "
@@ -393,19 +396,19 @@ def window_attention_backward(d_out, q, k, v, out, lse, batch, seq_len, n_heads,
         raise ValueError("window and sinks must not be negative")
     ctx, s = _launch_on(stream, d_out, q, k, v, out, lse, seq_lens, d_q, d_k, d_v)
     with ctx:
-        grads = []
+        grads, to = [], []
         for t, name, cols in ((d_q, "d_q", H), (d_k, "d_k", K), (d_v, "d_v", K)):
             if t is None:
                 t = torch.empty((rows, cols), dtype=q.dtype, device=q.device)
-            grads.append(_rows(t, name, rows, cols))
-        ws = torch.empty((lib.prichs_window_attention_backward_workspace(
-            batch, seq_len, n_heads, n_kv_heads, window, sinks),), dtype=torch.uint8,
-            device=q.device)
-        args = [x for t in (d_out, q, k, v, out) for x in (_a(t), _ld(t))]
+            ld = _rows(t, name, rows, cols)
+            grads.append(t)
+            to += (t.data_ptr(), ld)
+        need = lib.prichs_window_attention_backward_workspace(batch, seq_len, n_heads, n_kv_heads,
+                                                              window, sinks)
+        ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
         L.check(lib.prichs_window_attention_backward(
-            *args, _a(lse), _a(seq_lens), *[x for t in grads for x in (_a(t), _ld(t))], batch,
-            seq_len, n_heads, n_kv_heads, head_dim, window, sinks, dtype_code(q), _a(ws),
-            ws.numel(), s))
+            *args, lse.data_ptr(), _a(seq_lens), *to, batch, seq_len, n_heads, n_kv_heads,
+            head_dim, window, sinks, L.DTYPE_BF16, ws.data_ptr(), need, s))
     return tuple(grads)
 
 
@@ -428,11 +431,9 @@ def kv_cache_write(cache, page_table, start, k, v, batch, n, n_kv_heads, counts=
     quantised into position start[b] + i of sequence b, whose pages page_table
     (int32 device [batch, max_pages]) names; i < counts[b] where counts is given.
     start, counts: int32 device [batch]."""
-    lib = L.load()
     _kv_cache(cache, page_table, batch, n_kv_heads)
     cols = n_kv_heads * 128
-    for t, name in ((k, "k"), (v, "v")):
-        _rows(t, name, batch * n, cols, (torch.bfloat16, torch.float32))
+    ldk, ldv = _rows(k, "k", batch * n, cols, _FLOATS), _rows(v, "v", batch * n, cols, _FLOATS)
     if k.dtype != v.dtype:
         raise TypeError("k and v have different dtypes")
     _i32(start, "start", batch)
@@ -440,9 +441,10 @@ def kv_cache_write(cache, page_table, start, k, v, batch, n, n_kv_heads, counts=
         _i32(counts, "counts", batch)
     ctx, s = _launch_on(stream, cache, page_table, start, counts, k, v)
     with ctx:
-        L.check(lib.prichs_kv_cache_write(
-            _a(cache), cache.shape[0], _a(page_table), page_table.shape[1], _a(start), _a(counts),
-            _a(k), _ld(k), _a(v), _ld(v), batch, n, n_kv_heads, 128, dtype_code(k), s))
+        L.check(L.load().prichs_kv_cache_write(
+            cache.data_ptr(), cache.shape[0], page_table.data_ptr(), page_table.shape[1],
+            start.data_ptr(), _a(counts), k.data_ptr(), ldk, v.data_ptr(), ldv, batch, n,
+            n_kv_heads, 128, _TORCH_DTYPES[k.dtype], s))
 
 
 def kv_cache_read(cache, page_table, start, batch, n, n_kv_heads, counts=None,
@@ -450,26 +452,25 @@ def kv_cache_read(cache, page_table, start, batch, n, n_kv_heads, counts=None,
     """prichs_kv_cache_read: positions start[b] .. start[b] + n - 1 of every sequence
     -> (k, v) [batch * n, n_kv_heads * 128].  Rows past counts[b] keep what k and v
     held (zeros where this call allocates them)."""
-    lib = L.load()
     _kv_cache(cache, page_table, batch, n_kv_heads)
     _i32(start, "start", batch)
     if counts is not None:
         _i32(counts, "counts", batch)
-    shape = (batch * n, n_kv_heads * 128)
+    rows, cols = batch * n, n_kv_heads * 128
     ctx, s = _launch_on(stream, cache, page_table, start, counts, k, v)
     with ctx:
         make = torch.empty if counts is None else torch.zeros
-        got = []
-        for t, name in ((k, "k"), (v, "v")):
-            if t is None:
-                t = make(shape, dtype=out_dtype, device=cache.device)
-            got.append(_rows(t, name, *shape, (torch.bfloat16, torch.float32)))
-        k, v = got
+        if k is None:
+            k = make((rows, cols), dtype=out_dtype, device=cache.device)
+        if v is None:
+            v = make((rows, cols), dtype=out_dtype, device=cache.device)
+        ldk, ldv = _rows(k, "k", rows, cols, _FLOATS), _rows(v, "v", rows, cols, _FLOATS)
         if k.dtype != v.dtype:
             raise TypeError("k and v have different dtypes")
-        L.check(lib.prichs_kv_cache_read(
-            _a(cache), cache.shape[0], _a(page_table), page_table.shape[1], _a(start), _a(counts),
-            _a(k), _ld(k), _a(v), _ld(v), batch, n, n_kv_heads, 128, dtype_code(k), s))
+        L.check(L.load().prichs_kv_cache_read(
+            cache.data_ptr(), cache.shape[0], page_table.data_ptr(), page_table.shape[1],
+            start.data_ptr(), _a(counts), k.data_ptr(), ldk, v.data_ptr(), ldv, batch, n,
+            n_kv_heads, 128, _TORCH_DTYPES[k.dtype], s))
     return k, v
 
 
@@ -482,7 +483,7 @@ def kv_cache_attention(q, cache, page_table, lens, batch, n_q, n_heads, n_kv_hea
     lib = L.load()
     _kv_cache(cache, page_table, batch, n_kv_heads)
     rows, H = batch * n_q, n_heads * head_dim
-    _rows(q, "q", rows, H)
+    ldq = _rows(q, "q", rows, H)
     _i32(lens, "lens", batch)
     if window < 0 or sinks < 0:
         raise ValueError("window and sinks must not be negative")
@@ -490,15 +491,15 @@ def kv_cache_attention(q, cache, page_table, lens, batch, n_q, n_heads, n_kv_hea
     with ctx:
         if out is None:
             out = torch.empty((rows, H), dtype=q.dtype, device=q.device)
-        _rows(out, "out", rows, H)
+        ldo = _rows(out, "out", rows, H)
         lse = None
         if want_lse:
             lse = torch.empty((batch, n_heads, n_q), dtype=torch.float32, device=q.device)
         max_pages = page_table.shape[1]
-        ws = torch.empty((lib.prichs_kv_cache_attention_workspace(
-            batch, n_q, n_heads, n_kv_heads, max_pages),), dtype=torch.uint8, device=q.device)
+        need = lib.prichs_kv_cache_attention_workspace(batch, n_q, n_heads, n_kv_heads, max_pages)
+        ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
         L.check(lib.prichs_kv_cache_attention(
-            _a(q), _ld(q), _a(cache), cache.shape[0], _a(page_table), max_pages, _a(lens), _a(out),
-            _ld(out), _a(lse), batch, n_q, n_heads, n_kv_heads, head_dim, window, sinks,
-            dtype_code(q), _a(ws), ws.numel(), s))
+            q.data_ptr(), ldq, cache.data_ptr(), cache.shape[0], page_table.data_ptr(), max_pages,
+            lens.data_ptr(), out.data_ptr(), ldo, _a(lse), batch, n_q, n_heads, n_kv_heads,
+            head_dim, window, sinks, L.DTYPE_BF16, _a(ws), need, s))
     return out, lse
