@@ -2,7 +2,7 @@
 // 4-bit KV cache (kv_cache.hpp has the layout and the number format).
 //
 // All query rows that read one kv head (n_q tokens x G heads, row = token * G +
-// head) form tiles of 16 NB rows.  A wave takes whole pages of 64 keys:
+// head) form tiles of 16 rows.  A wave takes whole pages of 64 keys:
 //   S^T = K Q^T     v_mfma_f32_16x16x32_bf16: a lane holds 32 head dims (16 bytes
 //                   of codes, one scale) of a key, converted two at a time with
 //                   their scale -- exact in bf16 -- straight into the operand; the
@@ -14,13 +14,21 @@
 //                   holds two dims of one key; a byte permute of two keys' pairs
 //                   gives both dims' operands, and the product's row m of block jd
 //                   is dim 8 m + jd.
-// Nothing goes through LDS before the waves join, no lane exchange but the row
-// maximum, and a page is read once per row tile: 8704 bytes against 65 KB in f32 /
-// 32 KB in bf16.  Each wave reads its next page into registers while it computes one.
+// Nothing goes through LDS before the waves join, there is no lane exchange but the
+// row maximum, and a page is read once per row tile: 8704 bytes against 32 KB in
+// bf16.  Bound by HBM where the caches are long (MI355X, 12 + 3 heads, 32 sequences
+// of 16384 positions: 214 MB in 40 us, 5.3 TB/s), by the latency of a page (about 2
+// us from its table entry to its last product) where they are short (one token over
+// 8192 positions: 8 us, 3.3 MB).  Three workgroups a CU hide each other's loads: a
+// second set of registers for a wave's next page cost the third and was no faster
+// (32 x 3000 positions 15.2 -> 16.1 us).  Tiles of 32 rows share the conversions of
+// two row blocks but leave half the waves (8 x 8 queries over 4096: 15.7 us against
+// 14.7; 1 x 8: 10.9 against 8.7; only 32 x 6 over 2000 gains, 18.9 to 17.6).
 //
-// The visible pages of a tile are dealt to 4 n_split waves in contiguous runs; the
-// waves of a workgroup join in LDS, workgroups through the workspace and a second
-// kernel (n_split > 1).  The order of both is fixed, so results are reproducible.
+// The visible pages of a tile are dealt evenly to the waves of n_split workgroups in
+// contiguous runs; the waves of a workgroup join in LDS, workgroups through the
+// workspace and a second kernel (n_split > 1).  The order of both is fixed, so
+// results are reproducible.
 #include "attention_tile.hpp"
 #include "kv_cache.hpp"
 
@@ -29,10 +37,9 @@
 namespace prichs {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
+constexpr int kRows = 16;          // query rows of a tile
 constexpr int kLdRow = kKvHd + 4;  // LDS row of joined outputs: 16 rows on distinct banks
-constexpr float kLazy = 8.0f;  // log2 headroom of the lazily raised softmax max
+constexpr float kLazy = 8.0f;      // log2 headroom of the lazily raised softmax max
 
 struct AttendShape {
   int n_pages, max_pages, n_q, Hq, Hkv, window, sinks, tiles, n_split;
@@ -61,14 +68,22 @@ struct PageRegs {
   u32x4 vs;    // scales of v[0..3]
 };
 
-// NB: 16-row query blocks of a tile.
-template <int NB>
-__global__ __launch_bounds__(kThreads, NB == 1 ? 3 : 2) void kv_attend_kernel(
+// A part of a row (maximum mw, sum lw) joined to the row's maximum m: its weight, and
+// its share of the sum.
+__device__ __forceinline__ float part_weight(float mw, float m) {
+  return mw == m ? 1.f : fast_exp2(mw - m);
+}
+__device__ __forceinline__ float part_sum(float mw, float lw, float m) {
+  return mw == -INFINITY && m != -INFINITY ? 0.f : lw * part_weight(mw, m);
+}
+
+template <int kWaves>
+__global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 3 : 2) void kv_attend_kernel(
     const bf16_t *__restrict__ q, size_t ldq, const uint8_t *__restrict__ cache,
     const int32_t *__restrict__ table, const int32_t *__restrict__ lens, bf16_t *__restrict__ o,
     size_t ldo, float *__restrict__ lse, float *__restrict__ part_o, float2 *__restrict__ part_ml,
     AttendShape sh) {
-  constexpr int kRows = 16 * NB;
+  constexpr int kThreads = 64 * kWaves;
   __shared__ float s_ml[2][kWaves][kRows];
   __shared__ float s_o[kWaves][kRows * kLdRow];
 
@@ -83,18 +98,13 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 3 : 2) void kv_attend_kernel(
   // Positions of the tile's first and last row, and of this lane's rows.
   const int r0 = tile * kRows, r1 = min(r0 + kRows, rows) - 1;
   const int p0 = L - sh.n_q + r0 / G, p1 = L - sh.n_q + r1 / G;
-  int pos[NB];
-  u32x4 qf[NB][4];
+  u32x4 qf[4];
+  const int lrow = min(r0 + l16, rows - 1), lq = lrow / G;
+  const int pos = L - sh.n_q + lq;
+  const bf16_t *qrow = q + ((size_t)b * sh.n_q + lq) * ldq +
+                       (size_t)(kvh * G + lrow - lq * G) * kKvHd + 32 * g;
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int r = min(r0 + 16 * nb + l16, rows - 1);
-    const int iq = r / G;
-    pos[nb] = L - sh.n_q + iq;
-    const bf16_t *qrow = q + ((size_t)b * sh.n_q + iq) * ldq +
-                         (size_t)(kvh * G + r - iq * G) * kKvHd + 32 * g;
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) qf[nb][kk] = *reinterpret_cast<const u32x4 *>(qrow + 8 * kk);
-  }
+  for (int kk = 0; kk < 4; ++kk) qf[kk] = *reinterpret_cast<const u32x4 *>(qrow + 8 * kk);
 
   // The pages that some row sees: those of the sinks, then from the first row's
   // window on.
@@ -113,17 +123,11 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 3 : 2) void kv_attend_kernel(
     return p >= 0 && p < sh.n_pages ? p : -1;
   };
 
-  f32x4 oacc[8][NB], lsum[NB];
-  float m_ref[NB];
-  bool seen[NB];
+  f32x4 oacc[8], lsum = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-    for (int jd = 0; jd < 8; ++jd) oacc[jd][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
-    lsum[nb] = f32x4{0.f, 0.f, 0.f, 0.f};
-    m_ref[nb] = -INFINITY;
-    seen[nb] = false;
-  }
+  for (int jd = 0; jd < 8; ++jd) oacc[jd] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m_ref = -INFINITY;
+  bool seen = false;
   const u32x4 ones = u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 
   auto part_of = [&](int page) { return cache + ((size_t)page * sh.Hkv + kvh) * kKvPart; };
@@ -146,41 +150,36 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 3 : 2) void kv_attend_kernel(
   auto compute = [&](PageRegs &x, int i, int page) {
     if (page < 0) return;
     const int kv0 = block_of(i) * kKvPage;
-    f32x4 s[4][NB];
+    f32x4 s[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const float sc = kv_scale((x.ks >> (8 * c)) & 255u);
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) s[c][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+      s[c] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
         const u32x4 kf = eight(x.k[c][kk], sc);
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) s[c][nb] = mfma_u32(kf, qf[nb][kk], s[c][nb]);
+        s[c] = mfma_u32(kf, qf[kk], s[c]);
       }
     }
-    // s[c][nb][r]: query row 16 nb + l16 of the tile, key kv0 + 16 c + 4 g + r.
+    // s[c][r]: query row l16 of the tile, key kv0 + 16 c + 4 g + r.
     const bool whole = kv0 + kKvPage - 1 <= p0 &&
                        (sh.window == 0 || p1 - kv0 < sh.window || kv0 + kKvPage <= sh.sinks);
     bool nans = false;  // a V group without finite values in a page that not all rows see
     if (!whole) {
+      const int lim = pos - kv0 - 4 * g;
+      const int old = sh.window == 0 ? -64 : lim - sh.window;
+      const int sink = sh.sinks - kv0 - 4 * g;
+      bool any = false;
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const int lim = pos[nb] - kv0 - 4 * g;
-        const int old = sh.window == 0 ? -64 : lim - sh.window;
-        const int sink = sh.sinks - kv0 - 4 * g;
-        bool any = false;
+      for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int e = 16 * c + r;
-            const bool hidden = (e > lim) | ((e <= old) & (e >= sink));
-            any |= !hidden;
-            s[c][nb][r] = hidden ? -INFINITY : s[c][nb][r];
-          }
-        seen[nb] |= any;
-      }
+        for (int r = 0; r < 4; ++r) {
+          const int e = 16 * c + r;
+          const bool hidden = (e > lim) | ((e <= old) & (e >= sink));
+          any |= !hidden;
+          s[c][r] = hidden ? -INFINITY : s[c][r];
+        }
+      seen |= any;
       // A key that a row does not see has p = 0 there, but 0 times an infinity or
       // NaN of V is NaN: such groups (slots never written among them) count as
       // zeros here, and as NaN after the product for the rows that see them.
@@ -193,47 +192,38 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 3 : 2) void kv_attend_kernel(
             nans = true;
           }
     } else {
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) seen[nb] = true;
+      seen = true;
     }
 
-    u32x4 pf[NB][2];
-    float alpha[NB];
-    bool raised = false;
+    u32x4 pf[2];
+    float mloc = -INFINITY;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      float mloc = -INFINITY;
+    for (int c = 0; c < 4; ++c)
+      mloc = vmax(vmax(vmax(mloc, s[c][0]), s[c][1]), vmax(s[c][2], s[c][3]));
+    mloc = max_across_groups(mloc);
+    // The reference max is raised only when a page's passes it by 2^8 in p.
+    const float m_blk = mloc * sh.scale_log2;
+    const bool raise = m_blk > m_ref + kLazy;
+    const float m_new = raise ? m_blk : m_ref;
+    const float alpha = raise ? fast_exp2(m_ref - m_new) : 1.0f;
+    m_ref = m_new;
+    const float neg_m = m_new == -INFINITY ? 0.f : -m_new;
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        mloc = vmax(vmax(vmax(mloc, s[c][nb][0]), s[c][nb][1]), vmax(s[c][nb][2], s[c][nb][3]));
-      mloc = max_across_groups(mloc);
-      // The reference max is raised only when a page's passes it by 2^8 in p.
-      const float m_blk = mloc * sh.scale_log2;
-      const bool raise = m_blk > m_ref[nb] + kLazy;
-      const float m_new = raise ? m_blk : m_ref[nb];
-      alpha[nb] = raise ? fast_exp2(m_ref[nb] - m_new) : 1.0f;
-      m_ref[nb] = m_new;
-      raised |= raise;
-      const float neg_m = m_new == -INFINITY ? 0.f : -m_new;
+    for (int ks2 = 0; ks2 < 2; ++ks2) {
+      float p[8];
 #pragma unroll
-      for (int ks2 = 0; ks2 < 2; ++ks2) {
-        float p[8];
+      for (int h2 = 0; h2 < 2; ++h2)
 #pragma unroll
-        for (int h2 = 0; h2 < 2; ++h2)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            p[4 * h2 + r] = fast_exp2(fmaf(s[2 * ks2 + h2][nb][r], sh.scale_log2, neg_m));
-        pf[nb][ks2] = u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]),
-                            pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])};
-      }
+        for (int r = 0; r < 4; ++r)
+          p[4 * h2 + r] = fast_exp2(fmaf(s[2 * ks2 + h2][r], sh.scale_log2, neg_m));
+      // P rounded to bf16 for the product; its sum is that of the rounded values.
+      pf[ks2] = u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]),
+                      pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])};
     }
-    if (__any(raised)) {
+    if (__any(raise)) {
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-        for (int jd = 0; jd < 8; ++jd) oacc[jd][nb] = oacc[jd][nb] * alpha[nb];
-        lsum[nb] = lsum[nb] * alpha[nb];
-      }
+      for (int jd = 0; jd < 8; ++jd) oacc[jd] = oacc[jd] * alpha;
+      lsum = lsum * alpha;
     }
     auto v_block = [&](auto byte_c, int ks2, const float (&sa)[4], const float (&sb)[4]) {
       constexpr int BYTE = decltype(byte_c)::value;
@@ -249,11 +239,8 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 3 : 2) void kv_attend_kernel(
         lo[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x05040100);
         hi[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302);
       }
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        oacc[2 * BYTE][nb] = mfma_u32(lo, pf[nb][ks2], oacc[2 * BYTE][nb]);
-        oacc[2 * BYTE + 1][nb] = mfma_u32(hi, pf[nb][ks2], oacc[2 * BYTE + 1][nb]);
-      }
+      oacc[2 * BYTE] = mfma_u32(lo, pf[ks2], oacc[2 * BYTE]);
+      oacc[2 * BYTE + 1] = mfma_u32(hi, pf[ks2], oacc[2 * BYTE + 1]);
     };
 #pragma unroll
     for (int ks2 = 0; ks2 < 2; ++ks2) {
@@ -267,29 +254,24 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 3 : 2) void kv_attend_kernel(
       v_block(std::integral_constant<int, 1>{}, ks2, sa, sb);
       v_block(std::integral_constant<int, 2>{}, ks2, sa, sb);
       v_block(std::integral_constant<int, 3>{}, ks2, sa, sb);
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) lsum[nb] = mfma_u32(ones, pf[nb][ks2], lsum[nb]);
+      lsum = mfma_u32(ones, pf[ks2], lsum);
     }
     if (!whole && __any(nans)) {
       // The lane's dims 8 (4 g + r) + jd are group g's.
       const uint8_t *p = part_of(page);
-      bool hit[NB] = {};
+      bool hit = false;
 #pragma unroll 1
       for (int t = 0; t < kKvPage; ++t) {
         const bool off = p[kv_v_scale_off(t, g)] > 252;
         const int key = kv0 + t;
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-          hit[nb] |= off & (key <= pos[nb]) &
-                     ((sh.window == 0) | (pos[nb] - key < sh.window) | (key < sh.sinks));
+        hit |= off & (key <= pos) &
+               ((sh.window == 0) | (pos - key < sh.window) | (key < sh.sinks));
       }
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
+      for (int jd = 0; jd < 8; ++jd)
 #pragma unroll
-        for (int jd = 0; jd < 8; ++jd)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            oacc[jd][nb][r] = hit[nb] ? __uint_as_float(0x7fc00000u) : oacc[jd][nb][r];
+        for (int r = 0; r < 4; ++r)
+          oacc[jd][r] = hit ? __uint_as_float(0x7fc00000u) : oacc[jd][r];
     }
   };
 
@@ -301,37 +283,30 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 3 : 2) void kv_attend_kernel(
     compute(x, i, page);
   }
 
-  // The waves join.
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    // A row that saw keys but no score above -inf has no softmax: NaN.
-    const bool lost = __any(seen[nb] && m_ref[nb] == -INFINITY) != 0 && seen[nb] &&
-                      m_ref[nb] == -INFINITY;
-    int flag = lost ? 1 : 0;
-    flag |= __shfl_xor(flag, 16);
-    flag |= __shfl_xor(flag, 32);
-    if (g == 0) {
-      s_ml[0][wave][16 * nb + l16] = m_ref[nb];
-      s_ml[1][wave][16 * nb + l16] = flag ? __uint_as_float(0x7fc00000u) : lsum[nb][0];
-    }
+  // The waves join.  A score that is NaN makes the row's maximum NaN.  A row that saw
+  // keys but no score above -inf has no softmax: its sum is NaN, and counts where no
+  // other part of the row has a score (part_sum).
+  if (lsum[0] != lsum[0]) m_ref = lsum[0];
+  int lost = seen && m_ref == -INFINITY;
+  lost |= __shfl_xor(lost, 16);
+  lost |= __shfl_xor(lost, 32);
+  if (g == 0) {
+    s_ml[0][wave][l16] = m_ref;
+    s_ml[1][wave][l16] = lost ? __uint_as_float(0x7fc00000u) : lsum[0];
   }
   __syncthreads();
+  float m = -INFINITY;
+  for (int w = 0; w < kWaves; ++w) m = vmax(m, s_ml[0][w][l16]);
+  const float f = part_weight(m_ref, m);
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    float m = -INFINITY;
-    for (int w = 0; w < kWaves; ++w) m = vmax(m, s_ml[0][w][16 * nb + l16]);
-    const float f = m_ref[nb] == m ? 1.f : fast_exp2(m_ref[nb] - m);
+  for (int r = 0; r < 4; ++r)
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int j4 = 0; j4 < 2; ++j4) {
+      f32x4 t;
 #pragma unroll
-      for (int j4 = 0; j4 < 2; ++j4) {
-        f32x4 t;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) t[e] = oacc[4 * j4 + e][nb][r] * f;
-        *reinterpret_cast<f32x4 *>(
-            &s_o[wave][(16 * nb + l16) * kLdRow + 8 * (4 * g + r) + 4 * j4]) = t;
-      }
-  }
+      for (int e = 0; e < 4; ++e) t[e] = oacc[4 * j4 + e][r] * f;
+      *reinterpret_cast<f32x4 *>(&s_o[wave][l16 * kLdRow + 8 * (4 * g + r) + 4 * j4]) = t;
+    }
   __syncthreads();
   for (int x = tid; x < kRows * kKvHd / 4; x += kThreads) {
     const int row = x / (kKvHd / 4), d = 4 * (x - row * (kKvHd / 4));
@@ -341,7 +316,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 3 : 2) void kv_attend_kernel(
     f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int w = 0; w < kWaves; ++w) {
       const float mw = s_ml[0][w][row];
-      l += s_ml[1][w][row] * (mw == m ? 1.f : fast_exp2(mw - m));
+      l += part_sum(mw, s_ml[1][w][row], m);
       t = t + *reinterpret_cast<const f32x4 *>(&s_o[w][row * kLdRow + d]);
     }
     if (sh.n_split > 1) {
@@ -369,7 +344,7 @@ template <int KG>
 __global__ __launch_bounds__(256) void kv_join_kernel(const float *__restrict__ part_o,
                                                       const float2 *__restrict__ part_ml,
                                                       bf16_t *__restrict__ o, size_t ldo,
-                                                      float *__restrict__ lse, int tile_rows,
+                                                      float *__restrict__ lse,
                                                       AttendShape sh) {
   __shared__ f32x4 s_o[8][32];
   __shared__ float2 s_ml[8];
@@ -378,8 +353,8 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const float *__restrict__ 
   const int r = blockIdx.x * (8 / KG) + slot / KG;
   const int kvh = blockIdx.y, b = blockIdx.z;
   if (KG == 1 && r >= rows) return;  // with KG = 8 the grid is the rows
-  const int tile = r / tile_rows, row = r - tile * tile_rows;
-  const size_t base = (((size_t)b * sh.Hkv + kvh) * sh.tiles + tile) * sh.n_split * tile_rows + row;
+  const int tile = r / kRows, row = r - tile * kRows;
+  const size_t base = (((size_t)b * sh.Hkv + kvh) * sh.tiles + tile) * sh.n_split * kRows + row;
   float m = -INFINITY, l = 0.f;
   f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int s0 = k; s0 < sh.n_split; s0 += 8 * KG) {
@@ -391,7 +366,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const float *__restrict__ 
       ml[j] = make_float2(-INFINITY, 0.f);
       p[j] = f32x4{0.f, 0.f, 0.f, 0.f};
       if (s < sh.n_split) {
-        const size_t at = base + (size_t)s * tile_rows;
+        const size_t at = base + (size_t)s * kRows;
         ml[j] = part_ml[at];
         p[j] = *reinterpret_cast<const f32x4 *>(part_o + at * kKvHd + 4 * d4);
       }
@@ -399,14 +374,12 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const float *__restrict__ 
     float m2 = m;
 #pragma unroll
     for (int j = 0; j < 8; ++j) m2 = vmax(m2, ml[j].x);
-    const float f0 = m == m2 ? 1.f : fast_exp2(m - m2);
-    l *= f0;
-    t = t * f0;
+    l = part_sum(m, l, m2);
+    t = t * part_weight(m, m2);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float f = ml[j].x == m2 ? 1.f : fast_exp2(ml[j].x - m2);
-      l += ml[j].y * f;
-      t = t + p[j] * f;
+      l += part_sum(ml[j].x, ml[j].y, m2);
+      t = t + p[j] * part_weight(ml[j].x, m2);
     }
     m = m2;
   }
@@ -422,9 +395,8 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const float *__restrict__ 
     t = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < KG; ++j) {
-      const float f = s_ml[j].x == m ? 1.f : fast_exp2(s_ml[j].x - m);
-      l += s_ml[j].y * f;
-      t = t + s_o[j][d4] * f;
+      l += part_sum(s_ml[j].x, s_ml[j].y, m);
+      t = t + s_o[j][d4] * part_weight(s_ml[j].x, m);
     }
   }
   const int iq = r / G, h = kvh * G + r - iq * G;
@@ -437,26 +409,40 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const float *__restrict__ 
     lse[((size_t)b * sh.Hq + h) * sh.n_q + iq] = (m + log2f(l)) * 0.6931471805599453f;
 }
 
-// How a call is cut: 16 nb rows a tile, n_split workgroups over a tile's pages.
+// Pages up to which one workgroup of 8 waves takes a tile without a second kernel:
+// a page costs a wave some 2 us, the second kernel 2.5 on the device and 4 on the
+// host.  One token over 8 pages 7.4 -> 6.1 us (graph), over 16 pages 7.4 -> 8.2
+// (called from Python 15.2 -> 11), 32 and 80 sequences over 16 pages 9.2 -> 8.4 and
+// 14.6 -> 10.6, 32 over 32 pages 11.1 -> 13.3.
+constexpr size_t kShortPages = 16;
+
+// How a call is cut: n_split workgroups of `waves` waves over a
+// tile's pages.
 struct Plan {
-  int nb;
+  int waves;
   size_t tiles, n_split;
 };
 Plan plan_of(size_t batch, size_t n_q, size_t n_heads, size_t n_kv_heads, size_t pages) {
   const size_t rows = n_q * (n_heads / n_kv_heads);
   Plan p;
-  p.nb = rows <= 16 ? 1 : 2;
-  p.tiles = cdiv(rows, 16 * (size_t)p.nb);
-  // As many workgroups as fit the chip at once (three a CU with 16 rows, two with
-  // 32), and a page for each wave of a workgroup.
+  p.waves = 4;
+  p.tiles = cdiv(rows, (size_t)kRows);
   const size_t wgs = std::max<size_t>(batch * n_kv_heads * p.tiles, 1);
-  const size_t fit = p.nb == 1 ? 768 : 512;
-  p.n_split = std::max<size_t>(std::min(fit / wgs, cdiv(pages, kWaves)), 1);
+  // Few pages and a CU for every tile: one workgroup of 8 waves a tile, and no
+  // second kernel.
+  if (pages > 4 && pages <= kShortPages && wgs <= 256) {
+    p.waves = 8;
+    p.n_split = 1;
+    return p;
+  }
+  // As many workgroups as fit the chip at once (three a CU), and a page for each
+  // wave of a workgroup.
+  p.n_split = std::max<size_t>(std::min(768 / wgs, cdiv(pages, 4)), 1);
   return p;
 }
 size_t workspace_of(const Plan &p, size_t batch, size_t n_kv_heads) {
   if (p.n_split <= 1) return 0;
-  return batch * n_kv_heads * p.tiles * p.n_split * 16 * p.nb * (kKvHd + 2) * sizeof(float);
+  return batch * n_kv_heads * p.tiles * p.n_split * kRows * (kKvHd + 2) * sizeof(float);
 }
 
 }  // namespace
@@ -525,12 +511,12 @@ extern "C" int prichs_kv_cache_attention(const void *q, size_t ldq, const void *
                        (int)p.tiles,
                        (int)p.n_split,
                        (1.0f / sqrtf((float)head_dim)) * 1.4426950408889634f};
-  const size_t part_rows = batch * n_kv_heads * p.tiles * p.n_split * 16 * p.nb;
+  const size_t part_rows = batch * n_kv_heads * p.tiles * p.n_split * kRows;
   float *part_o = static_cast<float *>(workspace);
   float2 *part_ml = reinterpret_cast<float2 *>(part_o + (p.n_split > 1 ? part_rows * kKvHd : 0));
   const dim3 grid((unsigned)p.n_split, (unsigned)(n_kv_heads * p.tiles), (unsigned)batch);
-  auto kern = p.nb == 1 ? kv_attend_kernel<1> : kv_attend_kernel<2>;
-  hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, as_stream(stream),
+  auto kern = p.waves == 8 ? kv_attend_kernel<8> : kv_attend_kernel<4>;
+  hipLaunchKernelGGL(kern, grid, dim3((unsigned)(64 * p.waves)), 0, as_stream(stream),
                      static_cast<const bf16_t *>(q), ldq, static_cast<const uint8_t *>(cache),
                      page_table, lens, static_cast<bf16_t *>(o), ldo, lse, part_o, part_ml, sh);
   PRICHS_LAUNCH_CHECK("kv_cache_attention launch");
@@ -543,7 +529,7 @@ extern "C" int prichs_kv_cache_attention(const void *q, size_t ldq, const void *
                     (unsigned)batch);
     auto join_kern = wide ? kv_join_kernel<8> : kv_join_kernel<1>;
     hipLaunchKernelGGL(join_kern, join, dim3(256), 0, as_stream(stream), part_o, part_ml,
-                       static_cast<bf16_t *>(o), ldo, lse, 16 * p.nb, sh);
+                       static_cast<bf16_t *>(o), ldo, lse, sh);
     PRICHS_LAUNCH_CHECK("kv_cache_attention join launch");
   }
   return PRICHS_OK;

@@ -319,6 +319,27 @@ def test_flat_and_steep_scores(cuda, q_scale):
     check(ops.kv_cache_attention(dev(q), cache, table, i32(lens), 2, 2, 4, 2)[0], None, ref)
 
 
+@pytest.mark.parametrize("length", [50, 500, 3000])
+def test_queries_without_finite_scores(cuda, length):
+    """Scores of -inf have no weight; a row of nothing else, and one with a NaN or a
+    +inf, has no softmax.  The keys' first dim is 1 from position 40 on and 0 before
+    (0 times an infinity is NaN)."""
+    k = np.zeros((length, HD), np.float32)
+    v = synth.round_bf16(np.random.default_rng(1).standard_normal((length, HD)))
+    k[40:, 0] = 1
+    table, n_pages = table_of(1, -(-length // PAGE))
+    cache = filled(n_pages, 1)
+    ops.kv_cache_write(cache, table, i32([0]), dev(k), dev(v), 1, length, 1)
+    q = np.zeros((1, 4 * HD), np.float32)
+    q[0, 0], q[0, HD], q[0, 2 * HD] = -np.inf, np.inf, np.nan
+    for window in (0, length - 45):  # with and without keys whose score is NaN
+        out, lse = ops.kv_cache_attention(dev(q), cache, table, i32([length]), 1, 1, 4, 1, window,
+                                          want_lse=True)
+        h, hl = host(out).reshape(4, HD), host(lse).reshape(4)
+        assert np.isnan(h[:3]).all() and np.isnan(hl[:3]).all(), window
+        assert np.isfinite(h[3]).all() and np.isfinite(hl[3])
+
+
 def test_prefill_then_decode_steps_in_a_graph(cuda):
     """As a program uses them together: a prompt's window attention, its keys and
     values into the cache, then decode steps -- one captured graph whose table,
