@@ -87,8 +87,8 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 3 : 2) void kv_attend_ke
   __shared__ float s_ml[2][kWaves][kRows];
   __shared__ float s_o[kWaves][kRows * kLdRow];
 
-  const int split = blockIdx.x;
-  const int kvh = blockIdx.y / sh.tiles, tile = blockIdx.y - kvh * sh.tiles;
+  const int split = blockIdx.y;
+  const int kvh = blockIdx.x / sh.tiles, tile = blockIdx.x - kvh * sh.tiles;
   const int b = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -500,7 +500,7 @@ extern "C" int prichs_kv_cache_attention(const void *q, size_t ldq, const void *
       w == 0 ? max_pages
              : std::min(max_pages, cdiv(w + n_q, kKvPage) + 1 + cdiv(sk, kKvPage));
   const Plan p = plan_of(batch, n_q, n_heads, n_kv_heads, pages);
-  PRICHS_REQUIRE(n_kv_heads * p.tiles <= 65535, "%s: shape too large", who);
+  PRICHS_REQUIRE(n_kv_heads * p.tiles <= (size_t)1 << 23, "%s: shape too large", who);
   const AttendShape sh{(int)n_pages,
                        (int)max_pages,
                        (int)n_q,
@@ -514,7 +514,7 @@ extern "C" int prichs_kv_cache_attention(const void *q, size_t ldq, const void *
   const size_t part_rows = batch * n_kv_heads * p.tiles * p.n_split * kRows;
   float *part_o = static_cast<float *>(workspace);
   float2 *part_ml = reinterpret_cast<float2 *>(part_o + (p.n_split > 1 ? part_rows * kKvHd : 0));
-  const dim3 grid((unsigned)p.n_split, (unsigned)(n_kv_heads * p.tiles), (unsigned)batch);
+  const dim3 grid((unsigned)(n_kv_heads * p.tiles), (unsigned)p.n_split, (unsigned)batch);
   auto kern = p.waves == 8 ? kv_attend_kernel<8> : kv_attend_kernel<4>;
   hipLaunchKernelGGL(kern, grid, dim3((unsigned)(64 * p.waves)), 0, as_stream(stream),
                      static_cast<const bf16_t *>(q), ldq, static_cast<const uint8_t *>(cache),

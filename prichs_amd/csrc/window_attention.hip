@@ -815,7 +815,8 @@ int check_shape(const char *who, size_t batch, size_t seq_len, size_t n_heads, s
                  "%s: n_heads=%zu must be a positive multiple of n_kv_heads=%zu", who, n_heads,
                  n_kv_heads);
   PRICHS_REQUIRE(n_heads <= 65535 && batch <= 65535 && seq_len <= (size_t)1 << 21 &&
-                     batch * seq_len <= (size_t)INT32_MAX / 2,
+                     batch * seq_len <= (size_t)INT32_MAX / 2 &&
+                     (seq_len + 128) * (n_heads / n_kv_heads) <= (size_t)INT32_MAX,
                  "%s: shape too large", who);
   *sh = shape_of(seq_len, n_heads, n_kv_heads, window, sinks);
   *work = batch != 0 && seq_len != 0;
@@ -826,9 +827,10 @@ int check_shape(const char *who, size_t batch, size_t seq_len, size_t n_heads, s
 // 16-byte aligned.
 int check_rows(const char *who, const char *name, const void *p, size_t ld, size_t cols) {
   PRICHS_REQUIRE(p != nullptr, "%s: null pointer argument %s", who, name);
-  PRICHS_REQUIRE(ld >= cols && ld % 8 == 0 && ld < ((size_t)1 << 25),
+  // The kernels address up to 128 rows with 32-bit byte offsets.
+  PRICHS_REQUIRE(ld >= cols && ld % 8 == 0 && ld < ((size_t)1 << 24),
                  "%s: the leading dimension %zu of %s must be a multiple of 8 elements, at least "
-                 "%zu and below 2^25",
+                 "%zu and below 2^24",
                  who, ld, name, cols);
   PRICHS_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, "%s: %s must be 16-byte aligned", who,
                  name);

@@ -180,6 +180,9 @@ ATTEND = [
     (2, 5, [300, 3], 12, 3, 0, 0), (2, 3, [130, 66], 8, 1, 20, 2), (1, 4, [70], 5, 1, 0, 0),
     (3, 17, [400, 17, 20], 4, 1, 33, 1), (1, 40, [40], 8, 2, 0, 0), (1, 130, [450], 12, 3, 96, 4),
     (2, 70, [500, 100], 3, 3, 0, 0), (1, 1, [5000], 12, 3, 4096, 4), (1, 33, [1000], 16, 2, 300, 70),
+    # A few splits joined; more tiles than workgroups that fit at once.
+    (1, 1, [1500], 8, 2, 0, 0), (2, 40, [1300, 60], 12, 3, 0, 0), (9, 40, [300] * 9, 12, 3, 0, 0),
+    (2, 700, [750, 700], 12, 3, 200, 3),
 ]
 
 

@@ -49,6 +49,10 @@ CASES = [
     (1, 450, 2, 1, 65, 500, None), (1, 900, 4, 1, 130, 5, None),
     (3, 130, 6, 2, 50, 1, [0, 130, 77]), (4, 90, 2, 1, 0, 0, [1, 64, 500, -3]),
     (2, 400, 4, 1, 100, 4, [399, 130]),
+    # More workgroups than the short-row variants take, for 4, 2 and 1 heads that
+    # share a workgroup's tiles.
+    (3, 330, 48, 12, 100, 4, [330, 200, 17]), (6, 330, 24, 12, 90, 0, None),
+    (6, 330, 24, 24, 0, 0, [330, 1, 0, 129, 300, 64]),
 ]
 
 
