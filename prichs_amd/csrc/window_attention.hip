@@ -113,8 +113,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
   const Shape &sh = a.sh;
   const int group = sh.Hq / sh.Hkv, sets = group / HPW;
   const int kvh = blockIdx.x / sets, b = blockIdx.y;
-  const int n_qb = (sh.S + kRowsWg - 1) / kRowsWg;
-  const int qb = n_qb - 1 - (int)blockIdx.z;
+  const int qb = (int)(gridDim.z - 1 - blockIdx.z);  // long rows first
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = kvh * group + (blockIdx.x - kvh * sets) * HPW + wave % HPW;
@@ -913,7 +912,9 @@ extern "C" int prichs_window_attention_backward(
   const int hpw = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
   const size_t blocks = cdiv(seq_len, (size_t)kBlk), n_qb32 = cdiv(seq_len, (size_t)(128 / hpw));
   const bool few = 2 * (n_heads / hpw) * batch * n_qb32 <= 3 * 256;
-  const size_t n_qb = few ? cdiv(seq_len, (size_t)(64 / hpw)) : n_qb32;
+  // The d_q kernel writes the statistics of whole 32-row tiles, so its rows go to the
+  // end of the last one.
+  const size_t n_qb = few ? cdiv(roundup(seq_len, (size_t)kTr), (size_t)(64 / hpw)) : n_qb32;
   PRICHS_REQUIRE(n_qb <= 65535 && n_kv_heads <= 65535, "%s: shape too large", who);
   const auto bf = [](const void *p) { return static_cast<const bf16_t *>(p); };
   const auto out = [](void *p) { return static_cast<bf16_t *>(p); };

@@ -236,3 +236,25 @@ def test_wrapper_refusals(cuda):
         ops.window_attention_backward(g, q, k, v, out, lse[:, :1], *ok)
     out, lse = ops.window_attention(q[:0], k[:0], v[:0], 0, 8, 2, 1, 4, want_lse=True)
     assert out.shape == (0, 256) and lse.shape == (0, 2, 8)
+
+
+@pytest.mark.parametrize("S,H,K", [(10, 4, 1), (777, 8, 2), (33, 2, 1), (16, 3, 3)])
+def test_what_the_workspace_held_does_not_matter(cuda, S, H, K):
+    """NaN everywhere in it, sequences that end in the first half of a 32-row tile
+    among the cases."""
+    W, sinks = 40, 3
+    x = inputs(1, S, H, K, 7)
+    ref = R.batch_attention(*x[:3], 1, S, H, K, W, sinks, d_out=x[3])
+    q, k, v, d_o = (dev(a) for a in x)
+    out, lse = ops.window_attention(q, k, v, 1, S, H, K, W, sinks, want_lse=True)
+    lib = L.load()
+    need = lib.prichs_window_attention_backward_workspace(1, S, H, K, W, sinks)
+    ws = torch.full((need,), 0xff, dtype=torch.uint8, device="cuda")
+    grads = [torch.empty_like(t) for t in (q, k, v)]
+    args = [a for t in (d_o, q, k, v, out) for a in (t.data_ptr(), t.stride(0))]
+    to = [a for t in grads for a in (t.data_ptr(), t.stride(0))]
+    L.check(lib.prichs_window_attention_backward(
+        *args, lse.data_ptr(), None, *to, 1, S, H, K, HD, W, sinks, L.DTYPE_BF16, ws.data_ptr(),
+        need, torch.cuda.current_stream().cuda_stream))
+    for t, name in zip(grads, ("dq", "dk", "dv")):
+        near(t, ref, name)
