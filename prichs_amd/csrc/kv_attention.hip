@@ -480,7 +480,7 @@ extern "C" int prichs_kv_cache_attention(const void *q, size_t ldq, const void *
                  "%s: ldq and ldo must be multiples of 8 elements that hold all heads", who);
   const size_t cap = max_pages * kKvPage;
   if (batch == 0 || n_q == 0) return PRICHS_OK;
-  PRICHS_REQUIRE(q && o && lens && (cap == 0 || (cache && page_table)),
+  PRICHS_REQUIRE(q && o && lens && (cap == 0 || page_table) && (n_pages == 0 || cache),
                  "%s: null pointer argument", who);
   PRICHS_REQUIRE((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(o) |
                   reinterpret_cast<uintptr_t>(cache)) % 16 == 0,

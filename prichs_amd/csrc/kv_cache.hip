@@ -152,7 +152,8 @@ int kv_check(const char *who, const void *k, size_t ldk, const void *v, size_t l
                      max_pages <= (size_t)INT32_MAX / kKvPage,
                  "%s: shape too large", who);
   if (batch == 0 || n == 0) return PRICHS_OK;
-  PRICHS_REQUIRE(k && v && cache && page_table && start, "%s: null pointer argument", who);
+  PRICHS_REQUIRE(k && v && start && (n_pages == 0 || cache) && (max_pages == 0 || page_table),
+                 "%s: null pointer argument", who);
   const uintptr_t al = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
                        reinterpret_cast<uintptr_t>(cache);
   PRICHS_REQUIRE(al % 16 == 0, "%s: k, v and the cache must be 16-byte aligned", who);

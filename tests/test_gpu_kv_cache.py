@@ -430,3 +430,39 @@ def test_wrapper_refusals(cuda):
     none = torch.empty((1, 0), dtype=torch.int32, device="cuda")
     out, lse = ops.kv_cache_attention(q, cache, none, i32([5]), 1, 1, 4, kv, want_lse=True)
     assert not host(out).any() and np.isneginf(host(lse)).all()
+
+
+def test_without_pages_or_positions(cuda):
+    """A cache of no pages and a table of no columns: nothing is written, zeros are
+    read, and a query sees no key."""
+    for n_pages, cols in ((0, 0), (0, 2), (3, 0)):
+        say("case:", n_pages, cols)
+        cache = ops.kv_cache_pages(n_pages, 2)
+        cache.fill_(255)
+        table = torch.zeros((2, cols), dtype=torch.int32, device="cuda")
+        x = torch.ones((2 * 3, 2 * HD), dtype=torch.bfloat16, device="cuda")
+        ops.kv_cache_write(cache, table, i32([0, 1]), x, x, 2, 3, 2)
+        assert (cache == 255).all()
+        k, v = ops.kv_cache_read(cache, table, i32([0, 1]), 2, 3, 2)
+        assert (k == 0).all() and (v == 0).all()
+        out, lse = ops.kv_cache_attention(torch.ones((6, 4 * HD), dtype=torch.bfloat16, device="cuda"),
+                                          cache, table, i32([3, 70]), 2, 3, 4, 2, want_lse=True)
+        assert (out == 0).all() and torch.isneginf(lse).all()
+
+
+@pytest.mark.parametrize("batch,n_q,lens,heads,kv,window", [
+    (1, 1, [3000], 4, 1, 0), (3, 5, [1300, 0, 3], 6, 2, 0), (2, 40, [1500, 1100], 4, 2, 100)])
+def test_what_the_workspace_held_does_not_matter(cuda, batch, n_q, lens, heads, kv, window):
+    table, cache, q, kc, vc = attend_case(batch, n_q, lens, heads, kv, 11)
+    ref = attend_ref(q, kc, vc, lens, n_q, heads, kv, window, 2)
+    lib, pages, x = L.load(), table.shape[1], dev(q)
+    need = lib.prichs_kv_cache_attention_workspace(batch, n_q, heads, kv, pages)
+    assert need > 0
+    ws = torch.full((need,), 0xff, dtype=torch.uint8, device="cuda")
+    out, lens_d = torch.empty_like(x), i32(lens)
+    lse = torch.empty((batch, heads, n_q), dtype=torch.float32, device="cuda")
+    L.check(lib.prichs_kv_cache_attention(
+        x.data_ptr(), heads * HD, cache.data_ptr(), cache.shape[0], table.data_ptr(), pages,
+        lens_d.data_ptr(), out.data_ptr(), heads * HD, lse.data_ptr(), batch, n_q, heads, kv, HD,
+        window, 2, L.DTYPE_BF16, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream))
+    check(out, lse, ref)
