@@ -466,3 +466,26 @@ def test_what_the_workspace_held_does_not_matter(cuda, batch, n_q, lens, heads, 
         lens_d.data_ptr(), out.data_ptr(), heads * HD, lse.data_ptr(), batch, n_q, heads, kv, HD,
         window, 2, L.DTYPE_BF16, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream))
     check(out, lse, ref)
+
+
+def test_pages_past_32_bits(cuda):
+    """A cache of 4.7 GB whose used pages lie at its start and its end."""
+    kv, lens, n_q, heads = 2, [150, 200], 3, 4
+    n_pages = 270_000
+    assert n_pages * kv * L.KV_PAGE_BYTES > 1 << 32
+    cache = ops.kv_cache_pages(n_pages, kv)
+    table = torch.tensor([[n_pages - 1, 0, n_pages - 5, 7], [n_pages - 2, n_pages - 3, 1, 2]],
+                         dtype=torch.int32, device="cuda")
+    cache[table.flatten().long()] = 255
+    rng = np.random.default_rng(4)
+    k, v = (synth.round_bf16(rng.standard_normal((2 * 200, kv * HD))) for _ in range(2))
+    q = synth.round_bf16(rng.standard_normal((2 * n_q, heads * HD)))
+    ops.kv_cache_write(cache, table, i32([0, 0]), dev(k), dev(v), 2, 200, kv, counts=i32(lens))
+    kc, vc = (R.cached_values(x.reshape(-1, HD)).reshape(2, 200, kv * HD) for x in (k, v))
+    back = ops.kv_cache_read(cache, table, i32([0, 0]), 2, 150, kv)
+    for got, want in zip(back, (kc, vc)):
+        same(got, want[:, :150].reshape(300, kv * HD))
+    kc, vc = (x.reshape(2, 200, kv, HD) for x in (kc, vc))
+    ref = attend_ref(q, kc, vc, lens, n_q, heads, kv, 0, 0)
+    check(*ops.kv_cache_attention(dev(q), cache, table, i32(lens), 2, n_q, heads, kv,
+                                  want_lse=True), ref)

@@ -258,3 +258,22 @@ def test_what_the_workspace_held_does_not_matter(cuda, S, H, K):
         need, torch.cuda.current_stream().cuda_stream))
     for t, name in zip(grads, ("dq", "dk", "dv")):
         near(t, ref, name)
+
+
+def test_offsets_past_32_bits(cuda):
+    """All operands and gradients as columns of one buffer of 4.7 GB, with the largest
+    leading dimension there is."""
+    S, H, K, W, sinks, ld = 140, 2, 1, 60, 3, (1 << 24) - 8
+    x = inputs(1, S, H, K, 9)
+    ref = R.batch_attention(*x[:3], 1, S, H, K, W, sinks, d_out=x[3])
+    buf = torch.empty((S, ld), dtype=torch.bfloat16, device="cuda")
+    heads = [H, K, K, H, H, H, K, K]
+    q, k, v, d_o, out, dq, dk, dv = (buf[:, (e - n) * HD:e * HD]
+                                     for n, e in zip(heads, np.cumsum(heads)))
+    for t, a in zip((q, k, v, d_o), x):
+        t.copy_(dev(a))
+    _, lse = ops.window_attention(q, k, v, 1, S, H, K, W, sinks, out=out, want_lse=True)
+    ops.window_attention_backward(d_o, q, k, v, out, lse, 1, S, H, K, W, sinks, d_q=dq, d_k=dk,
+                                  d_v=dv)
+    for t, name in ((out, "out"), (dq, "dq"), (dk, "dk"), (dv, "dv")):
+        near(t, ref, name)
