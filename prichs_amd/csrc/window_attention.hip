@@ -435,19 +435,21 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
 
   // The step to compute next: its number and row tile.
   int cx = begin + sg, ct = tiles > 0 ? cx % tiles : 0;
-  // The step to fetch next: where its rows of q and d_o start, how many bytes the
-  // sequence has from there on (past them a copy gives zeros), and its statistics.
-  int fx = cx, ft = ct, fh = tiles > 0 ? cx / tiles : 0;
+  // Every wave of a step group moves kRowsEach of the step's rows of q and of d_o, and
+  // all of lse / delta (the same bytes).
+  constexpr int kRowsEach = kTr / kKg, kCopies = 3;
+  static_assert(kRowsEach == 4, "one copy of 16 bytes a lane each");
+  // The step to fetch next: where the wave's rows of q and d_o start, how many rows
+  // the sequence has from there on, and the step's statistics.
+  int fx = cx, ft = ct, fh = tiles > 0 ? cx / tiles : 0, left;
   const char *pq, *pd;
   const float *pr;
-  int64_t lq, ld;
   auto seek = [&]() {
-    const int h = kvh * G + fh, t0 = (t_lo + ft) * kTr;
+    const int h = kvh * G + fh, t0 = (t_lo + ft) * kTr + kRowsEach * kg;
     pq = reinterpret_cast<const char *>(a.q + (seq0 + t0) * a.ldq + (size_t)h * kHd);
     pd = reinterpret_cast<const char *>(a.d_o + (seq0 + t0) * a.ldd + (size_t)h * kHd);
-    lq = (int64_t)(L - 1 - t0) * 2 * a.ldq + 2 * kHd;
-    ld = (int64_t)(L - 1 - t0) * 2 * a.ldd + 2 * kHd;
     pr = a.rows + (((size_t)b * sh.Hq + h) * a.row_tiles + t_lo + ft) * 64;
+    left = L - t0;
   };
   seek();
   const uint32_t lds_base =
@@ -455,7 +457,7 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
   // V of the block, behind the steps' tiles.
   const uint32_t v_tile = 2 * kStages * kStepElems * 2u;
   {
-    const int left = L - blk * kBlk;
+    const int left = L - blk * kBlk;  // rows of V
     const uint64_t bytes = (uint64_t)(left - 1) * 2 * (uint64_t)a.ldv + 2 * kHd;
     const __amdgpu_buffer_rsrc_t r = buffer_rsrc(
         a.v + (seq0 + (left > 0 ? blk * kBlk : 0)) * a.ldv + (size_t)kvh * kHd,
@@ -467,33 +469,29 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
                lds_base + v_tile + (uint32_t)(2 * (kBlk / (2 * kKg) * wave + 4 * j) * kHd));
     }
   }
-  // Every wave of a step group moves 8 of the step's rows of q and of d_o, and all
-  // of lse / delta (the same bytes): 5 copies.  A step past the end copies nothing
-  // (an empty buffer: zeros), so that the count of copies in flight stays known.
-  constexpr int kRowsEach = kTr / kKg, kCopies = kRowsEach / 2 + 1;
+  // Row 4 kg + g of a step's tile has the key 2 g ^ `turn`.  A step past the end copies
+  // nothing (an empty buffer: zeros), so that the count of copies in flight stays known;
+  // rows past the sequence are zeros too.
+  const uint32_t turn = (uint32_t)tile_key(kRowsEach * kg);
   auto fetch = [&](int slot) {
     const uint32_t dst = lds_base + (uint32_t)((sg * kStages + slot) * kStepElems) * 2u;
-    const bool on = fx < end;
-    const int ln = lane_here();
-    auto rows = [&](const char *src, int64_t left, int pitch, int at) {
-      const __amdgpu_buffer_rsrc_t r =
-          buffer_rsrc(src, !on ? 0u : left > 0xffffffffll ? 0xffffffffu : (uint32_t)left);
-#pragma unroll
-      for (int j = 0; j < kRowsEach / 4; ++j) {
-        const int x = kRowsEach * kg + 4 * j + (ln >> 4);
-        copy_16b(r, 2u * ((uint32_t)x * (uint32_t)pitch + 8u * (uint32_t)((ln & 15) ^ tile_key(x))),
-                 dst + (uint32_t)(2 * (at + (kRowsEach * kg + 4 * j) * kHd)));
-      }
+    const int ln = lane_here(), n = fx < end ? min(left, kRowsEach) : 0;
+    const uint32_t gg = (uint32_t)ln >> 4, at = (((uint32_t)ln & 15) ^ (2 * gg) ^ turn) << 4;
+    auto rows = [&](const char *src, int pitch, int tile) {
+      copy_16b(buffer_rsrc(src, n <= 0 ? 0u : (uint32_t)(n - 1) * 2u * (uint32_t)pitch + 2 * kHd),
+               (2 * gg) * ((uint32_t)pitch & 0xffffffu) + at,
+               dst + (uint32_t)(2 * (tile + kRowsEach * kg * kHd)));
     };
-    rows(pq, lq, a.ldq, 0);
-    rows(pd, ld, a.ldd, kTr * kHd);
-    copy_4b(buffer_rsrc(pr, on ? 256u : 0u), 4u * (uint32_t)ln, dst + 4 * kTr * kHd);
+    rows(pq, a.ldq, 0);
+    rows(pd, a.ldd, kTr * kHd);
+    copy_4b(buffer_rsrc(pr, fx < end ? 256u : 0u), 4u * (uint32_t)ln, dst + 4 * kTr * kHd);
     fx += 2;
     ft += 2;
     if (ft < tiles) {
-      pq += 4 * kTr * (int64_t)a.ldq, lq -= 4 * kTr * (int64_t)a.ldq;
-      pd += 4 * kTr * (int64_t)a.ldd, ld -= 4 * kTr * (int64_t)a.ldd;
+      pq += 4 * kTr * (int64_t)a.ldq;
+      pd += 4 * kTr * (int64_t)a.ldd;
       pr += 2 * 64;
+      left -= 2 * kTr;
     } else if (tiles > 0) {
       while (ft >= tiles) ft -= tiles, ++fh;
       seek();
@@ -502,6 +500,7 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
 
   const uint32_t ra0 = 2u * (uint32_t)tile_off(l16, g);
   const uint32_t ta0 = 2u * (uint32_t)(tile_off(4 * g + (l16 >> 2), (l16 & 3) >> 1) + 4 * (l16 & 1));
+  const uint32_t g16 = 16u * (uint32_t)g;
   auto compute = [&](int slot) {
     const int t0 = (t_lo + ct) * kTr;
     const bool none = cx >= end || k0 >= L || t0 + kTr - 1 < k0 ||
@@ -511,10 +510,14 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
                                          k0 + 16 <= sh.sinks);
     const uint32_t at = (uint32_t)((sg * kStages + slot) * kStepElems) * 2u;
     const char *tile = reinterpret_cast<const char *>(lds) + at;
-    const uint32_t ra = at + ra0, ta = lds_base + at + ta0;
+    const uint32_t ra = lds_base + at + ra0, ta = lds_base + at + ta0;
     auto frag_at = [&](uint32_t lane_at, int kk, uint32_t off) {
-      return *reinterpret_cast<const bf16x8 *>(reinterpret_cast<const char *>(lds) +
-                                               (lane_at ^ (uint32_t)(64 * kk)) + off);
+      typedef const __attribute__((address_space(3))) bf16x8 *at_t;
+      return *(at_t)(uintptr_t)((lane_at ^ (uint32_t)(64 * kk)) + off);
+    };
+    auto stat_at = [&](uint32_t off) {
+      typedef const __attribute__((address_space(3))) f32x4 *at_t;
+      return *(at_t)(uintptr_t)(lds_base + at + 4 * kTr * kHd + g16 + off);
     };
     // x is 0 where the key's row does not see it.
     auto hide = [&](int qb, f32x4 &x) {
@@ -537,10 +540,9 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
 #pragma unroll
       for (int qb = 0; qb < 2; ++qb)
         x[qb] = mfma_bf16(frag_at(ra, kk, 2 * kHd * 16 * qb), kf[kk], x[qb]);
-    const float *st = reinterpret_cast<const float *>(tile + 4 * kTr * kHd) + 4 * g;
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
-      const f32x4 lse2 = *reinterpret_cast<const f32x4 *>(st + 16 * qb);
+      const f32x4 lse2 = stat_at(64 * qb);
 #pragma unroll
       for (int r = 0; r < 4; ++r) p[qb][r] = fast_exp2(fmaf(x[qb][r], sh.scale_log2, -lse2[r]));
     }
@@ -554,7 +556,8 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
       }
     }
     x[0] = x[1] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const uint32_t va = ra0 + v_tile + 2 * kHd * 16 * kg;
+    uint32_t va = lds_base + ra0 + v_tile + 2 * kHd * 16 * kg;
+    asm volatile("" : "+v"(va));  // its fragments' addresses are not kept over the steps
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
       const bf16x8 vf = frag_at(va, kk, 0);
@@ -565,7 +568,7 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
     f32x4 e[2];
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
-      const f32x4 delta = *reinterpret_cast<const f32x4 *>(st + kTr + 16 * qb);
+      const f32x4 delta = stat_at(4 * kTr + 64 * qb);
 #pragma unroll
       for (int r = 0; r < 4; ++r) e[qb][r] = p[qb][r] * (x[qb][r] - delta[r]);
     }
