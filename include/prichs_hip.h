@@ -357,8 +357,9 @@ int prichs_attention_forward_rope_q(const void *q, size_t ldq, const void *k,
  * its further rows of q/k/v are not used and get zeros in o.  lse (device f32
  * [batch, n_heads, seq_len], may be NULL): log of the sum of exp(score) over the
  * visible keys, for the backward (-inf past a sequence's length).  Keys that a
- * query does not see do not reach it, whatever they hold.  The reference has no
- * windowed attention. */
+ * query does not see do not reach it, whatever they hold.  Operands are 16-byte
+ * aligned; leading dimensions are multiples of 8 below 2^24, seq_len is at most
+ * 2^21.  The reference has no windowed attention. */
 int prichs_window_attention_forward(const void *q, size_t ldq, const void *k,
                                     size_t ldk, const void *v, size_t ldv, void *o,
                                     size_t ldo, float *lse, const int32_t *seq_lens,
@@ -397,10 +398,11 @@ int prichs_window_attention_backward(const void *d_o, size_t ldd, const void *q,
  * PRICHS_KV_PAGE]; sequences may share pages that none of them writes.
  *
  * Format: groups of 32 values along the head share a scale 2^(s - 127), one byte,
- * the least (1 <= s <= 252) with max|x| <= 7 * scale; a value is a 4-bit float (0, .5, 1,
- * 1.5, 2, 3, 4, 6 and a sign) times it, rounded to nearest, ties to the even code
- * (magnitudes past the largest level become it).  A group that holds an infinity or NaN reads back as NaN.  136 bytes per
- * position and kv head; what is read back is exact in bf16.
+ * the least (1 <= s <= 252) with max|x| <= 7 * scale; a value is a 4-bit float (0,
+ * .5, 1, 1.5, 2, 3, 4, 6 and a sign) times it, rounded to nearest, ties to the even
+ * code (magnitudes past the largest level become it).  A group that holds an
+ * infinity or NaN reads back as NaN.  136 bytes per position and kv head; what is
+ * read back is exact in bf16.
  *
  * write: rows b * n + i of k and v (bf16 or f32, leading dimensions ldk / ldv,
  * multiples of 8, 16-byte aligned; kv head j at column j * 128) become position
@@ -409,7 +411,7 @@ int prichs_window_attention_backward(const void *d_o, size_t ldd, const void *q,
  * skipped -- a read leaves them as they were.  Positions outside the table, and
  * pages outside [0, n_pages), are not written and read as zeros.  A position must
  * not be written twice in one call, nor read by a call that may run at the same
- * time. */
+ * time.  batch * n * n_kv_heads is below 2^28. */
 #define PRICHS_KV_PAGE 64
 #define PRICHS_KV_HEAD_DIM 128
 #define PRICHS_KV_PAGE_BYTES 8704 /* of one kv head */

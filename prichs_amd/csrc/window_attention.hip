@@ -85,21 +85,28 @@ struct BwdArgs {
   // d_o . o of the rows; a row past the sequence has +inf and 0 (p = 0).
   float *rows;
   int row_tiles;  // 32-row tiles of a (sequence, head) there
-  float *part;    // f32 partial d_k, d_v (dkv_kernel)
-  int budget;     // steps of a workgroup (dkv_kernel)
+  float *part;    // f32 partial d_k, d_v (window_dkv_kernel)
+  int budget;     // steps of a workgroup there
   Shape sh;
 };
 
 // ---------------------------------------------------------------- d_q --------
-// As the forward (attention.hip): a wave owns 32 query rows of one head, HPW heads
-// of a kv group share the K / V tiles that the workgroup streams through LDS (64
-// keys, two stages).
+// As the forward (attention.hip): a wave owns NB blocks of 16 query rows of one
+// head, HPW heads of a kv group share the K / V tiles that the workgroup streams
+// through LDS (64 keys, two stages).
 //   S^T = K Q^T, dP^T = V d_o^T   both operands' rows straight from LDS / registers
 //   dS^T = exp2(S scale log2(e) - lse) (dP - delta)   in the accumulator layout,
 //                   which is the operand layout of
 //   dQ^T += K^T dS^T              K^T by transposing LDS reads
-// The kernel also forms delta of its rows and leaves it, with lse, to dkv_kernel.
-constexpr int kTr = 32;  // rows of a step of dkv_kernel
+// The kernel also forms delta of its rows and leaves it, with lse, to
+// window_dkv_kernel.  12 + 3 heads: 4 x 2048, window 512, 69 us; 1 x 4096 whole 116
+// us (670 TFLOP/s); 3 x 500, window 128, 21 us.  Long windows are bound by the matrix
+// cores (busy 55% of the time) and the vector instructions between their products,
+// which the two waves of a SIMD overlap little; short ones by the latency of a block
+// (load, barrier, two dependent products: 1.5 us), twice for rows of few blocks.
+// Eight waves of 16 rows a workgroup on the same tiles were no faster (170 -> 167,
+// 1481 -> 1552 us for the whole backward of 4 x 2048 and of 1 x 16384, window 4096).
+constexpr int kTr = 32;  // rows of a step of window_dkv_kernel
 constexpr int kKeys = 64;
 constexpr int kQStage = 2 * kKeys * kHd;  // elements: K, then V
 constexpr int kExactBlocks = 4;  // delta in a sweep of its own up to so many blocks
@@ -338,25 +345,33 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
 
 // ------------------------------------------------------------ d_k, d_v -------
 // A workgroup owns 128 keys of one kv head and runs over the (query head, 32-row
-// tile) steps that see them.  8 waves: 4 key groups of 32 keys, whose K and V
-// fragments and f32 gradients stay in registers, times 2 step groups, which take
+// tile) steps that see them.  16 waves: 8 key groups of 16 keys, whose K fragments
+// and f32 gradients stay in registers and V in LDS, times 2 step groups, which take
 // every second step and join in LDS at the end.
 //   S = Q K^T, dP = d_o V^T       rows of the q and d_o tiles straight from LDS
 //   P, dS                         in the accumulator layout, which is the operand
 //                                 layout (a lane holds one key and 8 of 32 rows) of
 //   dV^T += d_o^T P, dK^T += Q^T dS   by transposing LDS reads
-// 64 products a step and wave against 32 KB of LDS reads: four waves a step group
-// take the LDS's whole bandwidth at the full rate of the matrix cores.
+// Tiles come in three stages, so that a step's copies have the time of two steps.
+// 12 + 3 heads: 4 x 2048, window 512, 98 us; 1 x 4096 whole 160 us (640 TFLOP/s), 1 x
+// 16384, window 4096, 900 us (800); 3 x 500, window 128, 21 us.  No single unit bounds it: without the copies it takes
+// 2 to 7% less, without the transposing reads 2 to 7%, without the exponentials 1.5%;
+// the matrix cores are busy 40% of the time, LDS 50%, and what is left is the latency of a step
+// (reads, four dependent products, exponentials, products) that four waves a SIMD,
+// held together by a barrier a step, do not hide.  With 32 keys a wave (two waves a
+// SIMD, half the LDS reads) the whole backward of 4 x 2048 takes 187 us instead of 157
+// and that of 1 x 16384, window 4096, 1390 instead of 1413; 64-key blocks, two
+// workgroups a CU, 195 and 1740.  No register may spill in the loop: a reload waits for
+// all copies in flight (7%).
 // Steps are cut into items of at most `budget` (a block that holds sinks is seen by
 // every later row); the items of one block meet in f32 partial sums that
-// dkv_join_kernel adds in order.
-constexpr int kBlk = 128;                       // keys of a workgroup
-constexpr int kKb = 1;                          // 16-key blocks of a wave
-constexpr int kKg = kBlk / (16 * kKb);          // key groups
+// window_dkv_join_kernel adds in order.
+constexpr int kBlk = 128;           // keys of a workgroup
+constexpr int kKg = kBlk / 16;      // key groups
 constexpr int kStages = 3;
-constexpr int kStepElems = 2 * kTr * kHd + 128; // q, d_o, then lse / delta (64 floats)
+constexpr int kStepElems = 2 * kTr * kHd + 128;  // q, d_o, then lse / delta (64 floats)
 constexpr size_t kKvLds = (2 * kStages * (size_t)kStepElems + kBlk * kHd) * sizeof(bf16_t);
-static_assert(kKvLds >= kKg * 8 * kKb * 64 * sizeof(f32x4), "the join of the step groups fits");
+static_assert(kKvLds >= kKg * 8 * 64 * sizeof(f32x4), "the join of the step groups fits");
 
 // Steps of key block j over sequences of S rows.
 __host__ __device__ inline int steps_of(const Shape &sh, int rows, int j) {
@@ -410,7 +425,7 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
 
   bf16x8 kf[4];
   f32x4 dk[8], dv[8];
-{
+  {
     const int key = k0 + l16;
     const size_t r = seq0 + min(key, sh.S - 1), c = (size_t)kvh * kHd + 8 * g;
     const bool live = key < L;
@@ -423,8 +438,7 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
     }
   }
 #pragma unroll
-  for (int jd = 0; jd < 8; ++jd)
-    dk[jd] = dv[jd] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int jd = 0; jd < 8; ++jd) dk[jd] = dv[jd] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   // This item's steps: step x is head x / tiles, row tile t_lo + x % tiles.
   const int steps = steps_of(sh, L, blk), tiles = steps / G;
@@ -531,6 +545,9 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
         x[r] = seen ? x[r] : 0.f;
       }
     };
+    // Softmax and first products before the other waves' last ones: 1 x 16384 window
+    // 4096 1411 -> 1390 us, 4 x 2048 158.7 -> 156.
+    __builtin_amdgcn_s_setprio(1);
     u32x4 pf, ds;  // P and dS rounded to bf16 for the products
     float z = 0.f;
     f32x4 p[2], x[2];  // of 16 rows each
@@ -588,6 +605,7 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
     // the products of a step that not every key's row sees.
     const bool rare = !whole && __any(!(z == 0.f)) != 0;
     constexpr int kDo = 2 * kTr * kHd;  // bytes to the d_o tile
+    __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int j0 = 0; j0 < 8; j0 += 4) {
       u32x4 f[4];
@@ -595,18 +613,16 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
       for (int t = 0; t < 4; ++t) f[t] = read_tr((ta ^ (uint32_t)(32 * (j0 + t))) + kDo);
       if (rare) finite_frags(f);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-          dv[j0 + t] = mfma_bf16(__builtin_bit_cast(bf16x8, f[t]), __builtin_bit_cast(bf16x8, pf),
-                                     dv[j0 + t]);
-      }
+      for (int t = 0; t < 4; ++t)
+        dv[j0 + t] = mfma_bf16(__builtin_bit_cast(bf16x8, f[t]), __builtin_bit_cast(bf16x8, pf),
+                               dv[j0 + t]);
 #pragma unroll
       for (int t = 0; t < 4; ++t) f[t] = read_tr(ta ^ (uint32_t)(32 * (j0 + t)));
       if (rare) finite_frags(f);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-          dk[j0 + t] = mfma_bf16(__builtin_bit_cast(bf16x8, f[t]), __builtin_bit_cast(bf16x8, ds),
-                                     dk[j0 + t]);
-      }
+      for (int t = 0; t < 4; ++t)
+        dk[j0 + t] = mfma_bf16(__builtin_bit_cast(bf16x8, f[t]), __builtin_bit_cast(bf16x8, ds),
+                               dk[j0 + t]);
     }
     if (rare) {
       // The infinities and NaN of d_o that were taken out, for the keys that their
@@ -620,16 +636,14 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
           asm volatile("" ::: "memory");  // one load after the other: registers
           const u32x2 raw = *reinterpret_cast<const u32x2 *>(
               tile + kDo + ((uint32_t)(2 * (tile_off(x, g >> 1) + 4 * (g & 1))) ^ (32u * jd)));
-{
-            const int key = k0 + l16;
-            const bool seen = (key <= row) & ((sh.window == 0) | (row - key < sh.window) |
-                                              (key < sh.sinks));
+          const int key = k0 + l16;
+          const bool seen = (key <= row) & ((sh.window == 0) | (row - key < sh.window) |
+                                            (key < sh.sinks));
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const uint32_t u = r & 1 ? raw[r / 2] & 0xffff0000u : raw[r / 2] << 16;
-              const bool off = (u & 0x7f800000u) == 0x7f800000u;
-              dv[jd][r] += (off & seen) ? __uint_as_float(u) : 0.f;
-            }
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t u = r & 1 ? raw[r / 2] & 0xffff0000u : raw[r / 2] << 16;
+            const bool off = (u & 0x7f800000u) == 0x7f800000u;
+            dv[jd][r] += (off & seen) ? __uint_as_float(u) : 0.f;
           }
         }
       }
@@ -659,14 +673,12 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
   auto joined = [&](f32x4 (&x)[8]) {
     if (sg == 1) {
 #pragma unroll
-      for (int jd = 0; jd < 8; ++jd)
-join[((jd) * kKg + kg) * 64 + le] = x[jd];
+      for (int jd = 0; jd < 8; ++jd) join[(jd * kKg + kg) * 64 + le] = x[jd];
     }
     __syncthreads();
     if (sg == 0) {
 #pragma unroll
-      for (int jd = 0; jd < 8; ++jd)
-          x[jd] = x[jd] + join[((jd) * kKg + kg) * 64 + le];
+      for (int jd = 0; jd < 8; ++jd) x[jd] = x[jd] + join[(jd * kKg + kg) * 64 + le];
     }
     __syncthreads();
   };
@@ -675,35 +687,32 @@ join[((jd) * kKg + kg) * 64 + le] = x[jd];
   if (sg != 0) return;
   if (n_split > 1) {
     float *part = a.part + ((((size_t)b * sh.Hkv + kvh) * gridDim.x + blockIdx.x) * 2) * kBlk * kHd;
-{
-      float *row = part + (16 * kg + l16e) * kHd + 4 * ge;
+    float *row = part + (16 * kg + l16e) * kHd + 4 * ge;
 #pragma unroll
-      for (int jd = 0; jd < 8; ++jd) {
-        *reinterpret_cast<f32x4 *>(row + 16 * jd) = dk[jd];
-        *reinterpret_cast<f32x4 *>(row + kBlk * kHd + 16 * jd) = dv[jd];
-      }
+    for (int jd = 0; jd < 8; ++jd) {
+      *reinterpret_cast<f32x4 *>(row + 16 * jd) = dk[jd];
+      *reinterpret_cast<f32x4 *>(row + kBlk * kHd + 16 * jd) = dv[jd];
     }
     return;
   }
-{
-    const int key = k0 + l16e;
-    if (key >= sh.S) return;
-    bf16_t *ok = a.dk + (seq0 + key) * a.lddk + (size_t)kvh * kHd + 4 * ge;
-    bf16_t *ov = a.dv + (seq0 + key) * a.lddv + (size_t)kvh * kHd + 4 * ge;
-    const bool live = key < L;
+  const int key = k0 + l16e;
+  if (key >= sh.S) return;
+  bf16_t *ok = a.dk + (seq0 + key) * a.lddk + (size_t)kvh * kHd + 4 * ge;
+  bf16_t *ov = a.dv + (seq0 + key) * a.lddv + (size_t)kvh * kHd + 4 * ge;
+  const bool live = key < L;
 #pragma unroll
-    for (int jd = 0; jd < 8; ++jd) {
-      const f32x4 x = dk[jd] * sh.scale, y = dv[jd];
-      const u32x2 ux = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
-      const u32x2 uy = u32x2{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])};
-      *reinterpret_cast<u32x2 *>(ok + 16 * jd) = live ? ux : u32x2{0, 0};
-      *reinterpret_cast<u32x2 *>(ov + 16 * jd) = live ? uy : u32x2{0, 0};
-    }
+  for (int jd = 0; jd < 8; ++jd) {
+    const f32x4 x = dk[jd] * sh.scale, y = dv[jd];
+    const u32x2 ux = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+    const u32x2 uy = u32x2{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])};
+    *reinterpret_cast<u32x2 *>(ok + 16 * jd) = live ? ux : u32x2{0, 0};
+    *reinterpret_cast<u32x2 *>(ov + 16 * jd) = live ? uy : u32x2{0, 0};
   }
 }
 
 // Adds the items of the blocks that were cut, in the items' order: a workgroup per
-// (block, kv head, sequence) and 16 of its keys.
+// (block, kv head, sequence) and 16 of its keys.  Bound by the latency of its loads
+// (3 x 500, window 128: 6 us).
 __global__ __launch_bounds__(256) void window_dkv_join_kernel(BwdArgs a, int items) {
   const Shape &sh = a.sh;
   const int blk = blockIdx.x / (kBlk / 16), kvh = blockIdx.y, b = blockIdx.z;
@@ -915,6 +924,10 @@ extern "C" int prichs_window_attention_backward(
   const int hpw = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
   const size_t blocks = cdiv(seq_len, (size_t)kBlk), n_qb32 = cdiv(seq_len, (size_t)(128 / hpw));
   const bool few = 2 * (n_heads / hpw) * batch * n_qb32 <= 3 * 256;
+  // Rows of a wave of the d_q kernel, by the forward's rule (attention.hip).  Whole
+  // backward, 32 -> 16 rows, us: 1 x 777 52 -> 46, 3 x 500 56 -> 50, 1 x 4096 277 ->
+  // 260, 4 x 1024 (384 workgroups) 81.6 -> 81.9, 4 x 2048 169 -> 173, 1 x 16384 1499 ->
+  // 1671.
   // The d_q kernel writes the statistics of whole 32-row tiles, so its rows go to the
   // end of the last one.
   const size_t n_qb = few ? cdiv(roundup(seq_len, (size_t)kTr), (size_t)(64 / hpw)) : n_qb32;
