@@ -236,23 +236,43 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
         if (!whole) {
           // What a row does not see must not reach it: hidden elements become p = 0,
           // and an infinity or NaN in K^T, which 0 would turn into NaN, is taken out
-          // of the product (a row that sees such a key has NaN in dS).
+          // of the product (a row that sees such a key has NaN in dS).  Rows past the
+          // sequence need no mask: their lse is +inf, and they reach no other row.
+          // The wave's rows decide which of the rules a block needs.
           float z = 0.f;
+          const bool ahead = kv0 + kKeys - 1 > q0;
+          const bool behind = sh.window != 0 && q0 + 16 * NB - 1 - kv0 >= sh.window &&
+                              kv0 + kKeys > sh.sinks;
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-              z = not_finite(s[c][nb], z);
-              const int row = q0 + 16 * nb + l16, key = kv0 + 32 * half + 16 * c + 4 * g;
+            for (int nb = 0; nb < NB; ++nb) z = not_finite(s[c][nb], z);
+          const int first_key = kv0 + 32 * half + 4 * g - (q0 + l16);
+          if (ahead) {
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const bool seen = (key + r <= row) & (row < L) &
-                                  ((sh.window == 0) | (row - key - r < sh.window) |
-                                   (key + r < sh.sinks));
-                s[c][nb][r] = seen ? s[c][nb][r] : -INFINITY;
-                dp[c][nb][r] = seen ? dp[c][nb][r] : 0.f;
-              }
-            }
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const bool hidden = first_key > 16 * nb - 16 * c - r;
+                  s[c][nb][r] = hidden ? -INFINITY : s[c][nb][r];
+                  dp[c][nb][r] = hidden ? 0.f : dp[c][nb][r];
+                }
+          }
+          if (behind) {
+            const int old = first_key + sh.window, sink = sh.sinks - (kv0 + 32 * half + 4 * g);
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const bool hidden = (old <= 16 * nb - 16 * c - r) & (sink <= 16 * c + r);
+                  s[c][nb][r] = hidden ? -INFINITY : s[c][nb][r];
+                  dp[c][nb][r] = hidden ? 0.f : dp[c][nb][r];
+                }
+          }
           rare = __any(!(z == 0.f)) != 0;
         }
         f(half_c, stage, s, dp, rare);
