@@ -53,6 +53,7 @@ struct WindowArgs {
   float *lse;
   const int32_t *seq_lens;
   int window, sinks;
+  int pairs;  // head sets times sequences
 };
 constexpr size_t kWinLdsBytes = kLdsBytes + 16;  // and a flag
 constexpr float kLazy = 8.0f;  // log2 headroom of the lazily raised softmax max
@@ -93,12 +94,13 @@ __device__ __forceinline__ bf16x8 rope_frag(bf16x8 f, float4 c4, float4 s4) {
 // NB: 16-row query blocks per wave.  WIN: window attention -- a sliding window,
 // sinks, sequences of their own lengths, and the log-sum-exp written (the
 // arguments in wa); row i of a sequence then sees the keys j <= i with i - j <
-// window (0: all) or j < sinks.  12 + 3 heads with a window: 1 x 16384 of 4096 400 us
-// (900 TFLOP/s), 4 x 2048 of 512 49 us (460), 1 x 4096 whole 76 us (680), bound as
+// window (0: all) or j < sinks.  DIE: workgroups dealt by die (attention_tile.hpp).
+// 12 + 3 heads with a window: 1 x 16384 of 4096 367 us
+// (980 TFLOP/s), 4 x 2048 of 512 49 us (460), 1 x 4096 whole 76 us (680), bound as
 // without one; a block of keys that some rows do not see costs its masks and a scan
 // of V (a whole causal 4 x 2048 takes 65 us here and 60 there).  1 x 777 of 256 13 us:
 // the latency of its five blocks of keys.
-template <int HPW, int NB, bool WIN>
+template <int HPW, int NB, bool WIN, bool DIE = false>
 __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
     const bf16_t *__restrict__ q, int ldq, const bf16_t *__restrict__ k, int ldk,
     const bf16_t *__restrict__ v, int ldv, bf16_t *__restrict__ o, int ldo, int S, int Hq,
@@ -112,13 +114,17 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
   // so every head set's longest causal rows (the last query block) go first.
   const int n_qb = (S + kRowsWg - 1) / kRowsWg;
   const int sets = group / HPW;  // head sets per kv group
-  const int kvh = blockIdx.x / sets;
-  const int b = blockIdx.y;
-  const int qb = n_qb - 1 - (int)blockIdx.z;
+  int x = blockIdx.x, b = blockIdx.y, qb = n_qb - 1 - (int)blockIdx.z;
+  if constexpr (DIE) {
+    int pair, rank;
+    if (!die_rank(blockIdx.x, wa.pairs, n_qb, &pair, &rank)) return;
+    b = pair / (Hq / HPW), x = pair - b * (Hq / HPW), qb = n_qb - 1 - rank;
+  }
+  const int kvh = x / sets;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int h = kvh * group + (blockIdx.x - kvh * sets) * HPW + wave % HPW;
+  const int h = kvh * group + (x - kvh * sets) * HPW + wave % HPW;
   const int g = lane >> 4;    // 0..3
   const int l16 = lane & 15;  // 0..15
 
@@ -636,17 +642,26 @@ int window_attention_launch(const void *q, size_t ldq, const void *k, size_t ldk
   const size_t n_qb = few ? cdiv(seq_len, (size_t)(16 * kWaves / hpw)) : n_qb32;
   PRICHS_REQUIRE(n_qb <= 65535, "window_attention: seq_len too large");
   const float scale_log2 = (1.0f / sqrtf((float)kHd)) * 1.4426950408889634f;
-  const dim3 grid((unsigned)(n_heads / hpw), (unsigned)batch, (unsigned)n_qb);
+  const size_t pairs = n_heads / hpw * batch;
+  const bool dies = !few && by_die(seq_len, window, pairs, n_qb);
+  const dim3 grid = dies ? dim3((unsigned)die_grid(pairs, n_qb))
+                         : dim3((unsigned)(n_heads / hpw), (unsigned)batch, (unsigned)n_qb);
   static const struct {
     decltype(&attn_fwd_kernel<4, 2, true>) kernel;
     int hpw;
-    bool few;
-  } kinds[] = {{attn_fwd_kernel<4, 1, true>, 4, true},  {attn_fwd_kernel<2, 1, true>, 2, true},
-               {attn_fwd_kernel<1, 1, true>, 1, true},  {attn_fwd_kernel<4, 2, true>, 4, false},
-               {attn_fwd_kernel<2, 2, true>, 2, false}, {attn_fwd_kernel<1, 2, true>, 1, false}};
-  static LdsLimit limits[6];
+    bool few, dies;
+  } kinds[] = {{attn_fwd_kernel<4, 1, true>, 4, true, false},
+               {attn_fwd_kernel<2, 1, true>, 2, true, false},
+               {attn_fwd_kernel<1, 1, true>, 1, true, false},
+               {attn_fwd_kernel<4, 2, true>, 4, false, false},
+               {attn_fwd_kernel<2, 2, true>, 2, false, false},
+               {attn_fwd_kernel<1, 2, true>, 1, false, false},
+               {attn_fwd_kernel<4, 2, true, true>, 4, false, true},
+               {attn_fwd_kernel<2, 2, true, true>, 2, false, true},
+               {attn_fwd_kernel<1, 2, true, true>, 1, false, true}};
+  static LdsLimit limits[9];
   int i = 0;
-  while (kinds[i].hpw != hpw || kinds[i].few != few) ++i;
+  while (kinds[i].hpw != hpw || kinds[i].few != few || kinds[i].dies != dies) ++i;
   const auto kern = kinds[i].kernel;
   if (int rc = raise_lds_limit(limits[i], reinterpret_cast<const void *>(kern), kWinLdsBytes,
                                "window_attention"))
@@ -656,7 +671,7 @@ int window_attention_launch(const void *q, size_t ldq, const void *k, size_t ldk
                      (int)ldk, static_cast<const bf16_t *>(v), (int)ldv,
                      static_cast<bf16_t *>(o), (int)ldo, (int)seq_len, (int)n_heads, group,
                      scale_log2, nullptr, nullptr, 0,
-                     WindowArgs{lse, seq_lens, (int)window, (int)sinks});
+                     WindowArgs{lse, seq_lens, (int)window, (int)sinks, (int)pairs});
   PRICHS_LAUNCH_CHECK("window_attention launch");
   return PRICHS_OK;
 }

@@ -87,4 +87,29 @@ __device__ __forceinline__ uint32_t finite_bf16x2(uint32_t u) {
   return u;
 }
 
+// Workgroups whose keys (or query rows) are their neighbours' too, on one die: of the
+// eight dies, each with an L2 of its own, workgroup `id` runs on die id % 8.  A launch
+// of die_grid(pairs, n) workgroups covers the ranks 0 .. n - 1 of `pairs` sequences'
+// heads in runs of kDieRun neighbouring ranks, low ranks first; false: none left.
+constexpr int kDieRun = 8;
+__device__ __forceinline__ bool die_rank(unsigned id, int pairs, int n, int *pair, int *rank) {
+  const int j = id >> 3, run = j / kDieRun * 8 + (id & 7), c = run / pairs;
+  *pair = run - c * pairs;
+  *rank = c * kDieRun + j % kDieRun;
+  return *rank < n;
+}
+inline size_t die_grid(size_t pairs, size_t n) {
+  return 8 * kDieRun * cdiv(pairs * cdiv(n, (size_t)kDieRun), (size_t)8);
+}
+// With a window, from this many rows on; below, neighbours mostly run at the same time
+// on all dies, and without one the longest rows would not all come first.  In launch
+// order -> by die, us: forward 1 x 16384 window 4096 393 -> 367, 1 x 8192 window 1024 79.1
+// -> 73.4, window 128 31.7 -> 29.4, 1 x 4096 window 512 34.2 -> 34.4, 2 x 8192 whole 389 ->
+// 395; backward 1 x 16384 1378 -> 1353, 1 x 8192 window 128 92.5 -> 88.7, 1 x 4096 104 -> 105.6.
+constexpr size_t kDieRows = 8192;
+inline bool by_die(size_t seq_len, size_t window, size_t pairs, size_t n) {
+  constexpr size_t kMost = (size_t)1 << 21;  // workgroups, of 1024 threads at most
+  return seq_len >= kDieRows && window != 0 && pairs <= kMost && die_grid(pairs, n) <= kMost;
+}
+
 }  // namespace prichs

@@ -87,6 +87,10 @@ struct BwdArgs {
   int row_tiles;  // 32-row tiles of a (sequence, head) there
   float *part;    // f32 partial d_k, d_v (window_dkv_kernel)
   int budget;     // steps of a workgroup there
+  int items;      // items of a (sequence, kv head) there
+  // For workgroups dealt by die: row blocks of window_dq_kernel, and the (sequence,
+  // head set) pairs there and (sequence, kv head) pairs in window_dkv_kernel.
+  int dq_blocks, dq_pairs, dkv_pairs;
   Shape sh;
 };
 
@@ -112,18 +116,23 @@ constexpr int kQStage = 2 * kKeys * kHd;  // elements: K, then V
 constexpr int kExactBlocks = 4;  // delta in a sweep of its own up to so many blocks
 constexpr size_t kQLds = 2 * (size_t)kQStage * sizeof(bf16_t);
 
-// NB: 16-row blocks of a wave.
-template <int HPW, int NB>
+// NB: 16-row blocks of a wave.  DIE: workgroups dealt by die (attention_tile.hpp).
+template <int HPW, int NB, bool DIE = false>
 __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
   constexpr int kRowsWg = 64 * NB / HPW;
   extern __shared__ __attribute__((aligned(16))) bf16_t lds[];
   const Shape &sh = a.sh;
   const int group = sh.Hq / sh.Hkv, sets = group / HPW;
-  const int kvh = blockIdx.x / sets, b = blockIdx.y;
-  const int qb = (int)(gridDim.z - 1 - blockIdx.z);  // long rows first
+  int x = blockIdx.x, b = blockIdx.y, qb = (int)(gridDim.z - 1 - blockIdx.z);  // long rows first
+  if constexpr (DIE) {
+    int pair, rank;
+    if (!die_rank(blockIdx.x, a.dq_pairs, a.dq_blocks, &pair, &rank)) return;
+    b = pair / (sh.Hq / HPW), x = pair - b * (sh.Hq / HPW), qb = a.dq_blocks - 1 - rank;
+  }
+  const int kvh = x / sets;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int h = kvh * group + (blockIdx.x - kvh * sets) * HPW + wave % HPW;
+  const int h = kvh * group + (x - kvh * sets) * HPW + wave % HPW;
   const int q0 = qb * kRowsWg + (wave / HPW) * 16 * NB;
   const int L = rows_of(a.seq_lens, b, sh.S);
   const size_t seq0 = (size_t)b * sh.S;
@@ -427,13 +436,19 @@ __device__ __forceinline__ void item_at(const Shape &sh, int budget, int item, i
   *block = blocks - 1, *split = 0;  // not reached: the grid holds the items
 }
 
+template <bool DIE>
 __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
   extern __shared__ __attribute__((aligned(16))) bf16_t lds[];
   const Shape &sh = a.sh;
   const int G = sh.Hq / sh.Hkv;
-  const int kvh = blockIdx.y, b = blockIdx.z;
+  int item = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+  if constexpr (DIE) {
+    int pair;
+    if (!die_rank(blockIdx.x, a.dkv_pairs, a.items, &pair, &item)) return;
+    b = pair / sh.Hkv, kvh = pair - b * sh.Hkv;
+  }
   int blk, split;
-  item_at(sh, a.budget, blockIdx.x, &blk, &split);
+  item_at(sh, a.budget, item, &blk, &split);
   blk = __builtin_amdgcn_readfirstlane(blk);
   const int n_split = splits_of(sh, a.budget, blk);
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, l16 = lane & 15;
@@ -706,7 +721,7 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
   joined(dv);
   if (sg != 0) return;
   if (n_split > 1) {
-    float *part = a.part + ((((size_t)b * sh.Hkv + kvh) * gridDim.x + blockIdx.x) * 2) * kBlk * kHd;
+    float *part = a.part + ((((size_t)b * sh.Hkv + kvh) * a.items + item) * 2) * kBlk * kHd;
     float *row = part + (16 * kg + l16e) * kHd + 4 * ge;
 #pragma unroll
     for (int jd = 0; jd < 8; ++jd) {
@@ -733,7 +748,7 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
 // Adds the items of the blocks that were cut, in the items' order: a workgroup per
 // (block, kv head, sequence) and 16 of its keys.  Bound by the latency of its loads
 // (3 x 500, window 128: 6 us).
-__global__ __launch_bounds__(256) void window_dkv_join_kernel(BwdArgs a, int items) {
+__global__ __launch_bounds__(256) void window_dkv_join_kernel(BwdArgs a) {
   const Shape &sh = a.sh;
   const int blk = blockIdx.x / (kBlk / 16), kvh = blockIdx.y, b = blockIdx.z;
   const int n_split = splits_of(sh, a.budget, blk);
@@ -747,7 +762,7 @@ __global__ __launch_bounds__(256) void window_dkv_join_kernel(BwdArgs a, int ite
   if (row >= sh.S) return;
   const bool live = row < rows_of(a.seq_lens, b, sh.S);
   const float *part =
-      a.part + ((((size_t)b * sh.Hkv + kvh) * items + item) * 2) * kBlk * kHd + key * kHd + d;
+      a.part + ((((size_t)b * sh.Hkv + kvh) * a.items + item) * 2) * kBlk * kHd + key * kHd + d;
   f32x4 t[2][2];
 #pragma unroll
   for (int w = 0; w < 2; ++w) t[w][0] = t[w][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -952,31 +967,43 @@ extern "C" int prichs_window_attention_backward(
   // end of the last one.
   const size_t n_qb = few ? cdiv(roundup(seq_len, (size_t)kTr), (size_t)(64 / hpw)) : n_qb32;
   PRICHS_REQUIRE(n_qb <= 65535 && n_kv_heads <= 65535, "%s: shape too large", who);
+  const size_t dq_pairs = n_heads / hpw * batch, dkv_pairs = n_kv_heads * batch;
+  const bool dq_dies = !few && by_die(seq_len, sh.window, dq_pairs, n_qb),
+             dkv_dies = by_die(seq_len, sh.window, dkv_pairs, plan.items);
   const auto bf = [](const void *p) { return static_cast<const bf16_t *>(p); };
   const auto out = [](void *p) { return static_cast<bf16_t *>(p); };
   BwdArgs a{bf(d_o), bf(q), bf(k), bf(v), bf(o), lse, seq_lens, out(d_q), out(d_k), out(d_v),
             (int)ldd, (int)ldq, (int)ldk, (int)ldv, (int)ldo, (int)lddq, (int)lddk, (int)lddv,
             static_cast<float *>(workspace), (int)cdiv(seq_len, (size_t)kTr),
-            reinterpret_cast<float *>(static_cast<char *>(workspace) + stats), plan.budget, sh};
+            reinterpret_cast<float *>(static_cast<char *>(workspace) + stats), plan.budget,
+            (int)plan.items, (int)n_qb, (int)dq_pairs, (int)dkv_pairs, sh};
   auto dq_kern = few ? (hpw == 4   ? window_dq_kernel<4, 1>
                         : hpw == 2 ? window_dq_kernel<2, 1>
                                    : window_dq_kernel<1, 1>)
-                     : (hpw == 4   ? window_dq_kernel<4, 2>
-                        : hpw == 2 ? window_dq_kernel<2, 2>
-                                   : window_dq_kernel<1, 2>);
-  hipLaunchKernelGGL(dq_kern, dim3((unsigned)(n_heads / hpw), (unsigned)batch, (unsigned)n_qb),
+                 : dq_dies ? (hpw == 4   ? window_dq_kernel<4, 2, true>
+                              : hpw == 2 ? window_dq_kernel<2, 2, true>
+                                         : window_dq_kernel<1, 2, true>)
+                           : (hpw == 4   ? window_dq_kernel<4, 2>
+                              : hpw == 2 ? window_dq_kernel<2, 2>
+                                         : window_dq_kernel<1, 2>);
+  hipLaunchKernelGGL(dq_kern,
+                     dq_dies ? dim3((unsigned)die_grid(dq_pairs, n_qb))
+                             : dim3((unsigned)(n_heads / hpw), (unsigned)batch, (unsigned)n_qb),
                      dim3(256), kQLds, as_stream(stream), a);
   PRICHS_LAUNCH_CHECK("window_attention_backward d_q launch");
-  static LdsLimit limit;
-  WINDOW_TRY(raise_lds_limit(limit, reinterpret_cast<const void *>(window_dkv_kernel), kKvLds, who));
-  hipLaunchKernelGGL(window_dkv_kernel,
-                     dim3((unsigned)plan.items, (unsigned)n_kv_heads, (unsigned)batch), dim3(128 * kKg),
+  static LdsLimit limits[2];
+  auto dkv_kern = dkv_dies ? window_dkv_kernel<true> : window_dkv_kernel<false>;
+  WINDOW_TRY(raise_lds_limit(limits[dkv_dies], reinterpret_cast<const void *>(dkv_kern), kKvLds, who));
+  hipLaunchKernelGGL(dkv_kern,
+                     dkv_dies ? dim3((unsigned)die_grid(dkv_pairs, plan.items))
+                              : dim3((unsigned)plan.items, (unsigned)n_kv_heads, (unsigned)batch),
+                     dim3(128 * kKg),
                      kKvLds, as_stream(stream), a);
   PRICHS_LAUNCH_CHECK("window_attention_backward d_k / d_v launch");
   if (plan.cut) {
     hipLaunchKernelGGL(window_dkv_join_kernel,
                        dim3((unsigned)(kBlk / 16 * blocks), (unsigned)n_kv_heads, (unsigned)batch),
-                       dim3(256), 0, as_stream(stream), a, (int)plan.items);
+                       dim3(256), 0, as_stream(stream), a);
     PRICHS_LAUNCH_CHECK("window_attention_backward join launch");
   }
   return PRICHS_OK;

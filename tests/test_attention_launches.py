@@ -45,14 +45,14 @@ def test_window_attention_variants():
     (_, big), (_, small), (_, two), (_, one) = window(
         [(4, 2048, 12, 3, 512, 4), (1, 777, 12, 3, 256, 4), (2, 300, 6, 3, 0, 0),
          (1, 300, 5, 5, 0, 0)])
-    assert big[0].kernel == "attn_fwd_kernel<4, 2, true>" and big[0].grid == [3, 4, 64]
-    assert big[1].kernel == "window_dq_kernel<4, 2>" and big[1].grid == [3, 4, 64]
-    assert small[0].kernel == "attn_fwd_kernel<4, 1, true>" and small[0].grid == [3, 1, 49]
-    assert small[1].kernel == "window_dq_kernel<4, 1>"
-    assert two[0].kernel == "attn_fwd_kernel<2, 1, true>"
-    assert one[0].kernel == "attn_fwd_kernel<1, 1, true>"
+    assert big[0].kernel == "attn_fwd_kernel<4, 2, true, false>" and big[0].grid == [3, 4, 64]
+    assert big[1].kernel == "window_dq_kernel<4, 2, false>" and big[1].grid == [3, 4, 64]
+    assert small[0].kernel == "attn_fwd_kernel<4, 1, true, false>" and small[0].grid == [3, 1, 49]
+    assert small[1].kernel == "window_dq_kernel<4, 1, false>"
+    assert two[0].kernel == "attn_fwd_kernel<2, 1, true, false>"
+    assert one[0].kernel == "attn_fwd_kernel<1, 1, true, false>"
     for launches in (big, small, two, one):
-        assert launches[2].kernel == "window_dkv_kernel" and launches[2].lds <= 160 * 1024
+        assert launches[2].kernel == "window_dkv_kernel<false>" and launches[2].lds <= 160 * 1024
 
 
 def test_key_blocks_are_cut_where_few_or_seen_by_many_rows():
@@ -69,6 +69,23 @@ def test_key_blocks_are_cut_where_few_or_seen_by_many_rows():
     # The partial sums of an item are 128 keys of d_k and of d_v in f32.
     stats = 4 * 12 * 64 * 64 * 4
     assert need0 == stats and need1 == stats + sinks[2].grid[0] * 12 * 2 * 128 * 128 * 4
+
+
+def test_long_sequences_are_dealt_to_the_dies():
+    # With a window from 8192 rows on: runs of 8 row blocks (8 key blocks) in a grid of one
+    # dimension.
+    (_, long), (_, ragged), (_, whole), (_, few) = window(
+        [(4, 8192, 12, 3, 512, 0), (1, 8200, 6, 3, 64, 0), (4, 8192, 12, 3, 0, 0),
+         (1, 8200, 4, 1, 64, 0)])
+    assert long[0].kernel == "attn_fwd_kernel<4, 2, true, true>" and long[0].grid == [3072, 1, 1]
+    assert long[1].kernel == "window_dq_kernel<4, 2, true>" and long[1].grid == [3072, 1, 1]
+    assert long[2].kernel == "window_dkv_kernel<true>" and long[2].grid == [64 * 12, 1, 1]
+    # 129 blocks of 64 rows: 17 runs for each of 3 pairs, in 7 rounds of the 8 dies.
+    assert ragged[0].grid == [7 * 64, 1, 1] and ragged[1].grid == [7 * 64, 1, 1]
+    assert whole[0].grid == [3, 4, 256] and whole[1].grid == [3, 4, 256]
+    assert whole[2].kernel == "window_dkv_kernel<false>"
+    assert few[0].grid == [1, 1, 513] and few[1].kernel == "window_dq_kernel<4, 1, false>"
+    assert few[2].kernel == "window_dkv_kernel<true>"
 
 
 @pytest.mark.parametrize("case,kernel,splits", [
@@ -92,12 +109,15 @@ def test_cache_attention_splits(case, kernel, splits):
 
 def test_the_gpu_tests_reach_every_variant():
     from tests.test_gpu_kv_cache import ATTEND, PAGE
-    from tests.test_gpu_window_attention import CASES
+    from tests.test_gpu_window_attention import CASES, LONG
 
-    names = {x.kernel for _, ls in window([c[:6] for c in CASES]) for x in ls}
-    want = {f"attn_fwd_kernel<{h}, {n}, true>" for h in (1, 2, 4) for n in (1, 2)}
-    want |= {f"window_dq_kernel<{h}, {n}>" for h in (1, 2, 4) for n in (1, 2)}
-    assert names == want | {"window_dkv_kernel", "window_dkv_join_kernel"}
+    cases = [c[:6] for c in CASES] + [(*c[:5], 0) for c in LONG]
+    names = {x.kernel for _, ls in window(cases) for x in ls}
+    kinds = [(h, n, d) for h in (1, 2, 4) for n, d in ((1, "false"), (2, "false"), (2, "true"))]
+    want = {f"attn_fwd_kernel<{h}, {n}, true, {d}>" for h, n, d in kinds}
+    want |= {f"window_dq_kernel<{h}, {n}, {d}>" for h, n, d in kinds}
+    assert names == want | {"window_dkv_kernel<false>", "window_dkv_kernel<true>",
+                            "window_dkv_join_kernel"}
     cases = [(b, n, -(-max(max(lens), 1) // PAGE), h, k, w, s) for b, n, lens, h, k, w, s in ATTEND]
     names = {x.kernel for _, ls in attend(cases) for x in ls}
     assert names == {"kv_attend_kernel<4>", "kv_attend_kernel<8>", "kv_join_kernel<1>",

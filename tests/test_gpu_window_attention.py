@@ -277,3 +277,43 @@ def test_offsets_past_32_bits(cuda):
                                   d_v=dv)
     for t, name in ((out, "out"), (dq, "dq"), (dk, "dk"), (dv, "dv")):
         near(t, ref, name)
+
+
+def by_pieces(q, k, v, d_out, B, S, H, K, W, lens):
+    """R.batch_attention without sinks, from pieces of rows and the keys they see."""
+    r = {e + n: np.zeros((B * S, (H if n in ("out", "dq") else K) * HD))
+         for n in ("out", "dq", "dk", "dv") for e in ("", "e_")}
+    for b, n in enumerate(lens):
+        for a in range(0, n, 1000):
+            lo, mid, end = max(0, a - W + 1), min(a + 1000, n), min(a + 1000 + W, n)
+            rows, keys, own = (slice(b * S + x, b * S + y) for x, y in ((a, end), (lo, end), (a, mid)))
+            for h in range(H):
+                c = slice(h * HD, (h + 1) * HD)
+                ck = slice(h // (H // K) * HD, (h // (H // K) + 1) * HD)
+                one = R.attention(q[rows, c], k[keys, ck], v[keys, ck], W, 0, first=a - lo,
+                                  d_out=d_out[rows, c])
+                for e in ("", "e_"):
+                    for name in ("out", "dq"):
+                        r[e + name][own, c] = one[e + name][:mid - a]
+                    for name in ("dk", "dv"):
+                        r[e + name][own, ck] += one[e + name][a - lo:mid - lo]
+    return r
+
+
+LONG = [(1, 8200, 8, 2, 150, [8200]), (1, 8195, 6, 3, 70, [8190]),
+        (2, 8193, 3, 3, 100, [8193, 1200])]
+
+
+@pytest.mark.parametrize("B,S,H,K,W,lens", LONG)
+def test_long_sequences_dealt_by_die(cuda, B, S, H, K, W, lens):
+    """Launches whose workgroups are dealt to the dies in runs, the last one ragged."""
+    say("case:", B, S, H, K, W, lens)
+    x = inputs(B, S, H, K, S + W)
+    ref = by_pieces(*x, B, S, H, K, W, lens)
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q, k, v, g = (dev(a) for a in x)
+    out, lse = ops.window_attention(q, k, v, B, S, H, K, W, 0, sl, want_lse=True)
+    near(out, ref, "out")
+    d = ops.window_attention_backward(g, q, k, v, out, lse, B, S, H, K, W, 0, sl)
+    for t, name in zip(d, ("dq", "dk", "dv")):
+        near(t, ref, name)
