@@ -103,7 +103,7 @@ struct BwdArgs {
 //                   which is the operand layout of
 //   dQ^T += K^T dS^T              K^T by transposing LDS reads
 // The kernel also forms delta of its rows and leaves it, with lse, to
-// window_dkv_kernel.  12 + 3 heads: 4 x 2048, window 512, 69 us; 1 x 4096 whole 116
+// window_dkv_kernel.  12 + 3 heads: 4 x 2048, window 512, 66 us; 1 x 4096 whole 116
 // us (670 TFLOP/s); 3 x 500, window 128, 21 us.  Long windows are bound by the matrix
 // cores (busy 55% of the time) and the vector instructions between their products,
 // which the two waves of a SIMD overlap little; short ones by the latency of a block
@@ -382,7 +382,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
 //                                 layout (a lane holds one key and 8 of 32 rows) of
 //   dV^T += d_o^T P, dK^T += Q^T dS   by transposing LDS reads
 // Tiles come in three stages, so that a step's copies have the time of two steps.
-// 12 + 3 heads: 4 x 2048, window 512, 98 us; 1 x 4096 whole 160 us (640 TFLOP/s), 1 x
+// 12 + 3 heads: 4 x 2048, window 512, 97 us; 1 x 4096 whole 156 us (660 TFLOP/s), 1 x
 // 16384, window 4096, 900 us (800); 3 x 500, window 128, 21 us.  No single unit bounds it: without the copies it takes
 // 2 to 7% less, without the transposing reads 2 to 7%, without the exponentials 1.5%;
 // the matrix cores are busy 40% of the time, LDS 50%, and what is left is the latency of a step
@@ -805,7 +805,9 @@ BwdPlan plan_bwd(const Shape &sh, size_t batch) {
   }
   // One workgroup fits a CU.  The time is about that of the longest item where all
   // items are resident, and the average load and half an item more beyond; an item
-  // of a cut block costs about 8 steps more (its sums go through memory).
+  // of a cut block costs about 8 steps more (its sums go through memory), and has 8
+  // steps at least (whole backward with at least 4, 8, 12, us: 3 x 500 46.9, 46.4, 49.6;
+  // 2 x 1000 47.2, 45.6, 48.6; 1 x 200 30.9, 33.0, 35.6).
   const int64_t wgs = (int64_t)batch * sh.Hkv, cus = 256;
   BwdPlan best;
   double best_cost = 0;
