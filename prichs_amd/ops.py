@@ -360,7 +360,7 @@ def window_attention(q, k, v, batch, seq_len, n_heads, n_kv_heads, window, sinks
     ctx, s = _launch_on(stream, q, k, v, seq_lens, out)
     with ctx:
         if out is None:
-            out = torch.empty((rows, H), dtype=q.dtype, device=q.device)
+            out = q.new_empty((rows, H))
         ldo = _rows(out, "out", rows, H)
         lse = None
         if want_lse:
@@ -462,6 +462,8 @@ def kv_cache_read(cache, page_table, start, batch, n, n_kv_heads, counts=None,
         make = torch.empty if counts is None else torch.zeros
         if k is None:
             k = make((rows, cols), dtype=out_dtype, device=cache.device)
+            if v is None and counts is None:
+                v = torch.empty_like(k)
         if v is None:
             v = make((rows, cols), dtype=out_dtype, device=cache.device)
         ldk, ldv = _rows(k, "k", rows, cols, _FLOATS), _rows(v, "v", rows, cols, _FLOATS)
@@ -490,14 +492,14 @@ def kv_cache_attention(q, cache, page_table, lens, batch, n_q, n_heads, n_kv_hea
     ctx, s = _launch_on(stream, q, cache, page_table, lens, out)
     with ctx:
         if out is None:
-            out = torch.empty((rows, H), dtype=q.dtype, device=q.device)
+            out = q.new_empty((rows, H))
         ldo = _rows(out, "out", rows, H)
         lse = None
         if want_lse:
             lse = torch.empty((batch, n_heads, n_q), dtype=torch.float32, device=q.device)
         max_pages = page_table.shape[1]
         need = lib.prichs_kv_cache_attention_workspace(batch, n_q, n_heads, n_kv_heads, max_pages)
-        ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
+        ws = q.new_empty((need + 1) // 2) if need else None  # of two bytes each: a faster call
         L.check(lib.prichs_kv_cache_attention(
             q.data_ptr(), ldq, cache.data_ptr(), cache.shape[0], page_table.data_ptr(), max_pages,
             lens.data_ptr(), out.data_ptr(), ldo, _a(lse), batch, n_q, n_heads, n_kv_heads,
