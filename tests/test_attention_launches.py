@@ -75,14 +75,14 @@ def test_long_sequences_are_dealt_to_the_dies():
     # With a window from 8192 rows on: runs of 8 row blocks (8 key blocks) in a grid of one
     # dimension.
     (_, long), (_, ragged), (_, whole), (_, few) = window(
-        [(4, 8192, 12, 3, 512, 0), (1, 8200, 6, 3, 64, 0), (4, 8192, 12, 3, 0, 0),
+        [(3, 8192, 12, 3, 512, 0), (1, 8200, 6, 3, 64, 0), (3, 8192, 12, 3, 0, 0),
          (1, 8200, 4, 1, 64, 0)])
-    assert long[0].kernel == "attn_fwd_kernel<4, 2, true, true>" and long[0].grid == [3072, 1, 1]
-    assert long[1].kernel == "window_dq_kernel<4, 2, true>" and long[1].grid == [3072, 1, 1]
-    assert long[2].kernel == "window_dkv_kernel<true>" and long[2].grid == [64 * 12, 1, 1]
+    assert long[0].kernel == "attn_fwd_kernel<4, 2, true, true>" and long[0].grid == [256 * 9, 1, 1]
+    assert long[1].kernel == "window_dq_kernel<4, 2, true>" and long[1].grid == [256 * 9, 1, 1]
+    assert long[2].kernel == "window_dkv_kernel<true>" and long[2].grid == [64 * 9, 1, 1]
     # 129 blocks of 64 rows: 17 runs for each of 3 pairs, in 7 rounds of the 8 dies.
     assert ragged[0].grid == [7 * 64, 1, 1] and ragged[1].grid == [7 * 64, 1, 1]
-    assert whole[0].grid == [3, 4, 256] and whole[1].grid == [3, 4, 256]
+    assert whole[0].grid == [3, 3, 256] and whole[1].grid == [3, 3, 256]
     assert whole[2].kernel == "window_dkv_kernel<false>"
     assert few[0].grid == [1, 1, 513] and few[1].kernel == "window_dq_kernel<4, 1, false>"
     assert few[2].kernel == "window_dkv_kernel<true>"
