@@ -411,7 +411,7 @@ int prichs_window_attention_backward(const void *d_o, size_t ldd, const void *q,
  * skipped -- a read leaves them as they were.  Positions outside the table, and
  * pages outside [0, n_pages), are not written and read as zeros.  A position must
  * not be written twice in one call, nor read by a call that may run at the same
- * time.  batch * n * n_kv_heads is below 2^28. */
+ * time.  batch * n * n_kv_heads is at most 2^28 - 16. */
 #define PRICHS_KV_PAGE 64
 #define PRICHS_KV_HEAD_DIM 128
 #define PRICHS_KV_PAGE_BYTES 8704 /* of one kv head */

@@ -17,7 +17,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // as a rule four positions of one head, whose V dwords are neighbours in the cache
 // -- and four heads where every sequence has one new token.
 constexpr int kItems = 16;  // items per workgroup of 256 threads
-constexpr size_t kMaxItems = ((size_t)1 << 28) - 1;  // 16 lanes each, below 2^32 in a launch
+// Whole workgroups of items whose lanes (16 an item) stay below 2^32 in a launch.
+constexpr size_t kMaxItems = ((size_t)1 << 28) - kItems;
 
 struct Item {
   int row, h, c, page, t;  // row of k / v; dword c; page (-1: none) and slot
