@@ -972,6 +972,10 @@ extern "C" int prichs_window_attention_backward(
   const size_t dq_pairs = n_heads / hpw * batch, dkv_pairs = n_kv_heads * batch;
   const bool dq_dies = !few && by_die(seq_len, sh.window, dq_pairs, n_qb),
              dkv_dies = by_die(seq_len, sh.window, dkv_pairs, plan.items);
+  // Before the first launch: a call that fails leaves nothing half done.
+  static LdsLimit limits[2];
+  auto dkv_kern = dkv_dies ? window_dkv_kernel<true> : window_dkv_kernel<false>;
+  WINDOW_TRY(raise_lds_limit(limits[dkv_dies], reinterpret_cast<const void *>(dkv_kern), kKvLds, who));
   const auto bf = [](const void *p) { return static_cast<const bf16_t *>(p); };
   const auto out = [](void *p) { return static_cast<bf16_t *>(p); };
   BwdArgs a{bf(d_o), bf(q), bf(k), bf(v), bf(o), lse, seq_lens, out(d_q), out(d_k), out(d_v),
@@ -993,9 +997,6 @@ extern "C" int prichs_window_attention_backward(
                              : dim3((unsigned)(n_heads / hpw), (unsigned)batch, (unsigned)n_qb),
                      dim3(256), kQLds, as_stream(stream), a);
   PRICHS_LAUNCH_CHECK("window_attention_backward d_q launch");
-  static LdsLimit limits[2];
-  auto dkv_kern = dkv_dies ? window_dkv_kernel<true> : window_dkv_kernel<false>;
-  WINDOW_TRY(raise_lds_limit(limits[dkv_dies], reinterpret_cast<const void *>(dkv_kern), kKvLds, who));
   hipLaunchKernelGGL(dkv_kern,
                      dkv_dies ? dim3((unsigned)die_grid(dkv_pairs, plan.items))
                               : dim3((unsigned)plan.items, (unsigned)n_kv_heads, (unsigned)batch),

@@ -1,5 +1,8 @@
 """Limits of the window attention and KV cache entry points as documented, on the
 CPU (tests/launch_log.py): the largest calls launch, the next ones are refused."""
+import os
+import subprocess
+
 import pytest
 
 from prichs_amd import _lib as L
@@ -27,3 +30,57 @@ def test_items_of_a_cache_call(name):
                          (5, ((1 << 28) - 1) // 15, 3)):
         assert ITEMS < batch * n * kv < 1 << 28
         assert cache_call(name, batch, n, kv) == [L.PRICHS_ERR_INVALID_ARGUMENT, []], (batch, n, kv)
+
+
+# Answers to hipFuncSetAttribute and to the count of compute units that a test
+# chooses, before launch_log's.
+STANDINS = r"""
+#define __HIP_PLATFORM_AMD__
+#include <hip/hip_runtime_api.h>
+#include <cstdlib>
+extern "C" hipError_t hipFuncSetAttribute(const void *, hipFuncAttribute, int) {
+  return std::getenv("REFUSE_LDS") ? hipErrorInvalidValue : hipSuccess;
+}
+extern "C" hipError_t hipDeviceGetAttribute(int *v, hipDeviceAttribute_t, int) {
+  const char *cus = std::getenv("CUS");
+  *v = cus ? std::atoi(cus) : 256;
+  return hipSuccess;
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def standins(tmp_path_factory):
+    """A library to load first (LD_PRELOAD) that reads REFUSE_LDS and CUS."""
+    at = tmp_path_factory.mktemp("standins")
+    (at / "standins.cpp").write_text(STANDINS)
+    so = at / "standins.so"
+    subprocess.run([os.environ.get("CXX", "g++"), "-std=c++17", "-fPIC", "-shared", "-w", "-I",
+                    os.path.join(ll.ROCM, "include"), str(at / "standins.cpp"), "-o", str(so)],
+                   check=True)
+    return str(so)
+
+
+def window_calls(cases, **env):
+    """For each (batch, seq_len, heads, kv heads, window, sinks): status and launches of
+    a forward, the workspace's size, status and launches of a backward."""
+    rows = ll.run(f"""
+result = []
+for b, S, h, k, w, s in {cases!r}:
+    H, K = 128 * h, 128 * k
+    f = lib.prichs_window_attention_forward(P, H, P, K, P, K, P, H, P, None, b, S, h, k, 128, w, s, 1,
+                                            None)
+    f = [f, launches()]
+    need = lib.prichs_window_attention_backward_workspace(b, S, h, k, w, s)
+    g = lib.prichs_window_attention_backward(P, H, P, H, P, K, P, K, P, H, P, None, P, H, P, K, P, K,
+                                             b, S, h, k, 128, w, s, 1, P, need, None)
+    result.append([*f, need, g, launches()])
+""", **env)
+    return [(f, ll.as_launches(x), need, g, ll.as_launches(y)) for f, x, need, g, y in rows]
+
+
+def test_no_launch_before_a_refused_lds_limit(standins):
+    for case in ((1, 100, 4, 1, 0, 0), (1, 9000, 48, 12, 64, 0)):
+        (f, fwd, _, g, bwd), = window_calls([case], LD_PRELOAD=standins, REFUSE_LDS="1")
+        assert (f, g) == (L.PRICHS_ERR_HIP, L.PRICHS_ERR_HIP)
+        assert fwd == [] and bwd == []
