@@ -631,7 +631,7 @@ int window_attention_launch(const void *q, size_t ldq, const void *k, size_t ldk
                             size_t batch, size_t seq_len, size_t n_heads, size_t n_kv_heads,
                             size_t window, size_t sinks, void *stream) {
   const int group = (int)(n_heads / n_kv_heads);
-  const int hpw = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+  const int hpw = window_heads((size_t)group, seq_len);
   const size_t n_qb32 = cdiv(seq_len, (size_t)(32 * kWaves / hpw));
   // 16 query rows per wave by attention's rule.  32 -> 16 rows, us: 1 x 777 window 256
   // 17.7 -> 12.8, 3 x 500 window 128 15.4 -> 11.6, 1 x 4096 whole 95.6 -> 76.0, 1 x 2048
@@ -640,7 +640,6 @@ int window_attention_launch(const void *q, size_t ldq, const void *k, size_t ldk
   const int cus = device_cu_count();
   const bool few = 2 * (n_heads / hpw) * batch * n_qb32 <= 3 * (size_t)std::max(cus, 0);
   const size_t n_qb = few ? cdiv(seq_len, (size_t)(16 * kWaves / hpw)) : n_qb32;
-  PRICHS_REQUIRE(n_qb <= 65535, "window_attention: seq_len too large");
   const float scale_log2 = (1.0f / sqrtf((float)kHd)) * 1.4426950408889634f;
   const size_t pairs = n_heads / hpw * batch;
   const bool dies = !few && by_die(seq_len, window, pairs, n_qb);

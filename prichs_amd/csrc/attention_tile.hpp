@@ -87,6 +87,15 @@ __device__ __forceinline__ uint32_t finite_bf16x2(uint32_t u) {
   return u;
 }
 
+// Query heads that share the K / V tiles of a window attention workgroup (128 / heads
+// rows of each): the largest of 4, 2, 1 that divides the GQA group and leaves at most
+// 65535 row blocks, a grid's third dimension (of four heads up to 2^21 - 32 rows).
+inline int window_heads(size_t group, size_t seq_len) {
+  int heads = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+  while (heads > 1 && cdiv(seq_len, (size_t)(128 / heads)) > 65535) heads /= 2;
+  return heads;
+}
+
 // Workgroups whose keys (or query rows) are their neighbours' too, on one die: of the
 // eight dies, each with an L2 of its own, workgroup `id` runs on die id % 8.  A launch
 // of die_grid(pairs, n) workgroups covers the ranks 0 .. n - 1 of `pairs` sequences'

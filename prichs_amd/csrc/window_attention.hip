@@ -957,8 +957,7 @@ extern "C" int prichs_window_attention_backward(
                 workspace_bytes, need);
   PRICHS_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
                  "%s: the workspace must be 16-byte aligned device memory", who);
-  const int group = (int)(n_heads / n_kv_heads);
-  const int hpw = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+  const int hpw = window_heads(n_heads / n_kv_heads, seq_len);
   const size_t blocks = cdiv(seq_len, (size_t)kBlk), n_qb32 = cdiv(seq_len, (size_t)(128 / hpw));
   const bool few = 2 * (n_heads / hpw) * batch * n_qb32 <= 3 * 256;
   // Rows of a wave of the d_q kernel, by the forward's rule (attention.hip).  Whole
@@ -968,7 +967,6 @@ extern "C" int prichs_window_attention_backward(
   // The d_q kernel writes the statistics of whole 32-row tiles, so its rows go to the
   // end of the last one.
   const size_t n_qb = few ? cdiv(roundup(seq_len, (size_t)kTr), (size_t)(64 / hpw)) : n_qb32;
-  PRICHS_REQUIRE(n_qb <= 65535 && n_kv_heads <= 65535, "%s: shape too large", who);
   const size_t dq_pairs = n_heads / hpw * batch, dkv_pairs = n_kv_heads * batch;
   const bool dq_dies = !few && by_die(seq_len, sh.window, dq_pairs, n_qb),
              dkv_dies = by_die(seq_len, sh.window, dkv_pairs, plan.items);

@@ -84,3 +84,25 @@ def test_no_launch_before_a_refused_lds_limit(standins):
         (f, fwd, _, g, bwd), = window_calls([case], LD_PRELOAD=standins, REFUSE_LDS="1")
         assert (f, g) == (L.PRICHS_ERR_HIP, L.PRICHS_ERR_HIP)
         assert fwd == [] and bwd == []
+
+
+@pytest.mark.parametrize("heads,kv", [(4, 1), (12, 3), (2, 1), (1, 1), (3, 3)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (64, 0), (4096, 4)])
+def test_the_longest_sequence(heads, kv, window, sinks):
+    """2^21 rows in both directions, whatever the heads, in grids of at most 65535 row
+    blocks; one row more is refused by all three entry points."""
+    longest, past = window_calls([(1, 1 << 21, heads, kv, window, sinks),
+                                  (1, (1 << 21) + 1, heads, kv, window, sinks)])
+    f, fwd, need, g, bwd = longest
+    assert (f, g) == (L.PRICHS_OK, L.PRICHS_OK) and need > 0
+    for x in (*fwd, *bwd):
+        assert x.grid[0] * x.block < 1 << 32 and max(x.grid[1:]) <= 65535, x
+    # 128 rows a workgroup, or 64 of each of two heads: all of them.
+    share = 1 if (heads // kv) % 2 else 2
+    for x in (fwd[0], bwd[0]):
+        n = (1 << 21) // (128 // share) * (heads // share)
+        assert f"<{share}, 2," in x.kernel
+        assert x.grid[0] * x.grid[1] * x.grid[2] == n, x
+    f, fwd, need, g, bwd = past
+    assert (f, need, g) == (L.PRICHS_ERR_INVALID_ARGUMENT, 0, L.PRICHS_ERR_INVALID_ARGUMENT)
+    assert fwd == [] and bwd == []
