@@ -36,8 +36,6 @@
 // lane i that column's 4 consecutive kv values.
 #include "attention_tile.hpp"
 
-#include <algorithm>
-
 namespace prichs {
 namespace {
 
@@ -607,8 +605,7 @@ int attention_forward_impl(const void *q, size_t ldq, const void *k, size_t ldk,
   // heads, 32 -> 16 rows, us: 1 x 333 11.2 -> 9.1, 1 x 777 19.1 -> 13.5, 1 x
   // 2048 41.2 -> 31.0, 4 x 1024 (384 workgroups) 26.6 -> 24.1, 4 x 2048 (768)
   // 60.3 -> 69.8.
-  const int cus = device_cu_count();
-  const bool few = 2 * (n_heads / hpw) * batch * (size_t)n_qb <= 3 * (size_t)std::max(cus, 0);
+  const bool few = few_workgroups((n_heads / hpw) * batch * (size_t)n_qb);
   if (few) n_qb = (int)cdiv(seq_len, (size_t)(16 * kWaves / hpw));
   const dim3 grid((unsigned)(n_heads / hpw), (unsigned)batch, (unsigned)n_qb);
   auto kern = few ? (hpw == 4   ? attn_fwd_kernel<4, 1, false>
@@ -637,8 +634,7 @@ int window_attention_launch(const void *q, size_t ldq, const void *k, size_t ldk
   // 17.7 -> 12.8, 3 x 500 window 128 15.4 -> 11.6, 1 x 4096 whole 95.6 -> 76.0, 1 x 2048
   // window 512 23.8 -> 22.0, 4 x 1024 window 256 (384 workgroups) 25.5 -> 26.4, 4 x 2048
   // window 512 48.8 -> 52.6, 1 x 16384 window 4096 414 -> 493.
-  const int cus = device_cu_count();
-  const bool few = 2 * (n_heads / hpw) * batch * n_qb32 <= 3 * (size_t)std::max(cus, 0);
+  const bool few = few_workgroups((n_heads / hpw) * batch * n_qb32);
   const size_t n_qb = few ? cdiv(seq_len, (size_t)(16 * kWaves / hpw)) : n_qb32;
   const float scale_log2 = (1.0f / sqrtf((float)kHd)) * 1.4426950408889634f;
   const size_t pairs = n_heads / hpw * batch;

@@ -2,6 +2,7 @@
 // reads, copies straight into LDS, exchanges between a query's lanes.
 #pragma once
 
+#include <algorithm>
 #include <type_traits>
 #include <utility>
 
@@ -94,6 +95,13 @@ inline int window_heads(size_t group, size_t seq_len) {
   int heads = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
   while (heads > 1 && cdiv(seq_len, (size_t)(128 / heads)) > 65535) heads /= 2;
   return heads;
+}
+
+// Whether a wave takes 16 query rows instead of 32: where the workgroups of 32 would
+// all be resident with room to spare (two fit a CU).  attention.hip and
+// window_attention.hip have what either takes.
+inline bool few_workgroups(size_t wgs32) {
+  return 2 * wgs32 <= 3 * (size_t)std::max(device_cu_count(), 0);
 }
 
 // Workgroups whose keys (or query rows) are their neighbours' too, on one die: of the

@@ -959,8 +959,8 @@ extern "C" int prichs_window_attention_backward(
                  "%s: the workspace must be 16-byte aligned device memory", who);
   const int hpw = window_heads(n_heads / n_kv_heads, seq_len);
   const size_t blocks = cdiv(seq_len, (size_t)kBlk), n_qb32 = cdiv(seq_len, (size_t)(128 / hpw));
-  const bool few = 2 * (n_heads / hpw) * batch * n_qb32 <= 3 * 256;
-  // Rows of a wave of the d_q kernel, by the forward's rule (attention.hip).  Whole
+  const bool few = few_workgroups((n_heads / hpw) * batch * n_qb32);
+  // Rows of a wave of the d_q kernel, by the forward's rule.  Whole
   // backward, 32 -> 16 rows, us: 1 x 777 52 -> 46, 3 x 500 56 -> 50, 1 x 4096 277 ->
   // 260, 4 x 1024 (384 workgroups) 81.6 -> 81.9, 4 x 2048 169 -> 173, 1 x 16384 1499 ->
   // 1671.

@@ -106,3 +106,18 @@ def test_the_longest_sequence(heads, kv, window, sinks):
     f, fwd, need, g, bwd = past
     assert (f, need, g) == (L.PRICHS_ERR_INVALID_ARGUMENT, 0, L.PRICHS_ERR_INVALID_ARGUMENT)
     assert fwd == [] and bwd == []
+
+
+def rows_a_wave(launch):
+    """16-row blocks of a wave of a forward or d_q kernel."""
+    return launch.kernel.split(",")[1].strip()
+
+
+@pytest.mark.parametrize("cus,rows", [(256, "1111"), (64, "1122"), (32, "1222"), (512, "1111")])
+def test_both_directions_take_16_rows_a_wave_by_one_rule(standins, cus, rows):
+    """Where the workgroups of 32 rows a wave are at most one and a half a CU of the
+    device: 75, 192 and 384 of 777, 2048 and 4096 rows, and 3 of one row."""
+    cases = [(1, S, 12, 3, 0, 0) for S in (1, 777, 2048, 4096)]
+    calls = window_calls(cases, LD_PRELOAD=standins, CUS=str(cus))
+    assert "".join(rows_a_wave(c[1][0]) for c in calls) == rows
+    assert "".join(rows_a_wave(c[4][0]) for c in calls) == rows
