@@ -88,6 +88,7 @@ struct BwdArgs {
   float *part;    // f32 partial d_k, d_v (window_dkv_kernel)
   int budget;     // steps of a workgroup there
   int items;      // items of a (sequence, kv head) there
+  int slots;      // of them, the first ones, those that have a place in part
   // For workgroups dealt by die: row blocks of window_dq_kernel, and the (sequence,
   // head set) pairs there and (sequence, kv head) pairs in window_dkv_kernel.
   int dq_blocks, dq_pairs, dkv_pairs;
@@ -721,7 +722,7 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
   joined(dv);
   if (sg != 0) return;
   if (n_split > 1) {
-    float *part = a.part + ((((size_t)b * sh.Hkv + kvh) * a.items + item) * 2) * kBlk * kHd;
+    float *part = a.part + ((((size_t)b * sh.Hkv + kvh) * a.slots + item) * 2) * kBlk * kHd;
     float *row = part + (16 * kg + l16e) * kHd + 4 * ge;
 #pragma unroll
     for (int jd = 0; jd < 8; ++jd) {
@@ -762,7 +763,7 @@ __global__ __launch_bounds__(256) void window_dkv_join_kernel(BwdArgs a) {
   if (row >= sh.S) return;
   const bool live = row < rows_of(a.seq_lens, b, sh.S);
   const float *part =
-      a.part + ((((size_t)b * sh.Hkv + kvh) * a.items + item) * 2) * kBlk * kHd + key * kHd + d;
+      a.part + ((((size_t)b * sh.Hkv + kvh) * a.slots + item) * 2) * kBlk * kHd + key * kHd + d;
   f32x4 t[2][2];
 #pragma unroll
   for (int w = 0; w < 2; ++w) t[w][0] = t[w][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -789,11 +790,13 @@ __global__ __launch_bounds__(256) void window_dkv_join_kernel(BwdArgs a) {
   }
 }
 
-// How the key blocks are cut: items of at most `budget` steps.
+// How the key blocks are cut: items of at most `budget` steps.  No block has more steps
+// than the one before it (the sinks' come first, and a window or the rows left are the
+// same or fewer from block to block), so the items of cut blocks are the first `cut`.
 struct BwdPlan {
   int budget = 0;
   size_t items = 0;
-  bool cut = false;
+  size_t cut = 0;
 };
 BwdPlan plan_bwd(const Shape &sh, size_t batch) {
   const int blocks = (int)cdiv((size_t)sh.S, (size_t)kBlk);
@@ -825,18 +828,28 @@ BwdPlan plan_bwd(const Shape &sh, size_t batch) {
       best_cost = cost;
       best.budget = budget;
       best.items = (size_t)items;
-      best.cut = extra != 0;
+      best.cut = (size_t)extra;
     }
     if (budget == 8) break;
   }
   return best;
+}
+// Items of a (sequence, kv head) that have a place among the partial sums: those of cut
+// blocks.  Up to 32 MiB all items have one, which is the size that callers of shapes
+// so small have known; where batches are large the uncut blocks' places are most of it
+// (16 x 8192 rows, 32 + 8 heads, window 512, 4 sinks: 1200 MiB with them, 192 without).
+size_t part_slots(const Shape &sh, size_t batch, const BwdPlan &p) {
+  constexpr size_t kSmall = (size_t)32 << 20;
+  const size_t all = batch * sh.Hkv * p.items * 2 * kBlk * kHd * sizeof(float);
+  return p.cut == 0 || all <= kSmall ? p.items : p.cut;
 }
 // Bytes of the row statistics and of the partial sums.
 size_t stat_bytes(const Shape &sh, size_t batch) {
   return roundup(batch * sh.Hq * cdiv((size_t)sh.S, (size_t)kTr) * 64 * sizeof(float), 256);
 }
 size_t part_bytes(const Shape &sh, size_t batch, const BwdPlan &p) {
-  return p.cut ? batch * sh.Hkv * p.items * 2 * kBlk * kHd * sizeof(float) : 0;
+  return p.cut == 0 ? 0
+                    : batch * sh.Hkv * part_slots(sh, batch, p) * 2 * kBlk * kHd * sizeof(float);
 }
 
 Shape shape_of(size_t seq_len, size_t n_heads, size_t n_kv_heads, size_t window, size_t sinks) {
@@ -980,7 +993,8 @@ extern "C" int prichs_window_attention_backward(
             (int)ldd, (int)ldq, (int)ldk, (int)ldv, (int)ldo, (int)lddq, (int)lddk, (int)lddv,
             static_cast<float *>(workspace), (int)cdiv(seq_len, (size_t)kTr),
             reinterpret_cast<float *>(static_cast<char *>(workspace) + stats), plan.budget,
-            (int)plan.items, (int)n_qb, (int)dq_pairs, (int)dkv_pairs, sh};
+            (int)plan.items, (int)part_slots(sh, batch, plan), (int)n_qb, (int)dq_pairs,
+            (int)dkv_pairs, sh};
   auto dq_kern = few ? (hpw == 4   ? window_dq_kernel<4, 1>
                         : hpw == 2 ? window_dq_kernel<2, 1>
                                    : window_dq_kernel<1, 1>)
@@ -1001,7 +1015,7 @@ extern "C" int prichs_window_attention_backward(
                      dim3(128 * kKg),
                      kKvLds, as_stream(stream), a);
   PRICHS_LAUNCH_CHECK("window_attention_backward d_k / d_v launch");
-  if (plan.cut) {
+  if (plan.cut != 0) {
     hipLaunchKernelGGL(window_dkv_join_kernel,
                        dim3((unsigned)(kBlk / 16 * blocks), (unsigned)n_kv_heads, (unsigned)batch),
                        dim3(256), 0, as_stream(stream), a);

@@ -121,3 +121,22 @@ def test_both_directions_take_16_rows_a_wave_by_one_rule(standins, cus, rows):
     calls = window_calls(cases, LD_PRELOAD=standins, CUS=str(cus))
     assert "".join(rows_a_wave(c[1][0]) for c in calls) == rows
     assert "".join(rows_a_wave(c[4][0]) for c in calls) == rows
+
+
+@pytest.mark.parametrize("B,S,H,K,W", [(64, 2048, 12, 3, 512), (6, 1500, 4, 4, 60),
+                                       (10, 1100, 4, 4, 60)])
+def test_workspace_holds_partial_sums_of_cut_blocks_only(B, S, H, K, W):
+    """With a few sinks the first block of 128 keys is cut into items and the others are
+    not; 128 KiB of f32 sums an item."""
+    (_, _, need, _, bwd), = window_calls([(B, S, H, K, W, 4)])
+    assert bwd[-1].kernel == "window_dkv_join_kernel"
+    items, blocks = bwd[1].grid[0], -(-S // 128)
+    stats = -(-S // 32) * 256 * B * H
+    assert 1 < items - (blocks - 1) < items
+    assert need == -(-stats // 256) * 256 + (items - (blocks - 1)) * B * K * (128 << 10)
+
+
+def test_workspace_of_a_large_batch_with_sinks():
+    (_, _, none, _, _), (_, _, few, _, _) = window_calls([(16, 8192, 32, 8, 512, s)
+                                                          for s in (0, 4)])
+    assert none == 32 << 20 and few <= 256 << 20

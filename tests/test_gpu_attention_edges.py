@@ -1,13 +1,23 @@
-"""Window attention of the longest sequence."""
+"""Window attention where its edges meet: the longest sequence, and the workspace of a
+batch whose first blocks of keys are cut."""
 import numpy as np
 import pytest
 import torch
 
 import attention_ref as R
-from prichs_amd import ops
+from prichs_amd import _lib as L
+from prichs_amd import ops, synth
 
 pytestmark = pytest.mark.gpu
 HD = 128
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a, dtype=np.float32)).to("cuda").bfloat16()
+
+
+def i32(a):
+    return torch.tensor(a, dtype=torch.int32, device="cuda")
 
 
 def host(t):
@@ -25,6 +35,11 @@ def near(got, want, bound, name):
     assert (err <= bound).all(), (name, err.flat[worst], bound.flat[worst])
 
 
+def inputs(B, S, H, K, seed):
+    rng = np.random.default_rng(seed)
+    return [synth.round_bf16(rng.standard_normal((B * S, n * HD))) for n in (H, K, K, H)]
+
+
 def piece(q, k, v, d_out, a, z, W, sinks):
     """R.attention of the rows a .. z - 1 of one head (window W > 0) and the keys that
     they see, and those keys.  The sinks before the window take the places right before
@@ -34,6 +49,27 @@ def piece(q, k, v, d_out, a, z, W, sinks):
     keys = np.concatenate([np.arange(s), np.arange(lo, z)])
     return R.attention(q[a:z], k[keys], v[keys], W, s if lo > s else sinks, first=a - lo + s,
                        d_out=d_out[a:z]), keys
+
+
+def by_pieces(q, k, v, d_out, B, S, H, K, W, sinks, lens):
+    """R.batch_attention from pieces of 1000 rows.  A key's gradients are sums over the
+    pieces, and so are their bounds."""
+    r = {e + n: np.zeros((B * S, (H if n in ("out", "dq") else K) * HD))
+         for n in ("out", "dq", "dk", "dv") for e in ("", "e_")}
+    for b, n in enumerate(lens):
+        for a in range(0, n, 1000):
+            z = min(a + 1000, n)
+            for h in range(H):
+                c = slice(h * HD, (h + 1) * HD)
+                ck = slice(h // (H // K) * HD, (h // (H // K) + 1) * HD)
+                seq = slice(b * S, b * S + n)
+                one, keys = piece(q[seq, c], k[seq, ck], v[seq, ck], d_out[seq, c], a, z, W, sinks)
+                for e in ("", "e_"):
+                    for name in ("out", "dq"):
+                        r[e + name][b * S + a:b * S + z, c] = one[e + name]
+                    for name in ("dk", "dv"):
+                        r[e + name][b * S + keys, ck] += one[e + name]
+    return r
 
 
 @pytest.mark.parametrize("spans", [[(0, 200), ((1 << 20) - 100, (1 << 20) + 100),
@@ -64,3 +100,28 @@ def test_the_longest_sequence(cuda, spans):
                 sums[name] = sums[name] + one[name][keys >= a - lo][:z - a]
         for name, t in (("dk", dk), ("dv", dv)):
             near(t[a:z], sums[name], sums["e_" + name], name)
+
+
+@pytest.mark.parametrize("B,S,H,K,W,sinks,lens", [
+    (6, 1500, 4, 4, 60, 4, [1500, 3, 0, 1400, 129, 700]), (10, 1100, 8, 4, 60, 200, [1100] * 9 + [64])])
+def test_a_workspace_of_the_size_asked_for_is_enough(cuda, B, S, H, K, W, sinks, lens):
+    """Batches whose partial sums are of the cut blocks only: the right gradients, and
+    nothing written behind the workspace."""
+    say("case:", B, S, H, K, W, sinks)
+    x = inputs(B, S, H, K, 5)
+    ref = by_pieces(*x, B, S, H, K, W, sinks, lens)
+    q, k, v, d_o = (dev(a) for a in x)
+    sl = i32(lens)
+    out, lse = ops.window_attention(q, k, v, B, S, H, K, W, sinks, sl, want_lse=True)
+    lib = L.load()
+    need = lib.prichs_window_attention_backward_workspace(B, S, H, K, W, sinks)
+    ws = torch.full((need + (4 << 20),), 0xff, dtype=torch.uint8, device="cuda")
+    grads = [torch.empty_like(t) for t in (q, k, v)]
+    args = [a for t in (d_o, q, k, v, out) for a in (t.data_ptr(), t.stride(0))]
+    to = [a for t in grads for a in (t.data_ptr(), t.stride(0))]
+    L.check(lib.prichs_window_attention_backward(
+        *args, lse.data_ptr(), sl.data_ptr(), *to, B, S, H, K, HD, W, sinks, L.DTYPE_BF16,
+        ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream))
+    for t, name in zip(grads, ("dq", "dk", "dv")):
+        near(t, ref[name], ref["e_" + name], name)
+    assert (ws[need:] == 0xff).all()
