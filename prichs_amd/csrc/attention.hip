@@ -90,16 +90,16 @@ __device__ __forceinline__ bf16x8 rope_frag(bf16x8 f, float4 c4, float4 s4) {
 }
 
 // NB: 16-row query blocks per wave.  WIN: window attention -- a sliding window,
-// sinks, sequences of their own lengths, and the log-sum-exp written (the
-// arguments in wa); row i of a sequence then sees the keys j <= i with i - j <
-// window (0: all) or j < sinks.  DIE: workgroups dealt by die (attention_tile.hpp).
+// sinks and sequences of their own lengths (the arguments in wa); row i of a
+// sequence then sees the keys j <= i with i - j < window (0: all) or j < sinks.
+// DIE: workgroups dealt by die (attention_tile.hpp).  LSE: the log-sum-exp is written.
 // 12 + 3 heads with a window: 1 x 16384 of 4096 367 us
 // (980 TFLOP/s), 4 x 2048 of 512 49 us (460), 1 x 4096 whole 76 us (680), bound as
 // without one; a block of keys that some rows do not see costs its masks and a scan
 // of V (a whole causal 4 x 2048 takes 65 us here and 60 there).  1 x 777 of 256 13 us:
 // the latency of its five blocks of keys.
-template <int HPW, int NB, bool WIN, bool DIE = false>
-__global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
+template <int HPW, int NB, bool WIN, bool DIE, bool LSE>
+__device__ __forceinline__ void attn_fwd(
     const bf16_t *__restrict__ q, int ldq, const bf16_t *__restrict__ k, int ldk,
     const bf16_t *__restrict__ v, int ldv, bf16_t *__restrict__ o, int ldo, int S, int Hq,
     int group, float scale_log2, const float *__restrict__ rcos, const float *__restrict__ rsin,
@@ -144,7 +144,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
         if (qrow >= S) continue;
         bf16_t *orow = o + (seq0 + qrow) * ldo + (size_t)h * kHd + 4 * g;
         for (int jd = 0; jd < 8; ++jd) *reinterpret_cast<u32x2 *>(orow + 16 * jd) = u32x2{0, 0};
-        if (wa.lse != nullptr && g == 0) wa.lse[((size_t)b * Hq + h) * S + qrow] = -INFINITY;
+        if (LSE && g == 0) wa.lse[((size_t)b * Hq + h) * S + qrow] = -INFINITY;
       }
       return;
     }
@@ -181,10 +181,14 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
   // Row sums of P, accumulated by MFMA against a ones fragment (every element
   // of lsum[nb] holds the sum of query row q0 + 16 nb + lane % 16).
   f32x4 lsum[NB];
+  // LSE: this lane's share of the sum of P before its rounding, for lse.  The output is
+  // divided by the sum of the rounded P, whose errors its own cancel with.
+  float psum[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     m_ref[nb] = -INFINITY;
     lsum[nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    psum[nb] = 0.f;
   }
   const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u,
                                                         0x3f803f80u});
@@ -393,6 +397,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
       // be NaN.  Only a masked block can leave a row without one.
       if constexpr (kMasked || WIN) m_use = m_new == -INFINITY ? 0.f : m_new;
       const float neg_m = -m_use;
+      float part[2];
 #pragma unroll
       for (int ks2 = 0; ks2 < 2; ++ks2) {
         // k slots 0..3: kv block 2 ks2 (rows 4g + r); slots 4..7: block 2 ks2 + 1.
@@ -402,14 +407,20 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             p[4 * h2 + r] = fast_exp2(fmaf(scur[2 * ks2 + h2][nb][r], scale_log2, neg_m));
+        if constexpr (LSE)
+          part[ks2] = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
         pf[nb][ks2] = u32x4{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]),
                             pack_bf16(p[6], p[7])};
       }
+      if constexpr (LSE) psum[nb] = fmaf(psum[nb], alpha[nb], part[0] + part[1]);
     }
     // Pin the P fragments here: otherwise the compiler sinks the exp work
     // past the branch below, out of reach of the S MFMAs it should overlap.
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) asm volatile("" ::"v"(pf[nb][0]), "v"(pf[nb][1]));
+    for (int nb = 0; nb < NB; ++nb) {
+      asm volatile("" ::"v"(pf[nb][0]), "v"(pf[nb][1]));
+      if constexpr (LSE) asm volatile("" : "+v"(psum[nb]));  // P need not live on for it
+    }
     // Rescale the output rows where the reference max was raised (rare).
     if (__any(raise[0] || raise[NB - 1])) {
 #pragma unroll
@@ -531,10 +542,14 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
     // every score is -inf, and 0 / 0 is the softmax of that.)
     const float inv = 1.0f / (WIN ? lsum[nb][0] : fmaxf(lsum[nb][0], 1e-30f));
     const int qrow = q0 + 16 * nb + l16;
-    if constexpr (WIN) {
-      if (wa.lse != nullptr && g == 0 && qrow < S)
+    if constexpr (LSE) {
+      float l = psum[nb] + __shfl_xor(psum[nb], 16);
+      l += __shfl_xor(l, 32);
+      if (g == 0 && qrow < S)
         wa.lse[((size_t)b * Hq + h) * S + qrow] =
-            qrow < L ? (m_ref[nb] + log2f(lsum[nb][0])) * 0.6931471805599453f : -INFINITY;
+            qrow < L ? (m_ref[nb] + log2f(l)) * 0.6931471805599453f : -INFINITY;
+    }
+    if constexpr (WIN) {
       if (qrow >= L && qrow < S) {
         bf16_t *orow = o + (seq0 + qrow) * ldo + (size_t)h * kHd + 4 * g;
 #pragma unroll
@@ -551,6 +566,29 @@ __global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
       }
     }
   }
+}
+
+// The whole attention, or (WIN) window attention with lse.
+template <int HPW, int NB, bool WIN, bool DIE = false>
+__global__ __launch_bounds__(kThreads, 2) void attn_fwd_kernel(
+    const bf16_t *__restrict__ q, int ldq, const bf16_t *__restrict__ k, int ldk,
+    const bf16_t *__restrict__ v, int ldv, bf16_t *__restrict__ o, int ldo, int S, int Hq,
+    int group, float scale_log2, const float *__restrict__ rcos, const float *__restrict__ rsin,
+    int pos_offset, WindowArgs wa) {
+  attn_fwd<HPW, NB, WIN, DIE, WIN>(q, ldq, k, ldk, v, ldv, o, ldo, S, Hq, group, scale_log2, rcos,
+                                   rsin, pos_offset, wa);
+}
+// Window attention without lse, whose sum costs 17 vector instructions for each 64 keys and
+// 16 rows (1 x 777 window 256 12.8 -> 13.0 us, 4 x 2048 window 512 48.3 -> 49.9, 1 x 16384
+// window 4096 365 -> 387).
+template <int HPW, int NB, bool DIE = false>
+__global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(
+    const bf16_t *__restrict__ q, int ldq, const bf16_t *__restrict__ k, int ldk,
+    const bf16_t *__restrict__ v, int ldv, bf16_t *__restrict__ o, int ldo, int S, int Hq,
+    int group, float scale_log2, const float *__restrict__ rcos, const float *__restrict__ rsin,
+    int pos_offset, WindowArgs wa) {
+  attn_fwd<HPW, NB, true, DIE, false>(q, ldq, k, ldk, v, ldv, o, ldo, S, Hq, group, scale_log2,
+                                      rcos, rsin, pos_offset, wa);
 }
 
 }  // namespace
@@ -642,23 +680,23 @@ int window_attention_launch(const void *q, size_t ldq, const void *k, size_t ldk
   const dim3 grid = dies ? dim3((unsigned)die_grid(pairs, n_qb))
                          : dim3((unsigned)(n_heads / hpw), (unsigned)batch, (unsigned)n_qb);
   static const struct {
-    decltype(&attn_fwd_kernel<4, 2, true>) kernel;
+    decltype(&attn_fwd_kernel<4, 2, true>) with_lse, without;
     int hpw;
     bool few, dies;
-  } kinds[] = {{attn_fwd_kernel<4, 1, true>, 4, true, false},
-               {attn_fwd_kernel<2, 1, true>, 2, true, false},
-               {attn_fwd_kernel<1, 1, true>, 1, true, false},
-               {attn_fwd_kernel<4, 2, true>, 4, false, false},
-               {attn_fwd_kernel<2, 2, true>, 2, false, false},
-               {attn_fwd_kernel<1, 2, true>, 1, false, false},
-               {attn_fwd_kernel<4, 2, true, true>, 4, false, true},
-               {attn_fwd_kernel<2, 2, true, true>, 2, false, true},
-               {attn_fwd_kernel<1, 2, true, true>, 1, false, true}};
-  static LdsLimit limits[9];
+  } kinds[] = {{attn_fwd_kernel<4, 1, true>, window_fwd_kernel<4, 1>, 4, true, false},
+               {attn_fwd_kernel<2, 1, true>, window_fwd_kernel<2, 1>, 2, true, false},
+               {attn_fwd_kernel<1, 1, true>, window_fwd_kernel<1, 1>, 1, true, false},
+               {attn_fwd_kernel<4, 2, true>, window_fwd_kernel<4, 2>, 4, false, false},
+               {attn_fwd_kernel<2, 2, true>, window_fwd_kernel<2, 2>, 2, false, false},
+               {attn_fwd_kernel<1, 2, true>, window_fwd_kernel<1, 2>, 1, false, false},
+               {attn_fwd_kernel<4, 2, true, true>, window_fwd_kernel<4, 2, true>, 4, false, true},
+               {attn_fwd_kernel<2, 2, true, true>, window_fwd_kernel<2, 2, true>, 2, false, true},
+               {attn_fwd_kernel<1, 2, true, true>, window_fwd_kernel<1, 2, true>, 1, false, true}};
+  static LdsLimit limits[9][2];
   int i = 0;
   while (kinds[i].hpw != hpw || kinds[i].few != few || kinds[i].dies != dies) ++i;
-  const auto kern = kinds[i].kernel;
-  if (int rc = raise_lds_limit(limits[i], reinterpret_cast<const void *>(kern), kWinLdsBytes,
+  const auto kern = lse != nullptr ? kinds[i].with_lse : kinds[i].without;
+  if (int rc = raise_lds_limit(limits[i][lse != nullptr], reinterpret_cast<const void *>(kern), kWinLdsBytes,
                                "window_attention"))
     return rc;
   hipLaunchKernelGGL(kern, grid, dim3(kThreads), kWinLdsBytes, as_stream(stream),

@@ -140,3 +140,24 @@ def test_workspace_of_a_large_batch_with_sinks():
     (_, _, none, _, _), (_, _, few, _, _) = window_calls([(16, 8192, 32, 8, 512, s)
                                                           for s in (0, 4)])
     assert none == 32 << 20 and few <= 256 << 20
+
+
+def test_window_attention_without_lse_has_kernels_of_its_own():
+    """One for each that forms it, in the same grids."""
+    from tests.test_gpu_attention_edges import WITHOUT_LSE
+
+    rows = ll.run(f"""
+result = []
+for b, S, h, k, w, s in {WITHOUT_LSE!r}:
+    for lse in (P, None):
+        H, K = 128 * h, 128 * k
+        L.check(lib.prichs_window_attention_forward(P, H, P, K, P, K, P, H, lse, None, b, S, h, k, 128,
+                                                    w, s, 1, None))
+    result.append(launches())
+""")
+    seen = set()
+    for one, two in (ll.as_launches(x) for x in rows):
+        kind = one.kernel[len("attn_fwd_kernel<"):].replace("true, ", "", 1)
+        assert two.kernel == "window_fwd_kernel<" + kind and one[2:] == two[2:]
+        seen.add(kind)
+    assert len(seen) == 9

@@ -1,5 +1,5 @@
-"""Window attention where its edges meet: the longest sequence, and the workspace of a
-batch whose first blocks of keys are cut."""
+"""Window attention where its edges meet: the longest sequence, the workspace of a batch
+whose first blocks of keys are cut, and the log-sum-exp against its f32 bound."""
 import numpy as np
 import pytest
 import torch
@@ -125,3 +125,61 @@ def test_a_workspace_of_the_size_asked_for_is_enough(cuda, B, S, H, K, W, sinks,
     for t, name in zip(grads, ("dq", "dk", "dv")):
         near(t, ref[name], ref["e_" + name], name)
     assert (ws[need:] == 0xff).all()
+
+
+# ------------------------------------------------------------ log-sum-exp --
+def lse_and_bound(q, k, first, W, sinks):
+    """lse of query rows q [n, 128] at positions first .. over keys k [L, 128], and how
+    far one formed in f32 may be off.  With ulp = 2^-23, which is also what a sum that
+    cuts off instead of rounding loses:
+      a score      128 additions, each of at most the terms' magnitudes;
+      an exponent  up to 8 roundings of the largest score (scale, product, maximum);
+      the sum      an addition for each visible key, and for each 64 keys a rescaling
+                   by a power that is off by its exponent's rounding, and a join;
+      the logarithm and what is added to it: 4 of the result and of the sum's."""
+    i, j = first + np.arange(len(q))[:, None], np.arange(len(k))[None]
+    ok = R.visible(i, j, W, sinks)
+    scale = 1 / np.sqrt(HD)
+    s = np.where(ok, q @ k.T * scale, -np.inf)
+    m = s.max(1)
+    lse = m + np.log(np.exp(s - m[:, None]).sum(1))
+    terms = np.where(ok, np.abs(q) @ np.abs(k).T * scale, 0).max(1)
+    top = np.where(ok, np.abs(s), 0).max(1)
+    n = ok.sum(1)
+    blocks = n // 64 + 2 + sinks // 64
+    return lse, 2.0 ** -23 * (128 * terms + 8 * top + n + 8 * blocks * (1 + top)
+                              + 4 * (np.abs(lse) + np.log(n) + 1))
+
+
+@pytest.mark.parametrize("S,H,K,W,sinks,lens", [
+    (1, 1, 1, 0, 0, None), (70, 4, 1, 2, 0, None), (70, 4, 2, 3, 1, None), (300, 6, 3, 0, 0, None),
+    (200, 2, 2, 17, 70, [133]), (2600, 4, 1, 300, 4, None), (1700, 48, 12, 5, 0, None)])
+def test_lse_is_formed_in_f32(cuda, S, H, K, W, sinks, lens):
+    """Of the unrounded exponentials, though the output's sum is of rounded ones."""
+    say("case:", S, H, K, W, sinks, lens)
+    q, k, v, _ = inputs(1, S, H, K, S + W)
+    _, lse = ops.window_attention(dev(q), dev(k), dev(v), 1, S, H, K, W, sinks,
+                                  None if lens is None else i32(lens), want_lse=True)
+    n = S if lens is None else lens[0]
+    for h in range(H):
+        c, ck = slice(h * HD, (h + 1) * HD), slice(h // (H // K) * HD, (h // (H // K) + 1) * HD)
+        want, bound = lse_and_bound(q[:n, c], k[:n, ck], 0, W, sinks)
+        near(lse[0, h, :n], want, bound, h)
+        assert torch.isneginf(lse[0, h, n:]).all()
+
+
+# 4, 2 and 1 heads that share tiles; few workgroups, many, and dealt by die.
+WITHOUT_LSE = [
+    (2, 200, 4, 1, 17, 3), (1, 300, 6, 3, 100, 70), (1, 257, 3, 3, 0, 0), (3, 330, 48, 12, 100, 4),
+    (6, 330, 24, 12, 90, 0), (6, 330, 24, 24, 0, 0), (1, 8200, 8, 2, 150, 4), (1, 8195, 6, 3, 70, 0),
+    (2, 8193, 3, 3, 100, 0)]
+
+
+@pytest.mark.parametrize("B,S,H,K,W,sinks", WITHOUT_LSE)
+def test_the_output_does_not_depend_on_whether_lse_is_wanted(cuda, B, S, H, K, W, sinks):
+    say("case:", B, S, H, K, W, sinks)
+    q, k, v = (dev(x) for x in inputs(B, S, H, K, S)[:3])
+    for lens in (None, i32([S - 70] * B)):
+        out, lse = ops.window_attention(q, k, v, B, S, H, K, W, sinks, lens, want_lse=True)
+        assert torch.isfinite(out).all() and torch.isfinite(lse[:, :, :S - 70]).all()
+        assert torch.equal(out, ops.window_attention(q, k, v, B, S, H, K, W, sinks, lens)[0])
