@@ -68,6 +68,12 @@ struct PageRegs {
   u32x4 vs;    // scales of v[0..3]
 };
 
+// The workspace, where a tile's pages are split: the parts of each row's output (kKvHd
+// floats), maximum and sum (2), then from here the sums of unrounded P (1).
+__device__ __forceinline__ size_t sums_at(const AttendShape &sh) {
+  return (size_t)gridDim.z * sh.Hkv * sh.tiles * sh.n_split * kRows * (kKvHd + 2);
+}
+
 // A part of a row (maximum mw, sum lw) joined to the row's maximum m: its weight, and
 // its share of the sum.
 __device__ __forceinline__ float part_weight(float mw, float m) {
@@ -77,14 +83,14 @@ __device__ __forceinline__ float part_sum(float mw, float lw, float m) {
   return mw == -INFINITY && m != -INFINITY ? 0.f : lw * part_weight(mw, m);
 }
 
-template <int kWaves>
-__global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 3 : 2) void kv_attend_kernel(
+template <int kWaves, bool LSE>
+__device__ __forceinline__ void kv_attend(
     const bf16_t *__restrict__ q, size_t ldq, const uint8_t *__restrict__ cache,
     const int32_t *__restrict__ table, const int32_t *__restrict__ lens, bf16_t *__restrict__ o,
     size_t ldo, float *__restrict__ lse, float *__restrict__ part_o, float2 *__restrict__ part_ml,
-    AttendShape sh) {
+    const AttendShape &sh) {
   constexpr int kThreads = 64 * kWaves;
-  __shared__ float s_ml[2][kWaves][kRows];
+  __shared__ float s_ml[LSE ? 3 : 2][kWaves][kRows];
   __shared__ float s_o[kWaves][kRows * kLdRow];
 
   const int split = blockIdx.y;
@@ -127,6 +133,9 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 3 : 2) void kv_attend_ke
 #pragma unroll
   for (int jd = 0; jd < 8; ++jd) oacc[jd] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m_ref = -INFINITY;
+  // LSE: the lane's share of the sum of P before its rounding, for lse.  The output is
+  // divided by the sum of the rounded P, lsum, whose errors its own cancel with.
+  float psum = 0.f;
   bool seen = false;
   const u32x4 ones = u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 
@@ -208,6 +217,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 3 : 2) void kv_attend_ke
     const float alpha = raise ? fast_exp2(m_ref - m_new) : 1.0f;
     m_ref = m_new;
     const float neg_m = m_new == -INFINITY ? 0.f : -m_new;
+    if constexpr (LSE) psum *= alpha;
 #pragma unroll
     for (int ks2 = 0; ks2 < 2; ++ks2) {
       float p[8];
@@ -216,6 +226,8 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 3 : 2) void kv_attend_ke
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           p[4 * h2 + r] = fast_exp2(fmaf(s[2 * ks2 + h2][r], sh.scale_log2, neg_m));
+      if constexpr (LSE)
+        psum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
       // P rounded to bf16 for the product; its sum is that of the rounded values.
       pf[ks2] = u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]),
                       pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])};
@@ -286,6 +298,10 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 3 : 2) void kv_attend_ke
   // The waves join.  A score that is NaN makes the row's maximum NaN.  A row that saw
   // keys but no score above -inf has no softmax: its sum is NaN, and counts where no
   // other part of the row has a score (part_sum).
+  if constexpr (LSE) {
+    psum += __shfl_xor(psum, 16);
+    psum += __shfl_xor(psum, 32);
+  }
   if (lsum[0] != lsum[0]) m_ref = lsum[0];
   int lost = seen && m_ref == -INFINITY;
   lost |= __shfl_xor(lost, 16);
@@ -293,6 +309,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 3 : 2) void kv_attend_ke
   if (g == 0) {
     s_ml[0][wave][l16] = m_ref;
     s_ml[1][wave][l16] = lost ? __uint_as_float(0x7fc00000u) : lsum[0];
+    if constexpr (LSE) s_ml[2][wave][l16] = lost ? __uint_as_float(0x7fc00000u) : psum;
   }
   __syncthreads();
   float m = -INFINITY;
@@ -311,12 +328,13 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 3 : 2) void kv_attend_ke
   for (int x = tid; x < kRows * kKvHd / 4; x += kThreads) {
     const int row = x / (kKvHd / 4), d = 4 * (x - row * (kKvHd / 4));
     if (r0 + row > r1) break;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, ls = 0.f;
     for (int w = 0; w < kWaves; ++w) m = vmax(m, s_ml[0][w][row]);
     f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int w = 0; w < kWaves; ++w) {
       const float mw = s_ml[0][w][row];
       l += part_sum(mw, s_ml[1][w][row], m);
+      if constexpr (LSE) ls += part_sum(mw, s_ml[2][w][row], m);
       t = t + *reinterpret_cast<const f32x4 *>(&s_o[w][row * kLdRow + d]);
     }
     if (sh.n_split > 1) {
@@ -324,6 +342,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 3 : 2) void kv_attend_ke
           ((((size_t)b * sh.Hkv + kvh) * sh.tiles + tile) * sh.n_split + split) * kRows + row;
       *reinterpret_cast<f32x4 *>(part_o + at * kKvHd + d) = t;
       if (d == 0) part_ml[at] = make_float2(m, l);
+      if (LSE && d == 0) part_o[sums_at(sh) + at] = ls;
       continue;
     }
     const int r = r0 + row, iq = r / G, h = kvh * G + r - iq * G;
@@ -332,22 +351,40 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 3 : 2) void kv_attend_ke
     u.x = pack_bf16x2(t[0] * inv, t[1] * inv);
     u.y = pack_bf16x2(t[2] * inv, t[3] * inv);
     *reinterpret_cast<uint2 *>(o + ((size_t)b * sh.n_q + iq) * ldo + (size_t)h * kKvHd + d) = u;
-    if (lse != nullptr && d == 0)
-      lse[((size_t)b * sh.Hq + h) * sh.n_q + iq] = (m + log2f(l)) * 0.6931471805599453f;
+    if (LSE && d == 0)
+      lse[((size_t)b * sh.Hq + h) * sh.n_q + iq] = (m + log2f(ls)) * 0.6931471805599453f;
   }
+}
+
+template <int kWaves>
+__global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 3 : 2) void kv_attend_kernel(
+    const bf16_t *__restrict__ q, size_t ldq, const uint8_t *__restrict__ cache,
+    const int32_t *__restrict__ table, const int32_t *__restrict__ lens, bf16_t *__restrict__ o,
+    size_t ldo, float *__restrict__ lse, float *__restrict__ part_o, float2 *__restrict__ part_ml,
+    AttendShape sh) {
+  kv_attend<kWaves, false>(q, ldq, cache, table, lens, o, ldo, lse, part_o, part_ml, sh);
+}
+// With lse: 10 registers more, and 0.2 to 1 us a call (one token over 8192 positions 8.6 ->
+// 9.1 us, 32 x 3000 16.1 -> 16.6, 8 x 5 over 4096 14.7 -> 15.3, 2 x 256 over 4352 35.9 -> 36.9).
+template <int kWaves>
+__global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 3 : 2) void kv_attend_lse_kernel(
+    const bf16_t *__restrict__ q, size_t ldq, const uint8_t *__restrict__ cache,
+    const int32_t *__restrict__ table, const int32_t *__restrict__ lens, bf16_t *__restrict__ o,
+    size_t ldo, float *__restrict__ lse, float *__restrict__ part_o, float2 *__restrict__ part_ml,
+    AttendShape sh) {
+  kv_attend<kWaves, true>(q, ldq, cache, table, lens, o, ldo, lse, part_o, part_ml, sh);
 }
 
 // Joins the splits of a query row: KG groups of 32 threads, thread d4 of group k
 // taking dims 4 d4 .. + 3 of splits k, k + KG, ..; all loads of up to 8 splits are
 // in flight at once (the partial results come from other dies' caches).
-template <int KG>
-__global__ __launch_bounds__(256) void kv_join_kernel(const float *__restrict__ part_o,
-                                                      const float2 *__restrict__ part_ml,
-                                                      bf16_t *__restrict__ o, size_t ldo,
-                                                      float *__restrict__ lse,
-                                                      AttendShape sh) {
+template <int KG, bool LSE>
+__device__ __forceinline__ void kv_join(
+    const float *__restrict__ part_o, const float2 *__restrict__ part_ml, bf16_t *__restrict__ o,
+    size_t ldo, float *__restrict__ lse, const AttendShape &sh) {
   __shared__ f32x4 s_o[8][32];
   __shared__ float2 s_ml[8];
+  __shared__ float s_s[8];
   const int G = sh.Hq / sh.Hkv, rows = sh.n_q * G;
   const int d4 = threadIdx.x & 31, slot = threadIdx.x >> 5, k = slot % KG;
   const int r = blockIdx.x * (8 / KG) + slot / KG;
@@ -355,19 +392,22 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const float *__restrict__ 
   if (KG == 1 && r >= rows) return;  // with KG = 8 the grid is the rows
   const int tile = r / kRows, row = r - tile * kRows;
   const size_t base = (((size_t)b * sh.Hkv + kvh) * sh.tiles + tile) * sh.n_split * kRows + row;
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f, ls = 0.f;
   f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int s0 = k; s0 < sh.n_split; s0 += 8 * KG) {
     f32x4 p[8];
     float2 ml[8];
+    float ps[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int s = s0 + j * KG;
       ml[j] = make_float2(-INFINITY, 0.f);
       p[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      ps[j] = 0.f;
       if (s < sh.n_split) {
         const size_t at = base + (size_t)s * kRows;
         ml[j] = part_ml[at];
+        if constexpr (LSE) ps[j] = part_o[sums_at(sh) + at];
         p[j] = *reinterpret_cast<const f32x4 *>(part_o + at * kKvHd + 4 * d4);
       }
     }
@@ -375,10 +415,12 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const float *__restrict__ 
 #pragma unroll
     for (int j = 0; j < 8; ++j) m2 = vmax(m2, ml[j].x);
     l = part_sum(m, l, m2);
+    ls = part_sum(m, ls, m2);
     t = t * part_weight(m, m2);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       l += part_sum(ml[j].x, ml[j].y, m2);
+      ls += part_sum(ml[j].x, ps[j], m2);
       t = t + p[j] * part_weight(ml[j].x, m2);
     }
     m = m2;
@@ -386,16 +428,18 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const float *__restrict__ 
   if (KG > 1) {
     s_o[slot][d4] = t;
     if (d4 == 0) s_ml[slot] = make_float2(m, l);
+    if (LSE && d4 == 0) s_s[slot] = ls;
     __syncthreads();
     if (k != 0) return;
     m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < KG; ++j) m = vmax(m, s_ml[j].x);
-    l = 0.f;
+    l = ls = 0.f;
     t = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < KG; ++j) {
       l += part_sum(s_ml[j].x, s_ml[j].y, m);
+      ls += part_sum(s_ml[j].x, s_s[j], m);
       t = t + s_o[j][d4] * part_weight(s_ml[j].x, m);
     }
   }
@@ -405,8 +449,20 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const float *__restrict__ 
   u.x = pack_bf16x2(t[0] * inv, t[1] * inv);
   u.y = pack_bf16x2(t[2] * inv, t[3] * inv);
   *reinterpret_cast<uint2 *>(o + ((size_t)b * sh.n_q + iq) * ldo + (size_t)h * kKvHd + 4 * d4) = u;
-  if (lse != nullptr && d4 == 0)
-    lse[((size_t)b * sh.Hq + h) * sh.n_q + iq] = (m + log2f(l)) * 0.6931471805599453f;
+  if (LSE && d4 == 0)
+    lse[((size_t)b * sh.Hq + h) * sh.n_q + iq] = (m + log2f(ls)) * 0.6931471805599453f;
+}
+template <int KG>
+__global__ __launch_bounds__(256) void kv_join_kernel(
+    const float *__restrict__ part_o, const float2 *__restrict__ part_ml, bf16_t *__restrict__ o,
+    size_t ldo, float *__restrict__ lse, AttendShape sh) {
+  kv_join<KG, false>(part_o, part_ml, o, ldo, lse, sh);
+}
+template <int KG>
+__global__ __launch_bounds__(256) void kv_join_lse_kernel(
+    const float *__restrict__ part_o, const float2 *__restrict__ part_ml, bf16_t *__restrict__ o,
+    size_t ldo, float *__restrict__ lse, AttendShape sh) {
+  kv_join<KG, true>(part_o, part_ml, o, ldo, lse, sh);
 }
 
 // Pages up to which one workgroup of 8 waves takes a tile without a second kernel:
@@ -442,7 +498,7 @@ Plan plan_of(size_t batch, size_t n_q, size_t n_heads, size_t n_kv_heads, size_t
 }
 size_t workspace_of(const Plan &p, size_t batch, size_t n_kv_heads) {
   if (p.n_split <= 1) return 0;
-  return batch * n_kv_heads * p.tiles * p.n_split * kRows * (kKvHd + 2) * sizeof(float);
+  return batch * n_kv_heads * p.tiles * p.n_split * kRows * (kKvHd + 3) * sizeof(float);
 }
 
 }  // namespace
@@ -515,7 +571,8 @@ extern "C" int prichs_kv_cache_attention(const void *q, size_t ldq, const void *
   float *part_o = static_cast<float *>(workspace);
   float2 *part_ml = reinterpret_cast<float2 *>(part_o + (p.n_split > 1 ? part_rows * kKvHd : 0));
   const dim3 grid((unsigned)(n_kv_heads * p.tiles), (unsigned)p.n_split, (unsigned)batch);
-  auto kern = p.waves == 8 ? kv_attend_kernel<8> : kv_attend_kernel<4>;
+  auto kern = lse == nullptr ? (p.waves == 8 ? kv_attend_kernel<8> : kv_attend_kernel<4>)
+                             : (p.waves == 8 ? kv_attend_lse_kernel<8> : kv_attend_lse_kernel<4>);
   hipLaunchKernelGGL(kern, grid, dim3((unsigned)(64 * p.waves)), 0, as_stream(stream),
                      static_cast<const bf16_t *>(q), ldq, static_cast<const uint8_t *>(cache),
                      page_table, lens, static_cast<bf16_t *>(o), ldo, lse, part_o, part_ml, sh);
@@ -527,7 +584,8 @@ extern "C" int prichs_kv_cache_attention(const void *q, size_t ldq, const void *
     const bool wide = p.n_split > 8;
     const dim3 join((unsigned)(wide ? rows : cdiv(rows, 8)), (unsigned)n_kv_heads,
                     (unsigned)batch);
-    auto join_kern = wide ? kv_join_kernel<8> : kv_join_kernel<1>;
+    auto join_kern = lse == nullptr ? (wide ? kv_join_kernel<8> : kv_join_kernel<1>)
+                                    : (wide ? kv_join_lse_kernel<8> : kv_join_lse_kernel<1>);
     hipLaunchKernelGGL(join_kern, join, dim3(256), 0, as_stream(stream), part_o, part_ml,
                        static_cast<bf16_t *>(o), ldo, lse, sh);
     PRICHS_LAUNCH_CHECK("kv_cache_attention join launch");

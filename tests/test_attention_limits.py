@@ -161,3 +161,24 @@ for b, S, h, k, w, s in {WITHOUT_LSE!r}:
         assert two.kernel == "window_fwd_kernel<" + kind and one[2:] == two[2:]
         seen.add(kind)
     assert len(seen) == 9
+
+
+def test_cache_attention_with_lse_has_kernels_of_its_own():
+    """One for each without, in the same grids, from workspaces of one size."""
+    rows = ll.run("""
+result = []
+for b, n, p in ((1, 1, 5), (1, 1, 16), (1, 1, 2), (1, 1, 128), (2, 256, 68)):
+    need = lib.prichs_kv_cache_attention_workspace(b, n, 12, 3, p)
+    for lse in (None, P):
+        L.check(lib.prichs_kv_cache_attention(P, 1536, P, 1000, P, p, P, P, 1536, lse, b, n, 12, 3, 128,
+                                              0, 0, 1, P, need, None))
+        result.append(launches())
+""")
+    seen = set()
+    for one, two in zip(*(map(ll.as_launches, rows[i::2]) for i in (0, 1))):
+        assert len(one) == len(two)
+        for x, y in zip(one, two):
+            assert y.kernel == x.kernel.replace("_kernel", "_lse_kernel") and x[2:4] == y[2:4]
+            seen.add(y.kernel)
+    assert seen == {"kv_attend_lse_kernel<4>", "kv_attend_lse_kernel<8>", "kv_join_lse_kernel<1>",
+                    "kv_join_lse_kernel<8>"}

@@ -1,5 +1,6 @@
-"""Window attention where its edges meet: the longest sequence, the workspace of a batch
-whose first blocks of keys are cut, and the log-sum-exp against its f32 bound."""
+"""Window attention and cache attention where their edges meet: the longest sequence, the
+workspace of a batch whose first blocks of keys are cut, and the log-sum-exp against its
+f32 bound."""
 import numpy as np
 import pytest
 import torch
@@ -9,7 +10,7 @@ from prichs_amd import _lib as L
 from prichs_amd import ops, synth
 
 pytestmark = pytest.mark.gpu
-HD = 128
+HD, PAGE = 128, L.KV_PAGE
 
 
 def dev(a):
@@ -183,3 +184,33 @@ def test_the_output_does_not_depend_on_whether_lse_is_wanted(cuda, B, S, H, K, W
         out, lse = ops.window_attention(q, k, v, B, S, H, K, W, sinks, lens, want_lse=True)
         assert torch.isfinite(out).all() and torch.isfinite(lse[:, :, :S - 70]).all()
         assert torch.equal(out, ops.window_attention(q, k, v, B, S, H, K, W, sinks, lens)[0])
+
+
+@pytest.mark.parametrize("n_q,lens,H,K,W,sinks", [
+    (1, [1, 2, 3, 60], 4, 1, 0, 0), (1, [300, 129], 4, 2, 0, 0), (5, [900, 70], 6, 2, 3, 1),
+    (1, [5000], 4, 1, 0, 0), (2, [1300, 1500], 4, 2, 0, 0), (40, [1500], 8, 2, 2, 0),
+    (300, [700], 12, 3, 100, 4)])
+def test_lse_over_the_cache_is_formed_in_f32(cuda, n_q, lens, H, K, W, sinks):
+    """By one workgroup a tile, and joined from parts."""
+    say("case:", n_q, lens, H, K, W, sinks)
+    rng = np.random.default_rng(sum(lens) + W)
+    batch, top = len(lens), max(lens)
+    pages = -(-top // PAGE)
+    table = i32(rng.permutation(batch * pages).reshape(batch, pages))
+    cache = ops.kv_cache_pages(batch * pages, K)
+    cache.fill_(255)
+    k, v = (synth.round_bf16(rng.standard_normal((batch * top, K * HD))) for _ in range(2))
+    q = synth.round_bf16(rng.standard_normal((batch * n_q, H * HD)))
+    ops.kv_cache_write(cache, table, i32([0] * batch), dev(k), dev(v), batch, top, K,
+                       counts=i32(lens))
+    out, lse = ops.kv_cache_attention(dev(q), cache, table, i32(lens), batch, n_q, H, K, W, sinks,
+                                      want_lse=True)
+    # The output is the same bits with and without it.
+    assert torch.equal(out, ops.kv_cache_attention(dev(q), cache, table, i32(lens), batch, n_q, H, K,
+                                                   W, sinks)[0])
+    kc = R.cached_values(k.reshape(-1, HD)).reshape(batch, top, K, HD)
+    for b, n in enumerate(lens):
+        for h in range(H):
+            want, bound = lse_and_bound(q[b * n_q:(b + 1) * n_q, h * HD:(h + 1) * HD],
+                                        kc[b, :n, h // (H // K)], n - n_q, W, sinks)
+            near(lse[b, h], want, bound, (b, h))
