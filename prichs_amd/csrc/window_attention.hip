@@ -558,6 +558,9 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
     if (none) return;
     const bool whole = t0 >= k0 + 16 - 1 && (sh.window == 0 || t0 + kTr - 1 - k0 < sh.window ||
                                          k0 + 16 <= sh.sinks);
+    // Rows past the sequence are zeros in the tiles, and p is 0 by their lse -- but not
+    // with a key that is not finite: their scores are NaN, and their dP.
+    const bool past = t0 + kTr > L;
     const uint32_t at = (uint32_t)((sg * kStages + slot) * kStepElems) * 2u;
     const char *tile = reinterpret_cast<const char *>(lds) + at;
     const uint32_t ra = lds_base + at + ra0, ta = lds_base + at + ta0;
@@ -580,6 +583,12 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
                                               (key < sh.sinks));
         x[r] = seen ? x[r] : 0.f;
       }
+    };
+    auto hide_past = [&](int qb, f32x4 &x) {
+      int row = t0 + 16 * qb + 4 * g;
+      asm volatile("" : "+v"(row));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = row + r < L ? x[r] : 0.f;
     };
     // Softmax and first products before the other waves' last ones: 1 x 16384 window
     // 4096 1411 -> 1390 us, 4 x 2048 158.7 -> 156.
@@ -608,6 +617,10 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
         hide(qb, p[qb]);
       }
     }
+    if (past) {
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) hide_past(qb, p[qb]);
+    }
     x[0] = x[1] = f32x4{0.f, 0.f, 0.f, 0.f};
     uint32_t va = lds_base + ra0 + v_tile + 2 * kHd * 16 * kg;
     asm volatile("" : "+v"(va));  // its fragments' addresses are not kept over the steps
@@ -631,6 +644,10 @@ __global__ __launch_bounds__(128 * kKg, 4) void window_dkv_kernel(BwdArgs a) {
         z = not_finite(x[qb], z);
         hide(qb, e[qb]);
       }
+    }
+    if (past) {
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) hide_past(qb, e[qb]);
     }
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {

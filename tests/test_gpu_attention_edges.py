@@ -1,6 +1,6 @@
 """Window attention and cache attention where their edges meet: the longest sequence, the
-workspace of a batch whose first blocks of keys are cut, and the log-sum-exp against its
-f32 bound."""
+workspace of a batch whose first blocks of keys are cut, the log-sum-exp against its f32
+bound, and keys that are not finite beside padding."""
 import numpy as np
 import pytest
 import torch
@@ -214,3 +214,54 @@ def test_lse_over_the_cache_is_formed_in_f32(cuda, n_q, lens, H, K, W, sinks):
             want, bound = lse_and_bound(q[b * n_q:(b + 1) * n_q, h * HD:(h + 1) * HD],
                                         kc[b, :n, h // (H // K)], n - n_q, W, sinks)
             near(lse[b, h], want, bound, (b, h))
+
+
+# ------------------------------------------------- keys that are not finite --
+def weightless(S, H, K, at, seed):
+    """Inputs where key `at` holds an infinity that gives it a score of -inf with every
+    query, and no weight."""
+    q, k, v, g = inputs(1, S, H, K, seed)
+    q[:, ::HD], k[:, ::HD] = -1, 0
+    k[at, ::HD] = np.inf
+    return q, k, v, g
+
+
+def without_key(q, k, v, g, H, K, W, sinks, at):
+    """R.batch_attention of whole sequences without key `at` (row `at` sees others)."""
+    S = len(q)
+    keep = np.ones(S, bool)
+    keep[at] = False
+    k = np.where(np.isfinite(k), k, 0)
+    r = {e + n: np.zeros((S, (H if n in ("out", "dq") else K) * HD))
+         for n in ("out", "dq", "dk", "dv") for e in ("", "e_")}
+    for h in range(H):
+        c, ck = slice(h * HD, (h + 1) * HD), slice(h // (H // K) * HD, (h // (H // K) + 1) * HD)
+        one = R.attention(q[:, c], k[:, ck], v[:, ck], W, sinks, d_out=g[:, c], keep=keep)
+        for n in ("out", "dq", "dk", "dv"):
+            for e in ("", "e_"):
+                r[e + n][:, c if n in ("out", "dq") else ck] += one[e + n]
+    return r
+
+
+@pytest.mark.parametrize("S,n,at", [(40, 40, 3), (40, 40, 33), (64, 40, 3), (96, 70, 66),
+                                    (400, 333, 200), (400, 333, 325)])
+def test_padding_does_not_reach_a_key_that_is_not_finite(cuda, S, n, at):
+    """Rows past a sequence's end are in the tiles of its last rows: a key without any
+    weight keeps gradients of zero, as it has without such rows."""
+    H, K, W, sinks = 4, 2, 100, 2
+    say("case:", S, n, at)
+    q, k, v, g = (x for x in weightless(n, H, K, at, 3))
+    ref = without_key(q, k, v, g, H, K, W, sinks, at)
+    t = []
+    for x in (q, k, v, g):
+        pad = torch.full((S, x.shape[1]), float("nan"), dtype=torch.bfloat16, device="cuda")
+        pad[:n] = dev(x)
+        t.append(pad)
+    sl = i32([n]) if S != n else None
+    out, lse = ops.window_attention(*t[:3], 1, S, H, K, W, sinks, sl, want_lse=True)
+    near(out[:n], ref["out"], ref["e_out"], "out")
+    _, dk, dv = ops.window_attention_backward(t[3], *t[:3], out, lse, 1, S, H, K, W, sinks, sl)
+    assert not host(dk[at]).any() and not host(dv[at]).any()
+    near(dk[:n], ref["dk"], ref["e_dk"], "dk")
+    near(dv[:n], ref["dv"], ref["e_dv"], "dv")
+    assert not host(dk[n:]).any() and not host(dv[n:]).any()
