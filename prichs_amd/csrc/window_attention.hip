@@ -204,8 +204,8 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
   const uint32_t tr_addr =
       lds_base + 2u * (uint32_t)(tile_off(4 * g + (l16 >> 2), (l16 & 3) >> 1) + 4 * (l16 & 1));
 
-  // One sweep over the blocks: f(half, S^T, dP^T, rare) for each half block that
-  // some row of the wave sees, hidden elements at -inf and 0.
+  // One sweep over the blocks: f(half, stage, first key, S^T, dP^T, rare) for each half
+  // block that some row of the wave sees, hidden elements at -inf and 0.
   auto sweep = [&](auto &&f) {
     if (n_blk > 0) issue(0);
 #pragma unroll 1
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
         if (!whole) {
           // What a row does not see must not reach it: hidden elements become p = 0,
           // and an infinity or NaN in K^T, which 0 would turn into NaN, is taken out
-          // of the product (a row that sees such a key has NaN in dS).  Rows past the
+          // of the product (see rare below).  Rows past the
           // sequence need no mask: their lse is +inf, and they reach no other row.
           // The wave's rows decide which of the rules a block needs.
           float z = 0.f;
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
           }
           rare = __any(!(z == 0.f)) != 0;
         }
-        f(half_c, stage, s, dp, rare);
+        f(half_c, stage, kv0 + 32 * half, s, dp, rare);
       });
     }
   };
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
   // sum p dP / sum p instead, in a sweep of their own (2 of the 3 products again).
   if (n_blk > 0 && n_blk <= kExactBlocks) {
     float num[NB] = {}, den[NB] = {};
-    sweep([&](auto, uint32_t, f32x4 (&s)[2][NB], f32x4 (&dp)[2][NB], bool) {
+    sweep([&](auto, uint32_t, int, f32x4 (&s)[2][NB], f32x4 (&dp)[2][NB], bool) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -326,7 +326,8 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
       rows[kTr + 16 * nb + l16] = delta[nb];
     }
 
-  sweep([&](auto half_c, uint32_t stage, f32x4 (&s)[2][NB], f32x4 (&dp)[2][NB], bool rare) {
+  sweep([&](auto half_c, uint32_t stage, int key0, f32x4 (&s)[2][NB], f32x4 (&dp)[2][NB],
+            bool rare) {
     constexpr int half = decltype(half_c)::value;
     u32x4 ds[NB];
 #pragma unroll
@@ -355,6 +356,33 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
         for (int nb = 0; nb < NB; ++nb)
           acc[j0 + t][nb] = mfma_bf16(__builtin_bit_cast(bf16x8, f[t]),
                                       __builtin_bit_cast(bf16x8, ds[nb]), acc[j0 + t][nb]);
+    }
+    if (rare) {
+      // A row that sees a key that is not finite: 0 (of a score of -inf) or NaN times
+      // what was taken out is NaN, in that element.
+      const char *kt = reinterpret_cast<const char *>(lds) + stage;
+#pragma unroll 1
+      for (int x = 0; x < 32; ++x) {
+        const int key = key0 + x;
+#pragma unroll
+        for (int jd = 0; jd < 8; ++jd) {
+          asm volatile("" ::: "memory");  // one load after the other: registers
+          const u32x2 raw = *reinterpret_cast<const u32x2 *>(
+              kt + ((uint32_t)(2 * (tile_off(32 * half + x, g >> 1) + 4 * (g & 1))) ^ (32u * jd)));
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            const int row = q0 + 16 * nb + l16;
+            const bool seen = (key <= row) & ((sh.window == 0) | (row - key < sh.window) |
+                                              (key < sh.sinks));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const uint32_t u = r & 1 ? raw[r / 2] & 0xffff0000u : raw[r / 2] << 16;
+              const bool off = (u & 0x7f800000u) == 0x7f800000u;
+              acc[jd][nb][r] = (off & seen) ? __uint_as_float(0x7fc00000u) : acc[jd][nb][r];
+            }
+          }
+        }
+      }
     }
   });
 

@@ -265,3 +265,24 @@ def test_padding_does_not_reach_a_key_that_is_not_finite(cuda, S, n, at):
     near(dk[:n], ref["dk"], ref["e_dk"], "dk")
     near(dv[:n], ref["dv"], ref["e_dv"], "dv")
     assert not host(dk[n:]).any() and not host(dv[n:]).any()
+
+
+@pytest.mark.parametrize("S,W,at", [(40, 0, 3), (300, 0, 70), (300, 100, 130), (900, 500, 310),
+                                    (900, 0, 5)])
+def test_d_q_of_a_row_that_sees_an_infinite_key(cuda, S, W, at):
+    """d_q = scale sum dS k: 0 times an infinity is NaN in that element, whether or not
+    the rows of the tile all see the key, and nothing elsewhere."""
+    H, K = 4, 2
+    q, k, v, g = weightless(S, H, K, at, 4)
+    ref = without_key(q, k, v, g, H, K, W, 0, at)
+    t = [dev(x) for x in (q, k, v, g)]
+    out, lse = ops.window_attention(*t[:3], 1, S, H, K, W, want_lse=True)
+    dq = ops.window_attention_backward(t[3], *t[:3], out, lse, 1, S, H, K, W)[0]
+    sees = (np.arange(S) >= at) & ((W == 0) | (np.arange(S) < at + W))
+    h = host(dq)
+    nan = np.zeros(h.shape, bool)
+    nan[sees, ::HD] = True
+    assert np.array_equal(np.isnan(h), nan)
+    dq[torch.from_numpy(nan).cuda()] = 0
+    ref["dq"][nan] = 0
+    near(dq, ref["dq"], ref["e_dq"], "dq")
