@@ -182,3 +182,14 @@ for b, n, p in ((1, 1, 5), (1, 1, 16), (1, 1, 2), (1, 1, 128), (2, 256, 68)):
             seen.add(y.kernel)
     assert seen == {"kv_attend_lse_kernel<4>", "kv_attend_lse_kernel<8>", "kv_join_lse_kernel<1>",
                     "kv_join_lse_kernel<8>"}
+
+
+def test_gpu_tests_deal_rows_and_key_blocks_and_join_cut_blocks_in_one_call():
+    from tests.test_gpu_attention_edges import DEALT
+
+    share = set()
+    for _, fwd, _, _, bwd in window_calls([c[:6] for c in DEALT]):
+        assert fwd[0].kernel.endswith("true, true>") and bwd[0].kernel.endswith("2, true>")
+        assert [x.kernel for x in bwd[1:]] == ["window_dkv_kernel<true>", "window_dkv_join_kernel"]
+        share.add(fwd[0].kernel)
+    assert len(share) == 3

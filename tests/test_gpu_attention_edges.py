@@ -1,6 +1,7 @@
 """Window attention and cache attention where their edges meet: the longest sequence, the
 workspace of a batch whose first blocks of keys are cut, the log-sum-exp against its f32
-bound, and keys that are not finite beside padding."""
+bound, keys that are not finite beside padding, and long sequences dealt by die with
+sinks."""
 import numpy as np
 import pytest
 import torch
@@ -286,3 +287,25 @@ def test_d_q_of_a_row_that_sees_an_infinite_key(cuda, S, W, at):
     dq[torch.from_numpy(nan).cuda()] = 0
     ref["dq"][nan] = 0
     near(dq, ref["dq"], ref["e_dq"], "dq")
+
+
+# ------------------------------------------------------------- dealt by die --
+# (batch, seq_len, heads, kv heads, window, sinks, lens): every one deals its rows and
+# its key blocks, and joins the blocks that the sinks cut (tests/test_attention_limits.py
+# checks that).
+DEALT = [(1, 8200, 8, 2, 150, 4, [8200]), (1, 8195, 6, 3, 70, 130, [8190]),
+         (2, 8193, 3, 3, 100, 9, [8193, 1200])]
+
+
+@pytest.mark.parametrize("B,S,H,K,W,sinks,lens", DEALT)
+def test_sinks_of_long_sequences_dealt_by_die(cuda, B, S, H, K, W, sinks, lens):
+    say("case:", B, S, H, K, W, sinks, lens)
+    x = inputs(B, S, H, K, S + W)
+    ref = by_pieces(*x, B, S, H, K, W, sinks, lens)
+    sl = i32(lens)
+    q, k, v, g = (dev(a) for a in x)
+    out, lse = ops.window_attention(q, k, v, B, S, H, K, W, sinks, sl, want_lse=True)
+    near(out, ref["out"], ref["e_out"], "out")
+    d = ops.window_attention_backward(g, q, k, v, out, lse, B, S, H, K, W, sinks, sl)
+    for t, name in zip(d, ("dq", "dk", "dv")):
+        near(t, ref[name], ref["e_" + name], name)
