@@ -356,8 +356,9 @@ int prichs_attention_forward_rope_q(const void *q, size_t ldq, const void *k,
  * [batch], may be NULL): sequence b has min(max(seq_lens[b], 0), seq_len) rows;
  * its further rows of q/k/v are not used and get zeros in o.  lse (device f32
  * [batch, n_heads, seq_len], may be NULL): log of the sum of exp(score) over the
- * visible keys, for the backward (-inf past a sequence's length).  Keys that a
- * query does not see do not reach it, whatever they hold.  Operands are 16-byte
+ * visible keys, in f32, for the backward (-inf past a sequence's length).  Keys that
+ * a query does not see do not reach it, whatever they hold.  o must not overlap k or
+ * v.  Operands are 16-byte
  * aligned; leading dimensions are multiples of 8 below 2^24, seq_len is at most
  * 2^21.  The reference has no windowed attention. */
 int prichs_window_attention_forward(const void *q, size_t ldq, const void *k,

@@ -93,8 +93,8 @@ __device__ __forceinline__ bf16x8 rope_frag(bf16x8 f, float4 c4, float4 s4) {
 // sinks and sequences of their own lengths (the arguments in wa); row i of a
 // sequence then sees the keys j <= i with i - j < window (0: all) or j < sinks.
 // DIE: workgroups dealt by die (attention_tile.hpp).  LSE: the log-sum-exp is written.
-// 12 + 3 heads with a window: 1 x 16384 of 4096 367 us
-// (980 TFLOP/s), 4 x 2048 of 512 49 us (460), 1 x 4096 whole 76 us (680), bound as
+// 12 + 3 heads with a window, without lse: 1 x 16384 of 4096 367 us
+// (980 TFLOP/s), 4 x 2048 of 512 48 us (470), 1 x 4096 whole 74 us (700), bound as
 // without one; a block of keys that some rows do not see costs its masks and a scan
 // of V (a whole causal 4 x 2048 takes 65 us here and 60 there).  1 x 777 of 256 13 us:
 // the latency of its five blocks of keys.

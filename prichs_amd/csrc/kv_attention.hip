@@ -16,10 +16,13 @@
 //                   is dim 8 m + jd.
 // Nothing goes through LDS before the waves join, there is no lane exchange but the
 // row maximum, and a page is read once per row tile: 8704 bytes against 32 KB in
-// bf16.  Bound by HBM where the caches are long (MI355X, 12 + 3 heads, 32 sequences
-// of 16384 positions: 214 MB in 40 us, 5.3 TB/s), by the latency of a page (about 2
+// bf16.  Bound by HBM where the caches are long (MI355X, 12 + 3 heads, 64 sequences
+// of 16384 positions: 428 MB, more than the last-level cache holds, in 89 us, 4.8
+// TB/s; 32 sequences, which it does hold, 41 us), by the latency of a page (about 2
 // us from its table entry to its last product) where they are short (one token over
-// 8192 positions: 8 us, 3.3 MB).  Three workgroups a CU hide each other's loads: a
+// 8192 positions: 8.6 us, 3.3 MB).  Some 80 scalar registers are spilled to lanes of
+// vector registers (none to memory), and about 80 of a page's 650 instructions move
+// them.  Three workgroups a CU hide each other's loads: a
 // second set of registers for a wave's next page cost the third and was no faster
 // (32 x 3000 positions 15.2 -> 16.1 us).  Tiles of 32 rows share the conversions of
 // two row blocks but leave half the waves (8 x 8 queries over 4096: 15.7 us against

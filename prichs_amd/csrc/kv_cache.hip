@@ -9,9 +9,11 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // Both kernels are bound by HBM (a read of 512 bytes and a write of 136 per
-// position and kv head in bf16, or the reverse): 32 sequences x 6000 positions x 3
-// heads, 373 MB, take 87 us either way (4.3 TB/s), 4 x 2048 positions 5.5 us, and one
-// new token of 32 sequences 3.3 us, which is the launch.  16 lanes hold one (position, kv
+// position and kv head in bf16, or the reverse; 1024 and 136 in f32).  32 sequences x
+// 6000 positions x 3 heads: 373 MB in bf16, written in 81 us and read in 93 back to
+// back (92 and 86 alone), 668 MB in f32, 137 and 175 (165 and 162): 4.0 to 4.9 TB/s.
+// 4 x 2048 positions: 5.2 and 5.5 us, f32 5.7 and 8.9; one new token of 32 sequences
+// 3.3 us, which is the launch.  16 lanes hold one (position, kv
 // head), 8 values each: one 16-byte access in bf16, one dword of codes.  Items run
 // over (sequence, head, row) with the row fastest, so that a wave's four items are
 // as a rule four positions of one head, whose V dwords are neighbours in the cache
