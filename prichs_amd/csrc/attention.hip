@@ -696,8 +696,8 @@ int window_attention_launch(const void *q, size_t ldq, const void *k, size_t ldk
   int i = 0;
   while (kinds[i].hpw != hpw || kinds[i].few != few || kinds[i].dies != dies) ++i;
   const auto kern = lse != nullptr ? kinds[i].with_lse : kinds[i].without;
-  if (int rc = raise_lds_limit(limits[i][lse != nullptr], reinterpret_cast<const void *>(kern), kWinLdsBytes,
-                               "window_attention"))
+  if (int rc = raise_lds_limit(limits[i][lse != nullptr], reinterpret_cast<const void *>(kern),
+                               kWinLdsBytes, "window_attention"))
     return rc;
   hipLaunchKernelGGL(kern, grid, dim3(kThreads), kWinLdsBytes, as_stream(stream),
                      static_cast<const bf16_t *>(q), (int)ldq, static_cast<const bf16_t *>(k),

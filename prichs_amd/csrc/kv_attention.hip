@@ -475,8 +475,8 @@ __global__ __launch_bounds__(256) void kv_join_lse_kernel(
 // 14.6 -> 10.6, 32 over 32 pages 11.1 -> 13.3.
 constexpr size_t kShortPages = 16;
 
-// How a call is cut: n_split workgroups of `waves` waves over a
-// tile's pages.
+// How a call is cut: n_split workgroups of `waves` waves over a tile's pages.  For 256
+// CUs whatever the current device has: a workspace's size may be asked for on another.
 struct Plan {
   int waves;
   size_t tiles, n_split;

@@ -246,9 +246,8 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(BwdArgs a) {
         if (!whole) {
           // What a row does not see must not reach it: hidden elements become p = 0,
           // and an infinity or NaN in K^T, which 0 would turn into NaN, is taken out
-          // of the product (see rare below).  Rows past the
-          // sequence need no mask: their lse is +inf, and they reach no other row.
-          // The wave's rows decide which of the rules a block needs.
+          // of the product (see rare below).  Rows past the sequence need no mask: they
+          // reach no other row.  The wave's rows decide which of the rules a block needs.
           float z = 0.f;
           const bool ahead = kv0 + kKeys - 1 > q0;
           const bool behind = sh.window != 0 && q0 + 16 * NB - 1 - kv0 >= sh.window &&
@@ -851,9 +850,10 @@ BwdPlan plan_bwd(const Shape &sh, size_t batch) {
     total += n;
     most = std::max<int64_t>(most, n);
   }
-  // One workgroup fits a CU.  The time is about that of the longest item where all
-  // items are resident, and the average load and half an item more beyond; an item
-  // of a cut block costs about 8 steps more (its sums go through memory), and has 8
+  // One workgroup fits a CU, of which 256 are counted on every device (a workspace's
+  // size may be asked for on another).  The time is about that of the longest item
+  // where all items are resident, and the average load and half an item more beyond; an
+  // item of a cut block costs about 8 steps more (its sums go through memory), and has 8
   // steps at least (whole backward with at least 4, 8, 12, us: 3 x 500 46.9, 46.4, 49.6;
   // 2 x 1000 47.2, 45.6, 48.6; 1 x 200 30.9, 33.0, 35.6).
   const int64_t wgs = (int64_t)batch * sh.Hkv, cus = 256;
