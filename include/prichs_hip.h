@@ -288,6 +288,44 @@ int prichs_rope_forward_ld(void *qk, size_t row_stride, int dtype,
                            size_t n_heads, size_t head_dim, size_t pos_offset,
                            int sign, void *stream);
 
+/* Queries and keys normed per head and rotated in one pass (memory-bound): head x of row
+ * r becomes R (x w / sqrt(mean(x^2) + eps)), R the rotation of prichs_rope_forward at the
+ * row's position: positions[r] (device int32 [rows]), or r % seq_len + pos_offset where
+ * positions is NULL.  q [rows, n_heads * head_dim] and k [rows, n_kv_heads * head_dim]
+ * with leading dimensions (multiples of 8), bf16 or f32 as their outputs; w_q, w_k f32
+ * [head_dim]; tables f32 [cache_rows, head_dim / 2]; arithmetic in f32, rounded once.
+ * Either of n_heads and n_kv_heads may be 0 (its operands are not used then).  Rows at
+ * positions outside the tables are padding: their outputs stay as they were.  An output
+ * may be its input (same address and leading dimension), and must not overlap an input
+ * otherwise.  head_dim is a multiple of 8 up to 256; operands are 16-byte aligned.  The
+ * reference has no norm of queries and keys. */
+int prichs_qk_norm_rope_forward(const void *q, size_t ldq, const void *k, size_t ldk,
+                                const float *w_q, const float *w_k, const float *cos_cache,
+                                const float *sin_cache, size_t cache_rows,
+                                const int32_t *positions, size_t seq_len,
+                                size_t pos_offset, void *q_out, size_t ldqo, void *k_out,
+                                size_t ldko, size_t rows, size_t n_heads,
+                                size_t n_kv_heads, size_t head_dim, float eps, int dtype,
+                                void *stream);
+/* Its gradients from those of the outputs and the inputs q, k.  With xh = x inv, inv = 1 /
+ * sqrt(mean(x^2) + eps), g = R^T d_out, t = g w:
+ *   d_x = inv (t - xh mean(t xh)),  d_w = sum over rows and heads of g xh
+ * (d_wq, d_wk f32 [head_dim]: beta * d_w + the sum, beta 0 or 1, as the MoE gradients).
+ * Padding rows get zeros and add nothing.  d_q and d_k may be the gradients of the outputs
+ * (same address and leading dimension).  Deterministic.  workspace: device memory, 16-byte
+ * aligned, of at least prichs_qk_norm_rope_backward_workspace bytes, used by this call
+ * alone until it has finished. */
+size_t prichs_qk_norm_rope_backward_workspace(size_t rows, size_t n_heads,
+                                              size_t n_kv_heads, size_t head_dim);
+int prichs_qk_norm_rope_backward(
+    const void *d_q_out, size_t lddqo, const void *d_k_out, size_t lddko, const void *q,
+    size_t ldq, const void *k, size_t ldk, const float *w_q, const float *w_k,
+    const float *cos_cache, const float *sin_cache, size_t cache_rows,
+    const int32_t *positions, size_t seq_len, size_t pos_offset, void *d_q, size_t lddq,
+    void *d_k, size_t lddk, float *d_wq, float *d_wk, int beta, size_t rows,
+    size_t n_heads, size_t n_kv_heads, size_t head_dim, float eps, int dtype,
+    void *workspace, size_t workspace_bytes, void *stream);
+
 /* out = a + b element-wise in f32 arithmetic; each operand bf16 or f32.
  * Replaces add_tensors (crates/prichs-core/src/ops.rs:250-267) for the
  * block's residual connections.  n % 8 == 0, 16-byte aligned operands. */
@@ -448,6 +486,79 @@ int prichs_kv_cache_attention(const void *q, size_t ldq, const void *cache,
                               size_t window, size_t sinks, int dtype,
                               void *workspace, size_t workspace_bytes,
                               void *stream);
+
+/* The same attention where groups of sequences share their first pages: sequences
+ * group_start[g] .. group_start[g + 1] - 1 (group_start: device int32 [n_groups + 1])
+ * hold their first shared[g] positions (device int32 [n_groups]; whole pages count) in
+ * the same pages, those of the group's first sequence's row of the table.  These are
+ * read, and their products formed, once for the group.  A start counts as no less than
+ * those before it, and as no less than 0 and no more than batch; sequences outside every
+ * group share nothing, a group may be empty.  Everything else as above. */
+size_t prichs_kv_cache_shared_attention_workspace(size_t batch, size_t n_q, size_t n_heads,
+                                                  size_t n_kv_heads, size_t max_pages,
+                                                  size_t n_groups);
+int prichs_kv_cache_shared_attention(const void *q, size_t ldq, const void *cache,
+                                     size_t n_pages, const int32_t *page_table,
+                                     size_t max_pages, const int32_t *lens,
+                                     const int32_t *group_start, const int32_t *shared,
+                                     size_t n_groups, void *o, size_t ldo, float *lse,
+                                     size_t batch, size_t n_q, size_t n_heads,
+                                     size_t n_kv_heads, size_t head_dim, size_t window,
+                                     size_t sinks, int dtype, void *workspace,
+                                     size_t workspace_bytes, void *stream);
+
+/* The pages of a cache, kept on the device: refs (device int32 [n_pages]) counts how many
+ * table entries (and other holders: a caller may add its own) name each page, 0 for a
+ * free one (a negative count is a free page too).  page_table: device int32 [batch]
+ * [max_pages], entries outside [0, n_pages) name no page, -1 being written for none.  Free pages are taken lowest first, items in their
+ * order, so results are those of the steps done one after the other.  Nothing is read on
+ * the host.  shortfall (device int32 [1], may be NULL) gets the number of pages that a
+ * call wanted and did not get; their entries are -1.  n_pages is at most 2^24, batch and
+ * n 2^20, batch * max_pages 2^31 - 1.  workspace: device memory, 16-byte aligned, of
+ * prichs_kv_pages_workspace bytes (for the call's n_pages, batch and n; n = 0 for
+ * reserve, batch = n = 0 for compact), used by the call alone until it has finished.
+ *
+ * reserve: every sequence gets pages for its positions lens[b] .. lens[b] + counts[b] - 1
+ *   (lens, counts: device int32 [batch]) where the table names none yet; entries past
+ *   the table count as not got.
+ * fork: for i < n table row children[i] becomes a copy of row parents[i] (device int32
+ *   [n], distinct rows of the table), lens[children[i]] the parent's length: whole pages
+ *   are shared (their counts rise by one), a partly filled last page is copied into a new
+ *   one, further entries are -1.  What the child's row held is overwritten, not given
+ *   back (release it first).  Left out: an item with a row outside the table, one whose
+ *   child an earlier item names too, and one whose parent is the child of any item.
+ * release: rows rows[i] (device int32 [n]) of the table keep the entries of their first
+ *   keep[i] positions (keep: device int32 [n], or NULL for none); the others give their
+ *   pages back and become -1.  Rows outside the table are left out; one named twice
+ *   keeps the least of its keeps.
+ * compact: with L pages in use, those at L and above move to the free pages below L, the
+ *   lowest to the lowest and so on; counts and table entries follow (an entry that names
+ *   a free page becomes -1).  new_page (device int32 [n_pages]) gets each old page's new
+ *   number, -1 for a free one, *n_live (device int32 [1]) L.  Pages from L on are free
+ *   afterwards; their bytes stay what they were. */
+size_t prichs_kv_pages_workspace(size_t n_pages, size_t batch, size_t n);
+int prichs_kv_pages_reserve(int32_t *refs, size_t n_pages, int32_t *page_table,
+                            size_t max_pages, const int32_t *lens, const int32_t *counts,
+                            size_t batch, int32_t *shortfall, void *workspace,
+                            size_t workspace_bytes, void *stream);
+int prichs_kv_pages_fork(void *cache, int32_t *refs, size_t n_pages, int32_t *page_table,
+                         size_t max_pages, int32_t *lens, size_t batch,
+                         const int32_t *parents, const int32_t *children, size_t n,
+                         size_t n_kv_heads, int32_t *shortfall, void *workspace,
+                         size_t workspace_bytes, void *stream);
+int prichs_kv_pages_release(int32_t *refs, size_t n_pages, int32_t *page_table,
+                            size_t max_pages, size_t batch, const int32_t *rows,
+                            const int32_t *keep, size_t n, void *stream);
+int prichs_kv_pages_compact(void *cache, int32_t *refs, size_t n_pages, int32_t *page_table,
+                            size_t max_pages, size_t batch, size_t n_kv_heads,
+                            int32_t *new_page, int32_t *n_live, void *workspace,
+                            size_t workspace_bytes, void *stream);
+/* Page from[i] of src becomes page to[i] of dst (device int32 [n]; pairs with a page
+ * outside either cache are left out): to a larger cache, or within one (dst = src), where
+ * no page may be both read and written.  No page may be written twice. */
+int prichs_kv_cache_copy(void *dst, size_t dst_pages, const void *src, size_t src_pages,
+                         const int32_t *to, const int32_t *from, size_t n,
+                         size_t n_kv_heads, void *stream);
 
 /* f32 causal attention of one sequence with the probabilities kept: the
  * per-head computation of crates/prichs-model/src/attention.rs:96-149 (scores

@@ -116,6 +116,13 @@ SIGNATURES = {
     "prichs_rope_forward": (_i, [_vp, _i, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _i, _vp]),
     "prichs_rope_cache": (_i, [_sz, _sz, _f, _vp, _vp]),
     "prichs_rope_forward_ld": (_i, [_vp, _sz, _i, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _i, _vp]),
+    "prichs_qk_norm_rope_forward": (_i, [_vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _sz,
+                                         _sz, _vp, _sz, _vp, _sz, _sz, _sz, _sz, _sz, _f, _i,
+                                         _vp]),
+    "prichs_qk_norm_rope_backward_workspace": (_sz, [_sz, _sz, _sz, _sz]),
+    "prichs_qk_norm_rope_backward": (_i, [_vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp,
+                                          _vp, _sz, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _vp,
+                                          _i, _sz, _sz, _sz, _sz, _f, _i, _vp, _sz, _vp]),
     "prichs_add": (_i, [_vp, _i, _vp, _i, _vp, _i, _sz, _vp]),
     "prichs_hbm_copy": (_i, [_vp, _vp, _sz, _vp]),
     "prichs_packed_weight_elems": (_sz, [_sz, _sz, _i]),
@@ -138,6 +145,17 @@ SIGNATURES = {
     "prichs_kv_cache_attention_workspace": (_sz, [_sz, _sz, _sz, _sz, _sz]),
     "prichs_kv_cache_attention": (_i, [_vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _sz, _vp, _sz, _sz,
                                        _sz, _sz, _sz, _sz, _sz, _i, _vp, _sz, _vp]),
+    "prichs_kv_cache_shared_attention_workspace": (_sz, [_sz, _sz, _sz, _sz, _sz, _sz]),
+    "prichs_kv_cache_shared_attention": (_i, [_vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _sz,
+                                              _vp, _sz, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _sz, _i,
+                                              _vp, _sz, _vp]),
+    "prichs_kv_pages_workspace": (_sz, [_sz, _sz, _sz]),
+    "prichs_kv_pages_reserve": (_i, [_vp, _sz, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _sz, _vp]),
+    "prichs_kv_pages_fork": (_i, [_vp, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _sz, _sz, _vp, _vp,
+                                  _sz, _vp]),
+    "prichs_kv_pages_release": (_i, [_vp, _sz, _vp, _sz, _sz, _vp, _vp, _sz, _vp]),
+    "prichs_kv_pages_compact": (_i, [_vp, _vp, _sz, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _sz, _vp]),
+    "prichs_kv_cache_copy": (_i, [_vp, _sz, _vp, _sz, _vp, _vp, _sz, _sz, _vp]),
     "prichs_attention_probs_f32": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _vp]),
     "prichs_checkpoint_open": (_i, [C.c_char_p, C.POINTER(_vp)]),
     "prichs_checkpoint_close": (_i, [_vp]),

@@ -505,3 +505,274 @@ def kv_cache_attention(q, cache, page_table, lens, batch, n_q, n_heads, n_kv_hea
             lens.data_ptr(), out.data_ptr(), ldo, _a(lse), batch, n_q, n_heads, n_kv_heads,
             head_dim, window, sinks, L.DTYPE_BF16, _a(ws), need, s))
     return out, lse
+
+
+def kv_cache_shared_attention(q, cache, page_table, lens, group_start, shared, batch, n_q, n_heads,
+                              n_kv_heads, window=0, sinks=0, head_dim=128, out=None,
+                              want_lse=False, stream=None):
+    """prichs_kv_cache_shared_attention: kv_cache_attention of a batch whose sequences
+    group_start[g] .. group_start[g + 1] - 1 hold their first shared[g] positions in the
+    same pages (group_start int32 device [n_groups + 1], shared [n_groups]), which are
+    read once for the group.  -> (out, lse f32 [batch, n_heads, n_q], or None)."""
+    lib = L.load()
+    _kv_cache(cache, page_table, batch, n_kv_heads)
+    rows, H = batch * n_q, n_heads * head_dim
+    ldq = _rows(q, "q", rows, H)
+    _i32(lens, "lens", batch)
+    n_groups = shared.shape[0] if shared.dim() == 1 else -1
+    _i32(shared, "shared", n_groups)
+    _i32(group_start, "group_start", n_groups + 1)
+    if window < 0 or sinks < 0:
+        raise ValueError("window and sinks must not be negative")
+    ctx, s = _launch_on(stream, q, cache, page_table, lens, group_start, shared, out)
+    with ctx:
+        if out is None:
+            out = q.new_empty((rows, H))
+        ldo = _rows(out, "out", rows, H)
+        lse = None
+        if want_lse:
+            lse = torch.empty((batch, n_heads, n_q), dtype=torch.float32, device=q.device)
+        max_pages = page_table.shape[1]
+        need = lib.prichs_kv_cache_shared_attention_workspace(batch, n_q, n_heads, n_kv_heads,
+                                                              max_pages, n_groups)
+        ws = q.new_empty((need + 1) // 2)  # of two bytes each: a faster call
+        L.check(lib.prichs_kv_cache_shared_attention(
+            q.data_ptr(), ldq, cache.data_ptr(), cache.shape[0], page_table.data_ptr(), max_pages,
+            lens.data_ptr(), group_start.data_ptr(), shared.data_ptr(), n_groups, out.data_ptr(),
+            ldo, _a(lse), batch, n_q, n_heads, n_kv_heads, head_dim, window, sinks, L.DTYPE_BF16,
+            ws.data_ptr(), need, s))
+    return out, lse
+
+
+# --------------------------------------------------- pages of the KV cache ----
+def kv_pages_refs(n_pages, device="cuda"):
+    """Counts for a cache whose pages are all free: int32 [n_pages], zeros."""
+    return torch.zeros((n_pages,), dtype=torch.int32, device=device)
+
+
+def _pages(refs, page_table):
+    _i32(refs, "refs", refs.shape[0] if refs.dim() == 1 else -1)
+    _i32(page_table, "page_table", page_table.shape[0] if page_table.dim() == 2 else -1, dim=2)
+    return refs.shape[0], page_table.shape[0], page_table.shape[1]
+
+
+def _pages_cache(cache, n_pages, n_kv_heads):
+    if cache.dtype != torch.uint8 or not cache.is_contiguous() or \
+            cache.shape != (n_pages, n_kv_heads, L.KV_PAGE_BYTES):
+        raise ValueError("cache: expected the pages of kv_cache_pages for these refs and kv heads")
+
+
+def _pages_work(lib, refs, n_pages, batch, n):
+    need = lib.prichs_kv_pages_workspace(n_pages, batch, n)
+    return refs.new_empty((need + 3) // 4), need
+
+
+def kv_pages_reserve(refs, page_table, lens, counts, shortfall=None, stream=None):
+    """prichs_kv_pages_reserve: pages for positions lens[b] .. lens[b] + counts[b] - 1 of
+    every sequence (int32 device [batch]) where page_table (int32 device [batch,
+    max_pages]) names none; refs: int32 device [n_pages], the count of each page's
+    holders.  shortfall: int32 device [1], gets the number of pages that were not to be
+    had."""
+    n_pages, batch, max_pages = _pages(refs, page_table)
+    _i32(lens, "lens", batch)
+    _i32(counts, "counts", batch)
+    if shortfall is not None:
+        _i32(shortfall, "shortfall", 1)
+    ctx, s = _launch_on(stream, refs, page_table, lens, counts, shortfall)
+    with ctx:
+        lib = L.load()
+        ws, need = _pages_work(lib, refs, n_pages, batch, 0)
+        L.check(lib.prichs_kv_pages_reserve(
+            refs.data_ptr(), n_pages, page_table.data_ptr(), max_pages, lens.data_ptr(),
+            counts.data_ptr(), batch, _a(shortfall), ws.data_ptr(), need, s))
+
+
+def kv_pages_fork(cache, refs, page_table, lens, parents, children, n_kv_heads, shortfall=None,
+                  stream=None):
+    """prichs_kv_pages_fork: row children[i] of the table and of lens becomes a copy of
+    row parents[i] (int32 device [n]); whole pages are shared, a partly filled last page
+    is copied into a new one.  The children's rows must hold no pages (release them
+    first).  shortfall as for kv_pages_reserve."""
+    n_pages, batch, max_pages = _pages(refs, page_table)
+    _pages_cache(cache, n_pages, n_kv_heads)
+    _i32(lens, "lens", batch)
+    n = parents.shape[0] if parents.dim() == 1 else -1
+    _i32(parents, "parents", n)
+    _i32(children, "children", n)
+    if shortfall is not None:
+        _i32(shortfall, "shortfall", 1)
+    ctx, s = _launch_on(stream, cache, refs, page_table, lens, parents, children, shortfall)
+    with ctx:
+        lib = L.load()
+        ws, need = _pages_work(lib, refs, n_pages, batch, n)
+        L.check(lib.prichs_kv_pages_fork(
+            cache.data_ptr(), refs.data_ptr(), n_pages, page_table.data_ptr(), max_pages,
+            lens.data_ptr(), batch, parents.data_ptr(), children.data_ptr(), n, n_kv_heads,
+            _a(shortfall), ws.data_ptr(), need, s))
+
+
+def kv_pages_release(refs, page_table, rows, keep=None, stream=None):
+    """prichs_kv_pages_release: rows rows[i] of the table (int32 device [n]) keep the
+    pages of their first keep[i] positions (int32 device [n]; None: no positions) and
+    give the others back."""
+    n_pages, batch, max_pages = _pages(refs, page_table)
+    n = rows.shape[0] if rows.dim() == 1 else -1
+    _i32(rows, "rows", n)
+    if keep is not None:
+        _i32(keep, "keep", n)
+    ctx, s = _launch_on(stream, refs, page_table, rows, keep)
+    with ctx:
+        L.check(L.load().prichs_kv_pages_release(
+            refs.data_ptr(), n_pages, page_table.data_ptr(), max_pages, batch, rows.data_ptr(),
+            _a(keep), n, s))
+
+
+def kv_pages_compact(cache, refs, page_table, n_kv_heads, stream=None):
+    """prichs_kv_pages_compact: the pages in use moved to the front of the cache.  ->
+    (number of pages in use int32 [1], each old page's new number int32 [n_pages], -1 for
+    a free one)."""
+    n_pages, batch, max_pages = _pages(refs, page_table)
+    _pages_cache(cache, n_pages, n_kv_heads)
+    ctx, s = _launch_on(stream, cache, refs, page_table)
+    with ctx:
+        lib = L.load()
+        ws, need = _pages_work(lib, refs, n_pages, 0, 0)
+        n_live, new_page = refs.new_empty(1), refs.new_empty(n_pages)
+        L.check(lib.prichs_kv_pages_compact(
+            cache.data_ptr(), refs.data_ptr(), n_pages, page_table.data_ptr(), max_pages, batch,
+            n_kv_heads, new_page.data_ptr(), n_live.data_ptr(), ws.data_ptr(), need, s))
+    return n_live, new_page
+
+
+def kv_cache_copy(dst, src, to, from_, n_kv_heads, stream=None):
+    """prichs_kv_cache_copy: page from_[i] of the cache src becomes page to[i] of dst
+    (int32 device [n]); dst may be src where no page is both."""
+    _pages_cache(dst, dst.shape[0], n_kv_heads)
+    _pages_cache(src, src.shape[0], n_kv_heads)
+    n = to.shape[0] if to.dim() == 1 else -1
+    _i32(to, "to", n)
+    _i32(from_, "from_", n)
+    ctx, s = _launch_on(stream, dst, src, to, from_)
+    with ctx:
+        L.check(L.load().prichs_kv_cache_copy(dst.data_ptr(), dst.shape[0], src.data_ptr(),
+                                              src.shape[0], to.data_ptr(), from_.data_ptr(), n,
+                                              n_kv_heads, s))
+    return dst
+
+
+# ------------------------------------- norms of queries and keys, rotated ----
+def _qk(q, k, n_heads, n_kv_heads, head_dim, names):
+    """Rows, row strides and dtype of a pair of operands, either of which is None where
+    it has no heads."""
+    lds, rows, dtype = [0, 0], None, None
+    for i, (t, h, name) in enumerate(((q, n_heads, names[0]), (k, n_kv_heads, names[1]))):
+        if h == 0:
+            continue
+        if t is None:
+            raise ValueError(f"{name}: missing")
+        if rows is None:
+            rows, dtype = t.shape[0], t.dtype
+        elif t.dtype != dtype:
+            raise TypeError(f"{names[0]} and {names[1]} have different dtypes")
+        elif t.shape[0] != rows:
+            raise ValueError(f"{names[0]} and {names[1]} have different numbers of rows")
+        lds[i] = _rows(t, name, rows, h * head_dim, _FLOATS)
+    if rows is None:
+        raise ValueError("no heads at all")
+    return rows, lds, dtype
+
+
+def _f32(t, name, n):
+    if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != n:
+        raise ValueError(f"{name}: expected contiguous f32 of {n} elements")
+
+
+def _norm_rope_args(w_q, w_k, cos, sin, n_heads, n_kv_heads, head_dim, positions, seq_len, rows):
+    if n_heads:
+        _f32(w_q, "w_q", head_dim)
+    if n_kv_heads:
+        _f32(w_k, "w_k", head_dim)
+    if cos.dim() != 2 or cos.shape[1] * 2 != head_dim:
+        raise ValueError("cos, sin: expected f32 [positions, head_dim / 2]")
+    for t, name in ((cos, "cos"), (sin, "sin")):
+        _f32(t, name, cos.shape[0] * cos.shape[1])
+    if positions is not None:
+        _i32(positions, "positions", rows)
+    return rows if seq_len is None else seq_len
+
+
+def qk_norm_rope(q, k, w_q, w_k, cos, sin, n_heads, n_kv_heads, head_dim=128, eps=1e-5,
+                 positions=None, seq_len=None, pos_offset=0, q_out=None, k_out=None, stream=None):
+    """prichs_qk_norm_rope_forward: each head of q and k (2-D row views, bf16 or f32)
+    normed with w_q / w_k (f32 [head_dim]) and rotated to its row's position: positions[r]
+    (int32 device [rows]), or r % seq_len + pos_offset (seq_len None: the rows are one
+    sequence).  cos, sin: f32 [positions, head_dim / 2].  q_out / k_out may be q / k.  With
+    n_heads or n_kv_heads 0 that operand is None.  -> (q_out, k_out)."""
+    rows, ld, dtype = _qk(q, k, n_heads, n_kv_heads, head_dim, ("q", "k"))
+    seq_len = _norm_rope_args(w_q, w_k, cos, sin, n_heads, n_kv_heads, head_dim, positions,
+                              seq_len, rows)
+    if pos_offset < 0 or seq_len < 0:
+        raise ValueError("seq_len and pos_offset must not be negative")
+    if not n_heads:
+        q = w_q = q_out = None
+    if not n_kv_heads:
+        k = w_k = k_out = None
+    ctx, s = _launch_on(stream, cos, q, k, w_q, w_k, sin, positions, q_out, k_out)
+    with ctx:
+        if q_out is None and n_heads:
+            q_out = q.new_empty((rows, n_heads * head_dim))
+        if k_out is None and n_kv_heads:
+            k_out = k.new_empty((rows, n_kv_heads * head_dim))
+        r2, ldo, d2 = _qk(q_out, k_out, n_heads, n_kv_heads, head_dim, ("q_out", "k_out"))
+        if r2 != rows or d2 != dtype:
+            raise ValueError("q_out, k_out: expected the rows and the dtype of q and k")
+        L.check(L.load().prichs_qk_norm_rope_forward(
+            _a(q), ld[0], _a(k), ld[1], _a(w_q), _a(w_k), cos.data_ptr(), sin.data_ptr(),
+            cos.shape[0], _a(positions), seq_len if rows else 1, pos_offset, _a(q_out), ldo[0],
+            _a(k_out), ldo[1], rows, n_heads, n_kv_heads, head_dim, eps, _TORCH_DTYPES[dtype], s))
+    return q_out, k_out
+
+
+def qk_norm_rope_backward(d_q_out, d_k_out, q, k, w_q, w_k, cos, sin, n_heads, n_kv_heads,
+                          head_dim=128, eps=1e-5, positions=None, seq_len=None, pos_offset=0,
+                          d_q=None, d_k=None, d_wq=None, d_wk=None, accumulate=False, stream=None):
+    """prichs_qk_norm_rope_backward -> (d_q, d_k, d_wq, d_wk): gradients of q and k (d_q /
+    d_k may be d_q_out / d_k_out) and, in f32, of the weights (added to d_wq and d_wk with
+    accumulate)."""
+    lib = L.load()
+    rows, ld, dtype = _qk(q, k, n_heads, n_kv_heads, head_dim, ("q", "k"))
+    r2, ldd, d2 = _qk(d_q_out, d_k_out, n_heads, n_kv_heads, head_dim, ("d_q_out", "d_k_out"))
+    if r2 != rows or d2 != dtype:
+        raise ValueError("d_q_out, d_k_out: expected the rows and the dtype of q and k")
+    seq_len = _norm_rope_args(w_q, w_k, cos, sin, n_heads, n_kv_heads, head_dim, positions,
+                              seq_len, rows)
+    if pos_offset < 0 or seq_len < 0:
+        raise ValueError("seq_len and pos_offset must not be negative")
+    if not n_heads:
+        q = w_q = d_q_out = d_q = d_wq = None
+    if not n_kv_heads:
+        k = w_k = d_k_out = d_k = d_wk = None
+    if accumulate and (n_heads and d_wq is None or n_kv_heads and d_wk is None):
+        raise ValueError("accumulate needs the d_wq and d_wk to add to")
+    ctx, s = _launch_on(stream, cos, d_q_out, d_k_out, q, k, w_q, w_k, sin, positions, d_q, d_k,
+                        d_wq, d_wk)
+    with ctx:
+        if n_heads:
+            d_q = q.new_empty((rows, n_heads * head_dim)) if d_q is None else d_q
+            d_wq = w_q.new_empty(head_dim) if d_wq is None else d_wq
+            _f32(d_wq, "d_wq", head_dim)
+        if n_kv_heads:
+            d_k = k.new_empty((rows, n_kv_heads * head_dim)) if d_k is None else d_k
+            d_wk = w_k.new_empty(head_dim) if d_wk is None else d_wk
+            _f32(d_wk, "d_wk", head_dim)
+        r2, ldo, d2 = _qk(d_q, d_k, n_heads, n_kv_heads, head_dim, ("d_q", "d_k"))
+        if r2 != rows or d2 != dtype:
+            raise ValueError("d_q, d_k: expected the rows and the dtype of q and k")
+        need = lib.prichs_qk_norm_rope_backward_workspace(rows, n_heads, n_kv_heads, head_dim)
+        ws = cos.new_empty((need + 3) // 4)
+        L.check(lib.prichs_qk_norm_rope_backward(
+            _a(d_q_out), ldd[0], _a(d_k_out), ldd[1], _a(q), ld[0], _a(k), ld[1], _a(w_q), _a(w_k),
+            cos.data_ptr(), sin.data_ptr(), cos.shape[0], _a(positions), seq_len if rows else 1,
+            pos_offset, _a(d_q), ldo[0], _a(d_k), ldo[1], _a(d_wq), _a(d_wk), int(accumulate), rows,
+            n_heads, n_kv_heads, head_dim, eps, _TORCH_DTYPES[dtype], ws.data_ptr(), need, s))
+    return d_q, d_k, d_wq, d_wk
