@@ -39,6 +39,13 @@ int fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
     if (!(cond)) return ::prichs::fail(PRICHS_ERR_INVALID_ARGUMENT, __VA_ARGS__); \
   } while (0)
 
+// Returns the status of a call that has failed (and recorded why).
+#define PRICHS_TRY(expr)              \
+  do {                                \
+    const int _rc = (expr);           \
+    if (_rc != PRICHS_OK) return _rc; \
+  } while (0)
+
 inline hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
 
 // Number of compute units of the current device (cached per device).

@@ -66,6 +66,27 @@ __device__ __forceinline__ u32x4 eight(uint32_t codes, float scale) {
                pair<3>(codes, scale)};
 }
 
+// Bit e: whether a row sees key e from some first key on, for a row at position `lim` from
+// that key, and sinks up to key `sink` (exclusive).
+__device__ __forceinline__ uint64_t bits_below(int n) {
+  return n >= 64 ? ~0ull : (1ull << max(n, 0)) - 1;
+}
+__device__ __forceinline__ uint64_t visible_keys(int lim, int window, int sink) {
+  const uint64_t old = window == 0 ? 0 : bits_below(lim - window + 1) & ~bits_below(sink);
+  return bits_below(lim + 1) & ~old;
+}
+// The score, or -inf where bit e of `vis` is not set: without comparisons, whose results
+// would take a pair of scalar registers each.
+__device__ __forceinline__ float or_hidden(uint64_t vis, int e, float s) {
+  const uint32_t half = e < 32 ? (uint32_t)vis : (uint32_t)(vis >> 32);
+  const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)half, e & 31, 1);
+  return __uint_as_float((m & __float_as_uint(s)) | (~m & 0xff800000u));
+}
+// The top bit of each byte of x that is greater than 252.
+__device__ __forceinline__ uint32_t bytes_past_252(uint32_t x) {
+  return ((x & 0x7f7f7f7fu) + 0x03030303u) & x & 0x80808080u;
+}
+
 // A page of one kv head as a lane holds it.
 struct PageRegs {
   u32x4 k[4];  // key 16 c + lane % 16, dims 32 g ..
@@ -78,13 +99,15 @@ struct PageRegs {
 // launch then has two kinds of workgroup: splits of a group's tiles over its shared pages,
 // and splits of each sequence's tiles over its own.  Each writes the parts of its rows
 // into a slot of its own, split_p slots for shared and split_s for own pages.
-struct NoGroups {};
+enum { kWholeRole, kSharedRole, kOwnRole };  // a call without groups; the two kinds
 struct Groups {
   const int32_t *start, *shared;
   int n, batch;
   int tiles_p, split_p, split_s;  // tiles over shared pages at most, of one kv head
 };
-template <typename G> constexpr bool has_groups = std::is_same<G, Groups>::value;
+__device__ __forceinline__ int shared_workgroups(const AttendShape &sh, const Groups &gr) {
+  return sh.Hkv * gr.tiles_p * gr.split_p;
+}
 
 // Whole pages that `positions` cover.
 __device__ __forceinline__ int whole_pages(int positions, int max_pages) {
@@ -98,11 +121,12 @@ __device__ __forceinline__ int shared_pages_of(const Groups &gr, int b, int max_
   const int lane = threadIdx.x & 63;
   for (int base = 0; base <= gr.n; base += 64) {
     const int i = base + lane;
-    const uint64_t past = __ballot((i <= gr.n ? gr.start[i] : 0x7fffffff) > b);
-    if (past != 0) {
-      const int g = base + __ffsll((unsigned long long)past) - 2;
-      return g >= 0 && g < gr.n ? whole_pages(gr.shared[g], max_pages) : 0;
-    }
+    const int start = i <= gr.n ? gr.start[i] : 0x7fffffff;
+    const int before = i >= 1 && i <= gr.n ? gr.shared[i - 1] : 0;  // of the group that ends here
+    const uint64_t past = __ballot(start > b);
+    if (past != 0)
+      return whole_pages(
+          __builtin_amdgcn_readlane(before, __ffsll((unsigned long long)past) - 1), max_pages);
   }
   return 0;
 }
@@ -147,8 +171,7 @@ __device__ __forceinline__ bool shared_tile(const Groups &gr, int tile, int per,
   }
   return false;
 }
-// Rows of a call, and the number of one of them, as the slots of a launch with groups
-// have them.
+// Rows of a call: the distance of two slots.
 __device__ __forceinline__ size_t all_rows(const AttendShape &sh, const Groups &gr) {
   return (size_t)gr.batch * sh.n_q * sh.Hq;
 }
@@ -168,16 +191,25 @@ __device__ __forceinline__ float part_sum(float mw, float lw, float m) {
   return mw == -INFINITY && m != -INFINITY ? 0.f : lw * part_weight(mw, m);
 }
 
-template <int kWaves, bool LSE, typename GroupsT = NoGroups>
+// LDS that the waves of a workgroup join in, 16 rows at a time.
+template <int kWaves> struct JoinLds {
+  float o[kWaves][kRows * kLdRow];
+  float ml[3][kWaves][kRows];
+};
+
+// A workgroup's tile of 16 NB rows; NB > 1 (with groups) shares a page's conversions among
+// more rows.
+template <int kWaves, bool LSE, int ROLE = kWholeRole, int NB = 1>
 __device__ __forceinline__ void kv_attend(
     const bf16_t *__restrict__ q, size_t ldq, const uint8_t *__restrict__ cache,
     const int32_t *__restrict__ table, const int32_t *__restrict__ lens, bf16_t *__restrict__ o,
     size_t ldo, float *__restrict__ lse, float *__restrict__ part_o, float2 *__restrict__ part_ml,
-    const AttendShape &sh, const GroupsT gr = {}) {
-  constexpr bool kGroups = has_groups<GroupsT>;
-  constexpr int kThreads = 64 * kWaves;
-  __shared__ float s_ml[LSE ? 3 : 2][kWaves][kRows];
-  __shared__ float s_o[kWaves][kRows * kLdRow];
+    const AttendShape &sh, JoinLds<kWaves> &s, const Groups &gr) {
+  constexpr bool kGroups = ROLE != kWholeRole;
+  static_assert(NB == 1 || kGroups, "whole sequences have tiles of 16 rows");
+  constexpr int kThreads = 64 * kWaves, kTileRows = 16 * NB;
+  auto &s_ml = s.ml;
+  auto &s_o = s.o;
 
   int split = blockIdx.y, n_split = sh.n_split;
   int kvh = blockIdx.x / sh.tiles, tile = blockIdx.x - kvh * sh.tiles;
@@ -190,40 +222,51 @@ __device__ __forceinline__ void kv_attend(
   // With groups: the pages that count, and the slot of the parts.
   int lo = 0, hi = sh.max_pages, slot = 0;
   bool alone = false;  // no workgroup writes the slots for shared pages of these rows
-  if constexpr (kGroups) {
+  if constexpr (ROLE == kSharedRole) {
     int id = blockIdx.x;
-    const int n_shared = sh.Hkv * gr.tiles_p * gr.split_p;
-    if (id < n_shared) {
-      split = id % gr.split_p, id /= gr.split_p;
-      kvh = id / gr.tiles_p;
-      if (!shared_tile(gr, id - kvh * gr.tiles_p, kRows, seq_rows, sh.max_pages, &b, &rows, &hi,
-                       &tile))
-        return;
-      n_split = gr.split_p;
-      slot = split;
-    } else {
-      id -= n_shared;
-      split = id % gr.split_s, id /= gr.split_s;
-      tile = id % sh.tiles, id /= sh.tiles;
-      b = id / sh.Hkv;
-      kvh = id - b * sh.Hkv;
-      lo = shared_pages_of(gr, b, sh.max_pages);
-      alone = lo == 0 && split == 0;
-      n_split = gr.split_s;
-      slot = gr.split_p + split;
-    }
+    split = id % gr.split_p, id /= gr.split_p;
+    kvh = id / gr.tiles_p;
+    if (!shared_tile(gr, id - kvh * gr.tiles_p, kTileRows, seq_rows, sh.max_pages, &b, &rows, &hi,
+                     &tile))
+      return;
+    n_split = gr.split_p;
+    slot = split;
+  } else if constexpr (ROLE == kOwnRole) {
+    int id = blockIdx.x - shared_workgroups(sh, gr);
+    split = id % gr.split_s, id /= gr.split_s;
+    tile = id % sh.tiles, id /= sh.tiles;
+    b = id / sh.Hkv;
+    kvh = id - b * sh.Hkv;
+    lo = shared_pages_of(gr, b, sh.max_pages);
+    alone = lo == 0 && split == 0;
+    n_split = gr.split_s;
+    slot = gr.split_p + split;
   }
 
-  // Positions of the tile's first and last row, and of this lane's rows.
-  const int r0 = tile * kRows, r1 = min(r0 + kRows, rows) - 1;
-  u32x4 qf[4];
-  const int lrow = min(r0 + l16, rows - 1);
-  const int lseq = kGroups ? lrow / seq_rows : 0, lq = (lrow - lseq * seq_rows) / G;
-  const int L = min(max(lens[b + lseq], 0), sh.max_pages * kKvPage);
-  const int pos = L - sh.n_q + lq;
-  int p0 = L - sh.n_q + r0 / G, p1 = L - sh.n_q + r1 / G;
-  if constexpr (kGroups) {  // the least and the greatest of the tile
-    p0 = p1 = pos;
+  // Positions of the tile's first and last row (with groups the least and the greatest),
+  // and of this lane's rows.
+  const int r0 = tile * kTileRows, r1 = min(r0 + kTileRows, rows) - 1;
+  u32x4 qf[NB][4];
+  int pos[NB], p0, p1;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int lrow = min(r0 + 16 * nb + l16, rows - 1);
+    const int lseq = ROLE == kSharedRole ? lrow / seq_rows : 0,
+              lq = (lrow - lseq * seq_rows) / G;
+    const int L = min(max(lens[b + lseq], 0), sh.max_pages * kKvPage);
+    pos[nb] = L - sh.n_q + lq;
+    if constexpr (ROLE == kSharedRole) {
+      p0 = nb == 0 ? pos[0] : min(p0, pos[nb]);
+      p1 = nb == 0 ? pos[0] : max(p1, pos[nb]);
+    } else {
+      p0 = L - sh.n_q + r0 / G, p1 = L - sh.n_q + r1 / G;
+    }
+    const bf16_t *qrow = q + ((size_t)(b + lseq) * sh.n_q + lq) * ldq +
+                         (size_t)(kvh * G + lrow - lseq * seq_rows - lq * G) * kKvHd + 32 * g;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) qf[nb][kk] = *reinterpret_cast<const u32x4 *>(qrow + 8 * kk);
+  }
+  if constexpr (ROLE == kSharedRole) {
 #pragma unroll
     for (int d = 1; d < 16; d <<= 1) {
       p0 = min(p0, __shfl_xor(p0, d));
@@ -232,10 +275,6 @@ __device__ __forceinline__ void kv_attend(
     p0 = __builtin_amdgcn_readfirstlane(p0);
     p1 = __builtin_amdgcn_readfirstlane(p1);
   }
-  const bf16_t *qrow = q + ((size_t)(b + lseq) * sh.n_q + lq) * ldq +
-                       (size_t)(kvh * G + lrow - lseq * seq_rows - lq * G) * kKvHd + 32 * g;
-#pragma unroll
-  for (int kk = 0; kk < 4; ++kk) qf[kk] = *reinterpret_cast<const u32x4 *>(qrow + 8 * kk);
 
   // The pages that some row sees: those of the sinks, then from the first row's
   // window on.
@@ -250,25 +289,45 @@ __device__ __forceinline__ void kv_attend(
     skip = from - n_sink;
     n_vis = n_sink + max(to - from, 0);
   }
+  // Without a window the shared pages are dealt whatever the rows' positions, whose loads
+  // they then need not wait for; a row that ends before them sees none of the rest.
+  if (ROLE == kSharedRole && sh.window == 0) n_sink = skip = 0, n_vis = hi;
   const int64_t worker = split * kWaves + wave, workers = n_split * kWaves;
   const int begin = (int)(n_vis * worker / workers), end = (int)(n_vis * (worker + 1) / workers);
   auto block_of = [&](int i) { return i >= n_sink ? i + skip : i + lo; };
   const int32_t *row_table = table + (size_t)b * sh.max_pages;
-  // Page of the i-th visible block (-1: none); the same for the whole wave.
-  auto page_at = [&](int i) {
-    if (i >= end) return -1;
-    const int p = __builtin_amdgcn_readfirstlane(row_table[block_of(i)]);
-    return p >= 0 && p < sh.n_pages ? p : -1;
+  // The wave's next visible block whose page exists (end: none), and its page.  It holds 64
+  // entries of the table at a time, and a bit for each that names a page.
+  int ids = -1, base = begin - 64;
+  uint64_t left = 0;
+  auto next_page = [&](int *page) {
+    while (left == 0) {
+      base += 64;
+      if (base >= end) return end;
+      ids = base + lane < end ? row_table[block_of(base + lane)] : -1;
+      left = __ballot(ids >= 0 && ids < sh.n_pages);
+    }
+    const int at = __ffsll((unsigned long long)left) - 1;
+    left &= left - 1;
+    *page = __builtin_amdgcn_readlane(ids, at);
+    return base + at;
   };
 
-  f32x4 oacc[8], lsum = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int jd = 0; jd < 8; ++jd) oacc[jd] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m_ref = -INFINITY;
+  f32x4 oacc[8][NB], lsum[NB];
+  float m_ref[NB];
   // LSE: the lane's share of the sum of P before its rounding, for lse.  The output is
   // divided by the sum of the rounded P, lsum, whose errors its own cancel with.
-  float psum = 0.f;
-  bool seen = false;
+  float psum[NB];
+  bool seen[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+    for (int jd = 0; jd < 8; ++jd) oacc[jd][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    lsum[nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m_ref[nb] = -INFINITY;
+    psum[nb] = 0.f;
+    seen[nb] = false;
+  }
   const u32x4 ones = u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 
   auto part_of = [&](int page) { return cache + ((size_t)page * sh.Hkv + kvh) * kKvPart; };
@@ -276,98 +335,116 @@ __device__ __forceinline__ void kv_attend(
   const uint32_t ko = kKvK + 64 * l16 + 16 * g, vo = kKvV + 256 * g + 16 * l16,
                  kso = kKvKScale + kKvPage * g + 4 * l16,
                  vso = kKvVScale + kKvPage * (l16 >> 2) + 16 * g;
-  auto load = [&](PageRegs &x, int page) {
-    if (page < 0) return;
+  auto load_k = [&](PageRegs &x, int page) {
     const uint8_t *p = part_of(page);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      x.k[c] = *reinterpret_cast<const u32x4 *>(p + ko + 1024 * c);
-      x.v[c] = *reinterpret_cast<const u32x4 *>(p + vo + 1024 * c);
-    }
+    for (int c = 0; c < 4; ++c) x.k[c] = *reinterpret_cast<const u32x4 *>(p + ko + 1024 * c);
     x.ks = *reinterpret_cast<const uint32_t *>(p + kso);
+  };
+  auto load_v = [&](PageRegs &x, int page) {
+    const uint8_t *p = part_of(page);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) x.v[c] = *reinterpret_cast<const u32x4 *>(p + vo + 1024 * c);
     x.vs = *reinterpret_cast<const u32x4 *>(p + vso);
   };
 
-  auto compute = [&](PageRegs &x, int i, int page) {
-    if (page < 0) return;
+  // K and V of a page each take the registers of the page before as soon as its products
+  // are formed, so that they are on their way during the other half of a page's work.
+  auto compute = [&](PageRegs &x, int i, int page, int next) {
     const int kv0 = block_of(i) * kKvPage;
-    f32x4 s[4];
+    f32x4 s[4][NB];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const float sc = kv_scale((x.ks >> (8 * c)) & 255u);
-      s[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) s[c][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
         const u32x4 kf = eight(x.k[c][kk], sc);
-        s[c] = mfma_u32(kf, qf[kk], s[c]);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) s[c][nb] = mfma_u32(kf, qf[nb][kk], s[c][nb]);
       }
     }
-    // s[c][r]: query row l16 of the tile, key kv0 + 16 c + 4 g + r.
+    __builtin_amdgcn_sched_barrier(0);
+    if (next >= 0) load_k(x, next);
+    __builtin_amdgcn_sched_barrier(0);
+    // s[c][nb][r]: query row 16 nb + l16 of the tile, key kv0 + 16 c + 4 g + r.
     const bool whole = kv0 + kKvPage - 1 <= p0 &&
                        (sh.window == 0 || p1 - kv0 < sh.window || kv0 + kKvPage <= sh.sinks);
     bool nans = false;  // a V group without finite values in a page that not all rows see
     if (!whole) {
-      const int lim = pos - kv0 - 4 * g;
-      const int old = sh.window == 0 ? -64 : lim - sh.window;
-      const int sink = sh.sinks - kv0 - 4 * g;
-      bool any = false;
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int nb = 0; nb < NB; ++nb) {
+        const uint64_t vis = visible_keys(pos[nb] - kv0 - 4 * g, sh.window, sh.sinks - kv0 - 4 * g);
+        seen[nb] |= (vis & 0x000f000f000f000full) != 0;  // the lane's keys are 16 c + r, r < 4
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int e = 16 * c + r;
-          const bool hidden = (e > lim) | ((e <= old) & (e >= sink));
-          any |= !hidden;
-          s[c][r] = hidden ? -INFINITY : s[c][r];
-        }
-      seen |= any;
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[c][nb][r] = or_hidden(vis, 16 * c + r, s[c][nb][r]);
+      }
       // A key that a row does not see has p = 0 there, but 0 times an infinity or
       // NaN of V is NaN: such groups (slots never written among them) count as
-      // zeros here, and as NaN after the product for the rows that see them.
+      // zeros here, and as NaN after the product for the rows that see them (past the last
+      // row's position there are none).
+      uint32_t bad[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < 4; ++c) bad[c] = bytes_past_252(x.vs[c]);
+      if (__any((bad[0] | bad[1] | bad[2] | bad[3]) != 0)) {
+        const int last = p1 - kv0 - 4 * g;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (((x.vs[c] >> (8 * j)) & 255u) > 252u) {
-            x.vs[c] &= ~(255u << (8 * j));
-            nans = true;
-          }
+        for (int c = 0; c < 4; ++c) {
+          x.vs[c] &= ~((bad[c] >> 7) * 255u);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            nans |= ((bad[c] >> (8 * j + 7)) & 1) != 0 && 16 * c + j <= last;
+        }
+      }
     } else {
-      seen = true;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) seen[nb] = true;
     }
 
-    u32x4 pf[2];
-    float mloc = -INFINITY;
+    u32x4 pf[NB][2];
+    float alpha[NB];
+    bool any_raise = false;
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      mloc = vmax(vmax(vmax(mloc, s[c][0]), s[c][1]), vmax(s[c][2], s[c][3]));
-    mloc = max_across_groups(mloc);
-    // The reference max is raised only when a page's passes it by 2^8 in p.
-    const float m_blk = mloc * sh.scale_log2;
-    const bool raise = m_blk > m_ref + kLazy;
-    const float m_new = raise ? m_blk : m_ref;
-    const float alpha = raise ? fast_exp2(m_ref - m_new) : 1.0f;
-    m_ref = m_new;
-    const float neg_m = m_new == -INFINITY ? 0.f : -m_new;
-    if constexpr (LSE) psum *= alpha;
+    for (int nb = 0; nb < NB; ++nb) {
+      float mloc = -INFINITY;
 #pragma unroll
-    for (int ks2 = 0; ks2 < 2; ++ks2) {
-      float p[8];
+      for (int c = 0; c < 4; ++c)
+        mloc = vmax(vmax(vmax(mloc, s[c][nb][0]), s[c][nb][1]), vmax(s[c][nb][2], s[c][nb][3]));
+      mloc = max_across_groups(mloc);
+      // The reference max is raised only when a page's passes it by 2^8 in p.
+      const float m_blk = mloc * sh.scale_log2;
+      const bool raise = m_blk > m_ref[nb] + kLazy;
+      any_raise |= raise;
+      const float m_new = raise ? m_blk : m_ref[nb];
+      alpha[nb] = raise ? fast_exp2(m_ref[nb] - m_new) : 1.0f;
+      m_ref[nb] = m_new;
+      const float neg_m = m_new == -INFINITY ? 0.f : -m_new;
+      if constexpr (LSE) psum[nb] *= alpha[nb];
 #pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2)
+      for (int ks2 = 0; ks2 < 2; ++ks2) {
+        float p[8];
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          p[4 * h2 + r] = fast_exp2(fmaf(s[2 * ks2 + h2][r], sh.scale_log2, neg_m));
-      if constexpr (LSE)
-        psum += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-      // P rounded to bf16 for the product; its sum is that of the rounded values.
-      pf[ks2] = u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]),
-                      pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])};
+        for (int h2 = 0; h2 < 2; ++h2)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            p[4 * h2 + r] = fast_exp2(fmaf(s[2 * ks2 + h2][nb][r], sh.scale_log2, neg_m));
+        if constexpr (LSE)
+          psum[nb] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        // P rounded to bf16 for the product; its sum is that of the rounded values.
+        pf[nb][ks2] = u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]),
+                            pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])};
+      }
     }
-    if (__any(raise)) {
+    if (__any(any_raise)) {
 #pragma unroll
-      for (int jd = 0; jd < 8; ++jd) oacc[jd] = oacc[jd] * alpha;
-      lsum = lsum * alpha;
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int jd = 0; jd < 8; ++jd) oacc[jd][nb] = oacc[jd][nb] * alpha[nb];
+        lsum[nb] = lsum[nb] * alpha[nb];
+      }
     }
     auto v_block = [&](auto byte_c, int ks2, const float (&sa)[4], const float (&sb)[4]) {
       constexpr int BYTE = decltype(byte_c)::value;
@@ -383,8 +460,11 @@ __device__ __forceinline__ void kv_attend(
         lo[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x05040100);
         hi[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302);
       }
-      oacc[2 * BYTE] = mfma_u32(lo, pf[ks2], oacc[2 * BYTE]);
-      oacc[2 * BYTE + 1] = mfma_u32(hi, pf[ks2], oacc[2 * BYTE + 1]);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        oacc[2 * BYTE][nb] = mfma_u32(lo, pf[nb][ks2], oacc[2 * BYTE][nb]);
+        oacc[2 * BYTE + 1][nb] = mfma_u32(hi, pf[nb][ks2], oacc[2 * BYTE + 1][nb]);
+      }
     };
 #pragma unroll
     for (int ks2 = 0; ks2 < 2; ++ks2) {
@@ -398,123 +478,142 @@ __device__ __forceinline__ void kv_attend(
       v_block(std::integral_constant<int, 1>{}, ks2, sa, sb);
       v_block(std::integral_constant<int, 2>{}, ks2, sa, sb);
       v_block(std::integral_constant<int, 3>{}, ks2, sa, sb);
-      lsum = mfma_u32(ones, pf[ks2], lsum);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) lsum[nb] = mfma_u32(ones, pf[nb][ks2], lsum[nb]);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    if (next >= 0) load_v(x, next);
+    __builtin_amdgcn_sched_barrier(0);
     if (!whole && __any(nans)) {
       // The lane's dims 8 (4 g + r) + jd are group g's.
       const uint8_t *p = part_of(page);
-      bool hit = false;
+      bool hit[NB] = {};
 #pragma unroll 1
       for (int t = 0; t < kKvPage; ++t) {
         const bool off = p[kv_v_scale_off(t, g)] > 252;
         const int key = kv0 + t;
-        hit |= off & (key <= pos) &
-               ((sh.window == 0) | (pos - key < sh.window) | (key < sh.sinks));
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+          hit[nb] |= off & (key <= pos[nb]) &
+                     ((sh.window == 0) | (pos[nb] - key < sh.window) | (key < sh.sinks));
       }
 #pragma unroll
-      for (int jd = 0; jd < 8; ++jd)
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          oacc[jd][r] = hit ? __uint_as_float(0x7fc00000u) : oacc[jd][r];
+        for (int jd = 0; jd < 8; ++jd)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            oacc[jd][nb][r] = hit[nb] ? __uint_as_float(0x7fc00000u) : oacc[jd][nb][r];
     }
   };
 
-#pragma unroll 1
-  for (int i = begin; i < end; ++i) {
-    const int page = page_at(i);
+  int page = -1;
+  int i = next_page(&page);
+  if (i < end) {
     PageRegs x;
-    load(x, page);
-    compute(x, i, page);
+    load_k(x, page);
+    load_v(x, page);
+#pragma unroll 1
+    while (i < end) {
+      int page2 = -1;
+      const int j = next_page(&page2);
+      compute(x, i, page, page2);
+      i = j, page = page2;
+    }
   }
 
   // The waves join.  A score that is NaN makes the row's maximum NaN.  A row that saw
   // keys but no score above -inf has no softmax: its sum is NaN, and counts where no
   // other part of the row has a score (part_sum).
-  if constexpr (LSE) {
-    psum += __shfl_xor(psum, 16);
-    psum += __shfl_xor(psum, 32);
-  }
-  if (lsum[0] != lsum[0]) m_ref = lsum[0];
-  int lost = seen && m_ref == -INFINITY;
-  lost |= __shfl_xor(lost, 16);
-  lost |= __shfl_xor(lost, 32);
-  if (g == 0) {
-    s_ml[0][wave][l16] = m_ref;
-    s_ml[1][wave][l16] = lost ? __uint_as_float(0x7fc00000u) : lsum[0];
-    if constexpr (LSE) s_ml[2][wave][l16] = lost ? __uint_as_float(0x7fc00000u) : psum;
-  }
-  __syncthreads();
-  float m = -INFINITY;
-  for (int w = 0; w < kWaves; ++w) m = vmax(m, s_ml[0][w][l16]);
-  const float f = part_weight(m_ref, m);
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
-#pragma unroll
-    for (int j4 = 0; j4 < 2; ++j4) {
-      f32x4 t;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) t[e] = oacc[4 * j4 + e][r] * f;
-      *reinterpret_cast<f32x4 *>(&s_o[wave][l16 * kLdRow + 8 * (4 * g + r) + 4 * j4]) = t;
+  for (int nb = 0; nb < NB; ++nb) {
+    if (nb > 0) __syncthreads();  // the rows before have been read
+    if constexpr (LSE) {
+      psum[nb] += __shfl_xor(psum[nb], 16);
+      psum[nb] += __shfl_xor(psum[nb], 32);
     }
-  __syncthreads();
-  for (int x = tid; x < kRows * kKvHd / 4; x += kThreads) {
-    const int row = x / (kKvHd / 4), d = 4 * (x - row * (kKvHd / 4));
-    if (r0 + row > r1) break;
-    float m = -INFINITY, l = 0.f, ls = 0.f;
-    for (int w = 0; w < kWaves; ++w) m = vmax(m, s_ml[0][w][row]);
-    f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int w = 0; w < kWaves; ++w) {
-      const float mw = s_ml[0][w][row];
-      l += part_sum(mw, s_ml[1][w][row], m);
-      if constexpr (LSE) ls += part_sum(mw, s_ml[2][w][row], m);
-      t = t + *reinterpret_cast<const f32x4 *>(&s_o[w][row * kLdRow + d]);
+    float mr = m_ref[nb];
+    if (lsum[nb][0] != lsum[nb][0]) mr = lsum[nb][0];
+    int lost = seen[nb] && mr == -INFINITY;
+    lost |= __shfl_xor(lost, 16);
+    lost |= __shfl_xor(lost, 32);
+    if (g == 0) {
+      s_ml[0][wave][l16] = mr;
+      s_ml[1][wave][l16] = lost ? __uint_as_float(0x7fc00000u) : lsum[nb][0];
+      if constexpr (LSE) s_ml[2][wave][l16] = lost ? __uint_as_float(0x7fc00000u) : psum[nb];
     }
-    if constexpr (kGroups) {
-      const int r = r0 + row, iq = r / G, h = kvh * G + r - iq * G;  // iq: token from b's first
-      const size_t n = all_rows(sh, gr), id = ((size_t)b * sh.n_q + iq) * sh.Hq + h;
-      const size_t at = slot * n + id;
-      // A part without keys is known by its maximum and sum.
-      if (m != -INFINITY || l != 0.f)
-        *reinterpret_cast<f32x4 *>(part_o + at * kKvHd + d) = t;
-      if (d == 0) {
-        float *sums = part_o + n * (gr.split_p + gr.split_s) * (kKvHd + 2);
-        part_ml[at] = make_float2(m, l);
-        if (LSE) sums[at] = ls;
-        if (alone)
-          for (int s = 0; s < gr.split_p; ++s) {
-            part_ml[s * n + id] = make_float2(-INFINITY, 0.f);
-            if (LSE) sums[s * n + id] = 0.f;
-          }
+    __syncthreads();
+    float m = -INFINITY;
+    for (int w = 0; w < kWaves; ++w) m = vmax(m, s_ml[0][w][l16]);
+    const float f = part_weight(mr, m);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j4 = 0; j4 < 2; ++j4) {
+        f32x4 t;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = oacc[4 * j4 + e][nb][r] * f;
+        *reinterpret_cast<f32x4 *>(&s_o[wave][l16 * kLdRow + 8 * (4 * g + r) + 4 * j4]) = t;
       }
-      continue;
+    __syncthreads();
+    for (int x = tid; x < kRows * kKvHd / 4; x += kThreads) {
+      const int row = x / (kKvHd / 4), d = 4 * (x - row * (kKvHd / 4));
+      const int r = r0 + 16 * nb + row;
+      if (r > r1) break;
+      float m = -INFINITY, l = 0.f, ls = 0.f;
+      for (int w = 0; w < kWaves; ++w) m = vmax(m, s_ml[0][w][row]);
+      f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int w = 0; w < kWaves; ++w) {
+        const float mw = s_ml[0][w][row];
+        l += part_sum(mw, s_ml[1][w][row], m);
+        if constexpr (LSE) ls += part_sum(mw, s_ml[2][w][row], m);
+        t = t + *reinterpret_cast<const f32x4 *>(&s_o[w][row * kLdRow + d]);
+      }
+      const int iq = r / G, h = kvh * G + r - iq * G;  // iq: token from b's first
+      if constexpr (kGroups) {
+        const size_t n = all_rows(sh, gr), id = ((size_t)b * sh.n_q + iq) * sh.Hq + h;
+        const size_t at = slot * n + id;
+        // A part without keys is known by its maximum and sum.
+        if (m != -INFINITY || l != 0.f)
+          *reinterpret_cast<f32x4 *>(part_o + at * kKvHd + d) = t;
+        if (d == 0) {
+          float *sums = part_o + n * (gr.split_p + gr.split_s) * (kKvHd + 2);
+          part_ml[at] = make_float2(m, l);
+          if (LSE) sums[at] = ls;
+          if (alone)
+            for (int s = 0; s < gr.split_p; ++s) {
+              part_ml[s * n + id] = make_float2(-INFINITY, 0.f);
+              if (LSE) sums[s * n + id] = 0.f;
+            }
+        }
+        continue;
+      }
+      if (sh.n_split > 1) {
+        const size_t at =
+            ((((size_t)b * sh.Hkv + kvh) * sh.tiles + tile) * sh.n_split + split) * kRows + row;
+        *reinterpret_cast<f32x4 *>(part_o + at * kKvHd + d) = t;
+        if (d == 0) part_ml[at] = make_float2(m, l);
+        if (LSE && d == 0) part_o[sums_at(sh) + at] = ls;
+        continue;
+      }
+      const float inv = l == 0.f ? 0.f : 1.0f / l;  // l = 0: no key seen
+      uint2 u;
+      u.x = pack_bf16x2(t[0] * inv, t[1] * inv);
+      u.y = pack_bf16x2(t[2] * inv, t[3] * inv);
+      *reinterpret_cast<uint2 *>(o + ((size_t)b * sh.n_q + iq) * ldo + (size_t)h * kKvHd + d) = u;
+      if (LSE && d == 0)
+        lse[((size_t)b * sh.Hq + h) * sh.n_q + iq] = (m + log2f(ls)) * 0.6931471805599453f;
     }
-    if (sh.n_split > 1) {
-      const size_t at =
-          ((((size_t)b * sh.Hkv + kvh) * sh.tiles + tile) * sh.n_split + split) * kRows + row;
-      *reinterpret_cast<f32x4 *>(part_o + at * kKvHd + d) = t;
-      if (d == 0) part_ml[at] = make_float2(m, l);
-      if (LSE && d == 0) part_o[sums_at(sh) + at] = ls;
-      continue;
-    }
-    const int r = r0 + row, iq = r / G, h = kvh * G + r - iq * G;
-    const float inv = l == 0.f ? 0.f : 1.0f / l;  // l = 0: no key seen
-    uint2 u;
-    u.x = pack_bf16x2(t[0] * inv, t[1] * inv);
-    u.y = pack_bf16x2(t[2] * inv, t[3] * inv);
-    *reinterpret_cast<uint2 *>(o + ((size_t)b * sh.n_q + iq) * ldo + (size_t)h * kKvHd + d) = u;
-    if (LSE && d == 0)
-      lse[((size_t)b * sh.Hq + h) * sh.n_q + iq] = (m + log2f(ls)) * 0.6931471805599453f;
   }
 }
 
 // Joins the splits of a query row: KG groups of 32 threads, thread d4 of group k
 // taking dims 4 d4 .. + 3 of splits k, k + KG, ..; all loads of up to 8 splits are
 // in flight at once (the partial results come from other dies' caches).
-template <int KG, bool LSE, typename GroupsT = NoGroups>
+template <int KG, bool LSE, bool GROUPS = false>
 __device__ __forceinline__ void kv_join(
     const float *__restrict__ part_o, const float2 *__restrict__ part_ml, bf16_t *__restrict__ o,
-    size_t ldo, float *__restrict__ lse, const AttendShape &sh, const GroupsT gr = {}) {
-  constexpr bool kGroups = has_groups<GroupsT>;
+    size_t ldo, float *__restrict__ lse, const AttendShape &sh, const Groups &gr) {
   __shared__ f32x4 s_o[8][32];
   __shared__ float2 s_ml[8];
   __shared__ float s_s[8];
@@ -523,7 +622,7 @@ __device__ __forceinline__ void kv_join(
   // The row's parts: the first, and the distance to the next.
   size_t base, step = kRows, sums;
   int b = blockIdx.z, iq, h, n_split = sh.n_split;
-  if constexpr (kGroups) {
+  if constexpr (GROUPS) {
     step = all_rows(sh, gr);
     if ((size_t)r >= step) return;  // with KG = 8 the grid is the rows
     iq = r / sh.Hq, h = r - iq * sh.Hq;
@@ -558,7 +657,7 @@ __device__ __forceinline__ void kv_join(
         p[j] = *reinterpret_cast<const f32x4 *>(part_o + at * kKvHd + 4 * d4);
       }
     }
-    if constexpr (kGroups)  // parts without keys were not written
+    if constexpr (GROUPS)  // parts without keys were not written
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (ml[j].x == -INFINITY && ml[j].y == 0.f) p[j] = f32x4{0.f, 0.f, 0.f, 0.f};

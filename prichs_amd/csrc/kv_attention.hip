@@ -12,7 +12,8 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 3 : 2) void kv_attend_ke
     const int32_t *__restrict__ table, const int32_t *__restrict__ lens, bf16_t *__restrict__ o,
     size_t ldo, float *__restrict__ lse, float *__restrict__ part_o, float2 *__restrict__ part_ml,
     AttendShape sh) {
-  kv_attend<kWaves, false>(q, ldq, cache, table, lens, o, ldo, lse, part_o, part_ml, sh);
+  __shared__ JoinLds<kWaves> s;
+  kv_attend<kWaves, false>(q, ldq, cache, table, lens, o, ldo, lse, part_o, part_ml, sh, s, Groups{});
 }
 // With lse: 10 registers more, and 0.2 to 1 us a call (one token over 8192 positions 8.6 ->
 // 9.1 us, 32 x 3000 16.1 -> 16.6, 8 x 5 over 4096 14.7 -> 15.3, 2 x 256 over 4352 35.9 -> 36.9).
@@ -22,20 +23,21 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 3 : 2) void kv_attend_ls
     const int32_t *__restrict__ table, const int32_t *__restrict__ lens, bf16_t *__restrict__ o,
     size_t ldo, float *__restrict__ lse, float *__restrict__ part_o, float2 *__restrict__ part_ml,
     AttendShape sh) {
-  kv_attend<kWaves, true>(q, ldq, cache, table, lens, o, ldo, lse, part_o, part_ml, sh);
+  __shared__ JoinLds<kWaves> s;
+  kv_attend<kWaves, true>(q, ldq, cache, table, lens, o, ldo, lse, part_o, part_ml, sh, s, Groups{});
 }
 
 template <int KG>
 __global__ __launch_bounds__(256) void kv_join_kernel(
     const float *__restrict__ part_o, const float2 *__restrict__ part_ml, bf16_t *__restrict__ o,
     size_t ldo, float *__restrict__ lse, AttendShape sh) {
-  kv_join<KG, false>(part_o, part_ml, o, ldo, lse, sh);
+  kv_join<KG, false>(part_o, part_ml, o, ldo, lse, sh, Groups{});
 }
 template <int KG>
 __global__ __launch_bounds__(256) void kv_join_lse_kernel(
     const float *__restrict__ part_o, const float2 *__restrict__ part_ml, bf16_t *__restrict__ o,
     size_t ldo, float *__restrict__ lse, AttendShape sh) {
-  kv_join<KG, true>(part_o, part_ml, o, ldo, lse, sh);
+  kv_join<KG, true>(part_o, part_ml, o, ldo, lse, sh, Groups{});
 }
 
 // Pages up to which one workgroup of 8 waves takes a tile without a second kernel:

@@ -483,11 +483,6 @@ int page_check(const char *who, const void *cache, size_t n_pages, size_t n_kv_h
                  "%s: the cache must be 16-byte aligned", who);
   return PRICHS_OK;
 }
-#define PRICHS_TRY(expr)                \
-  do {                                  \
-    const int _rc = (expr);             \
-    if (_rc != PRICHS_OK) return _rc;   \
-  } while (0)
 
 }  // namespace
 }  // namespace prichs

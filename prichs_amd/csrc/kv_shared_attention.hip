@@ -10,44 +10,66 @@
 namespace prichs {
 namespace {
 
-constexpr int kPartWaves = 4;
+constexpr int kWaves = 4;
 
-template <bool LSE>
-__global__ __launch_bounds__(64 * kPartWaves, 3) void kv_shared_kernel(
+// Workgroups over shared pages, with tiles of 16 NB rows, then those over own pages.
+template <int NB, bool LSE>
+__global__ __launch_bounds__(64 * kWaves, NB == 1 ? 3 : 2) void kv_shared_kernel(
     const bf16_t *__restrict__ q, size_t ldq, const uint8_t *__restrict__ cache,
     const int32_t *__restrict__ table, const int32_t *__restrict__ lens,
     float *__restrict__ part_o, float2 *__restrict__ part_ml, AttendShape sh, Groups gr) {
-  kv_attend<kPartWaves, LSE, Groups>(q, ldq, cache, table, lens, nullptr, 0, nullptr, part_o,
-                                     part_ml, sh, gr);
+  __shared__ JoinLds<kWaves> s;
+  if ((int)blockIdx.x < shared_workgroups(sh, gr))
+    kv_attend<kWaves, LSE, kSharedRole, NB>(q, ldq, cache, table, lens, nullptr, 0, nullptr,
+                                            part_o, part_ml, sh, s, gr);
+  else
+    kv_attend<kWaves, LSE, kOwnRole>(q, ldq, cache, table, lens, nullptr, 0, nullptr, part_o,
+                                     part_ml, sh, s, gr);
 }
 template <int KG, bool LSE>
 __global__ __launch_bounds__(256) void kv_shared_join_kernel(
     const float *__restrict__ part_o, const float2 *__restrict__ part_ml, bf16_t *__restrict__ o,
     size_t ldo, float *__restrict__ lse, AttendShape sh, Groups gr) {
-  kv_join<KG, LSE, Groups>(part_o, part_ml, o, ldo, lse, sh, gr);
+  kv_join<KG, LSE, true>(part_o, part_ml, o, ldo, lse, sh, gr);
 }
 
 // How a call is cut.  For 256 CUs whatever the current device has: a workspace's size may
-// be asked for on another.
+// be asked for on another.  12 + 3 heads, us of a captured call (kernel and join):
+//   sequences x shared positions   8 x 1000  20 x 4096  64 x 8192  256 x 8192  256 x 32768
+//   tiles of 16 rows, 512            10.1      11.4       20.4        41.5        132
+//   tiles of 32 rows, 256            12.3      13.5       20.2        38.2        118
+//   tiles of 32 rows, 512            12.3      13.6       24.6        37.2         91
+// (the second number: workgroups that the shared pages are dealt to).  24 x 8000 with six
+// tokens each 26.2, 24.7, 30.5; 128 x 16384 36.3, 34.5, 38.1; 200 x 16384 52, 48, 45.
+// Tiles of 48 and 64 rows have one wave a SIMD: 140 and 166 us at 256 x 32768.  A form that
+// converts each page once into LDS for 128 rows took 95 to 101 us there and 36 to 39 at 24 x
+// 8000: its waves wait for each other at every page.
 struct Plan {
+  int blocks;               // of 16 rows in a tile over shared pages
   size_t tiles_p, split_p;  // tiles over shared pages of a kv head at most, splits of each
   size_t tiles_s, split_s;  // the same of a sequence's own pages
 };
+constexpr size_t kManySteps = 4096, kMoreSteps = 32768;  // pages of all tiles of 16 rows
 Plan plan_of(size_t batch, size_t n_q, size_t n_heads, size_t n_kv_heads, size_t max_pages,
              size_t n_groups) {
   const size_t rows = n_q * (n_heads / n_kv_heads);  // of a sequence
-  const size_t most = std::max<size_t>(cdiv(max_pages, 4), 1);
+  const size_t most = std::max<size_t>(cdiv(max_pages, (size_t)kWaves), 1);
+  // Only groups of some sequence have tiles, and the last of each may be short.
+  const size_t groups = std::min(n_groups, batch);
+  const size_t steps = cdiv(batch * rows, (size_t)kRows) * n_kv_heads * max_pages;
   Plan p;
-  // The last tile of each group may be short; only groups of some sequence have tiles.
-  p.tiles_p = n_groups == 0
-                  ? 0
-                  : (batch * rows + std::min(n_groups, batch) * (kRows - 1)) / kRows;
-  p.split_p = n_groups == 0
-                  ? 0
-                  : std::max<size_t>(std::min(768 / (n_kv_heads * p.tiles_p), most), 1);
+  p.blocks = batch * rows >= 2 * kRows * groups && steps >= kManySteps ? 2 : 1;
+  const size_t per = (size_t)kRows * p.blocks;
+  p.tiles_p = p.split_p = 0;
+  if (groups > 0) {
+    p.tiles_p = (batch * rows + groups * (per - 1)) / per;
+    const size_t wgs = p.blocks == 1 || steps >= kMoreSteps ? 512 : 256;
+    p.split_p = std::max<size_t>(std::min(wgs / (n_kv_heads * p.tiles_p), most), 1);
+  }
+  // Own pages: as a rule few, of a number that only the device knows.
   p.tiles_s = cdiv(rows, (size_t)kRows);
-  p.split_s =
-      std::max<size_t>(std::min(768 / (batch * n_kv_heads * p.tiles_s), std::min<size_t>(most, 8)), 1);
+  p.split_s = std::max<size_t>(
+      std::min({256 / (batch * n_kv_heads * p.tiles_s), most, (size_t)8}), 1);
   return p;
 }
 size_t workspace_of(const Plan &p, size_t rows) {
@@ -118,18 +140,20 @@ extern "C" int prichs_kv_cache_shared_attention(
                        (int)p.tiles_s,
                        1,
                        (1.0f / sqrtf((float)head_dim)) * 1.4426950408889634f};
-  const Groups gr{group_start,    shared,          (int)n_groups,  (int)batch,
+  const Groups gr{group_start,    shared,         (int)n_groups, (int)batch,
                   (int)p.tiles_p, (int)p.split_p, (int)p.split_s};
   float *part_o = static_cast<float *>(workspace);
   float2 *part_ml =
       reinterpret_cast<float2 *>(part_o + rows * (p.split_p + p.split_s) * kKvHd);
   const hipStream_t s = as_stream(stream);
-  const dim3 grid((unsigned)wgs);
-  auto kern = lse == nullptr ? kv_shared_kernel<false> : kv_shared_kernel<true>;
-  hipLaunchKernelGGL(kern, grid, dim3(64 * kPartWaves), 0, s, static_cast<const bf16_t *>(q), ldq,
-                     static_cast<const uint8_t *>(cache), page_table, lens, part_o, part_ml, sh,
-                     gr);
+  auto kern = p.blocks == 2
+                  ? (lse == nullptr ? kv_shared_kernel<2, false> : kv_shared_kernel<2, true>)
+                  : (lse == nullptr ? kv_shared_kernel<1, false> : kv_shared_kernel<1, true>);
+  hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(64 * kWaves), 0, s,
+                     static_cast<const bf16_t *>(q), ldq, static_cast<const uint8_t *>(cache),
+                     page_table, lens, part_o, part_ml, sh, gr);
   PRICHS_LAUNCH_CHECK("kv_cache_shared_attention launch");
+  // Eight groups of threads a row where it has more parts than one can load at once.
   const bool wide = p.split_p + p.split_s > 8;
   auto join = lse == nullptr
                   ? (wide ? kv_shared_join_kernel<8, false> : kv_shared_join_kernel<1, false>)

@@ -91,10 +91,22 @@ CASES = [
 ]
 
 
-@pytest.mark.parametrize("groups,lens,n_q,heads,kv,window,sinks", CASES)
-def test_groups(cuda, groups, lens, n_q, heads, kv, window, sinks):
-    say("case:", groups[:3], lens[:3], n_q, heads, kv, window, sinks)
-    s = Scene(groups, lens, n_q, heads, kv, n_q + sum(lens))
+def columns(batch, n_q, heads, kv):
+    """Columns of a table with which a call has 4096 tiles of 16 rows times pages, from where
+    on groups of 32 rows and more take tiles of 32."""
+    return -(-4096 // (-(-batch * n_q * (heads // kv) // 16) * kv))
+
+
+# The same with tiles of 32 rows (long tables, most of whose entries nobody reaches).
+MANY = [CASES[i] for i in (3, 5, 6, 7, 8, 9, 10, 11, 13, 14, 18, 19)]
+
+
+@pytest.mark.parametrize("groups,lens,n_q,heads,kv,window,sinks,wide", [
+    (*c, w) for cases, w in ((CASES, False), (MANY, True)) for c in cases])
+def test_groups(cuda, groups, lens, n_q, heads, kv, window, sinks, wide):
+    say("case:", groups[:3], lens[:3], n_q, heads, kv, window, sinks, wide)
+    s = Scene(groups, lens, n_q, heads, kv, n_q + sum(lens),
+              max_pages=columns(len(lens), n_q, heads, kv) if wide else None)
     ref = s.ref(window, sinks)
     wide = torch.full((s.batch * n_q + 1, heads * HD + 8), float("nan"), dtype=torch.bfloat16,
                       device="cuda")
@@ -109,6 +121,11 @@ def test_groups(cuda, groups, lens, n_q, heads, kv, window, sinks):
         (h[:, rows[1].stop:] == 7).all()
     again, none = s.run(window, sinks, want_lse=False)
     assert none is None and torch.equal(again, out[rows].contiguous())
+
+
+def wide(size, heads=8, kv=2):
+    """Columns for tiles of 32 rows where a group has 40 sequences."""
+    return columns(size, 1, heads, kv) if size == 40 else None
 
 
 def test_starts_of_every_kind(cuda):
@@ -137,7 +154,7 @@ def test_whole_table_shared_and_lens_past_it(cuda):
 
 @pytest.mark.parametrize("size", [3, 40])
 def test_pages_that_do_not_exist(cuda, size):
-    s = Scene([(size, 320)], [400 + i for i in range(size)], 1, 8, 2, 33)
+    s = Scene([(size, 320)], [400 + i for i in range(size)], 1, 8, 2, 33, max_pages=wide(size))
     s.table[0, 1], s.table[0, 4], s.table[1, 5] = s.n_pages, -1, 1 << 30
     keep = [np.ones(500, bool) for _ in range(size)]
     for k in keep:
@@ -158,7 +175,7 @@ def test_what_a_row_does_not_see_does_not_reach_it(cuda, size, bad):
     lens = [330 + 7 * i for i in range(size)]
     lens[1] = 150
     W = 120
-    s = Scene([(size, 320)], lens, 1, 4, 1, 34)
+    s = Scene([(size, 320)], lens, 1, 4, 1, 34, max_pages=wide(size, 4, 1))
     x = synth.round_bf16(np.random.default_rng(1).standard_normal((2, HD)))
     k, v = x[:1].copy(), x[1:].copy()
     one = s.table[:1].contiguous()
@@ -178,7 +195,8 @@ def test_what_a_row_does_not_see_does_not_reach_it(cuda, size, bad):
 @pytest.mark.parametrize("size", [3, 40])
 @pytest.mark.parametrize("q_scale", [0.0, 40.0])
 def test_flat_and_steep_scores(cuda, size, q_scale):
-    s = Scene([(size, 640)], [700 + i for i in range(size)], 1, 4, 2, 35, q_scale=q_scale)
+    s = Scene([(size, 640)], [700 + i for i in range(size)], 1, 4, 2, 35, q_scale=q_scale,
+              max_pages=wide(size, 4))
     ref = s.ref()
     # A score is off by 128 roundings of 2^-24 of its terms, and p by that.
     ref["e_out"] *= 1 + 2 * (q_scale * 16 * HD ** 0.5 * 128 * 2.0 ** -24) / R.U
@@ -193,7 +211,7 @@ def test_rows_without_finite_scores(cuda, size):
     """Scores of -inf alone, in the shared pages, in the own ones or in both, and a +inf or
     NaN: as for a sequence that shares nothing."""
     n, kv = 150, 1
-    s = Scene([(size, 128)], [n] * size, 1, 4, kv, 36)
+    s = Scene([(size, 128)], [n] * size, 1, 4, kv, 36, max_pages=wide(size, 4, 1))
     k = np.zeros((n, HD), np.float32)
     v = synth.round_bf16(np.random.default_rng(1).standard_normal((n, HD)))
     k[:, 0], k[128:, 1], k[:128, 2] = 1, 1, 1
@@ -215,7 +233,8 @@ def test_rows_without_finite_scores(cuda, size):
 
 @pytest.mark.parametrize("size,n_q", [(3, 1), (40, 1), (12, 9)])
 def test_what_the_workspace_held_does_not_matter(cuda, size, n_q):
-    s = Scene([(size, 640), (2, 0)], [700 + i for i in range(size)] + [90, 0], n_q, 8, 2, 37)
+    s = Scene([(size, 640), (2, 0)], [700 + i for i in range(size)] + [90, 0], n_q, 8, 2, 37,
+              max_pages=wide(size))
     lib, pages, x, lens = L.load(), s.table.shape[1], dev(s.q), i32(s.lens)
     need = lib.prichs_kv_cache_shared_attention_workspace(s.batch, n_q, 8, 2, pages, 2)
     ws = torch.full((need + 64,), 0xff, dtype=torch.uint8, device="cuda")
@@ -232,7 +251,7 @@ def test_what_the_workspace_held_does_not_matter(cuda, size, n_q):
 
 def test_pages_past_32_bits(cuda):
     """A cache of 4.7 GB whose shared and own pages lie at its start and its end."""
-    s = Scene([(40, 256)], [300 + i for i in range(40)], 1, 4, 2, 38)
+    s = Scene([(40, 256)], [300 + i for i in range(40)], 1, 4, 2, 38, max_pages=wide(40, 4))
     n = 270_000
     far = ops.kv_cache_pages(n, 2)
     old = torch.arange(s.n_pages, dtype=torch.int32, device="cuda")

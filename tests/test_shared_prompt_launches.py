@@ -1,0 +1,102 @@
+"""Which kernels the norms with rotation, the page calls and the attention over shared
+pages launch, on the CPU (tests/launch_log.py), and that the GPU tests reach them all."""
+import pytest
+
+from tests import launch_log as ll
+
+
+def attend(cases):
+    """Launches for each (batch, n_q, max_pages, heads, kv heads, groups, with lse)."""
+    rows = ll.run(f"""
+result = []
+for b, n, p, h, k, g, lse in {cases!r}:
+    need = lib.prichs_kv_cache_shared_attention_workspace(b, n, h, k, p, g)
+    L.check(lib.prichs_kv_cache_shared_attention(P, 128 * h, P, 1000, P, p, P, P, P, g, P, 128 * h,
+                                                 P if lse else None, b, n, h, k, 128, 0, 0, 1, P,
+                                                 need, None))
+    result.append([need, launches()])
+""")
+    return [(need, ll.as_launches(x)) for need, x in rows]
+
+
+# (case, blocks of 16 rows in a tile, tiles x splits over shared pages of a kv head, splits
+# of own pages): nothing shared; few rows; many rows and few pages; many of both; more tiles
+# than workgroups; groups that could each have a short tile; more groups than sequences.
+@pytest.mark.parametrize("case,blocks,tiles,split_p,split_s", [
+    ((4, 1, 20, 12, 3, 0), 1, 0, 0, 5), ((8, 1, 17, 12, 3, 1), 1, 2, 5, 5),
+    ((24, 6, 133, 12, 3, 1), 2, 18, 4, 1), ((256, 1, 528, 12, 3, 1), 2, 32, 5, 1),
+    ((64, 1, 136, 12, 3, 1), 2, 8, 10, 1), ((64, 1, 37, 12, 3, 16), 1, 31, 5, 1),
+    ((200, 16, 8, 8, 2, 2), 2, 401, 1, 1), ((3, 1, 50, 4, 4, 100), 1, 3, 13, 8),
+    ((1, 1, 0, 4, 4, 1), 1, 1, 1, 1)])
+def test_how_a_call_is_cut(case, blocks, tiles, split_p, split_s):
+    b, n, p, h, k, g = case
+    for lse in (0, 1):
+        (need, got), = attend([(*case, lse)])
+        own = b * k * -(-n * (h // k) // 16)
+        flag = "true" if lse else "false"
+        assert got[0].kernel == f"kv_shared_kernel<{blocks}, {flag}>"
+        assert got[0].grid == [k * tiles * split_p + own * split_s, 1, 1]
+        parts = split_p + split_s
+        wide = parts > 8
+        assert got[1].kernel == f"kv_shared_join_kernel<{8 if wide else 1}, {flag}>"
+        assert got[1].grid[0] == (b * n * h if wide else -(-b * n * h // 8)) and len(got) == 2
+        assert need == b * n * h * parts * 131 * 4
+
+
+def test_a_launch_too_large_is_refused():
+    out = ll.run("""
+need = lib.prichs_kv_cache_shared_attention_workspace(65535, 1, 1024, 1024, 4, 1)
+rc = lib.prichs_kv_cache_shared_attention(P, 1 << 17, P, 1000, P, 4, P, P, P, 1, P, 1 << 17, None,
+                                          65535, 1, 1024, 1024, 128, 0, 0, 1, P, need, None)
+result = [rc, launches()]
+""")
+    assert out == [-1, []]
+
+
+def test_the_gpu_tests_reach_every_variant():
+    from tests import test_gpu_kv_shared as t
+
+    calls = []
+    for cases, wide in ((t.CASES, False), (t.MANY, True)):
+        for groups, lens, n_q, heads, kv, _, _ in cases:
+            pages = t.columns(len(lens), n_q, heads, kv) if wide else -(-max(lens) // t.PAGE)
+            assert pages >= -(-max(lens) // t.PAGE)
+            calls += [(len(lens), n_q, pages, heads, kv, len(groups), lse) for lse in (0, 1)]
+    names = {x.kernel for _, ls in attend(calls) for x in ls}
+    assert names == {f"kv_shared_{k}<{n}, {f}>" for f in ("true", "false")
+                     for k, n in (("kernel", 1), ("kernel", 2), ("join_kernel", 1),
+                                  ("join_kernel", 8))}
+    (_, got), = attend([(40, 1, t.wide(40), 8, 2, 1, 0)])
+    assert got[0].kernel == "kv_shared_kernel<2, false>"
+
+
+def rotate(cases):
+    """Launches of a forward and a backward for each (rows, heads, kv heads, head dim, dtype)."""
+    return [ll.as_launches(x) for x in ll.run(f"""
+result = []
+for r, h, k, d, dt in {cases!r}:
+    H, K = d * h, d * k
+    L.check(lib.prichs_qk_norm_rope_forward(P, H, P, K, P, P, P, P, 9, P, 0, 0, P, H, P, K, r, h, k,
+                                            d, 1e-5, dt, None))
+    need = lib.prichs_qk_norm_rope_backward_workspace(r, h, k, d)
+    L.check(lib.prichs_qk_norm_rope_backward(P, H, P, K, P, H, P, K, P, P, P, P, 9, P, 0, 0, P, H,
+                                             P, K, P, P, 0, r, h, k, d, 1e-5, dt, P, need, None))
+    result.append(launches())
+""")]
+
+
+def test_rotation_takes_the_lanes_that_a_head_needs():
+    from tests.test_gpu_qk_norm_rope import SHAPES
+
+    cases = [(*s, dt) for s in SHAPES for dt in (0, 1)]
+    names = set()
+    for (rows, h, k, d, dt), got in zip(cases, rotate(cases)):
+        lanes = 4 if d <= 32 else 8 if d <= 64 else 16 if d <= 128 else 32
+        t = "unsigned short" if dt else "float"
+        fwd, bwd, dw = got
+        assert fwd.kernel == f"qk_norm_rope_kernel<{t}, {lanes}>"
+        assert bwd.kernel == f"qk_norm_rope_bwd_kernel<{t}, {lanes}>"
+        assert dw.kernel == "qk_norm_dw_kernel" and dw.grid[0] == -(-2 * d // 32)
+        assert bwd.grid[0] <= 1024
+        names |= {fwd.kernel, bwd.kernel}
+    assert len(names) == 16
