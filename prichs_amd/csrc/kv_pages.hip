@@ -3,12 +3,12 @@
 // page's layout, which nothing here looks into.
 //
 // Free pages are taken lowest first, so every result is that of the steps done one after
-// the other, whatever runs at the same time.  A call that needs the free pages in order
-// takes three launches: `count` counts them in blocks of kBlockPages, `list` ranks them
-// behind the blocks before (and one more workgroup scans what the call's items want), and
-// the call's own kernel applies it.  Counts and tables are some bytes a page: the launches
-// are the cost (MI355X: 2 us each on the device), until data is copied, which runs at the
-// rate of the memory.
+// the other, whatever runs at the same time.  Counts and tables are some bytes a page:
+// launches and round trips to memory are the cost, until data is copied, which runs at the
+// rate of the memory.  Up to kSmallPages pages and kSmallRows rows one workgroup of 1024
+// threads finds the free pages (16 of them a thread in one round trip) and ranks them in one
+// launch; beyond, workgroups count them in blocks of kBlockPages and a second launch ranks
+// them behind the blocks before.
 #include "kv_cache.hpp"
 
 #include <climits>
@@ -22,8 +22,19 @@ constexpr int kThreads = 256;
 constexpr int kSteps = 16;                          // pages of a lane
 constexpr int kBlockPages = kThreads * kSteps;      // pages of a workgroup
 constexpr int kCopyUnroll = 4;
-constexpr int kChunk = kThreads * kCopyUnroll;      // 16-byte pieces of a copying workgroup
+// A page in equal chunks of at most so many 16-byte pieces, one for a copying workgroup.
+constexpr int kChunk = kThreads * kCopyUnroll;
+struct Chunks {
+  int pieces, chunks, chunk;  // of a page; of a chunk
+  explicit Chunks(size_t n_kv_heads)
+      : pieces((int)(n_kv_heads * kKvPart / 16)),
+        chunks((int)cdiv(pieces, kChunk)),
+        chunk((int)cdiv(pieces, chunks)) {}
+};
 constexpr size_t kMaxPages = (size_t)1 << 24, kMaxRows = (size_t)1 << 20;
+constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+constexpr int kRound = kPlanThreads * kSteps;       // pages that a workgroup has in registers
+constexpr size_t kSmallPages = 4 * kRound, kSmallRows = 4 * kPlanThreads;
 
 // The workspace, in int32: block counts; what the first page list holds; then by call.
 struct Work {
@@ -54,15 +65,20 @@ __device__ __forceinline__ int wave_sum(int v) {
   for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m);
   return v;
 }
-// Sum over the workgroup, in every thread (s: 4 ints of LDS).
+// Sum over the workgroup, in every thread (s: an int of LDS for each of its waves).
+template <int WAVES>
 __device__ __forceinline__ int block_sum(int v, int *s) {
   v = wave_sum(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
   __syncthreads();
-  return s[0] + s[1] + s[2] + s[3];
+  int all = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) all += s[w];
+  return all;
 }
 // Sum of v over the threads before this one; *all: over the workgroup.
+template <int WAVES>
 __device__ __forceinline__ int block_before(int v, int *s, int *all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int x = v;
@@ -74,9 +90,13 @@ __device__ __forceinline__ int block_before(int v, int *s, int *all) {
   __syncthreads();
   if (lane == 63) s[wave] = x;
   __syncthreads();
-  int before = 0;
-  for (int w = 0; w < wave; ++w) before += s[w];
-  *all = s[0] + s[1] + s[2] + s[3];
+  int before = 0, sum = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    before += w < wave ? s[w] : 0;
+    sum += s[w];
+  }
+  *all = sum;
   return before + x - v;
 }
 
@@ -87,13 +107,12 @@ __device__ __forceinline__ int free_masks(const int32_t *refs, int n_pages, int 
   int r[kSteps];
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
-    const int p = p0 + 64 * i + lane;
-    r[i] = p < n_pages ? refs[p] : 1;
+    r[i] = refs[min(p0 + 64 * i + lane, n_pages - 1)];  // all loads at once
   }
   int n = 0;
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
-    mask[i] = __ballot(r[i] <= 0);
+    mask[i] = __ballot(r[i] <= 0 && p0 + 64 * i + lane < n_pages);
     n += __popcll(mask[i]);
   }
   return n;
@@ -118,8 +137,8 @@ __device__ __forceinline__ int free_before(const int32_t *counts, int blocks, in
     total += c;
     before += i < at ? c : 0;
   }
-  *all = block_sum(total, s);
-  return block_sum(before, s);
+  *all = block_sum<4>(total, s);
+  return block_sum<4>(before, s);
 }
 
 // The table entries of row b that hold positions from .. from + n - 1 (clipped to the
@@ -158,6 +177,39 @@ __global__ __launch_bounds__(kThreads) void reserve_count_kernel(
   if (lane == 0) w.a[b] = n;
 }
 
+// A wave's free pages take their ranks, those below `most`.
+__device__ __forceinline__ void list_wave(const uint64_t (&mask)[kSteps], int p0, int rank,
+                                          int most, int32_t *free_of) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int k = rank + __popcll(mask[i] & ((1ull << lane) - 1));
+    if (((mask[i] >> lane) & 1) && k < most) free_of[k] = p0 + 64 * i + lane;
+    rank += __popcll(mask[i]);
+  }
+}
+// One workgroup of kPlanThreads: the lowest `want` free pages into free_of (all threads
+// return how many it found, those of the last round included).
+__device__ __forceinline__ int list_free(const int32_t *refs, int n_pages, int want,
+                                         int32_t *free_of, int *s) {
+  const int wave = threadIdx.x >> 6;
+  int found = 0;
+  for (int r0 = 0; r0 < n_pages && found < want; r0 += kRound) {
+    uint64_t mask[kSteps];
+    const int p0 = r0 + wave * 64 * kSteps, n = free_masks(refs, n_pages, p0, mask);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s[wave] = n;
+    __syncthreads();
+    int rank = found;
+#pragma unroll
+    for (int v = 0; v < kPlanWaves; ++v) {
+      rank += v < wave ? s[v] : 0;
+      found += s[v];
+    }
+    list_wave(mask, p0, rank, want, free_of);
+  }
+  return found;
+}
 // Ranks the free pages of its block.
 __device__ __forceinline__ void list_block(const int32_t *refs, int n_pages, int blocks,
                                            const Work &w) {
@@ -169,12 +221,7 @@ __device__ __forceinline__ void list_block(const int32_t *refs, int n_pages, int
   if (lane == 0) s_wave[wave] = n;
   __syncthreads();
   for (int v = 0; v < wave; ++v) rank += s_wave[v];
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    if ((mask[i] >> lane) & 1)
-      w.free_of[rank + __popcll(mask[i] & ((1ull << lane) - 1))] = p0 + 64 * i + lane;
-    rank += __popcll(mask[i]);
-  }
+  list_wave(mask, p0, rank, INT_MAX, w.free_of);
 }
 // Writes the free pages in all and what of `wanted` (and of pages past the table) is missing.
 __device__ __forceinline__ void tell(long long wanted, long long beyond, int blocks,
@@ -214,7 +261,7 @@ __global__ __launch_bounds__(kThreads) void reserve_list_kernel(
         beyond += more;
       }
     }
-    int all, at = base + block_before(sum, s, &all);
+    int all, at = base + block_before<4>(sum, s, &all);
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       const int b = b0 + kRows * threadIdx.x + i;
@@ -256,18 +303,117 @@ __global__ __launch_bounds__(kThreads) void reserve_apply_kernel(
   }
 }
 
+// All of it in one workgroup, a thread for each row.
+__global__ __launch_bounds__(kPlanThreads) void reserve_small_kernel(
+    int32_t *refs, int n_pages, int32_t *table, int max_pages, const int32_t *lens,
+    const int32_t *counts, int batch, int32_t *shortfall, Work w) {
+  __shared__ int s[kPlanWaves];
+  __shared__ unsigned long long s_beyond;
+  if (threadIdx.x == 0) s_beyond = 0;
+  __syncthreads();
+  int base = 0;
+  for (int b0 = 0; b0 < batch; b0 += kPlanThreads) {
+    const int b = b0 + threadIdx.x;
+    int e0 = 0, e1 = 0, n = 0;
+    long long beyond = 0;
+    if (b < batch && entries_of(lens, counts, b, max_pages, &e0, &e1, &beyond)) {
+#pragma unroll 8
+      for (int e = e0; e < e1; ++e) n += !names(table[(size_t)b * max_pages + e], n_pages);
+      if (beyond) atomicAdd(&s_beyond, (unsigned long long)beyond);
+    }
+    int all;
+    const int at = base + block_before<kPlanWaves>(n, s, &all);
+    if (b < batch) w.b[b] = n ? at : -1;  // read by the same thread
+    base += all;
+  }
+  const int found = list_free(refs, n_pages, base, w.free_of, s);
+  __syncthreads();  // the list is written
+  if (threadIdx.x == 0 && shortfall != nullptr) {
+    const long long missing = (long long)s_beyond + (base > found ? base - found : 0);
+    *shortfall = (int32_t)min(missing, (long long)INT_MAX);
+  }
+  for (int b = threadIdx.x; b < batch; b += kPlanThreads) {
+    int at = w.b[b], e0, e1;
+    long long beyond;
+    if (at < 0 || !entries_of(lens, counts, b, max_pages, &e0, &e1, &beyond)) continue;
+    for (int e = e0; e < e1; ++e) {
+      int32_t *entry = table + (size_t)b * max_pages + e;
+      if (names(*entry, n_pages)) continue;
+      const int p = at < found ? w.free_of[at] : -1;
+      ++at;
+      *entry = p;
+      if (p >= 0) refs[p] = 1;
+    }
+  }
+}
+
 // --------------------------------------------------------------------- fork --
 __global__ __launch_bounds__(kThreads) void count_kernel(const int32_t *refs, int n_pages,
                                                          Work w) {
   count_block(refs, n_pages, w.counts);
 }
 
-__device__ __forceinline__ int owner_at(const int32_t *owner, int row) {
-  return __hip_atomic_load(owner + row, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// The first item that names a row as its child has it: owners of rows in LDS, or, past
+// kSmallRows, in memory, where atomics and accesses beside them have to meet.
+struct LdsOwners {
+  int *at;
+  __device__ void clear(int r) { at[r] = INT_MAX; }
+  __device__ void claim(int r, int i) { atomicMin(at + r, i); }
+  __device__ int of(int r) { return at[r]; }
+  __device__ void join() { __syncthreads(); }
+};
+struct MemoryOwners {
+  int32_t *at;
+  __device__ void clear(int r) {
+    __hip_atomic_store(at + r, INT_MAX, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __device__ void claim(int r, int i) { atomicMin(at + r, i); }
+  __device__ int of(int r) {
+    return __hip_atomic_load(at + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __device__ void join() {
+    __threadfence();
+    __syncthreads();
+  }
+};
+
+// One workgroup: of each item the rank of its new page among the free ones, -1 where it
+// needs none, -2 where the item is left out.  Returns how many want a page.
+template <int WAVES, typename Owners>
+__device__ __forceinline__ int fork_items(Owners own, int n_pages, const int32_t *table,
+                                          int max_pages,
+                                          const int32_t *lens, int batch, const int32_t *parents,
+                                          const int32_t *children, int n, const Work &w, int *s) {
+  constexpr int kT = 64 * WAVES;
+  for (int r = threadIdx.x; r < batch; r += kT) own.clear(r);
+  own.join();
+  for (int i = threadIdx.x; i < n; i += kT) {
+    const int c = children[i];
+    if (c >= 0 && c < batch) own.claim(c, i);
+  }
+  own.join();
+  int base = 0;
+  for (int i0 = 0; i0 < n; i0 += kT) {
+    const int i = i0 + threadIdx.x;
+    bool ok = false, want = false;
+    if (i < n) {
+      const int c = children[i], p = parents[i];
+      ok = c >= 0 && c < batch && p >= 0 && p < batch && own.of(c) == i &&
+           own.of(p) == INT_MAX;
+      if (ok) {
+        const int L = min(max(lens[p], 0), max_pages * kKvPage);
+        want = L % kKvPage != 0 &&
+               names(table[(size_t)p * max_pages + L / kKvPage], n_pages);
+      }
+    }
+    int all;
+    const int at = base + block_before<WAVES>(want ? 1 : 0, s, &all);
+    if (i < n) w.b[i] = !ok ? -2 : want ? at : -1;
+    base += all;
+  }
+  return base;
 }
 
-// Of each item the rank of its new page among the free ones, -1 where it needs none, -2
-// where the item is left out.
 __global__ __launch_bounds__(kThreads) void fork_list_kernel(
     const int32_t *refs, int n_pages, int blocks, const int32_t *table, int max_pages,
     const int32_t *lens, int batch, const int32_t *parents, const int32_t *children, int n,
@@ -277,70 +423,53 @@ __global__ __launch_bounds__(kThreads) void fork_list_kernel(
     return;
   }
   __shared__ int s[4];
-  // The first item that names a row as its child has it.
-  for (int r = threadIdx.x; r < batch; r += kThreads)
-    __hip_atomic_store(w.a + r, INT_MAX, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __threadfence();
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const int c = children[i];
-    if (c >= 0 && c < batch) atomicMin(w.a + c, i);
-  }
-  __threadfence();
-  __syncthreads();
-  int base = 0;
-  for (int i0 = 0; i0 < n; i0 += kThreads) {
-    const int i = i0 + threadIdx.x;
-    bool ok = false, want = false;
-    if (i < n) {
-      const int c = children[i], p = parents[i];
-      ok = c >= 0 && c < batch && p >= 0 && p < batch && owner_at(w.a, c) == i &&
-           owner_at(w.a, p) == INT_MAX;
-      if (ok) {
-        const int L = min(max(lens[p], 0), max_pages * kKvPage);
-        want = L % kKvPage != 0 &&
-               names(table[(size_t)p * max_pages + L / kKvPage], n_pages);
-      }
-    }
-    int all;
-    const int at = base + block_before(want ? 1 : 0, s, &all);
-    if (i < n) w.b[i] = !ok ? -2 : want ? at : -1;
-    base += all;
-  }
-  tell(base, 0, blocks, w, shortfall, s);
+  const int want =
+      fork_items<4>(MemoryOwners{w.a}, n_pages, table, max_pages, lens, batch, parents, children,
+                    n, w, s);
+  tell(want, 0, blocks, w, shortfall, s);
+}
+__global__ __launch_bounds__(kPlanThreads) void fork_small_kernel(
+    const int32_t *refs, int n_pages, const int32_t *table, int max_pages, const int32_t *lens,
+    int batch, const int32_t *parents, const int32_t *children, int n, int32_t *shortfall,
+    Work w) {
+  __shared__ int s[kPlanWaves], s_owner[kSmallRows];
+  const int want = fork_items<kPlanWaves>(LdsOwners{s_owner}, n_pages, table, max_pages, lens,
+                                          batch, parents, children, n, w, s);
+  const int found = list_free(refs, n_pages, want, w.free_of, s);
+  if (threadIdx.x != 0) return;
+  w.head[0] = found;
+  if (shortfall != nullptr) *shortfall = want > found ? want - found : 0;
 }
 
-// 16-byte pieces at .. at + kChunk - 1 of a page of n16 pieces.
-__device__ __forceinline__ void copy_chunk(const uint8_t *src, uint8_t *dst, int n16, int at) {
-  const u32x4 *from = reinterpret_cast<const u32x4 *>(src);
-  u32x4 *to = reinterpret_cast<u32x4 *>(dst);
+// Chunk `ch` of a page.
+__device__ __forceinline__ void copy_chunk(const uint8_t *cache_from, int from, uint8_t *cache_to,
+                                           int to, const Chunks &c, int ch) {
+  const size_t bytes = (size_t)c.pieces * 16;
+  const u32x4 *src = reinterpret_cast<const u32x4 *>(cache_from + from * bytes) + ch * c.chunk;
+  u32x4 *dst = reinterpret_cast<u32x4 *>(cache_to + to * bytes) + ch * c.chunk;
+  const int n = min(c.chunk, c.pieces - ch * c.chunk);
   u32x4 v[kCopyUnroll];
 #pragma unroll
-  for (int j = 0; j < kCopyUnroll; ++j) {
-    const int x = at + j * kThreads + threadIdx.x;
-    if (x < n16) v[j] = from[x];
-  }
+  for (int j = 0; j < kCopyUnroll; ++j)  // without a branch: all loads at once
+    v[j] = src[min(j * kThreads + (int)threadIdx.x, n - 1)];
 #pragma unroll
   for (int j = 0; j < kCopyUnroll; ++j) {
-    const int x = at + j * kThreads + threadIdx.x;
-    if (x < n16) to[x] = v[j];
+    const int x = j * kThreads + threadIdx.x;
+    if (x < n) dst[x] = v[j];
   }
 }
 
 // Grid (items, chunks of a page): the first chunk's workgroups write the table too.
 __global__ __launch_bounds__(kThreads) void fork_apply_kernel(
     uint8_t *cache, int32_t *refs, int n_pages, int32_t *table, int max_pages, int32_t *lens,
-    const int32_t *parents, const int32_t *children, int n16, Work w) {
+    const int32_t *parents, const int32_t *children, Chunks c16, Work w) {
   const int i = blockIdx.x, slot = w.b[i];
   if (slot == -2) return;
   const int c = children[i], p = parents[i];
   const int L = min(max(lens[p], 0), max_pages * kKvPage), full = L / kKvPage;
   const int32_t *from = table + (size_t)p * max_pages;
   const int fresh = slot >= 0 && slot < w.head[0] ? w.free_of[slot] : -1;
-  if (fresh >= 0) {
-    const size_t bytes = (size_t)n16 * 16;
-    copy_chunk(cache + from[full] * bytes, cache + fresh * bytes, n16, blockIdx.y * kChunk);
-  }
+  if (fresh >= 0) copy_chunk(cache, from[full], cache, fresh, c16, blockIdx.y);
   if (blockIdx.y != 0) return;
   int32_t *to = table + (size_t)c * max_pages;
   for (int e = threadIdx.x; e < max_pages; e += kThreads) {
@@ -379,22 +508,9 @@ __global__ __launch_bounds__(kThreads) void release_kernel(int32_t *refs, int n_
 // With n_live pages in use, those at n_live and above move to the free ones below; both
 // are equally many (head[1]).  a: the moving pages, highest first; b: of every page its
 // index in a, -1 where it is in use and stays, -2 where it is free.
-__global__ __launch_bounds__(kThreads) void compact_list_kernel(const int32_t *refs, int n_pages,
-                                                                int blocks, int32_t *n_live,
-                                                                Work w) {
-  __shared__ int s[4], s_wave[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, p0 = first_page();
-  uint64_t mask[kSteps];
-  const int n = free_masks(refs, n_pages, p0, mask);
-  int all, rank = free_before(w.counts, blocks, blockIdx.x, &all, s);
-  if (lane == 0) s_wave[wave] = n;
-  __syncthreads();
-  for (int v = 0; v < wave; ++v) rank += s_wave[v];
-  const int live = n_pages - all;
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    *n_live = live;
-    if (live == n_pages) w.head[1] = 0;
-  }
+__device__ __forceinline__ void compact_wave(const uint64_t (&mask)[kSteps], int p0, int rank,
+                                             int n_pages, int live, const Work &w) {
+  const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
     const int p = p0 + 64 * i + lane, f = rank + __popcll(mask[i] & ((1ull << lane) - 1));
@@ -412,17 +528,73 @@ __global__ __launch_bounds__(kThreads) void compact_list_kernel(const int32_t *r
     rank += __popcll(mask[i]);
   }
 }
+__global__ __launch_bounds__(kThreads) void compact_list_kernel(const int32_t *refs, int n_pages,
+                                                                int blocks, int32_t *n_live,
+                                                                Work w) {
+  __shared__ int s[4], s_wave[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, p0 = first_page();
+  uint64_t mask[kSteps];
+  const int n = free_masks(refs, n_pages, p0, mask);
+  int all, rank = free_before(w.counts, blocks, blockIdx.x, &all, s);
+  if (lane == 0) s_wave[wave] = n;
+  __syncthreads();
+  for (int v = 0; v < wave; ++v) rank += s_wave[v];
+  const int live = n_pages - all;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    *n_live = live;
+    if (live == n_pages) w.head[1] = 0;
+  }
+  compact_wave(mask, p0, rank, n_pages, live, w);
+}
+__global__ __launch_bounds__(kPlanThreads) void compact_small_kernel(const int32_t *refs,
+                                                                     int n_pages,
+                                                                     int32_t *n_live, Work w) {
+  __shared__ int s[kPlanWaves];
+  const int wave = threadIdx.x >> 6;
+  uint64_t mask[kSteps];
+  int n = 0, all = 0;
+  for (int r0 = 0; r0 < n_pages; r0 += kRound) {
+    const int m = free_masks(refs, n_pages, r0 + wave * 64 * kSteps, mask);
+    n += (threadIdx.x & 63) == 0 ? m : 0;
+  }
+  all = block_sum<kPlanWaves>(n, s);
+  const int live = n_pages - all;
+  if (threadIdx.x == 0) {
+    *n_live = live;
+    if (live == n_pages) w.head[1] = 0;
+  }
+  int before = 0;
+  for (int r0 = 0; r0 < n_pages; r0 += kRound) {
+    const int p0 = r0 + wave * 64 * kSteps;
+    // Up to kRound pages the masks are still here.
+    const int m = n_pages <= kRound ? 0 : free_masks(refs, n_pages, p0, mask);
+    int mine = m;
+    if (n_pages <= kRound) {
+      mine = 0;
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) mine += __popcll(mask[i]);
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s[wave] = mine;
+    __syncthreads();
+    int rank = before;
+#pragma unroll
+    for (int v = 0; v < kPlanWaves; ++v) {
+      rank += v < wave ? s[v] : 0;
+      before += s[v];
+    }
+    compact_wave(mask, p0, rank, n_pages, live, w);
+  }
+}
 
 __global__ __launch_bounds__(kThreads) void compact_apply_kernel(
-    uint8_t *cache, int32_t *refs, int n_pages, int32_t *table, size_t entries, int n16,
-    int chunks, int32_t *new_page, Work w) {
+    uint8_t *cache, int32_t *refs, int n_pages, int32_t *table, size_t entries, Chunks c16,
+    int32_t *new_page, Work w) {
   const int moves = w.head[1];
-  const size_t bytes = (size_t)n16 * 16;
-  const long long units = (long long)moves * chunks;
+  const long long units = (long long)moves * c16.chunks;
   for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-    const int r = (int)(u / chunks), ch = (int)(u - (long long)r * chunks);
-    copy_chunk(cache + w.a[moves - 1 - r] * bytes, cache + w.free_of[r] * bytes, n16,
-               ch * kChunk);
+    const int r = (int)(u / c16.chunks), ch = (int)(u - (long long)r * c16.chunks);
+    copy_chunk(cache, w.a[moves - 1 - r], cache, w.free_of[r], c16, ch);
   }
   const size_t first = (size_t)blockIdx.x * kThreads + threadIdx.x,
                step = (size_t)gridDim.x * kThreads;
@@ -449,12 +621,11 @@ __global__ __launch_bounds__(kThreads) void compact_apply_kernel(
 __global__ __launch_bounds__(kThreads) void copy_kernel(uint8_t *dst, int dst_pages,
                                                         const uint8_t *src, int src_pages,
                                                         const int32_t *to, const int32_t *from,
-                                                        int n, int n16) {
-  const size_t bytes = (size_t)n16 * 16;
+                                                        int n, Chunks c16) {
   for (int i = blockIdx.y; i < n; i += gridDim.y) {
     const int t = to[i], f = from[i];
     if (names(t, dst_pages) && names(f, src_pages))
-      copy_chunk(src + f * bytes, dst + t * bytes, n16, blockIdx.x * kChunk);
+      copy_chunk(src, f, dst, t, c16, blockIdx.x);
   }
 }
 
@@ -506,6 +677,12 @@ extern "C" int prichs_kv_pages_reserve(int32_t *refs, size_t n_pages, int32_t *p
                         prichs_kv_pages_workspace(n_pages, batch, 0)));
   const Work w = work_of(workspace, n_pages, batch);
   const hipStream_t s = as_stream(stream);
+  if (n_pages <= kSmallPages && batch <= kSmallRows) {
+    hipLaunchKernelGGL(reserve_small_kernel, dim3(1), dim3(kPlanThreads), 0, s, refs, (int)n_pages,
+                       page_table, (int)max_pages, lens, counts, (int)batch, shortfall, w);
+    PRICHS_LAUNCH_CHECK("kv_pages_reserve launch");
+    return PRICHS_OK;
+  }
   const unsigned blocks = (unsigned)blocks_of(n_pages), rows = (unsigned)cdiv(batch, 4);
   if (blocks + rows > 0) {
     hipLaunchKernelGGL(reserve_count_kernel, dim3(blocks + rows), dim3(kThreads), 0, s, refs,
@@ -542,20 +719,26 @@ extern "C" int prichs_kv_pages_fork(void *cache, int32_t *refs, size_t n_pages,
                         prichs_kv_pages_workspace(n_pages, batch, n)));
   const Work w = work_of(workspace, n_pages, batch > n ? batch : n);
   const hipStream_t s = as_stream(stream);
-  const unsigned blocks = (unsigned)blocks_of(n_pages);
-  if (blocks > 0) {
-    hipLaunchKernelGGL(count_kernel, dim3(blocks), dim3(kThreads), 0, s, refs, (int)n_pages, w);
-    PRICHS_LAUNCH_CHECK("kv_pages_fork count launch");
+  if (n_pages <= kSmallPages && batch <= kSmallRows && n <= kSmallRows) {
+    hipLaunchKernelGGL(fork_small_kernel, dim3(1), dim3(kPlanThreads), 0, s, refs, (int)n_pages,
+                       page_table, (int)max_pages, lens, (int)batch, parents, children, (int)n,
+                       shortfall, w);
+  } else {
+    const unsigned blocks = (unsigned)blocks_of(n_pages);
+    if (blocks > 0) {
+      hipLaunchKernelGGL(count_kernel, dim3(blocks), dim3(kThreads), 0, s, refs, (int)n_pages, w);
+      PRICHS_LAUNCH_CHECK("kv_pages_fork count launch");
+    }
+    hipLaunchKernelGGL(fork_list_kernel, dim3(blocks + 1), dim3(kThreads), 0, s, refs,
+                       (int)n_pages, (int)blocks, page_table, (int)max_pages, lens, (int)batch,
+                       parents, children, (int)n, shortfall, w);
   }
-  hipLaunchKernelGGL(fork_list_kernel, dim3(blocks + 1), dim3(kThreads), 0, s, refs, (int)n_pages,
-                     (int)blocks, page_table, (int)max_pages, lens, (int)batch, parents, children,
-                     (int)n, shortfall, w);
   PRICHS_LAUNCH_CHECK("kv_pages_fork list launch");
   if (n > 0) {
-    const size_t n16 = n_kv_heads * kKvPart / 16;
-    hipLaunchKernelGGL(fork_apply_kernel, dim3((unsigned)n, (unsigned)cdiv(n16, kChunk)),
+    const Chunks c16(n_kv_heads);
+    hipLaunchKernelGGL(fork_apply_kernel, dim3((unsigned)n, (unsigned)c16.chunks),
                        dim3(kThreads), 0, s, static_cast<uint8_t *>(cache), refs, (int)n_pages,
-                       page_table, (int)max_pages, lens, parents, children, (int)n16, w);
+                       page_table, (int)max_pages, lens, parents, children, c16, w);
     PRICHS_LAUNCH_CHECK("kv_pages_fork launch");
   }
   return PRICHS_OK;
@@ -589,24 +772,27 @@ extern "C" int prichs_kv_pages_compact(void *cache, int32_t *refs, size_t n_page
                         prichs_kv_pages_workspace(n_pages, 0, 0)));
   const Work w = work_of(workspace, n_pages, 0);
   const hipStream_t s = as_stream(stream);
-  const unsigned blocks = (unsigned)blocks_of(n_pages);
-  if (blocks > 0) {
+  if (n_pages <= kSmallPages) {
+    hipLaunchKernelGGL(compact_small_kernel, dim3(1), dim3(kPlanThreads), 0, s, refs,
+                       (int)n_pages, n_live, w);
+  } else {
+    const unsigned blocks = (unsigned)blocks_of(n_pages);
     hipLaunchKernelGGL(count_kernel, dim3(blocks), dim3(kThreads), 0, s, refs, (int)n_pages, w);
     PRICHS_LAUNCH_CHECK("kv_pages_compact count launch");
+    hipLaunchKernelGGL(compact_list_kernel, dim3(blocks), dim3(kThreads), 0, s, refs,
+                       (int)n_pages, (int)blocks, n_live, w);
   }
-  hipLaunchKernelGGL(compact_list_kernel, dim3(blocks > 0 ? blocks : 1), dim3(kThreads), 0, s,
-                     refs, (int)n_pages, (int)blocks, n_live, w);
   PRICHS_LAUNCH_CHECK("kv_pages_compact list launch");
   if (n_pages == 0) return PRICHS_OK;
-  const size_t n16 = n_kv_heads * kKvPart / 16, chunks = cdiv(n16, kChunk),
-               entries = batch * max_pages;
+  const Chunks c16(n_kv_heads);
+  const size_t entries = batch * max_pages;
   // At most half of the pages move; workgroups loop over what there is.
-  size_t grid = cdiv(n_pages, 2) * chunks;
+  size_t grid = cdiv(n_pages, 2) * c16.chunks;
   const size_t small = cdiv(n_pages > entries ? n_pages : entries, (size_t)kThreads);
   grid = grid > small ? grid : small;
   hipLaunchKernelGGL(compact_apply_kernel, dim3((unsigned)(grid < 2048 ? grid : 2048)),
                      dim3(kThreads), 0, s, static_cast<uint8_t *>(cache), refs, (int)n_pages,
-                     page_table, entries, (int)n16, (int)chunks, new_page, w);
+                     page_table, entries, c16, new_page, w);
   PRICHS_LAUNCH_CHECK("kv_pages_compact launch");
   return PRICHS_OK;
 }
@@ -622,11 +808,11 @@ extern "C" int prichs_kv_cache_copy(void *dst, size_t dst_pages, const void *src
                  "%s: shape too large", who);
   PRICHS_REQUIRE(n == 0 || (to && from), "%s: null pointer argument", who);
   if (n == 0 || dst_pages == 0 || src_pages == 0) return PRICHS_OK;
-  const size_t n16 = n_kv_heads * kKvPart / 16;
-  hipLaunchKernelGGL(copy_kernel, dim3((unsigned)cdiv(n16, kChunk), (unsigned)(n < 65535 ? n : 65535)),
+  const Chunks c16(n_kv_heads);
+  hipLaunchKernelGGL(copy_kernel, dim3((unsigned)c16.chunks, (unsigned)(n < 65535 ? n : 65535)),
                      dim3(kThreads), 0, as_stream(stream), static_cast<uint8_t *>(dst),
                      (int)dst_pages, static_cast<const uint8_t *>(src), (int)src_pages, to, from,
-                     (int)n, (int)n16);
+                     (int)n, c16);
   PRICHS_LAUNCH_CHECK("kv_cache_copy launch");
   return PRICHS_OK;
 }

@@ -57,9 +57,11 @@ def same(ref, cache, refs, table, lens):
 
 
 # (pages, rows, columns, kv heads): one page, less than a block of pages, several blocks;
-# tables of one column and of more than a workgroup has threads.
+# tables of one column and of more than a workgroup has threads; more pages than a workgroup
+# takes in one round, and more pages or rows than one workgroup plans for.
 SCENES = [(1, 1, 1, 1), (70, 6, 8, 3), (300, 40, 7, 1), (5000, 100, 40, 1), (9000, 17, 600, 1),
-          (4096, 3, 1300, 1), (40, 9, 3, 5), (4097, 2100, 2, 1)]
+          (4096, 3, 1300, 1), (40, 9, 3, 5), (4097, 2100, 2, 1), (20000, 50, 300, 1),
+          (16384, 30, 400, 1), (66000, 20, 3000, 1), (500, 4100, 2, 1), (70000, 4200, 9, 1)]
 
 
 @pytest.mark.parametrize("n_pages,batch,width,kv", SCENES)

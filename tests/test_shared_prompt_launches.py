@@ -100,3 +100,34 @@ def test_rotation_takes_the_lanes_that_a_head_needs():
         assert bwd.grid[0] <= 1024
         names |= {fwd.kernel, bwd.kernel}
     assert len(names) == 16
+
+
+def pages(cases):
+    """Names of the launches of a reserve, a fork and a compaction for each (pages, rows)."""
+    return ll.run(f"""
+result = []
+for n, b in {cases!r}:
+    one = []
+    need = lib.prichs_kv_pages_workspace(n, b, b)
+    L.check(lib.prichs_kv_pages_reserve(P, n, P, 9, P, P, b, None, P, need, None))
+    one.append([x[0] for x in launches()])
+    L.check(lib.prichs_kv_pages_fork(P, P, n, P, 9, P, b, P, P, b, 3, None, P, need, None))
+    one.append([x[0] for x in launches()])
+    L.check(lib.prichs_kv_pages_compact(P, P, n, P, 9, b, 3, P, P, P, need, None))
+    one.append([x[0] for x in launches()])
+    result.append(one)
+""")
+
+
+def test_one_workgroup_plans_for_few_pages_and_rows():
+    from tests.test_gpu_kv_pages import SCENES
+
+    few = [["reserve_small_kernel"], ["fork_small_kernel", "fork_apply_kernel"],
+           ["compact_small_kernel", "compact_apply_kernel"]]
+    many = [["reserve_count_kernel", "reserve_list_kernel", "reserve_apply_kernel"],
+            ["count_kernel", "fork_list_kernel", "fork_apply_kernel"],
+            ["count_kernel", "compact_list_kernel", "compact_apply_kernel"]]
+    got = pages([(65536, 4096), (65537, 4), (4, 4097), (0, 4)])
+    assert got == [few, many, many[:2] + few[2:], few[:2] + [few[2][:1]]]
+    seen = {x for one in pages([s[:2] for s in SCENES]) for call in one for x in call}
+    assert seen == {x for one in (few, many) for call in one for x in call}
