@@ -8,9 +8,13 @@
 // Everything is f32 between the load and the one rounding of a result.
 //
 // `LANES` lanes hold one head of one row, 8 values (4 whole pairs) each, so sums over a
-// head are a few lane exchanges.  Such a group of lanes takes up to kHeads heads of its
-// row, kHeads loads in flight, with one load of the position's cos and sin (32 bytes a
-// lane against 16 of a bf16 head).
+// head are a few lane exchanges.  Such a group of lanes takes kHeads heads of its row, whose
+// loads are all in flight, with one load of the position's cos and sin (32 bytes a lane
+// against 16 of a bf16 head).  Bound by HBM where there are many rows: 4 x 2048 of 12 + 3
+// heads in bf16 (64 MB; MI355X) 13.3 us forward, 4.8 TB/s, and 19.6 backward (98 MB, 5.0);
+// by the launch where there are few (32 rows 4.0 us).  Heads a group, us of a captured
+// forward, and of a forward and backward: 1 15.0 and 38.2, 2 13.7 and 35.9, 3 13.3 and 35.0,
+// 4 13.1 and 37.9, 5 13.7 and 47.4 (registers).
 #include "common.hpp"
 
 namespace prichs {
@@ -20,21 +24,27 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
-constexpr int kHeads = 4;  // heads of a group of lanes
+constexpr int kHeads = 3;  // heads of a group of lanes
 
-__device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
-  const f32x4 a = *reinterpret_cast<const f32x4 *>(p), b = *reinterpret_cast<const f32x4 *>(p + 4);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
-}
-__device__ __forceinline__ void load8(const bf16_t *p, float (&x)[8]) {
-  const u32x4 u = *reinterpret_cast<const u32x4 *>(p);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    x[2 * e] = __uint_as_float(u[e] << 16);
-    x[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u);
+// 8 values as they were loaded; taken apart where they are used, which keeps the registers
+// of loads in flight few.
+template <typename T> struct Raw8;
+template <> struct Raw8<float> {
+  f32x4 a, b;
+  __device__ __forceinline__ void load(const float *p) {
+    a = *reinterpret_cast<const f32x4 *>(p), b = *reinterpret_cast<const f32x4 *>(p + 4);
   }
-}
+  __device__ __forceinline__ void clear() { a = b = f32x4{0.f, 0.f, 0.f, 0.f}; }
+  __device__ __forceinline__ float operator[](int e) const { return e < 4 ? a[e] : b[e - 4]; }
+};
+template <> struct Raw8<bf16_t> {
+  u32x4 u;
+  __device__ __forceinline__ void load(const bf16_t *p) { u = *reinterpret_cast<const u32x4 *>(p); }
+  __device__ __forceinline__ void clear() { u = u32x4{0, 0, 0, 0}; }
+  __device__ __forceinline__ float operator[](int e) const {
+    return __uint_as_float(e & 1 ? u[e / 2] & 0xffff0000u : u[e / 2] << 16);
+  }
+};
 __device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
   *reinterpret_cast<f32x4 *>(p) = f32x4{x[0], x[1], x[2], x[3]};
   *reinterpret_cast<f32x4 *>(p + 4) = f32x4{x[4], x[5], x[6], x[7]};
@@ -60,65 +70,68 @@ struct Args {
   size_t ldx[2], ldd[2], ldo[2];
   const float *w[2], *cs, *sn;
   const int32_t *positions;
-  long long rows, cache_rows, pos_offset, seq_len;
-  int Hq, H, hd, per_row;  // per_row: groups of lanes of a row
+  uint32_t rows, cache_rows, pos_offset, seq_len;
+  int Hq, H, hd;
+  uint32_t per_row;  // groups of lanes of a row
   float inv_hd, eps;
 };
 
-// Position of a row, or -1 outside the tables.
+// Position of a row; cache_rows or more outside the tables.
 template <typename T>
-__device__ __forceinline__ long long position(const Args<T> &a, long long row) {
-  const long long p =
-      a.positions != nullptr ? (long long)a.positions[row] : row % a.seq_len + a.pos_offset;
-  return p < a.cache_rows ? p : -1;
+__device__ __forceinline__ uint32_t position(const Args<T> &a, uint32_t row) {
+  return a.positions != nullptr ? (uint32_t)a.positions[row] : row % a.seq_len + a.pos_offset;
+}
+// Row and first head of a group of lanes: the `at`-th of workgroup `block`, `groups` a workgroup.
+template <typename T>
+__device__ __forceinline__ void unit_of(const Args<T> &a, uint64_t block, int groups, int at,
+                                        uint64_t *row, int *s) {
+  const uint64_t u0 = block * groups, r0 = u0 / a.per_row;  // the same for the workgroup
+  const uint32_t x = (uint32_t)(u0 - r0 * a.per_row) + at, r = x / a.per_row;
+  *row = r0 + r;
+  *s = (int)(x - r * a.per_row);
 }
 
-// Head h of a row in q (or k) and its like.
-template <typename T>
-__device__ __forceinline__ T *head_at(T *const (&p)[2], const size_t (&ld)[2], long long row,
-                                      int h, int Hq, int hd) {
-  const bool isk = h >= Hq;
-  return (isk ? p[1] : p[0]) + (size_t)row * (isk ? ld[1] : ld[0]) +
-         (size_t)(h - (isk ? Hq : 0)) * hd;
-}
+// A lane's values of the heads s, s + per_row, .. of a row: in q (or its like) up to Hq, then
+// in k, which gets an address of its own that lies Hq heads before k's row.
+template <typename T> struct Heads {
+  T *q, *k;
+  __device__ __forceinline__ Heads(T *const (&p)[2], const size_t (&ld)[2], uint64_t row, int at,
+                                   int Hq, int hd)
+      : q(p[0] + row * ld[0] + at), k(p[1] + row * ld[1] + (at - Hq * hd)) {}
+  __device__ __forceinline__ T *at(bool isk, int step) const { return (isk ? k : q) + step; }
+};
 
 // Unit u: row u / per_row; heads u % per_row + per_row j, so that neighbouring groups of
 // lanes read neighbouring heads.
+// Lanes past the head's end and heads past the last load what the group's first ones do,
+// so that all loads are in flight without a branch between them.
 template <typename T, int LANES>
-__global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(Args<T> a) {
+__global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(Args<T> a, uint64_t blocks) {
   constexpr int kGroups = kThreads / LANES;
   const int c = threadIdx.x % LANES;
   const bool lane = 8 * c < a.hd;  // of the lanes' 8 LANES values hd are the head's
-  const long long units = a.rows * a.per_row;
-  for (long long u = (long long)blockIdx.x * kGroups + threadIdx.x / LANES; u < units;
-       u += (long long)gridDim.x * kGroups) {
-    const long long row = u / a.per_row;
-    const int s = (int)(u - row * a.per_row);
-    const long long pos = position(a, row);
-    if (pos < 0) continue;  // the lanes of a group agree
-    float x[kHeads][8], w[2][8], cs[4], sn[4];
+  const int col = lane ? 8 * c : 0;
+  for (uint64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
+    uint64_t row;
+    int s;
+    unit_of(a, block, kGroups, threadIdx.x / LANES, &row, &s);
+    if (row >= a.rows) continue;  // the lanes of a group agree
+    const uint32_t pos = position(a, (uint32_t)row);
+    if (pos >= a.cache_rows) continue;
+    const int step = (int)a.per_row * a.hd;  // from a head to the next of the group
+    const Heads<const T> xs(a.x, a.ldx, row, s * a.hd + col, a.Hq, a.hd);
+    Raw8<T> x[kHeads];
 #pragma unroll
     for (int j = 0; j < kHeads; ++j) {
-      const int h = s + a.per_row * j;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[j][e] = 0.f;
-      if (lane && h < a.H) load8(head_at(a.x, a.ldx, row, h, a.Hq, a.hd) + 8 * c, x[j]);
+      const int h = s + a.per_row * j, jj = h < a.H ? j : 0;
+      x[j].load(xs.at(s + (int)a.per_row * jj >= a.Hq, jj * step));
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) cs[e] = sn[e] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[i][e] = 0.f;
-    if (lane) {
-      const size_t at = (size_t)pos * (a.hd / 2) + 4 * c;
-      const f32x4 c4 = *reinterpret_cast<const f32x4 *>(a.cs + at);
-      const f32x4 s4 = *reinterpret_cast<const f32x4 *>(a.sn + at);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) cs[e] = c4[e], sn[e] = s4[e];
-      if (a.Hq > 0) load8(a.w[0] + 8 * c, w[0]);
-      if (a.H > a.Hq) load8(a.w[1] + 8 * c, w[1]);
-    }
+    const size_t at = (size_t)pos * (a.hd / 2) + col / 2;
+    const f32x4 cs = *reinterpret_cast<const f32x4 *>(a.cs + at);
+    const f32x4 sn = *reinterpret_cast<const f32x4 *>(a.sn + at);
+    Raw8<float> wq, wk;
+    wq.load(a.w[0] + col), wk.load(a.w[1] + col);
+    const Heads<T> os(a.out, a.ldo, row, s * a.hd + col, a.Hq, a.hd);
 #pragma unroll
     for (int j = 0; j < kHeads; ++j) {
       const int h = s + a.per_row * j;
@@ -126,68 +139,67 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(Args<T> a) {
       float ss = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss = fmaf(x[j][e], x[j][e], ss);
-      ss = lanes_sum<LANES>(ss);
-      const float inv = 1.0f / sqrtf(fmaf(ss, a.inv_hd, a.eps));
+      ss = lanes_sum<LANES>(lane ? ss : 0.f);
+      const float inv = rsqrtf(fmaf(ss, a.inv_hd, a.eps));
       float o[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float y0 = x[j][2 * i] * inv * (isk ? w[1][2 * i] : w[0][2 * i]);
-        const float y1 = x[j][2 * i + 1] * inv * (isk ? w[1][2 * i + 1] : w[0][2 * i + 1]);
+        const float y0 = x[j][2 * i] * inv * (isk ? wk[2 * i] : wq[2 * i]);
+        const float y1 = x[j][2 * i + 1] * inv * (isk ? wk[2 * i + 1] : wq[2 * i + 1]);
         o[2 * i] = y0 * cs[i] - y1 * sn[i];
         o[2 * i + 1] = y0 * sn[i] + y1 * cs[i];
       }
-      if (lane && h < a.H) store8(head_at(a.out, a.ldo, row, h, a.Hq, a.hd) + 8 * c, o);
+      if (lane && h < a.H) store8(os.at(isk, j * step), o);
     }
   }
 }
 
 // The gradients.  part: f32 [gridDim.x][2][hd], each workgroup's sums of d_wq and d_wk.
 template <typename T, int LANES>
-__global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd_kernel(Args<T> a,
-                                                                    float *__restrict__ part) {
+__global__ __launch_bounds__(kThreads, 4) void qk_norm_rope_bwd_kernel(Args<T> a, uint64_t blocks,
+                                                                       float *__restrict__ part) {
   constexpr int kGroups = kThreads / LANES;
   __shared__ float s_dw[kGroups][2][8 * LANES];
   const int c = threadIdx.x % LANES, grp = threadIdx.x / LANES;
   const bool lane = 8 * c < a.hd;
-  float w[2][8], dw[2][8];
+  const int col = lane ? 8 * c : 0;
+  Raw8<float> wq, wk;
+  wq.load(a.w[0] + col), wk.load(a.w[1] + col);
+  float dw[2][8];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[i][e] = dw[i][e] = 0.f;
-  if (lane && a.Hq > 0) load8(a.w[0] + 8 * c, w[0]);
-  if (lane && a.H > a.Hq) load8(a.w[1] + 8 * c, w[1]);
-  const long long units = a.rows * a.per_row;
-  for (long long u = (long long)blockIdx.x * kGroups + grp; u < units;
-       u += (long long)gridDim.x * kGroups) {
-    const long long row = u / a.per_row;
-    const int s = (int)(u - row * a.per_row);
-    const long long pos = position(a, row);
-    const bool live = lane && pos >= 0;
-    float x[kHeads][8], d[kHeads][8], cs[4], sn[4];
+    for (int e = 0; e < 8; ++e) dw[i][e] = 0.f;
+  for (uint64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
+    uint64_t row;
+    int s;
+    unit_of(a, block, kGroups, grp, &row, &s);
+    if (row >= a.rows) continue;
+    const uint32_t pos = position(a, (uint32_t)row);
+    const bool live = pos < a.cache_rows;
+    const int step = (int)a.per_row * a.hd;  // from a head to the next of the group
+    const Heads<const T> xs(a.x, a.ldx, row, s * a.hd + col, a.Hq, a.hd);
+    const Heads<const T> ds(a.d, a.ldd, row, s * a.hd + col, a.Hq, a.hd);
+    Raw8<T> x[kHeads], d[kHeads];
 #pragma unroll
     for (int j = 0; j < kHeads; ++j) {
-      const int h = s + a.per_row * j;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[j][e] = d[j][e] = 0.f;
-      if (live && h < a.H) {
-        load8(head_at(a.x, a.ldx, row, h, a.Hq, a.hd) + 8 * c, x[j]);
-        load8(head_at(a.d, a.ldd, row, h, a.Hq, a.hd) + 8 * c, d[j]);
-      }
+      const int h = s + a.per_row * j, jj = h < a.H ? j : 0;
+      const bool isk = s + (int)a.per_row * jj >= a.Hq;
+      x[j].load(xs.at(isk, jj * step));
+      d[j].load(ds.at(isk, jj * step));
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) cs[e] = sn[e] = 0.f;
-    if (live) {
-      const size_t at = (size_t)pos * (a.hd / 2) + 4 * c;
-      const f32x4 c4 = *reinterpret_cast<const f32x4 *>(a.cs + at);
-      const f32x4 s4 = *reinterpret_cast<const f32x4 *>(a.sn + at);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) cs[e] = c4[e], sn[e] = s4[e];
+    const size_t at = (size_t)(live ? pos : 0) * (a.hd / 2) + col / 2;
+    f32x4 cs = f32x4{0.f, 0.f, 0.f, 0.f}, sn = cs;
+    if (a.cache_rows > 0) {
+      cs = *reinterpret_cast<const f32x4 *>(a.cs + at);
+      sn = *reinterpret_cast<const f32x4 *>(a.sn + at);
     }
+    const Heads<T> os(a.out, a.ldo, row, s * a.hd + col, a.Hq, a.hd);
 #pragma unroll
     for (int j = 0; j < kHeads; ++j) {
       const int h = s + a.per_row * j;
       const bool isk = h >= a.Hq;
-      float g[8], t[8], ss = 0.f, tx = 0.f;
+      float g[8], ss = 0.f, tx = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         g[2 * i] = d[j][2 * i] * cs[i] + d[j][2 * i + 1] * sn[i];
@@ -195,29 +207,27 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd_kernel(Args<T> a,
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        t[e] = g[e] * (isk ? w[1][e] : w[0][e]);
         ss = fmaf(x[j][e], x[j][e], ss);
-        tx = fmaf(t[e], x[j][e], tx);
+        tx = fmaf(g[e] * (isk ? wk[e] : wq[e]), x[j][e], tx);
       }
-      ss = lanes_sum<LANES>(ss);
-      tx = lanes_sum<LANES>(tx);
-      const float inv = 1.0f / sqrtf(fmaf(ss, a.inv_hd, a.eps));
+      ss = lanes_sum<LANES>(lane ? ss : 0.f);
+      tx = lanes_sum<LANES>(lane ? tx : 0.f);
+      const float inv = rsqrtf(fmaf(ss, a.inv_hd, a.eps));
       const float m = tx * inv * a.inv_hd;  // mean(t xh)
       float o[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float xh = x[j][e] * inv;
-        o[e] = inv * (t[e] - xh * m);
+        o[e] = inv * (g[e] * (isk ? wk[e] : wq[e]) - xh * m);
         // A group without a position or past the last head adds nothing, whatever inv is.
         const float p = live && h < a.H ? g[e] * xh : 0.f;
         dw[0][e] += isk ? 0.f : p;
         dw[1][e] += isk ? p : 0.f;
       }
       if (lane && h < a.H) {
-        if (pos < 0)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = 0.f;
-        store8(head_at(a.out, a.ldo, row, h, a.Hq, a.hd) + 8 * c, o);
+        for (int e = 0; e < 8; ++e) o[e] = live ? o[e] : 0.f;
+        store8(os.at(isk, j * step), o);
       }
     }
   }
@@ -235,24 +245,27 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_bwd_kernel(Args<T> a,
   }
 }
 
-// d_w[v] (+)= the workgroups' sums, added in a fixed order: 32 columns a workgroup, 32
-// threads a column, whose loads are all in flight.
+// d_w[v] (+)= the workgroups' sums, added in a fixed order: kCols columns a workgroup, the
+// other threads of which share the rows of a column and have all their loads in flight.
+constexpr int kCols = 8;
 __global__ __launch_bounds__(1024) void qk_norm_dw_kernel(const float *__restrict__ part, int n,
                                                           int hd, float *d_wq, float *d_wk,
                                                           int beta) {
-  __shared__ float s[32][33];
-  const int col = threadIdx.x & 31, r = threadIdx.x >> 5, v = blockIdx.x * 32 + col;
+  constexpr int kParts = 1024 / kCols;
+  __shared__ float s[16][kCols];
+  const int col = threadIdx.x % kCols, r = threadIdx.x / kCols, v = blockIdx.x * kCols + col;
   float sum = 0.f;
-  if (v < 2 * hd) {
 #pragma unroll 8
-    for (int i = r; i < n; i += 32) sum += part[(size_t)i * 2 * hd + v];
-  }
-  s[r][col] = sum;
+  for (int i = r; i < n; i += kParts) sum += part[(size_t)i * 2 * hd + v];
+  // The 8 parts of a column that a wave holds, then the 16 waves'.
+#pragma unroll
+  for (int m = kCols; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
+  if ((threadIdx.x & 63) < kCols) s[threadIdx.x >> 6][col] = sum;
   __syncthreads();
-  if (r != 0 || v >= 2 * hd) return;
+  if (threadIdx.x >= kCols) return;
   sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) sum += s[i][col];
+  for (int i = 0; i < 16; ++i) sum += s[i][col];
   float *out = v < hd ? d_wq : d_wk;
   if (out == nullptr) return;  // a call without queries or without keys
   out += v < hd ? v : v - hd;
@@ -260,12 +273,16 @@ __global__ __launch_bounds__(1024) void qk_norm_dw_kernel(const float *__restric
 }
 
 // Workgroups of the backward: the sums of the weights' gradients end in one row of `part`
-// each.
+// each.  1024 are all resident (four a CU); 512 and 2048 take 36.9 and 38.4 us where these
+// take 35.9 (4 x 2048 rows, forward and backward, at two heads a group).
 constexpr size_t kBwdBlocks = 1024;
 int lanes_of(size_t hd) { return hd <= 32 ? 4 : hd <= 64 ? 8 : hd <= 128 ? 16 : 32; }
 size_t per_row_of(size_t heads) { return cdiv(heads, (size_t)kHeads); }
+size_t blocks_of(size_t rows, size_t heads, size_t hd) {
+  return cdiv(rows * per_row_of(heads), (size_t)(kThreads / lanes_of(hd)));
+}
 size_t bwd_blocks(size_t rows, size_t heads, size_t hd) {
-  const size_t blocks = cdiv(rows * per_row_of(heads), (size_t)(kThreads / lanes_of(hd)));
+  const size_t blocks = blocks_of(rows, heads, hd);
   return blocks < kBwdBlocks ? blocks : kBwdBlocks;
 }
 
@@ -333,13 +350,14 @@ Args<T> args_of(const Call &c) {
     a.d[i] = static_cast<const T *>(c.d[i]);
     a.out[i] = static_cast<T *>(c.out[i]);
     a.ldx[i] = c.ldx[i], a.ldd[i] = c.ldd[i], a.ldo[i] = c.ldo[i];
-    a.w[i] = c.w[i];
+    // A side without heads is never stored; its weights are loaded from the other's.
+    a.w[i] = c.heads[i] ? c.w[i] : c.w[1 - i];
   }
   a.cs = c.cs, a.sn = c.sn, a.positions = c.positions;
-  a.rows = (long long)c.rows, a.cache_rows = (long long)c.cache_rows;
-  a.pos_offset = (long long)c.pos_offset, a.seq_len = (long long)(c.positions ? 1 : c.seq_len);
+  a.rows = (uint32_t)c.rows, a.cache_rows = (uint32_t)c.cache_rows;
+  a.pos_offset = (uint32_t)c.pos_offset, a.seq_len = (uint32_t)(c.positions ? 1 : c.seq_len);
   a.Hq = (int)c.heads[0], a.H = (int)(c.heads[0] + c.heads[1]), a.hd = (int)c.hd;
-  a.per_row = (int)per_row_of(c.heads[0] + c.heads[1]);
+  a.per_row = (uint32_t)per_row_of(c.heads[0] + c.heads[1]);
   a.inv_hd = 1.0f / (float)c.hd, a.eps = c.eps;
   return a;
 }
@@ -347,23 +365,24 @@ Args<T> args_of(const Call &c) {
 template <typename T>
 void launch_forward(const Call &c, hipStream_t s) {
   const int lanes = lanes_of(c.hd);
-  const size_t units = c.rows * per_row_of(c.heads[0] + c.heads[1]);
-  const size_t blocks = cdiv(units, (size_t)(kThreads / lanes));
+  const size_t blocks = blocks_of(c.rows, c.heads[0] + c.heads[1], c.hd);
   const dim3 grid((unsigned)(blocks < (1u << 20) ? blocks : 1u << 20));
   auto kern = lanes == 4    ? qk_norm_rope_kernel<T, 4>
               : lanes == 8  ? qk_norm_rope_kernel<T, 8>
               : lanes == 16 ? qk_norm_rope_kernel<T, 16>
                             : qk_norm_rope_kernel<T, 32>;
-  hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, s, args_of<T>(c));
+  hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, s, args_of<T>(c),
+                     (uint64_t)blocks);
 }
 template <typename T>
-void launch_backward(const Call &c, size_t blocks, float *part, hipStream_t s) {
+void launch_backward(const Call &c, size_t grid, float *part, hipStream_t s) {
   const int lanes = lanes_of(c.hd);
   auto kern = lanes == 4    ? qk_norm_rope_bwd_kernel<T, 4>
               : lanes == 8  ? qk_norm_rope_bwd_kernel<T, 8>
               : lanes == 16 ? qk_norm_rope_bwd_kernel<T, 16>
                             : qk_norm_rope_bwd_kernel<T, 32>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(kThreads), 0, s, args_of<T>(c), part);
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(kThreads), 0, s, args_of<T>(c),
+                     (uint64_t)blocks_of(c.rows, c.heads[0] + c.heads[1], c.hd), part);
 }
 
 }  // namespace
@@ -467,7 +486,7 @@ extern "C" int prichs_qk_norm_rope_backward(
       launch_backward<float>(c, blocks, part, s);
     PRICHS_LAUNCH_CHECK("qk_norm_rope_backward launch");
   }
-  hipLaunchKernelGGL(qk_norm_dw_kernel, dim3((unsigned)cdiv(2 * head_dim, 32)), dim3(1024), 0, s,
+  hipLaunchKernelGGL(qk_norm_dw_kernel, dim3((unsigned)(2 * head_dim / kCols)), dim3(1024), 0, s,
                      part, (int)blocks, (int)head_dim, n_heads ? d_wq : nullptr,
                      n_kv_heads ? d_wk : nullptr, beta);
   PRICHS_LAUNCH_CHECK("qk_norm_rope_backward weights launch");

@@ -96,7 +96,7 @@ def test_rotation_takes_the_lanes_that_a_head_needs():
         fwd, bwd, dw = got
         assert fwd.kernel == f"qk_norm_rope_kernel<{t}, {lanes}>"
         assert bwd.kernel == f"qk_norm_rope_bwd_kernel<{t}, {lanes}>"
-        assert dw.kernel == "qk_norm_dw_kernel" and dw.grid[0] == -(-2 * d // 32)
+        assert dw.kernel == "qk_norm_dw_kernel" and dw.grid[0] == 2 * d // 8
         assert bwd.grid[0] <= 1024
         names |= {fwd.kernel, bwd.kernel}
     assert len(names) == 16
