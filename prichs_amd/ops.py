@@ -662,43 +662,48 @@ def kv_cache_copy(dst, src, to, from_, n_kv_heads, stream=None):
 
 # ------------------------------------- norms of queries and keys, rotated ----
 def _qk(q, k, n_heads, n_kv_heads, head_dim, names):
-    """Rows, row strides and dtype of a pair of operands, either of which is None where
-    it has no heads."""
-    lds, rows, dtype = [0, 0], None, None
-    for i, (t, h, name) in enumerate(((q, n_heads, names[0]), (k, n_kv_heads, names[1]))):
-        if h == 0:
-            continue
-        if t is None:
-            raise ValueError(f"{name}: missing")
-        if rows is None:
-            rows, dtype = t.shape[0], t.dtype
-        elif t.dtype != dtype:
-            raise TypeError(f"{names[0]} and {names[1]} have different dtypes")
-        elif t.shape[0] != rows:
-            raise ValueError(f"{names[0]} and {names[1]} have different numbers of rows")
-        lds[i] = _rows(t, name, rows, h * head_dim, _FLOATS)
-    if rows is None:
-        raise ValueError("no heads at all")
-    return rows, lds, dtype
+    """(rows, row strides of q and k, dtype) of a pair of operands, either of which is None
+    where it has no heads."""
+    first = q if n_heads else k
+    if first is None or n_heads and q is None or n_kv_heads and k is None:
+        raise ValueError(f"{names[0]}, {names[1]}: missing, or no heads at all")
+    rows, dtype = first.shape[0], first.dtype
+    ldq = _rows(q, names[0], rows, n_heads * head_dim, _FLOATS) if n_heads else 0
+    if not n_kv_heads:
+        return rows, ldq, 0, dtype
+    ldk = _rows(k, names[1], rows, n_kv_heads * head_dim, _FLOATS)
+    if k.dtype != dtype:
+        raise TypeError(f"{names[0]} and {names[1]} have different dtypes")
+    if k.shape[0] != rows:
+        raise ValueError(f"{names[0]} and {names[1]} have different numbers of rows")
+    return rows, ldq, ldk, dtype
 
 
 def _f32(t, name, n):
-    if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != n:
+    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{name}: expected contiguous f32 of {n} elements")
 
 
-def _norm_rope_args(w_q, w_k, cos, sin, n_heads, n_kv_heads, head_dim, positions, seq_len, rows):
+def _norm_rope_args(w_q, w_k, cos, sin, n_heads, n_kv_heads, head_dim, positions, seq_len,
+                    pos_offset, rows):
+    """Checks them and returns (positions of the tables, seq_len)."""
     if n_heads:
         _f32(w_q, "w_q", head_dim)
     if n_kv_heads:
         _f32(w_k, "w_k", head_dim)
-    if cos.dim() != 2 or cos.shape[1] * 2 != head_dim:
+    shape = cos.shape
+    if len(shape) != 2 or shape[1] * 2 != head_dim:
         raise ValueError("cos, sin: expected f32 [positions, head_dim / 2]")
-    for t, name in ((cos, "cos"), (sin, "sin")):
-        _f32(t, name, cos.shape[0] * cos.shape[1])
+    n = shape[0] * shape[1]
+    _f32(cos, "cos", n)
+    _f32(sin, "sin", n)
     if positions is not None:
         _i32(positions, "positions", rows)
-    return rows if seq_len is None else seq_len
+    if seq_len is None:
+        seq_len = rows
+    if pos_offset < 0 or seq_len < 0:
+        raise ValueError("seq_len and pos_offset must not be negative")
+    return shape[0], seq_len if rows else 1
 
 
 def qk_norm_rope(q, k, w_q, w_k, cos, sin, n_heads, n_kv_heads, head_dim=128, eps=1e-5,
@@ -708,28 +713,32 @@ def qk_norm_rope(q, k, w_q, w_k, cos, sin, n_heads, n_kv_heads, head_dim=128, ep
     (int32 device [rows]), or r % seq_len + pos_offset (seq_len None: the rows are one
     sequence).  cos, sin: f32 [positions, head_dim / 2].  q_out / k_out may be q / k.  With
     n_heads or n_kv_heads 0 that operand is None.  -> (q_out, k_out)."""
-    rows, ld, dtype = _qk(q, k, n_heads, n_kv_heads, head_dim, ("q", "k"))
-    seq_len = _norm_rope_args(w_q, w_k, cos, sin, n_heads, n_kv_heads, head_dim, positions,
-                              seq_len, rows)
-    if pos_offset < 0 or seq_len < 0:
-        raise ValueError("seq_len and pos_offset must not be negative")
+    rows, ldq, ldk, dtype = _qk(q, k, n_heads, n_kv_heads, head_dim, ("q", "k"))
+    n_pos, seq_len = _norm_rope_args(w_q, w_k, cos, sin, n_heads, n_kv_heads, head_dim, positions,
+                                     seq_len, pos_offset, rows)
     if not n_heads:
         q = w_q = q_out = None
     if not n_kv_heads:
         k = w_k = k_out = None
     ctx, s = _launch_on(stream, cos, q, k, w_q, w_k, sin, positions, q_out, k_out)
     with ctx:
-        if q_out is None and n_heads:
-            q_out = q.new_empty((rows, n_heads * head_dim))
-        if k_out is None and n_kv_heads:
-            k_out = k.new_empty((rows, n_kv_heads * head_dim))
-        r2, ldo, d2 = _qk(q_out, k_out, n_heads, n_kv_heads, head_dim, ("q_out", "k_out"))
-        if r2 != rows or d2 != dtype:
-            raise ValueError("q_out, k_out: expected the rows and the dtype of q and k")
+        ldqo, ldko = n_heads * head_dim, n_kv_heads * head_dim
+        if q_out is None and k_out is None:  # of q's and k's rows and dtype, without gaps
+            q_out = q.new_empty((rows, ldqo)) if n_heads else None
+            k_out = k.new_empty((rows, ldko)) if n_kv_heads else None
+        else:
+            if q_out is None and n_heads:
+                q_out = q.new_empty((rows, ldqo))
+            if k_out is None and n_kv_heads:
+                k_out = k.new_empty((rows, ldko))
+            r2, ldqo, ldko, d2 = _qk(q_out, k_out, n_heads, n_kv_heads, head_dim,
+                                     ("q_out", "k_out"))
+            if r2 != rows or d2 != dtype:
+                raise ValueError("q_out, k_out: expected the rows and the dtype of q and k")
         L.check(L.load().prichs_qk_norm_rope_forward(
-            _a(q), ld[0], _a(k), ld[1], _a(w_q), _a(w_k), cos.data_ptr(), sin.data_ptr(),
-            cos.shape[0], _a(positions), seq_len if rows else 1, pos_offset, _a(q_out), ldo[0],
-            _a(k_out), ldo[1], rows, n_heads, n_kv_heads, head_dim, eps, _TORCH_DTYPES[dtype], s))
+            _a(q), ldq, _a(k), ldk, _a(w_q), _a(w_k), cos.data_ptr(), sin.data_ptr(), n_pos,
+            _a(positions), seq_len, pos_offset, _a(q_out), ldqo, _a(k_out), ldko, rows, n_heads,
+            n_kv_heads, head_dim, eps, _TORCH_DTYPES[dtype], s))
     return q_out, k_out
 
 
@@ -740,14 +749,13 @@ def qk_norm_rope_backward(d_q_out, d_k_out, q, k, w_q, w_k, cos, sin, n_heads, n
     d_k may be d_q_out / d_k_out) and, in f32, of the weights (added to d_wq and d_wk with
     accumulate)."""
     lib = L.load()
-    rows, ld, dtype = _qk(q, k, n_heads, n_kv_heads, head_dim, ("q", "k"))
-    r2, ldd, d2 = _qk(d_q_out, d_k_out, n_heads, n_kv_heads, head_dim, ("d_q_out", "d_k_out"))
+    rows, ldq, ldk, dtype = _qk(q, k, n_heads, n_kv_heads, head_dim, ("q", "k"))
+    r2, lddqo, lddko, d2 = _qk(d_q_out, d_k_out, n_heads, n_kv_heads, head_dim,
+                               ("d_q_out", "d_k_out"))
     if r2 != rows or d2 != dtype:
         raise ValueError("d_q_out, d_k_out: expected the rows and the dtype of q and k")
-    seq_len = _norm_rope_args(w_q, w_k, cos, sin, n_heads, n_kv_heads, head_dim, positions,
-                              seq_len, rows)
-    if pos_offset < 0 or seq_len < 0:
-        raise ValueError("seq_len and pos_offset must not be negative")
+    n_pos, seq_len = _norm_rope_args(w_q, w_k, cos, sin, n_heads, n_kv_heads, head_dim, positions,
+                                     seq_len, pos_offset, rows)
     if not n_heads:
         q = w_q = d_q_out = d_q = d_wq = None
     if not n_kv_heads:
@@ -757,22 +765,29 @@ def qk_norm_rope_backward(d_q_out, d_k_out, q, k, w_q, w_k, cos, sin, n_heads, n
     ctx, s = _launch_on(stream, cos, d_q_out, d_k_out, q, k, w_q, w_k, sin, positions, d_q, d_k,
                         d_wq, d_wk)
     with ctx:
+        lddq, lddk = n_heads * head_dim, n_kv_heads * head_dim
+        given = d_q is not None or d_k is not None
         if n_heads:
-            d_q = q.new_empty((rows, n_heads * head_dim)) if d_q is None else d_q
-            d_wq = w_q.new_empty(head_dim) if d_wq is None else d_wq
-            _f32(d_wq, "d_wq", head_dim)
+            d_q = q.new_empty((rows, lddq)) if d_q is None else d_q
+            if d_wq is None:
+                d_wq = w_q.new_empty(head_dim)
+            else:
+                _f32(d_wq, "d_wq", head_dim)
         if n_kv_heads:
-            d_k = k.new_empty((rows, n_kv_heads * head_dim)) if d_k is None else d_k
-            d_wk = w_k.new_empty(head_dim) if d_wk is None else d_wk
-            _f32(d_wk, "d_wk", head_dim)
-        r2, ldo, d2 = _qk(d_q, d_k, n_heads, n_kv_heads, head_dim, ("d_q", "d_k"))
-        if r2 != rows or d2 != dtype:
-            raise ValueError("d_q, d_k: expected the rows and the dtype of q and k")
+            d_k = k.new_empty((rows, lddk)) if d_k is None else d_k
+            if d_wk is None:
+                d_wk = w_k.new_empty(head_dim)
+            else:
+                _f32(d_wk, "d_wk", head_dim)
+        if given:
+            r2, lddq, lddk, d2 = _qk(d_q, d_k, n_heads, n_kv_heads, head_dim, ("d_q", "d_k"))
+            if r2 != rows or d2 != dtype:
+                raise ValueError("d_q, d_k: expected the rows and the dtype of q and k")
         need = lib.prichs_qk_norm_rope_backward_workspace(rows, n_heads, n_kv_heads, head_dim)
         ws = cos.new_empty((need + 3) // 4)
         L.check(lib.prichs_qk_norm_rope_backward(
-            _a(d_q_out), ldd[0], _a(d_k_out), ldd[1], _a(q), ld[0], _a(k), ld[1], _a(w_q), _a(w_k),
-            cos.data_ptr(), sin.data_ptr(), cos.shape[0], _a(positions), seq_len if rows else 1,
-            pos_offset, _a(d_q), ldo[0], _a(d_k), ldo[1], _a(d_wq), _a(d_wk), int(accumulate), rows,
-            n_heads, n_kv_heads, head_dim, eps, _TORCH_DTYPES[dtype], ws.data_ptr(), need, s))
+            _a(d_q_out), lddqo, _a(d_k_out), lddko, _a(q), ldq, _a(k), ldk, _a(w_q), _a(w_k),
+            cos.data_ptr(), sin.data_ptr(), n_pos, _a(positions), seq_len, pos_offset, _a(d_q),
+            lddq, _a(d_k), lddk, _a(d_wq), _a(d_wk), int(accumulate), rows, n_heads, n_kv_heads,
+            head_dim, eps, _TORCH_DTYPES[dtype], ws.data_ptr(), need, s))
     return d_q, d_k, d_wq, d_wk

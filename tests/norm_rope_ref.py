@@ -46,8 +46,9 @@ def norm_rope(x, w, cos, sin, eps, dtype, d=None):
     # t is off by 4 roundings of its terms, the mean by 14 more and inv's 10 twice; the
     # difference and the product with inv by 3 and inv's 10.
     e_dx = inv * F * (20 * mag * np.abs(w) + 64 * np.abs(xh) * mag_m) + u * np.abs(dx)
-    # A lane adds up what its rows and 4 heads give, at most 1024 workgroups of 8 groups or
-    # more share the rows; then 16 to 64 groups and 1024 / 32 + 32 sums.
+    # A lane adds up what its rows and heads (at most 4 of a row) give, at most 1024
+    # workgroups of 8 groups or more share the rows; then 8 to 64 groups, and the workgroups'
+    # sums by way of a thread's 8, 3 exchanges and 16 waves.
     chain = 4 * -(-rows * x.shape[1] // (4 * 1024 * 8)) + 64 + 64 + 20
     dw, mag_w = (g * xh).sum((0, 1)), (mag * np.abs(xh)).sum((0, 1))
     r.update(dx=flat(dx), e_dx=flat(e_dx * (1 + u)), dw=dw, e_dw=chain * F * mag_w)
