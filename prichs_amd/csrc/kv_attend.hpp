@@ -19,15 +19,13 @@
 // row maximum, and a page is read once per row tile: 8704 bytes against 32 KB in
 // bf16.  Bound by HBM where the caches are long (MI355X, 12 + 3 heads, 64 sequences
 // of 16384 positions: 428 MB, more than the last-level cache holds, in 89 us, 4.8
-// TB/s; 32 sequences, which it does hold, 41 us), by the latency of a page (about 2
-// us from its table entry to its last product) where they are short (one token over
-// 8192 positions: 8.6 us, 3.3 MB).  Some 80 scalar registers are spilled to lanes of
-// vector registers (none to memory), and about 80 of a page's 650 instructions move
-// them.  Three workgroups a CU hide each other's loads: a
-// second set of registers for a wave's next page cost the third and was no faster
-// (32 x 3000 positions 15.2 -> 16.1 us).  Tiles of 32 rows share the conversions of
-// two row blocks but leave half the waves (8 x 8 queries over 4096: 15.7 us against
-// 14.7; 1 x 8: 10.9 against 8.7; only 32 x 6 over 2000 gains, 18.9 to 17.6).
+// TB/s; 32 sequences, which it does hold, 41 us), by the latency of a page where they
+// are short (one token over 8192 positions: 8.2 us, 3.3 MB).  K and V of a wave's next
+// page take the registers of this one's as soon as its products are formed (32 x 6000
+// windowed 17.5 -> 16 us, 2 x 256 over 4352 26 -> 24, with what follows); a second set of
+// registers cost the third workgroup a CU and was no faster.  Masks are bit fields: as
+// comparisons their results took so many scalar registers that some 80 others were held
+// in lanes of vector registers, which 80 of a page's 650 instructions moved.
 //
 // The visible pages of a tile are dealt evenly to the waves of n_split workgroups in
 // contiguous runs; the waves of a workgroup join in LDS, workgroups through the
@@ -105,8 +103,14 @@ struct Groups {
   int n, batch;
   int tiles_p, split_p, split_s;  // tiles over shared pages at most, of one kv head
 };
+// Workgroups over shared pages: an equal number on each of the eight dies, on which
+// workgroup `id` runs by id % 8, so that tiles that read the same pages (of one kv head and
+// split) do so through one L2.
+__host__ __device__ __forceinline__ int on_a_die(int kv_heads, const Groups &gr) {
+  return (kv_heads * gr.tiles_p * gr.split_p + 7) / 8;
+}
 __device__ __forceinline__ int shared_workgroups(const AttendShape &sh, const Groups &gr) {
-  return sh.Hkv * gr.tiles_p * gr.split_p;
+  return 8 * on_a_die(sh.Hkv, gr);
 }
 
 // Whole pages that `positions` cover.
@@ -223,11 +227,11 @@ __device__ __forceinline__ void kv_attend(
   int lo = 0, hi = sh.max_pages, slot = 0;
   bool alone = false;  // no workgroup writes the slots for shared pages of these rows
   if constexpr (ROLE == kSharedRole) {
-    int id = blockIdx.x;
-    split = id % gr.split_p, id /= gr.split_p;
-    kvh = id / gr.tiles_p;
-    if (!shared_tile(gr, id - kvh * gr.tiles_p, kTileRows, seq_rows, sh.max_pages, &b, &rows, &hi,
-                     &tile))
+    const int id = (blockIdx.x & 7) * on_a_die(sh.Hkv, gr) + (blockIdx.x >> 3);
+    const int pages = id / gr.tiles_p;  // kv head and split
+    kvh = pages / gr.split_p, split = pages - kvh * gr.split_p;
+    if (kvh >= sh.Hkv || !shared_tile(gr, id - pages * gr.tiles_p, kTileRows, seq_rows,
+                                      sh.max_pages, &b, &rows, &hi, &tile))
       return;
     n_split = gr.split_p;
     slot = split;

@@ -5,6 +5,10 @@
 // exponentials over part p of the keys,
 //   o = sum_p exp(m_p - m) o_p / sum_p exp(m_p - m) l_p,  m = max_p m_p.
 // kv_attend.hpp has the tiles and the join.
+//
+// MI355X, 12 + 3 heads, us from Python (kernel and join): 8 sequences of one prompt of 1000
+// positions 15 (10 captured), 16 prompts of 2048 with 4 sequences each 15.5, 24 x 6 tokens
+// behind 8000 shared positions 25, 256 sequences behind 32768 80: 52 GFLOP, 650 TFLOP/s.
 #include "kv_attend.hpp"
 
 namespace prichs {
@@ -41,9 +45,13 @@ __global__ __launch_bounds__(256) void kv_shared_join_kernel(
 //   tiles of 32 rows, 512            12.3      13.6       24.6        37.2         91
 // (the second number: workgroups that the shared pages are dealt to).  24 x 8000 with six
 // tokens each 26.2, 24.7, 30.5; 128 x 16384 36.3, 34.5, 38.1; 200 x 16384 52, 48, 45.
-// Tiles of 48 and 64 rows have one wave a SIMD: 140 and 166 us at 256 x 32768.  A form that
-// converts each page once into LDS for 128 rows took 95 to 101 us there and 36 to 39 at 24 x
-// 8000: its waves wait for each other at every page.
+// Dealt by die (kv_attend.hpp) the last three are 24.5, 32.7 and 44.2.
+// What bounds a large call is the vector instructions of a page, some 460 for 32 rows (128
+// conversions, 64 permutes, the softmax), which two waves a SIMD issue 56% of the time.
+// Measured and not kept, at 256 x 32768: tiles of 48 and 64 rows, one wave a SIMD, 140 and
+// 166 us; each page converted once into LDS for 128 rows, whose waves wait for each other at
+// every page, 95 to 101 (and 36 to 39 at 24 x 8000); queries in LDS, which leaves registers
+// for a third wave, 98 to 109; own pages first 98; wave priorities, the same to 1%.
 struct Plan {
   int blocks;               // of 16 rows in a tile over shared pages
   size_t tiles_p, split_p;  // tiles over shared pages of a kv head at most, splits of each
@@ -121,7 +129,8 @@ extern "C" int prichs_kv_cache_shared_attention(
                  "%s: q, o and the cache must be 16-byte aligned", who);
   const Plan p = plan_of(batch, n_q, n_heads, n_kv_heads, max_pages, n_groups);
   // Workgroups of 256 threads, fewer than 2^32 in a launch.
-  const size_t wgs = n_kv_heads * (p.tiles_p * p.split_p + batch * p.tiles_s * p.split_s);
+  const size_t wgs = roundup(n_kv_heads * p.tiles_p * p.split_p, 8) +
+                     n_kv_heads * batch * p.tiles_s * p.split_s;
   PRICHS_REQUIRE(wgs < (size_t)1 << 24, "%s: shape too large", who);
   const size_t rows = batch * n_q * n_heads, need = workspace_of(p, rows);
   if (workspace_bytes < need)

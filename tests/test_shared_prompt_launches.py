@@ -35,7 +35,7 @@ def test_how_a_call_is_cut(case, blocks, tiles, split_p, split_s):
         own = b * k * -(-n * (h // k) // 16)
         flag = "true" if lse else "false"
         assert got[0].kernel == f"kv_shared_kernel<{blocks}, {flag}>"
-        assert got[0].grid == [k * tiles * split_p + own * split_s, 1, 1]
+        assert got[0].grid == [-(-k * tiles * split_p // 8) * 8 + own * split_s, 1, 1]
         parts = split_p + split_s
         wide = parts > 8
         assert got[1].kernel == f"kv_shared_join_kernel<{8 if wide else 1}, {flag}>"
