@@ -510,13 +510,18 @@ int prichs_kv_cache_shared_attention(const void *q, size_t ldq, const void *cach
 /* The pages of a cache, kept on the device: refs (device int32 [n_pages]) counts how many
  * table entries (and other holders: a caller may add its own) name each page, 0 for a
  * free one (a negative count is a free page too).  page_table: device int32 [batch]
- * [max_pages], entries outside [0, n_pages) name no page, -1 being written for none.  Free pages are taken lowest first, items in their
- * order, so results are those of the steps done one after the other.  Nothing is read on
- * the host.  shortfall (device int32 [1], may be NULL) gets the number of pages that a
- * call wanted and did not get; their entries are -1.  n_pages is at most 2^24, batch and
- * n 2^20, batch * max_pages 2^31 - 1.  workspace: device memory, 16-byte aligned, of
- * prichs_kv_pages_workspace bytes (for the call's n_pages, batch and n; n = 0 for
- * reserve, batch = n = 0 for compact), used by the call alone until it has finished.
+ * [max_pages]; entries outside [0, n_pages) name no page, -1 is written for none.  Free
+ * pages are taken lowest first, items in their order, so results are those of the items
+ * done one after the other.  Nothing is read on the host.  shortfall (device int32 [1],
+ * may be NULL) gets the number of pages that a call wanted and did not get; their entries
+ * are -1.  n_pages is at most 2^24, batch and n 2^20, batch * max_pages 2^31 - 1.
+ * workspace: device memory, 16-byte aligned, of prichs_kv_pages_workspace bytes (for the
+ * call's n_pages, batch and n; n = 0 for reserve, batch = n = 0 for compact), used by the
+ * call alone until it has finished.  Calls on the same refs, table or cache are ordered by
+ * the caller (one stream, or events): two at a time would take the same pages.  Nor is it
+ * checked that a page which a call writes keys into is held by one row: a row that was
+ * cut back inside a page that others hold is forked, which copies that page, and goes on
+ * as the child.
  *
  * reserve: every sequence gets pages for its positions lens[b] .. lens[b] + counts[b] - 1
  *   (lens, counts: device int32 [batch]) where the table names none yet; entries past

@@ -18,8 +18,8 @@
 // Nothing goes through LDS before the waves join, there is no lane exchange but the
 // row maximum, and a page is read once per row tile: 8704 bytes against 32 KB in
 // bf16.  Bound by HBM where the caches are long (MI355X, 12 + 3 heads, 64 sequences
-// of 16384 positions: 428 MB, more than the last-level cache holds, in 89 us, 4.8
-// TB/s; 32 sequences, which it does hold, 41 us), by the latency of a page where they
+// of 16384 positions: 428 MB, more than the last-level cache holds, in 87 us, 4.9
+// TB/s; 32 sequences, which it does hold, 40 us), by the latency of a page where they
 // are short (one token over 8192 positions: 8.2 us, 3.3 MB).  K and V of a wave's next
 // page take the registers of this one's as soon as its products are formed (32 x 6000
 // windowed 17.5 -> 16 us, 2 x 256 over 4352 26 -> 24, with what follows); a second set of

@@ -15,8 +15,8 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 3 : 2) void kv_attend_ke
   __shared__ JoinLds<kWaves> s;
   kv_attend<kWaves, false>(q, ldq, cache, table, lens, o, ldo, lse, part_o, part_ml, sh, s, Groups{});
 }
-// With lse: 10 registers more, and 0.2 to 1 us a call (one token over 8192 positions 8.6 ->
-// 9.1 us, 32 x 3000 16.1 -> 16.6, 8 x 5 over 4096 14.7 -> 15.3, 2 x 256 over 4352 35.9 -> 36.9).
+// With lse: up to 0.8 us a call (one token over 8192 positions 8.2 -> 8.8 us, 32 x 3000 15.5
+// -> 15.9, 8 x 5 over 4096 13.8 -> 14.6, 2 x 256 over 4352 34.6 -> 35.1).
 template <int kWaves>
 __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 3 : 2) void kv_attend_lse_kernel(
     const bf16_t *__restrict__ q, size_t ldq, const uint8_t *__restrict__ cache,
@@ -42,9 +42,10 @@ __global__ __launch_bounds__(256) void kv_join_lse_kernel(
 
 // Pages up to which one workgroup of 8 waves takes a tile without a second kernel:
 // a page costs a wave some 2 us, the second kernel 2.5 on the device and 4 on the
-// host.  One token over 8 pages 7.4 -> 6.1 us (graph), over 16 pages 7.4 -> 8.2
-// (called from Python 15.2 -> 11), 32 and 80 sequences over 16 pages 9.2 -> 8.4 and
-// 14.6 -> 10.6, 32 over 32 pages 11.1 -> 13.3.
+// host.  Captured, us (from Python in brackets), one kernel and two: one token over 8
+// pages 6.5, 7.3 (9.6, 13.3), over 16 pages 8.1, 7.5 (9.6, 13.4), over 32 pages 11.2, 7.7
+// (10.6, 13.5); 32 and 80 sequences over 16 pages 8.5, 9.3 and 9.6, 13.8, over 32 pages
+// 12.2, 11.1 and 15.6, 19.9.
 constexpr size_t kShortPages = 16;
 
 // How a call is cut: n_split workgroups of `waves` waves over a tile's pages.  For 256

@@ -2,13 +2,15 @@
 // sequences, moved together.  prichs_hip.h has what each call does; kv_cache.hpp the
 // page's layout, which nothing here looks into.
 //
-// Free pages are taken lowest first, so every result is that of the steps done one after
-// the other, whatever runs at the same time.  Counts and tables are some bytes a page:
+// Free pages are taken lowest first, so every result is that of the items done one after
+// the other, in whatever order workgroups run.  Counts and tables are some bytes a page:
 // launches and round trips to memory are the cost, until data is copied, which runs at the
 // rate of the memory.  Up to kSmallPages pages and kSmallRows rows one workgroup of 1024
 // threads finds the free pages (16 of them a thread in one round trip) and ranks them in one
 // launch; beyond, workgroups count them in blocks of kBlockPages and a second launch ranks
-// them behind the blocks before.
+// them behind the blocks before.  MI355X: the kernels that plan and write tables take 3 to
+// 9 us each; fork_apply 4.4 us for 7 items and 6.0 for 224; compact_apply 39 us where 3661
+// pages of three heads move (191 MB read and written, 4.9 TB/s).
 #include "kv_cache.hpp"
 
 #include <climits>
@@ -33,8 +35,14 @@ struct Chunks {
 };
 constexpr size_t kMaxPages = (size_t)1 << 24, kMaxRows = (size_t)1 << 20;
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
-constexpr int kRound = kPlanThreads * kSteps;       // pages that a workgroup has in registers
-constexpr size_t kSmallPages = 4 * kRound, kSmallRows = 4 * kPlanThreads;
+// What one workgroup plans for: the pages that it has in registers.  A call in a captured
+// graph, us, one workgroup and many, none of the pages free (the longest scan), 32 rows:
+//                     reserve      fork, 16 items   compact, nothing moves
+//      1024 pages    6.4, 11.3      8.5,  9.4           6.9, 8.3
+//     16384          6.5, 11.3      8.4,  9.4           7.9, 9.0
+//     65536         15.0, 11.0     17.0,  9.8          26.0, 9.3 (one workgroup: four rounds)
+//     16384 pages, 1024 rows: 7.8, 12.1 and 13.8, 17.6; 4096: 15.9, 18.6 and 33.8, 45.1.
+constexpr size_t kSmallPages = kPlanThreads * kSteps, kSmallRows = 4 * kPlanThreads;
 
 // The workspace, in int32: block counts; what the first page list holds; then by call.
 struct Work {
@@ -158,6 +166,50 @@ __device__ __forceinline__ bool entries_of(const int32_t *lens, const int32_t *c
 __device__ __forceinline__ bool names(int p, int n_pages) { return p >= 0 && p < n_pages; }
 
 // ------------------------------------------------------------------ reserve --
+// Entries of a lane that are in flight at a time: a row may want thousands.  One row of 2048
+// entries 14 us, of 8192 35; one entry after the other took a thread 418 and 1631.
+constexpr int kEntrySteps = 8;
+// One wave: how many of a row's entries e0 .. e1 - 1 name no page.
+__device__ __forceinline__ int row_wants(const int32_t *row, int e0, int e1, int n_pages) {
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+  for (int e = e0; e < e1; e += 64 * kEntrySteps) {
+    int32_t v[kEntrySteps];
+#pragma unroll
+    for (int i = 0; i < kEntrySteps; ++i) v[i] = row[min(e + 64 * i + lane, e1 - 1)];
+#pragma unroll
+    for (int i = 0; i < kEntrySteps; ++i)
+      n += e + 64 * i + lane < e1 && !names(v[i], n_pages);
+  }
+  return wave_sum(n);
+}
+// One wave: those entries take the free pages from rank `at`, -1 where there are no more.
+__device__ __forceinline__ void row_takes(int32_t *row, int e0, int e1, int at, int n_free,
+                                          const int32_t *free_of, int32_t *refs, int n_pages) {
+  const int lane = threadIdx.x & 63;
+  for (int e = e0; e < e1; e += 64 * kEntrySteps) {
+    int32_t v[kEntrySteps];
+    int k[kEntrySteps];
+#pragma unroll
+    for (int i = 0; i < kEntrySteps; ++i) v[i] = row[min(e + 64 * i + lane, e1 - 1)];
+#pragma unroll
+    for (int i = 0; i < kEntrySteps; ++i) {
+      const bool want = e + 64 * i + lane < e1 && !names(v[i], n_pages);
+      const uint64_t mask = __ballot(want);
+      k[i] = want ? at + __popcll(mask & ((1ull << lane) - 1)) : -1;
+      at += __popcll(mask);
+    }
+#pragma unroll
+    for (int i = 0; i < kEntrySteps; ++i)
+      v[i] = k[i] >= 0 && k[i] < n_free ? free_of[k[i]] : -1;
+#pragma unroll
+    for (int i = 0; i < kEntrySteps; ++i) {
+      if (k[i] < 0) continue;
+      row[e + 64 * i + lane] = v[i];
+      if (v[i] >= 0) refs[v[i]] = 1;
+    }
+  }
+}
 // Workgroups past the blocks of pages: a wave counts what a row of the table wants.
 __global__ __launch_bounds__(kThreads) void reserve_count_kernel(
     const int32_t *refs, int n_pages, int blocks, const int32_t *table, int max_pages,
@@ -171,9 +223,7 @@ __global__ __launch_bounds__(kThreads) void reserve_count_kernel(
   int e0, e1, n = 0;
   long long beyond;
   if (entries_of(lens, counts, b, max_pages, &e0, &e1, &beyond))
-    for (int e = e0 + lane; e < e1; e += 64)
-      n += !names(table[(size_t)b * max_pages + e], n_pages);
-  n = wave_sum(n);
+    n = row_wants(table + (size_t)b * max_pages, e0, e1, n_pages);
   if (lane == 0) w.a[b] = n;
 }
 
@@ -188,26 +238,24 @@ __device__ __forceinline__ void list_wave(const uint64_t (&mask)[kSteps], int p0
     rank += __popcll(mask[i]);
   }
 }
-// One workgroup of kPlanThreads: the lowest `want` free pages into free_of (all threads
-// return how many it found, those of the last round included).
+// One workgroup of kPlanThreads, at most kSmallPages: the lowest `want` free pages into
+// free_of; returns how many are free.
 __device__ __forceinline__ int list_free(const int32_t *refs, int n_pages, int want,
                                          int32_t *free_of, int *s) {
-  const int wave = threadIdx.x >> 6;
-  int found = 0;
-  for (int r0 = 0; r0 < n_pages && found < want; r0 += kRound) {
-    uint64_t mask[kSteps];
-    const int p0 = r0 + wave * 64 * kSteps, n = free_masks(refs, n_pages, p0, mask);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) s[wave] = n;
-    __syncthreads();
-    int rank = found;
+  if (n_pages == 0 || want == 0) return 0;
+  const int wave = threadIdx.x >> 6, p0 = wave * 64 * kSteps;
+  uint64_t mask[kSteps];
+  const int n = free_masks(refs, n_pages, p0, mask);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s[wave] = n;
+  __syncthreads();
+  int rank = 0, found = 0;
 #pragma unroll
-    for (int v = 0; v < kPlanWaves; ++v) {
-      rank += v < wave ? s[v] : 0;
-      found += s[v];
-    }
-    list_wave(mask, p0, rank, want, free_of);
+  for (int v = 0; v < kPlanWaves; ++v) {
+    rank += v < wave ? s[v] : 0;
+    found += s[v];
   }
+  list_wave(mask, p0, rank, want, free_of);
   return found;
 }
 // Ranks the free pages of its block.
@@ -282,48 +330,57 @@ __global__ __launch_bounds__(kThreads) void reserve_list_kernel(
 __global__ __launch_bounds__(kThreads) void reserve_apply_kernel(
     int32_t *refs, int n_pages, int32_t *table, int max_pages, const int32_t *lens,
     const int32_t *counts, int batch, Work w) {
-  const int b = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int b = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (b >= batch || w.a[b] == 0) return;
   int e0, e1;
   long long beyond;
   if (!entries_of(lens, counts, b, max_pages, &e0, &e1, &beyond)) return;
-  const int n_free = w.head[0];
-  int at = w.b[b];
-  for (int e = e0; e < e1; e += 64) {
-    int32_t *entry = table + (size_t)b * max_pages + e + lane;
-    const bool want = e + lane < e1 && !names(*entry, n_pages);
-    const uint64_t mask = __ballot(want);
-    if (want) {
-      const int k = at + __popcll(mask & ((1ull << lane) - 1));
-      const int p = k < n_free ? w.free_of[k] : -1;
-      *entry = p;
-      if (p >= 0) refs[p] = 1;
-    }
-    at += __popcll(mask);
-  }
+  row_takes(table + (size_t)b * max_pages, e0, e1, w.b[b], w.head[0], w.free_of, refs, n_pages);
 }
 
-// All of it in one workgroup, a thread for each row.
+// All of it in one workgroup: a thread for each row, a wave for one of more than kShortRow
+// entries.
+constexpr int kShortRow = 4;
 __global__ __launch_bounds__(kPlanThreads) void reserve_small_kernel(
     int32_t *refs, int n_pages, int32_t *table, int max_pages, const int32_t *lens,
     const int32_t *counts, int batch, int32_t *shortfall, Work w) {
-  __shared__ int s[kPlanWaves];
+  // Of each row what it wants, then the rank of its first page; the rows with many entries.
+  __shared__ int s[kPlanWaves], s_row[kSmallRows], s_long[kSmallRows], n_long;
   __shared__ unsigned long long s_beyond;
-  if (threadIdx.x == 0) s_beyond = 0;
+  const int wave = threadIdx.x >> 6;
+  if (threadIdx.x == 0) {
+    s_beyond = 0;
+    n_long = 0;
+  }
+  __syncthreads();
+  int e0, e1;
+  long long beyond;
+  for (int b = threadIdx.x; b < batch; b += kPlanThreads) {
+    int n = 0;
+    if (entries_of(lens, counts, b, max_pages, &e0, &e1, &beyond)) {
+      if (beyond) atomicAdd(&s_beyond, (unsigned long long)beyond);
+      if (e1 - e0 > kShortRow) {
+        s_long[atomicAdd(&n_long, 1)] = b;  // in any order: each is counted by itself
+      } else {
+        for (int e = e0; e < e1; ++e) n += !names(table[(size_t)b * max_pages + e], n_pages);
+      }
+    }
+    s_row[b] = n;
+  }
+  __syncthreads();
+  for (int i = wave; i < n_long; i += kPlanWaves) {
+    const int b = s_long[i];
+    (void)entries_of(lens, counts, b, max_pages, &e0, &e1, &beyond);
+    const int n = row_wants(table + (size_t)b * max_pages, e0, e1, n_pages);
+    if ((threadIdx.x & 63) == 0) s_row[b] = n;
+  }
   __syncthreads();
   int base = 0;
   for (int b0 = 0; b0 < batch; b0 += kPlanThreads) {
-    const int b = b0 + threadIdx.x;
-    int e0 = 0, e1 = 0, n = 0;
-    long long beyond = 0;
-    if (b < batch && entries_of(lens, counts, b, max_pages, &e0, &e1, &beyond)) {
-#pragma unroll 8
-      for (int e = e0; e < e1; ++e) n += !names(table[(size_t)b * max_pages + e], n_pages);
-      if (beyond) atomicAdd(&s_beyond, (unsigned long long)beyond);
-    }
+    const int b = b0 + threadIdx.x, n = b < batch ? s_row[b] : 0;
     int all;
     const int at = base + block_before<kPlanWaves>(n, s, &all);
-    if (b < batch) w.b[b] = n ? at : -1;  // read by the same thread
+    if (b < batch) s_row[b] = at;
     base += all;
   }
   const int found = list_free(refs, n_pages, base, w.free_of, s);
@@ -332,10 +389,15 @@ __global__ __launch_bounds__(kPlanThreads) void reserve_small_kernel(
     const long long missing = (long long)s_beyond + (base > found ? base - found : 0);
     *shortfall = (int32_t)min(missing, (long long)INT_MAX);
   }
+  for (int i = wave; i < n_long; i += kPlanWaves) {
+    const int b = s_long[i];
+    (void)entries_of(lens, counts, b, max_pages, &e0, &e1, &beyond);
+    row_takes(table + (size_t)b * max_pages, e0, e1, s_row[b], found, w.free_of, refs, n_pages);
+  }
   for (int b = threadIdx.x; b < batch; b += kPlanThreads) {
-    int at = w.b[b], e0, e1;
-    long long beyond;
-    if (at < 0 || !entries_of(lens, counts, b, max_pages, &e0, &e1, &beyond)) continue;
+    if (!entries_of(lens, counts, b, max_pages, &e0, &e1, &beyond) || e1 - e0 > kShortRow)
+      continue;
+    int at = s_row[b];
     for (int e = e0; e < e1; ++e) {
       int32_t *entry = table + (size_t)b * max_pages + e;
       if (names(*entry, n_pages)) continue;
@@ -550,41 +612,23 @@ __global__ __launch_bounds__(kPlanThreads) void compact_small_kernel(const int32
                                                                      int n_pages,
                                                                      int32_t *n_live, Work w) {
   __shared__ int s[kPlanWaves];
-  const int wave = threadIdx.x >> 6;
+  const int wave = threadIdx.x >> 6, p0 = wave * 64 * kSteps;
   uint64_t mask[kSteps];
-  int n = 0, all = 0;
-  for (int r0 = 0; r0 < n_pages; r0 += kRound) {
-    const int m = free_masks(refs, n_pages, r0 + wave * 64 * kSteps, mask);
-    n += (threadIdx.x & 63) == 0 ? m : 0;
+  const int n = n_pages == 0 ? 0 : free_masks(refs, n_pages, p0, mask);
+  if ((threadIdx.x & 63) == 0) s[wave] = n;
+  __syncthreads();
+  int rank = 0, all = 0;
+#pragma unroll
+  for (int v = 0; v < kPlanWaves; ++v) {
+    rank += v < wave ? s[v] : 0;
+    all += s[v];
   }
-  all = block_sum<kPlanWaves>(n, s);
   const int live = n_pages - all;
   if (threadIdx.x == 0) {
     *n_live = live;
     if (live == n_pages) w.head[1] = 0;
   }
-  int before = 0;
-  for (int r0 = 0; r0 < n_pages; r0 += kRound) {
-    const int p0 = r0 + wave * 64 * kSteps;
-    // Up to kRound pages the masks are still here.
-    const int m = n_pages <= kRound ? 0 : free_masks(refs, n_pages, p0, mask);
-    int mine = m;
-    if (n_pages <= kRound) {
-      mine = 0;
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) mine += __popcll(mask[i]);
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) s[wave] = mine;
-    __syncthreads();
-    int rank = before;
-#pragma unroll
-    for (int v = 0; v < kPlanWaves; ++v) {
-      rank += v < wave ? s[v] : 0;
-      before += s[v];
-    }
-    compact_wave(mask, p0, rank, n_pages, live, w);
-  }
+  if (n_pages != 0) compact_wave(mask, p0, rank, n_pages, live, w);
 }
 
 __global__ __launch_bounds__(kThreads) void compact_apply_kernel(

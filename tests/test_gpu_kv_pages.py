@@ -149,6 +149,30 @@ def test_reserve_past_the_table_and_of_long_rows(cuda):
     assert refs.tolist() == ref.refs and table.tolist() == ref.table
 
 
+@pytest.mark.parametrize("n_pages,batch,width", [
+    (9000, 40, 1100),     # one workgroup
+    (9000, 1500, 70),     # more rows than its threads
+    (66000, 33, 1100),    # many workgroups
+])
+def test_reserve_for_rows_of_every_length(cuda, n_pages, batch, width):
+    """Rows that want one page beside rows that want hundreds, in tables with gaps; where there
+    are many rows until the pages are all taken."""
+    print("case:", n_pages, batch, width, flush=True)
+    rng, ref, cache, refs, table, lens = scene(batch, n_pages, batch, width, 1, used=0.3)
+    spans, short = [1, 2, 4, 5, 6, 63, 64, 65, 511, 512, 513, width], i32([0])
+    for turn in range(3):
+        for b in range(batch):  # gaps: entries that name no page behind a row's last position
+            for e in range(ref.lens[b] // PAGE + 1, width):
+                if ref.table[b][e] < 0 and rng.random() < 0.2:
+                    ref.table[b][e] = int(rng.choice([-1, -7, n_pages, n_pages + 5]))
+        table = i32(ref.table)
+        counts = PAGE * rng.choice(spans, batch) - rng.integers(0, PAGE, batch)
+        counts[rng.random(batch) < 0.5] = 0
+        ops.kv_pages_reserve(refs, table, lens, i32(counts), shortfall=short)
+        assert short.item() == ref.reserve(counts), turn
+        same(ref, cache, refs, table, lens)
+
+
 def test_compact_with_entries_that_name_free_pages(cuda):
     rng = np.random.default_rng(8)
     cache = random_cache(rng, 9, 2)
