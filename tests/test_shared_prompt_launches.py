@@ -127,7 +127,7 @@ def test_one_workgroup_plans_for_few_pages_and_rows():
     many = [["reserve_count_kernel", "reserve_list_kernel", "reserve_apply_kernel"],
             ["count_kernel", "fork_list_kernel", "fork_apply_kernel"],
             ["count_kernel", "compact_list_kernel", "compact_apply_kernel"]]
-    got = pages([(65536, 4096), (65537, 4), (4, 4097), (0, 4)])
+    got = pages([(16384, 4096), (16385, 4), (4, 4097), (0, 4)])
     assert got == [few, many, many[:2] + few[2:], few[:2] + [few[2][:1]]]
     seen = {x for one in pages([s[:2] for s in SCENES]) for call in one for x in call}
     assert seen == {x for one in (few, many) for call in one for x in call}
