@@ -120,8 +120,10 @@ __device__ __forceinline__ int whole_pages(int positions, int max_pages) {
 // A start counts as no less than those before it and lies in 0 .. batch, so that groups
 // never overlap, whatever the arrays hold.
 //
-// Shared pages of sequence b: its group ends at the first start past b.
+// Shared pages of sequence b: its group ends at the first start past b.  Without groups
+// there may be no starts.
 __device__ __forceinline__ int shared_pages_of(const Groups &gr, int b, int max_pages) {
+  if (gr.n == 0) return 0;
   const int lane = threadIdx.x & 63;
   for (int base = 0; base <= gr.n; base += 64) {
     const int i = base + lane;

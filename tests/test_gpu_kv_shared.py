@@ -143,6 +143,25 @@ def test_starts_of_every_kind(cuda):
         check(*s.run(start=i32(start), shared=i32(shared)), ref)
 
 
+@pytest.mark.parametrize("n_q,window", [(1, 0), (5, 100)])
+def test_no_groups_and_no_arrays_of_them(cuda, n_q, window):
+    """n_groups 0 with NULL for both arrays: every sequence shares nothing."""
+    s = Scene([], [300, 1, 0, 129], n_q, 4, 2, 33)
+    say("case:", n_q, window)
+    q, lens = dev(s.q), i32(s.lens)
+    out = torch.full_like(q, 7)
+    lse = torch.empty((4, 4, n_q), device="cuda")
+    max_pages, lib = s.table.shape[1], L.load()
+    need = lib.prichs_kv_cache_shared_attention_workspace(4, n_q, 4, 2, max_pages, 0)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    L.check(lib.prichs_kv_cache_shared_attention(
+        q.data_ptr(), q.stride(0), s.cache.data_ptr(), s.n_pages, s.table.data_ptr(), max_pages,
+        lens.data_ptr(), None, None, 0, out.data_ptr(), out.stride(0), lse.data_ptr(), 4, n_q, 4,
+        2, HD, window, 0, L.DTYPE_BF16, ws.data_ptr(), need,
+        torch.cuda.current_stream().cuda_stream))
+    check(out, lse, s.ref(window))
+
+
 def test_whole_table_shared_and_lens_past_it(cuda):
     """Sequences that hold nothing of their own, and lengths past the table."""
     s = Scene([(6, 256)], [256, 256, 255, 100, 200, 1], 1, 8, 2, 32, max_pages=4)
