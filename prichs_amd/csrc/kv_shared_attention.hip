@@ -7,7 +7,7 @@
 // kv_attend.hpp has the tiles and the join.
 //
 // MI355X, 12 + 3 heads, us from Python (kernel and join): 8 sequences of one prompt of 1000
-// positions 15 (10 captured), 16 prompts of 2048 with 4 sequences each 15.5, 24 x 6 tokens
+// positions 15 (10 captured), 16 prompts of 2048 with 4 sequences each 15, 24 x 6 tokens
 // behind 8000 shared positions 25, 256 sequences behind 32768 80: 52 GFLOP, 650 TFLOP/s.
 #include "kv_attend.hpp"
 
@@ -46,17 +46,25 @@ __global__ __launch_bounds__(256) void kv_shared_join_kernel(
 // (the second number: workgroups that the shared pages are dealt to).  24 x 8000 with six
 // tokens each 26.2, 24.7, 30.5; 128 x 16384 36.3, 34.5, 38.1; 200 x 16384 52, 48, 45.
 // Dealt by die (kv_attend.hpp) the last three are 24.5, 32.7 and 44.2.
+// With tiles of 16 rows three workgroups fit a CU: half of that round for shared and half
+// for own pages instead of 512 and 256: 16 prompts of 2048 x 4 sequences 15.4 -> 14.3, with
+// some 2000 positions of their own each 23.8 -> 19.0, 32 x 8000 with 1000 each 17.1 -> 16.0, but
+// 20 x 4096 11.5 -> 12.0 and 8 x 8 x 4096 16.5 -> 17.2.
 // What bounds a large call is the vector instructions of a page, some 460 for 32 rows (128
 // conversions, 64 permutes, the softmax), which two waves a SIMD issue 56% of the time.
 // Measured and not kept, at 256 x 32768: tiles of 48 and 64 rows, one wave a SIMD, 140 and
 // 166 us; each page converted once into LDS for 128 rows, whose waves wait for each other at
 // every page, 95 to 101 (and 36 to 39 at 24 x 8000); queries in LDS, which leaves registers
-// for a third wave, 98 to 109; own pages first 98; wave priorities, the same to 1%.
+// for a third wave, 98 to 109; own pages first 98; wave priorities, the same to 1%.  K's codes
+// in products without a conversion (queries as sums of two e4m3 parts, scores of the next
+// page formed between the products with V): 80.4 -> 77.8, but 64 x 8192 19.7 -> 20.4, and 24
+// registers in memory where lse is wanted.
 struct Plan {
   int blocks;               // of 16 rows in a tile over shared pages
   size_t tiles_p, split_p;  // tiles over shared pages of a kv head at most, splits of each
   size_t tiles_s, split_s;  // the same of a sequence's own pages
 };
+constexpr size_t kHalfRound = 384;
 constexpr size_t kManySteps = 4096, kMoreSteps = 32768;  // pages of all tiles of 16 rows
 Plan plan_of(size_t batch, size_t n_q, size_t n_heads, size_t n_kv_heads, size_t max_pages,
              size_t n_groups) {
@@ -71,13 +79,14 @@ Plan plan_of(size_t batch, size_t n_q, size_t n_heads, size_t n_kv_heads, size_t
   p.tiles_p = p.split_p = 0;
   if (groups > 0) {
     p.tiles_p = (batch * rows + groups * (per - 1)) / per;
-    const size_t wgs = p.blocks == 1 || steps >= kMoreSteps ? 512 : 256;
+    const size_t wgs = p.blocks == 1 ? kHalfRound : steps >= kMoreSteps ? 512 : 256;
     p.split_p = std::max<size_t>(std::min(wgs / (n_kv_heads * p.tiles_p), most), 1);
   }
   // Own pages: as a rule few, of a number that only the device knows.
   p.tiles_s = cdiv(rows, (size_t)kRows);
   p.split_s = std::max<size_t>(
-      std::min({256 / (batch * n_kv_heads * p.tiles_s), most, (size_t)8}), 1);
+      std::min({(p.blocks == 1 ? kHalfRound : 256) / (batch * n_kv_heads * p.tiles_s), most, (size_t)8}),
+      1);
   return p;
 }
 size_t workspace_of(const Plan &p, size_t rows) {

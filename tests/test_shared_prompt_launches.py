@@ -25,7 +25,7 @@ for b, n, p, h, k, g, lse in {cases!r}:
 @pytest.mark.parametrize("case,blocks,tiles,split_p,split_s", [
     ((4, 1, 20, 12, 3, 0), 1, 0, 0, 5), ((8, 1, 17, 12, 3, 1), 1, 2, 5, 5),
     ((24, 6, 133, 12, 3, 1), 2, 18, 4, 1), ((256, 1, 528, 12, 3, 1), 2, 32, 5, 1),
-    ((64, 1, 136, 12, 3, 1), 2, 8, 10, 1), ((64, 1, 37, 12, 3, 16), 1, 31, 5, 1),
+    ((64, 1, 136, 12, 3, 1), 2, 8, 10, 1), ((64, 1, 37, 12, 3, 16), 1, 31, 4, 2),
     ((200, 16, 8, 8, 2, 2), 2, 401, 1, 1), ((3, 1, 50, 4, 4, 100), 1, 3, 13, 8),
     ((1, 1, 0, 4, 4, 1), 1, 1, 1, 1)])
 def test_how_a_call_is_cut(case, blocks, tiles, split_p, split_s):
