@@ -84,9 +84,9 @@ Plan plan_of(size_t batch, size_t n_q, size_t n_heads, size_t n_kv_heads, size_t
   }
   // Own pages: as a rule few, of a number that only the device knows.
   p.tiles_s = cdiv(rows, (size_t)kRows);
+  const size_t own = p.blocks == 1 ? kHalfRound : 256;
   p.split_s = std::max<size_t>(
-      std::min({(p.blocks == 1 ? kHalfRound : 256) / (batch * n_kv_heads * p.tiles_s), most, (size_t)8}),
-      1);
+      std::min({own / (batch * n_kv_heads * p.tiles_s), most, (size_t)8}), 1);
   return p;
 }
 size_t workspace_of(const Plan &p, size_t rows) {

@@ -280,6 +280,65 @@ def test_pages_past_32_bits(cuda):
     check(*s.run(cache=far, table=table), s.ref())
 
 
+def test_two_graphs_at_once_and_a_stream_of_its_own(cuda):
+    """Two captured calls replayed at the same time on two streams, each with a workspace of
+    its own; the page calls and the attention on a stream that is not the current one."""
+    scenes = [Scene([(12, 1280)], [1290 + 70 * i for i in range(12)], 1, 12, 3, 40),
+              Scene([(3, 640), (4, 256)], [700, 650, 900, 300, 260, 257, 400], 2, 8, 2, 41)]
+    refs = [s.ref() for s in scenes]
+    lens = [i32(s.lens) for s in scenes]
+    qs = [dev(s.q) for s in scenes]
+
+    def call(i, stream=None):
+        s = scenes[i]
+        return ops.kv_cache_shared_attention(qs[i], s.cache, s.table, lens[i], s.start, s.shared,
+                                             s.batch, s.n_q, s.heads, s.kv, want_lse=True,
+                                             stream=stream)
+
+    graphs, outs = [], []
+    for i in range(2):
+        check(*call(i), refs[i])
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            outs.append(call(i))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(4):
+        for o, lse in outs:
+            o.fill_(7), lse.fill_(7)
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for g, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    g.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            check(*outs[i], refs[i])
+    side = streams[0]
+    side.wait_stream(torch.cuda.current_stream())
+    got = [call(i, side) for i in range(2)]
+    side.synchronize()
+    for i in range(2):
+        check(*got[i], refs[i])
+
+    # Pages taken, shared, given back and moved on that stream.
+    refs, table = ops.kv_pages_refs(20), torch.full((3, 4), -1, dtype=torch.int32, device="cuda")
+    cache, held, short = ops.kv_cache_pages(20, 2), i32([0] * 3), i32([9])
+    counts, now, kids, parents, first = (i32(x) for x in ([0, 130, 0], [0, 130, 0], [0, 2],
+                                                         [1, 1], [1]))
+    side.wait_stream(torch.cuda.current_stream())
+    ops.kv_pages_reserve(refs, table, held, counts, shortfall=short, stream=side)
+    with torch.cuda.stream(side):
+        held.copy_(now)
+    ops.kv_pages_fork(cache, refs, table, held, parents, kids, 2, stream=side)
+    ops.kv_pages_release(refs, table, first, stream=side)
+    n_live, new = ops.kv_pages_compact(cache, refs, table, 2, stream=side)
+    side.synchronize()
+    assert (short.item(), n_live.item(), held.tolist()) == (0, 4, [130] * 3)
+    assert table.tolist() == [[0, 1, 3, -1], [-1] * 4, [0, 1, 2, -1]]
+    assert refs.tolist() == [2, 2, 1, 1] + [0] * 16 and new.tolist()[:5] == [0, 1, -1, 3, 2]
+
+
 def test_forked_continuations_in_a_graph(cuda):
     """As a program uses the calls together: prompts normed, rotated and cached, forked into
     continuations, and decode steps in one captured graph (pages reserved, the token's keys
