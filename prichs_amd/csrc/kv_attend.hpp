@@ -96,8 +96,10 @@ struct PageRegs {
 // Groups of sequences that share their first pages (prichs_kv_cache_shared_attention).  A
 // launch then has two kinds of workgroup: splits of a group's tiles over its shared pages,
 // and splits of each sequence's tiles over its own.  Each writes the parts of its rows
-// into a slot of its own, split_p slots for shared and split_s for own pages.
-enum { kWholeRole, kSharedRole, kOwnRole };  // a call without groups; the two kinds
+// into a slot of its own, split_p slots for shared and split_s for own pages.  Or, where
+// there are few pages, one kind: a sequence's tile over all its pages, the shared ones
+// where its group's first sequence names them.
+enum { kWholeRole, kSharedRole, kOwnRole, kRowRole };  // a call without groups; these kinds
 struct Groups {
   const int32_t *start, *shared;
   int n, batch;
@@ -121,18 +123,26 @@ __device__ __forceinline__ int whole_pages(int positions, int max_pages) {
 // never overlap, whatever the arrays hold.
 //
 // Shared pages of sequence b: its group ends at the first start past b.  Without groups
-// there may be no starts.
-__device__ __forceinline__ int shared_pages_of(const Groups &gr, int b, int max_pages) {
+// there may be no starts.  *first (where wanted): the group's first sequence.
+__device__ __forceinline__ int shared_pages_of(const Groups &gr, int b, int max_pages,
+                                               int *first = nullptr) {
   if (gr.n == 0) return 0;
   const int lane = threadIdx.x & 63;
+  int low = 0;  // the group starts at the greatest start up to b
   for (int base = 0; base <= gr.n; base += 64) {
     const int i = base + lane;
     const int start = i <= gr.n ? gr.start[i] : 0x7fffffff;
     const int before = i >= 1 && i <= gr.n ? gr.shared[i - 1] : 0;  // of the group that ends here
     const uint64_t past = __ballot(start > b);
-    if (past != 0)
-      return whole_pages(
-          __builtin_amdgcn_readlane(before, __ffsll((unsigned long long)past) - 1), max_pages);
+    const int at = past == 0 ? 64 : __ffsll((unsigned long long)past) - 1;
+    if (first != nullptr) {
+      int s = lane < at ? start : 0;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) s = max(s, __shfl_xor(s, d));
+      low = max(low, s);
+      *first = __builtin_amdgcn_readfirstlane(low);
+    }
+    if (past != 0) return whole_pages(__builtin_amdgcn_readlane(before, at), max_pages);
   }
   return 0;
 }
@@ -211,7 +221,7 @@ __device__ __forceinline__ void kv_attend(
     const int32_t *__restrict__ table, const int32_t *__restrict__ lens, bf16_t *__restrict__ o,
     size_t ldo, float *__restrict__ lse, float *__restrict__ part_o, float2 *__restrict__ part_ml,
     const AttendShape &sh, JoinLds<kWaves> &s, const Groups &gr) {
-  constexpr bool kGroups = ROLE != kWholeRole;
+  constexpr bool kGroups = ROLE == kSharedRole || ROLE == kOwnRole;
   static_assert(NB == 1 || kGroups, "whole sequences have tiles of 16 rows");
   constexpr int kThreads = 64 * kWaves, kTileRows = 16 * NB;
   auto &s_ml = s.ml;
@@ -301,7 +311,16 @@ __device__ __forceinline__ void kv_attend(
   const int64_t worker = split * kWaves + wave, workers = n_split * kWaves;
   const int begin = (int)(n_vis * worker / workers), end = (int)(n_vis * (worker + 1) / workers);
   auto block_of = [&](int i) { return i >= n_sink ? i + skip : i + lo; };
-  const int32_t *row_table = table + (size_t)b * sh.max_pages;
+  const int32_t *row_table = table + (size_t)b * sh.max_pages, *first_table = row_table;
+  int n_shared = 0;  // kRowRole: pages that stand in first_table
+  if constexpr (ROLE == kRowRole) {
+    int first_b = 0;
+    n_shared = shared_pages_of(gr, b, sh.max_pages, &first_b);
+    if (n_shared > 0) first_table = table + (size_t)first_b * sh.max_pages;
+  }
+  auto entry = [&](int block) {
+    return ROLE == kRowRole && block < n_shared ? first_table[block] : row_table[block];
+  };
   // The wave's next visible block whose page exists (end: none), and its page.  It holds 64
   // entries of the table at a time, and a bit for each that names a page.
   int ids = -1, base = begin - 64;
@@ -310,7 +329,7 @@ __device__ __forceinline__ void kv_attend(
     while (left == 0) {
       base += 64;
       if (base >= end) return end;
-      ids = base + lane < end ? row_table[block_of(base + lane)] : -1;
+      ids = base + lane < end ? entry(block_of(base + lane)) : -1;
       left = __ballot(ids >= 0 && ids < sh.n_pages);
     }
     const int at = __ffsll((unsigned long long)left) - 1;

@@ -6,15 +6,15 @@
 //   o = sum_p exp(m_p - m) o_p / sum_p exp(m_p - m) l_p,  m = max_p m_p.
 // kv_attend.hpp has the tiles and the join.
 //
-// MI355X, 12 + 3 heads, us from Python (kernel and join): 8 sequences of one prompt of 1000
-// positions 15 (10 captured), 16 prompts of 2048 with 4 sequences each 15, 24 x 6 tokens
+// MI355X, 12 + 3 heads, us from Python (kernels): 8 sequences of one prompt of 1000
+// positions 11 (10 captured), 16 prompts of 2048 with 4 sequences each 15, 24 x 6 tokens
 // behind 8000 shared positions 25, 256 sequences behind 32768 80: 52 GFLOP, 650 TFLOP/s.
 #include "kv_attend.hpp"
 
 namespace prichs {
 namespace {
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 4, kRowWaves = 8;
 
 // Workgroups over shared pages, with tiles of 16 NB rows, then those over own pages.
 template <int NB, bool LSE>
@@ -29,6 +29,16 @@ __global__ __launch_bounds__(64 * kWaves, NB == 1 ? 3 : 2) void kv_shared_kernel
   else
     kv_attend<kWaves, LSE, kOwnRole>(q, ldq, cache, table, lens, nullptr, 0, nullptr, part_o,
                                      part_ml, sh, s, gr);
+}
+// Few pages: a workgroup for each tile of a sequence, and no second kernel.
+template <bool LSE>
+__global__ __launch_bounds__(64 * kRowWaves, 2) void kv_shared_rows_kernel(
+    const bf16_t *__restrict__ q, size_t ldq, const uint8_t *__restrict__ cache,
+    const int32_t *__restrict__ table, const int32_t *__restrict__ lens, bf16_t *__restrict__ o,
+    size_t ldo, float *__restrict__ lse, AttendShape sh, Groups gr) {
+  __shared__ JoinLds<kRowWaves> s;
+  kv_attend<kRowWaves, LSE, kRowRole>(q, ldq, cache, table, lens, o, ldo, lse, nullptr, nullptr,
+                                      sh, s, gr);
 }
 template <int KG, bool LSE>
 __global__ __launch_bounds__(256) void kv_shared_join_kernel(
@@ -63,11 +73,20 @@ struct Plan {
   int blocks;               // of 16 rows in a tile over shared pages
   size_t tiles_p, split_p;  // tiles over shared pages of a kv head at most, splits of each
   size_t tiles_s, split_s;  // the same of a sequence's own pages
+  bool rows;                // few pages: tiles_s tiles over all of a sequence's pages, one launch
 };
+// Up to so many pages, and a CU for each tile of a sequence, one launch takes each sequence by
+// itself.  Captured, us (from Python in brackets), so and apart with a join: 8 sequences of 8
+// pages 7.1, 9.4 (10.7, 14.5), 16 pages 8.8, 9.6 (10.6, 14.4), 24 pages 10.4, 10.2 (10.7, 14.5), 32
+// pages 12.0, 10.2 (11.4, 14.5); one of 24 pages 10.2, 9.5; 80 of 24 10.9, 13.3; 20 of 24 with
+// eight tokens each 10.9, 16.0.  100 sequences, more tiles than CUs: 8 pages 11.8, 10.7 (11.3,
+// 14.9), 24 pages 18.6, 13.7.
+constexpr size_t kFewPages = 24;
 constexpr size_t kHalfRound = 384;
 constexpr size_t kManySteps = 4096, kMoreSteps = 32768;  // pages of all tiles of 16 rows
+// `pages`: that a sequence's tile sees at most.
 Plan plan_of(size_t batch, size_t n_q, size_t n_heads, size_t n_kv_heads, size_t max_pages,
-             size_t n_groups) {
+             size_t n_groups, size_t pages) {
   const size_t rows = n_q * (n_heads / n_kv_heads);  // of a sequence
   const size_t most = std::max<size_t>(cdiv(max_pages, (size_t)kWaves), 1);
   // Only groups of some sequence have tiles, and the last of each may be short.
@@ -84,12 +103,14 @@ Plan plan_of(size_t batch, size_t n_q, size_t n_heads, size_t n_kv_heads, size_t
   }
   // Own pages: as a rule few, of a number that only the device knows.
   p.tiles_s = cdiv(rows, (size_t)kRows);
+  p.rows = pages <= kFewPages && batch * n_kv_heads * p.tiles_s <= 256;
   const size_t own = p.blocks == 1 ? kHalfRound : 256;
   p.split_s = std::max<size_t>(
       std::min({own / (batch * n_kv_heads * p.tiles_s), most, (size_t)8}), 1);
   return p;
 }
 size_t workspace_of(const Plan &p, size_t rows) {
+  if (p.rows) return 0;
   return rows * (p.split_p + p.split_s) * (kKvHd + 3) * sizeof(float);
 }
 
@@ -102,7 +123,7 @@ extern "C" size_t prichs_kv_cache_shared_attention_workspace(size_t batch, size_
                                                              size_t n_heads, size_t n_kv_heads,
                                                              size_t max_pages, size_t n_groups) {
   if (n_kv_heads == 0 || n_heads < n_kv_heads || batch == 0 || n_q == 0) return 0;
-  return workspace_of(plan_of(batch, n_q, n_heads, n_kv_heads, max_pages, n_groups),
+  return workspace_of(plan_of(batch, n_q, n_heads, n_kv_heads, max_pages, n_groups, max_pages),
                       batch * n_q * n_heads);
 }
 
@@ -136,7 +157,11 @@ extern "C" int prichs_kv_cache_shared_attention(
   PRICHS_REQUIRE((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(o) |
                   reinterpret_cast<uintptr_t>(cache)) % 16 == 0,
                  "%s: q, o and the cache must be 16-byte aligned", who);
-  const Plan p = plan_of(batch, n_q, n_heads, n_kv_heads, max_pages, n_groups);
+  // A window past the table hides nothing.
+  const size_t w = window >= cap ? 0 : window, sk = std::min(sinks, cap);
+  const size_t pages =
+      w == 0 ? max_pages : std::min(max_pages, cdiv(w + n_q, kKvPage) + 1 + cdiv(sk, kKvPage));
+  const Plan p = plan_of(batch, n_q, n_heads, n_kv_heads, max_pages, n_groups, pages);
   // Workgroups of 256 threads, fewer than 2^32 in a launch.
   const size_t wgs = roundup(n_kv_heads * p.tiles_p * p.split_p, 8) +
                      n_kv_heads * batch * p.tiles_s * p.split_s;
@@ -145,21 +170,30 @@ extern "C" int prichs_kv_cache_shared_attention(
   if (workspace_bytes < need)
     return fail(PRICHS_ERR_CAPACITY, "%s: workspace of %zu bytes, %zu needed", who,
                 workspace_bytes, need);
-  PRICHS_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+  PRICHS_REQUIRE(need == 0 ||
+                     (workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                  "%s: the workspace must be 16-byte aligned device memory", who);
-  // A window past the table hides nothing.
   const AttendShape sh{(int)n_pages,
                        (int)max_pages,
                        (int)n_q,
                        (int)n_heads,
                        (int)n_kv_heads,
-                       (int)(window >= cap ? 0 : window),
-                       (int)std::min(sinks, cap),
+                       (int)w,
+                       (int)sk,
                        (int)p.tiles_s,
                        1,
                        (1.0f / sqrtf((float)head_dim)) * 1.4426950408889634f};
   const Groups gr{group_start,    shared,         (int)n_groups, (int)batch,
                   (int)p.tiles_p, (int)p.split_p, (int)p.split_s};
+  if (p.rows) {
+    hipLaunchKernelGGL(lse == nullptr ? kv_shared_rows_kernel<false> : kv_shared_rows_kernel<true>,
+                       dim3((unsigned)(n_kv_heads * p.tiles_s), 1, (unsigned)batch),
+                       dim3(64 * kRowWaves), 0, as_stream(stream), static_cast<const bf16_t *>(q),
+                       ldq, static_cast<const uint8_t *>(cache), page_table, lens,
+                       static_cast<bf16_t *>(o), ldo, lse, sh, gr);
+    PRICHS_LAUNCH_CHECK("kv_cache_shared_attention launch");
+    return PRICHS_OK;
+  }
   float *part_o = static_cast<float *>(workspace);
   float2 *part_ml =
       reinterpret_cast<float2 *>(part_o + rows * (p.split_p + p.split_s) * kKvHd);

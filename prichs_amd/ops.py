@@ -526,21 +526,23 @@ def kv_cache_shared_attention(q, cache, page_table, lens, group_start, shared, b
         raise ValueError("window and sinks must not be negative")
     ctx, s = _launch_on(stream, q, cache, page_table, lens, group_start, shared, out)
     with ctx:
+        ldo = H
         if out is None:
             out = q.new_empty((rows, H))
-        ldo = _rows(out, "out", rows, H)
+        else:
+            ldo = _rows(out, "out", rows, H)
         lse = None
         if want_lse:
             lse = torch.empty((batch, n_heads, n_q), dtype=torch.float32, device=q.device)
         max_pages = page_table.shape[1]
         need = lib.prichs_kv_cache_shared_attention_workspace(batch, n_q, n_heads, n_kv_heads,
                                                               max_pages, n_groups)
-        ws = q.new_empty((need + 1) // 2)  # of two bytes each: a faster call
+        ws = q.new_empty((need + 1) // 2) if need else None  # of two bytes each: a faster call
         L.check(lib.prichs_kv_cache_shared_attention(
             q.data_ptr(), ldq, cache.data_ptr(), cache.shape[0], page_table.data_ptr(), max_pages,
             lens.data_ptr(), group_start.data_ptr(), shared.data_ptr(), n_groups, out.data_ptr(),
             ldo, _a(lse), batch, n_q, n_heads, n_kv_heads, head_dim, window, sinks, L.DTYPE_BF16,
-            ws.data_ptr(), need, s))
+            _a(ws), need, s))
     return out, lse
 
 

@@ -88,6 +88,10 @@ CASES = [
     ([(1, 64)] * 130 + [(20, 128)], [100] * 130 + [200] * 20, 1, 4, 2, 0, 0),
     ([(25, 192), (31, 128)], [250] * 25 + [129] * 31, 6, 3, 3, 0, 0),
     ([(70, 1280)], [1281 + 5 * i for i in range(70)], 2, 4, 2, 700, 130),
+    ([(90, 640)], [650 + 2 * i for i in range(90)], 1, 6, 3, 200, 70),
+    ([(130, 320), (140, 128)], [400 + i for i in range(130)] + [130 + i for i in range(140)], 1, 4,
+     1, 64, 0),
+    ([(30, 2000)], [1900 + 15 * i for i in range(30)], 2, 4, 2, 1600, 130),
 ]
 
 
@@ -97,16 +101,25 @@ def columns(batch, n_q, heads, kv):
     return -(-4096 // (-(-batch * n_q * (heads // kv) // 16) * kv))
 
 
-# The same with tiles of 32 rows (long tables, most of whose entries nobody reaches).
-MANY = [CASES[i] for i in (3, 5, 6, 7, 8, 9, 10, 11, 13, 14, 18, 19)]
+# A call of few pages has a workgroup for each tile of a sequence.  The same with tables so
+# long that shared and own pages are taken apart, and so long that there are tiles of 32 rows
+# (most entries of either nobody reaches).
+LONG = [CASES[i] for i in (0, 1, 2, 3, 4, 5, 6, 7, 11, 12, 16)]
+MANY = [CASES[i] for i in (3, 5, 6, 7, 8, 9, 10, 11, 13, 14, 18, 19, 20, 21, 22)]
+FORMS = [(*c, form) for cases, form in ((CASES, 0), (LONG, 1), (MANY, 2)) for c in cases]
 
 
-@pytest.mark.parametrize("groups,lens,n_q,heads,kv,window,sinks,wide", [
-    (*c, w) for cases, w in ((CASES, False), (MANY, True)) for c in cases])
-def test_groups(cuda, groups, lens, n_q, heads, kv, window, sinks, wide):
-    say("case:", groups[:3], lens[:3], n_q, heads, kv, window, sinks, wide)
+def pages_of(lens, n_q, heads, kv, form):
+    """Columns of a case's table."""
+    need = -(-max(lens) // PAGE)
+    return (need, max(need, 25), max(need, columns(len(lens), n_q, heads, kv)))[form]
+
+
+@pytest.mark.parametrize("groups,lens,n_q,heads,kv,window,sinks,form", FORMS)
+def test_groups(cuda, groups, lens, n_q, heads, kv, window, sinks, form):
+    say("case:", groups[:3], lens[:3], n_q, heads, kv, window, sinks, form)
     s = Scene(groups, lens, n_q, heads, kv, n_q + sum(lens),
-              max_pages=columns(len(lens), n_q, heads, kv) if wide else None)
+              max_pages=pages_of(lens, n_q, heads, kv, form))
     ref = s.ref(window, sinks)
     wide = torch.full((s.batch * n_q + 1, heads * HD + 8), float("nan"), dtype=torch.bfloat16,
                       device="cuda")
@@ -124,15 +137,17 @@ def test_groups(cuda, groups, lens, n_q, heads, kv, window, sinks, wide):
 
 
 def wide(size, heads=8, kv=2):
-    """Columns for tiles of 32 rows where a group has 40 sequences."""
-    return columns(size, 1, heads, kv) if size == 40 else None
+    """Columns by the sequences of a group: shared and own pages apart with 4, tiles of 32 rows
+    with 40 and 264."""
+    return columns(size, 1, heads, kv) if size in (40, 264) else 30 if size == 4 else None
 
 
-def test_starts_of_every_kind(cuda):
+@pytest.mark.parametrize("max_pages", [None, 25])
+def test_starts_of_every_kind(cuda, max_pages):
     """Starts below zero, past the batch, that fall, and sequences before and behind the
     groups: each counts as no less than those before it."""
     lens = [300, 280, 400, 350, 129, 200, 260]
-    s = Scene([(2, 256), (3, 128)], lens, 1, 4, 2, 31, first=1)
+    s = Scene([(2, 256), (3, 128)], lens, 1, 4, 2, 31, first=1, max_pages=max_pages)
     ref = s.ref()
     check(*s.run(), ref)
     kinds = [([1, 3, 6], [256, 128]), ([1, 3, 2, 6], [256, 1 << 30, 128]),
@@ -143,11 +158,11 @@ def test_starts_of_every_kind(cuda):
         check(*s.run(start=i32(start), shared=i32(shared)), ref)
 
 
-@pytest.mark.parametrize("n_q,window", [(1, 0), (5, 100)])
-def test_no_groups_and_no_arrays_of_them(cuda, n_q, window):
+@pytest.mark.parametrize("n_q,window,max_pages", [(1, 0, None), (5, 100, None), (1, 0, 30)])
+def test_no_groups_and_no_arrays_of_them(cuda, n_q, window, max_pages):
     """n_groups 0 with NULL for both arrays: every sequence shares nothing."""
-    s = Scene([], [300, 1, 0, 129], n_q, 4, 2, 33)
-    say("case:", n_q, window)
+    s = Scene([], [300, 1, 0, 129], n_q, 4, 2, 33, max_pages=max_pages)
+    say("case:", n_q, window, max_pages)
     q, lens = dev(s.q), i32(s.lens)
     out = torch.full_like(q, 7)
     lse = torch.empty((4, 4, n_q), device="cuda")
@@ -171,7 +186,7 @@ def test_whole_table_shared_and_lens_past_it(cuda):
     check(*s.run(), s.ref())
 
 
-@pytest.mark.parametrize("size", [3, 40])
+@pytest.mark.parametrize("size", [3, 4, 40])
 def test_pages_that_do_not_exist(cuda, size):
     s = Scene([(size, 320)], [400 + i for i in range(size)], 1, 8, 2, 33, max_pages=wide(size))
     s.table[0, 1], s.table[0, 4], s.table[1, 5] = s.n_pages, -1, 1 << 30
@@ -187,11 +202,11 @@ def test_pages_that_do_not_exist(cuda, size):
 
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
-@pytest.mark.parametrize("size", [3, 40])
+@pytest.mark.parametrize("size", [3, 260, 264])
 def test_what_a_row_does_not_see_does_not_reach_it(cuda, size, bad):
     """Values that are not finite in a shared page: rows behind a window, and a sequence
     that ends before them, are as without them."""
-    lens = [330 + 7 * i for i in range(size)]
+    lens = [330 + 7 * (i % 40) for i in range(size)]
     lens[1] = 150
     W = 120
     s = Scene([(size, 320)], lens, 1, 4, 1, 34, max_pages=wide(size, 4, 1))
@@ -211,7 +226,7 @@ def test_what_a_row_does_not_see_does_not_reach_it(cuda, size, bad):
     assert not np.isfinite(h[:, :, 1]).any() and np.isfinite(h[:, :, [0, 2, 3]]).all()
 
 
-@pytest.mark.parametrize("size", [3, 40])
+@pytest.mark.parametrize("size", [3, 4, 40])
 @pytest.mark.parametrize("q_scale", [0.0, 40.0])
 def test_flat_and_steep_scores(cuda, size, q_scale):
     s = Scene([(size, 640)], [700 + i for i in range(size)], 1, 4, 2, 35, q_scale=q_scale,
@@ -225,7 +240,7 @@ def test_flat_and_steep_scores(cuda, size, q_scale):
     check(s.run()[0], None, ref)
 
 
-@pytest.mark.parametrize("size", [2, 40])
+@pytest.mark.parametrize("size", [2, 4, 40])
 def test_rows_without_finite_scores(cuda, size):
     """Scores of -inf alone, in the shared pages, in the own ones or in both, and a +inf or
     NaN: as for a sequence that shares nothing."""
@@ -235,7 +250,8 @@ def test_rows_without_finite_scores(cuda, size):
     v = synth.round_bf16(np.random.default_rng(1).standard_normal((n, HD)))
     k[:, 0], k[128:, 1], k[:128, 2] = 1, 1, 1
     for b in range(size):
-        ops.kv_cache_write(s.cache, s.table[b:b + 1].contiguous(), i32([0]), dev(k), dev(v), 1, n, kv)
+        ops.kv_cache_write(s.cache, s.table[b:b + 1].contiguous(), i32([0]), dev(k), dev(v), 1, n,
+                           kv)
     for dim in range(3):
         for x in (-np.inf, np.inf, np.nan):
             q = np.zeros((size, 4 * HD), np.float32)
@@ -250,7 +266,7 @@ def test_rows_without_finite_scores(cuda, size):
             assert np.array_equal(np.isnan(host(lse)), np.isnan(host(want_lse)))
 
 
-@pytest.mark.parametrize("size,n_q", [(3, 1), (40, 1), (12, 9)])
+@pytest.mark.parametrize("size,n_q", [(3, 1), (4, 1), (4, 9), (40, 1), (12, 9)])
 def test_what_the_workspace_held_does_not_matter(cuda, size, n_q):
     s = Scene([(size, 640), (2, 0)], [700 + i for i in range(size)] + [90, 0], n_q, 8, 2, 37,
               max_pages=wide(size))

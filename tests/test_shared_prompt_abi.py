@@ -25,7 +25,7 @@ RELEASE = dict(refs=P, n_pages=9, page_table=P, max_pages=4, batch=3, rows=P, ke
 COMPACT = dict(cache=P, refs=P, n_pages=9, page_table=P, max_pages=4, batch=3, n_kv_heads=2,
                new_page=P, n_live=P, workspace=P, workspace_bytes=BIG, stream=None)
 COPY = dict(dst=P, dst_pages=9, src=P, src_pages=9, to=P, frm=P, n=2, n_kv_heads=2, stream=None)
-SHARED = dict(q=P, ldq=512, cache=P, n_pages=4, page_table=P, max_pages=2, lens=P, group_start=P,
+SHARED = dict(q=P, ldq=512, cache=P, n_pages=4, page_table=P, max_pages=40, lens=P, group_start=P,
               shared=P, n_groups=1, o=P, ldo=512, lse=None, batch=2, n_q=1, n_heads=4,
               n_kv_heads=2, head_dim=128, window=0, sinks=0, dtype=1, workspace=P,
               workspace_bytes=BIG, stream=None)
@@ -115,7 +115,7 @@ def test_workspaces(lib):
     need = lib.prichs_kv_pages_workspace(9, 3, 2)
     assert call(lib, "prichs_kv_pages_fork", {**FORK, "workspace_bytes": need - 1}) == CAP
     assert lib.prichs_kv_pages_workspace(1 << 25, 1, 1) == 0
-    need = lib.prichs_kv_cache_shared_attention_workspace(2, 1, 4, 2, 2, 1)
+    need = lib.prichs_kv_cache_shared_attention_workspace(2, 1, 4, 2, 40, 1)
     assert need >= 2 * 4 * 2 * 130 * 4
     assert call(lib, "prichs_kv_cache_shared_attention",
                 {**SHARED, "workspace_bytes": need - 1}) == CAP

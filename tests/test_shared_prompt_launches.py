@@ -6,13 +6,15 @@ from tests import launch_log as ll
 
 
 def attend(cases):
-    """Launches for each (batch, n_q, max_pages, heads, kv heads, groups, with lse)."""
+    """Launches for each (batch, n_q, max_pages, heads, kv heads, groups, with lse, window,
+    sinks)."""
     rows = ll.run(f"""
 result = []
-for b, n, p, h, k, g, lse in {cases!r}:
+for b, n, p, h, k, g, lse, window, sinks in {cases!r}:
     need = lib.prichs_kv_cache_shared_attention_workspace(b, n, h, k, p, g)
     L.check(lib.prichs_kv_cache_shared_attention(P, 128 * h, P, 1000, P, p, P, P, P, g, P, 128 * h,
-                                                 P if lse else None, b, n, h, k, 128, 0, 0, 1, P,
+                                                 P if lse else None, b, n, h, k, 128, window, sinks,
+                                                 1, P,
                                                  need, None))
     result.append([need, launches()])
 """)
@@ -23,15 +25,14 @@ for b, n, p, h, k, g, lse in {cases!r}:
 # of own pages): nothing shared; few rows; many rows and few pages; many of both; more tiles
 # than workgroups; groups that could each have a short tile; more groups than sequences.
 @pytest.mark.parametrize("case,blocks,tiles,split_p,split_s", [
-    ((4, 1, 20, 12, 3, 0), 1, 0, 0, 5), ((8, 1, 17, 12, 3, 1), 1, 2, 5, 5),
+    ((4, 1, 40, 12, 3, 0), 1, 0, 0, 8), ((8, 1, 37, 12, 3, 1), 1, 2, 10, 8),
     ((24, 6, 133, 12, 3, 1), 2, 18, 4, 1), ((256, 1, 528, 12, 3, 1), 2, 32, 5, 1),
     ((64, 1, 136, 12, 3, 1), 2, 8, 10, 1), ((64, 1, 37, 12, 3, 16), 1, 31, 4, 2),
-    ((200, 16, 8, 8, 2, 2), 2, 401, 1, 1), ((3, 1, 50, 4, 4, 100), 1, 3, 13, 8),
-    ((1, 1, 0, 4, 4, 1), 1, 1, 1, 1)])
+    ((200, 16, 8, 8, 2, 2), 2, 401, 1, 1), ((3, 1, 50, 4, 4, 100), 1, 3, 13, 8)])
 def test_how_a_call_is_cut(case, blocks, tiles, split_p, split_s):
     b, n, p, h, k, g = case
     for lse in (0, 1):
-        (need, got), = attend([(*case, lse)])
+        (need, got), = attend([(*case, lse, 0, 0)])
         own = b * k * -(-n * (h // k) // 16)
         flag = "true" if lse else "false"
         assert got[0].kernel == f"kv_shared_kernel<{blocks}, {flag}>"
@@ -41,6 +42,26 @@ def test_how_a_call_is_cut(case, blocks, tiles, split_p, split_s):
         assert got[1].kernel == f"kv_shared_join_kernel<{8 if wide else 1}, {flag}>"
         assert got[1].grid[0] == (b * n * h if wide else -(-b * n * h // 8)) and len(got) == 2
         assert need == b * n * h * parts * 131 * 4
+
+
+# Few pages: of a table, or that a window leaves.
+@pytest.mark.parametrize("case,window,sinks,rows", [
+    ((8, 1, 24, 12, 3, 1), 0, 0, True), ((8, 1, 25, 12, 3, 1), 0, 0, False),
+    ((85, 1, 4, 12, 3, 1), 0, 0, True), ((86, 1, 4, 12, 3, 1), 0, 0, False),
+    ((1, 1, 0, 4, 4, 1), 0, 0, True), ((4, 20, 9, 8, 2, 0), 0, 0, True),
+    ((8, 1, 500, 12, 3, 1), 1400, 4, True), ((8, 1, 500, 12, 3, 1), 1472, 64, False),
+    ((8, 1, 500, 12, 3, 1), 1 << 20, 0, False)])
+def test_few_pages_take_one_launch(case, window, sinks, rows):
+    b, n, p, h, k, g = case
+    for lse in (0, 1):
+        (need, got), = attend([(*case, lse, window, sinks)])
+        if rows:
+            flag = "true" if lse else "false"
+            assert [x.kernel for x in got] == [f"kv_shared_rows_kernel<{flag}>"]
+            assert got[0].grid == [k * -(-n * (h // k) // 16), 1, b]
+            assert (need == 0) == (window == 0)
+        else:
+            assert len(got) == 2
 
 
 def test_a_launch_too_large_is_refused():
@@ -56,18 +77,29 @@ result = [rc, launches()]
 def test_the_gpu_tests_reach_every_variant():
     from tests import test_gpu_kv_shared as t
 
-    calls = []
-    for cases, wide in ((t.CASES, False), (t.MANY, True)):
-        for groups, lens, n_q, heads, kv, _, _ in cases:
-            pages = t.columns(len(lens), n_q, heads, kv) if wide else -(-max(lens) // t.PAGE)
-            assert pages >= -(-max(lens) // t.PAGE)
-            calls += [(len(lens), n_q, pages, heads, kv, len(groups), lse) for lse in (0, 1)]
-    names = {x.kernel for _, ls in attend(calls) for x in ls}
-    assert names == {f"kv_shared_{k}<{n}, {f}>" for f in ("true", "false")
-                     for k, n in (("kernel", 1), ("kernel", 2), ("join_kernel", 1),
-                                  ("join_kernel", 8))}
-    (_, got), = attend([(40, 1, t.wide(40), 8, 2, 1, 0)])
-    assert got[0].kernel == "kv_shared_kernel<2, false>"
+    calls, forms = [], []
+    for groups, lens, n_q, heads, kv, window, sinks, form in t.FORMS:
+        pages = t.pages_of(lens, n_q, heads, kv, form)
+        for lse in (0, 1):
+            calls.append((len(lens), n_q, pages, heads, kv, len(groups), lse, window, sinks))
+            forms.append((form, window))
+    got = [{x.kernel for x in ls} for _, ls in attend(calls)]
+    kinds = {f"kv_shared_{k}<{n}{f}>" for f in ("true", "false")
+             for k, n in (("kernel", "1, "), ("kernel", "2, "), ("join_kernel", "1, "),
+                          ("join_kernel", "8, "), ("rows_kernel", ""))}
+    assert set.union(*got) == kinds
+    # With a window as well.
+    assert {x.split("<")[0] + x.split("<")[1][0] for g, (_, w) in zip(got, forms) if w for x in g} \
+        >= {"kv_shared_kernel1", "kv_shared_kernel2", "kv_shared_rows_kernelt"}
+    assert all(not any("rows" in x for x in g) for g, f in zip(got, forms) if f[0] == 1)
+
+    def kernel(size, heads, kv, pages, window=0):
+        (_, got), = attend([(size, 1, t.wide(size, heads, kv) or pages, heads, kv, 1, 0, window,
+                             0)])
+        return got[0].kernel
+    assert kernel(3, 8, 2, 7) == "kv_shared_rows_kernel<false>"
+    assert kernel(4, 8, 2, 7) == kernel(260, 4, 1, 10, 120) == "kv_shared_kernel<1, false>"
+    assert kernel(40, 8, 2, 7) == kernel(264, 4, 1, 10, 120) == "kv_shared_kernel<2, false>"
 
 
 def rotate(cases):
