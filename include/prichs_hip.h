@@ -295,7 +295,8 @@ int prichs_rope_forward_ld(void *qk, size_t row_stride, int dtype,
  * with leading dimensions (multiples of 8), bf16 or f32 as their outputs; w_q, w_k f32
  * [head_dim]; tables f32 [cache_rows, head_dim / 2]; arithmetic in f32, rounded once.
  * Either of n_heads and n_kv_heads may be 0 (its operands are not used then).  Rows at
- * positions outside the tables are padding: their outputs stay as they were.  An output
+ * positions outside the tables are padding: their outputs stay as they were, or become
+ * zeros (_zeros: for outputs that hold nothing yet).  An output
  * may be its input (same address and leading dimension), and must not overlap an input
  * otherwise.  head_dim is a multiple of 8 up to 256; operands are 16-byte aligned.  The
  * reference has no norm of queries and keys. */
@@ -307,6 +308,12 @@ int prichs_qk_norm_rope_forward(const void *q, size_t ldq, const void *k, size_t
                                 size_t ldko, size_t rows, size_t n_heads,
                                 size_t n_kv_heads, size_t head_dim, float eps, int dtype,
                                 void *stream);
+int prichs_qk_norm_rope_forward_zeros(
+    const void *q, size_t ldq, const void *k, size_t ldk, const float *w_q,
+    const float *w_k, const float *cos_cache, const float *sin_cache, size_t cache_rows,
+    const int32_t *positions, size_t seq_len, size_t pos_offset, void *q_out, size_t ldqo,
+    void *k_out, size_t ldko, size_t rows, size_t n_heads, size_t n_kv_heads,
+    size_t head_dim, float eps, int dtype, void *stream);
 /* Its gradients from those of the outputs and the inputs q, k.  With xh = x inv, inv = 1 /
  * sqrt(mean(x^2) + eps), g = R^T d_out, t = g w:
  *   d_x = inv (t - xh mean(t xh)),  d_w = sum over rows and heads of g xh

@@ -119,6 +119,9 @@ SIGNATURES = {
     "prichs_qk_norm_rope_forward": (_i, [_vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _sz,
                                          _sz, _vp, _sz, _vp, _sz, _sz, _sz, _sz, _sz, _f, _i,
                                          _vp]),
+    "prichs_qk_norm_rope_forward_zeros": (_i, [_vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp,
+                                               _sz, _sz, _vp, _sz, _vp, _sz, _sz, _sz, _sz, _sz,
+                                               _f, _i, _vp]),
     "prichs_qk_norm_rope_backward_workspace": (_sz, [_sz, _sz, _sz, _sz]),
     "prichs_qk_norm_rope_backward": (_i, [_vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp,
                                           _vp, _sz, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _vp,

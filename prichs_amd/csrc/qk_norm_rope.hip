@@ -105,8 +105,11 @@ template <typename T> struct Heads {
 // lanes read neighbouring heads.
 // Lanes past the head's end and heads past the last load what the group's first ones do,
 // so that all loads are in flight without a branch between them.
-template <typename T, int LANES>
-__global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(Args<T> a, uint64_t blocks) {
+// ZEROS: rows outside the tables become zeros (otherwise they stay as they were), by way of
+// the others' loads and products, at no cost (4 x 2048 rows by position 12.8 us either way): a
+// branch of their own took nine registers a lane from all rows and 3% of the time.
+template <typename T, int LANES, bool ZEROS>
+__device__ __forceinline__ void norm_rope(const Args<T> &a, uint64_t blocks) {
   constexpr int kGroups = kThreads / LANES;
   const int c = threadIdx.x % LANES;
   const bool lane = 8 * c < a.hd;  // of the lanes' 8 LANES values hd are the head's
@@ -117,7 +120,8 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(Args<T> a, uint6
     unit_of(a, block, kGroups, threadIdx.x / LANES, &row, &s);
     if (row >= a.rows) continue;  // the lanes of a group agree
     const uint32_t pos = position(a, (uint32_t)row);
-    if (pos >= a.cache_rows) continue;
+    const bool live = pos < a.cache_rows;
+    if (!ZEROS && !live) continue;
     const int step = (int)a.per_row * a.hd;  // from a head to the next of the group
     const Heads<const T> xs(a.x, a.ldx, row, s * a.hd + col, a.Hq, a.hd);
     Raw8<T> x[kHeads];
@@ -126,9 +130,12 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(Args<T> a, uint6
       const int h = s + a.per_row * j, jj = h < a.H ? j : 0;
       x[j].load(xs.at(s + (int)a.per_row * jj >= a.Hq, jj * step));
     }
-    const size_t at = (size_t)pos * (a.hd / 2) + col / 2;
-    const f32x4 cs = *reinterpret_cast<const f32x4 *>(a.cs + at);
-    const f32x4 sn = *reinterpret_cast<const f32x4 *>(a.sn + at);
+    const size_t at = (size_t)(!ZEROS || live ? pos : 0) * (a.hd / 2) + col / 2;
+    f32x4 cs = f32x4{0.f, 0.f, 0.f, 0.f}, sn = cs;
+    if (!ZEROS || a.cache_rows > 0) {
+      cs = *reinterpret_cast<const f32x4 *>(a.cs + at);
+      sn = *reinterpret_cast<const f32x4 *>(a.sn + at);
+    }
     Raw8<float> wq, wk;
     wq.load(a.w[0] + col), wk.load(a.w[1] + col);
     const Heads<T> os(a.out, a.ldo, row, s * a.hd + col, a.Hq, a.hd);
@@ -149,9 +156,21 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(Args<T> a, uint6
         o[2 * i] = y0 * cs[i] - y1 * sn[i];
         o[2 * i + 1] = y0 * sn[i] + y1 * cs[i];
       }
+      if constexpr (ZEROS) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = live ? o[e] : 0.f;
+      }
       if (lane && h < a.H) store8(os.at(isk, j * step), o);
     }
   }
+}
+template <typename T, int LANES>
+__global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(Args<T> a, uint64_t blocks) {
+  norm_rope<T, LANES, false>(a, blocks);
+}
+template <typename T, int LANES>
+__global__ __launch_bounds__(kThreads) void qk_norm_rope_zeros_kernel(Args<T> a, uint64_t blocks) {
+  norm_rope<T, LANES, true>(a, blocks);
 }
 
 // The gradients.  part: f32 [gridDim.x][2][hd], each workgroup's sums of d_wq and d_wk.
@@ -299,6 +318,7 @@ struct Call {
   size_t seq_len, pos_offset, rows, heads[2], hd;
   float eps;
   int dtype;
+  bool zeros;  // forward: in rows outside the tables
 };
 int check(const char *who, const Call &c, bool backward, bool *work) {
   *work = false;
@@ -362,15 +382,20 @@ Args<T> args_of(const Call &c) {
   return a;
 }
 
+template <typename T, int LANES>
+auto forward_kernel(bool zeros) {
+  return zeros ? qk_norm_rope_zeros_kernel<T, LANES> : qk_norm_rope_kernel<T, LANES>;
+}
 template <typename T>
 void launch_forward(const Call &c, hipStream_t s) {
   const int lanes = lanes_of(c.hd);
   const size_t blocks = blocks_of(c.rows, c.heads[0] + c.heads[1], c.hd);
   const dim3 grid((unsigned)(blocks < (1u << 20) ? blocks : 1u << 20));
-  auto kern = lanes == 4    ? qk_norm_rope_kernel<T, 4>
-              : lanes == 8  ? qk_norm_rope_kernel<T, 8>
-              : lanes == 16 ? qk_norm_rope_kernel<T, 16>
-                            : qk_norm_rope_kernel<T, 32>;
+  const bool zeros = c.zeros && c.positions != nullptr;  // without them no row is outside
+  auto kern = lanes == 4    ? forward_kernel<T, 4>(zeros)
+              : lanes == 8  ? forward_kernel<T, 8>(zeros)
+              : lanes == 16 ? forward_kernel<T, 16>(zeros)
+                            : forward_kernel<T, 32>(zeros);
   hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, s, args_of<T>(c),
                      (uint64_t)blocks);
 }
@@ -385,46 +410,79 @@ void launch_backward(const Call &c, size_t grid, float *part, hipStream_t s) {
                      (uint64_t)blocks_of(c.rows, c.heads[0] + c.heads[1], c.hd), part);
 }
 
-}  // namespace
-}  // namespace prichs
-
-using namespace prichs;
-
-extern "C" int prichs_qk_norm_rope_forward(const void *q, size_t ldq, const void *k, size_t ldk,
-                                           const float *w_q, const float *w_k,
-                                           const float *cos_cache, const float *sin_cache,
-                                           size_t cache_rows, const int32_t *positions,
-                                           size_t seq_len, size_t pos_offset, void *q_out,
-                                           size_t ldqo, void *k_out, size_t ldko, size_t rows,
-                                           size_t n_heads, size_t n_kv_heads, size_t head_dim,
-                                           float eps, int dtype, void *stream) {
-  const Call c{{q, k},
-               {nullptr, nullptr},
-               {q_out, k_out},
-               {ldq, ldk},
-               {0, 0},
-               {ldqo, ldko},
-               {w_q, w_k},
-               cos_cache,
-               sin_cache,
-               cache_rows,
-               positions,
-               seq_len,
-               pos_offset,
-               rows,
-               {n_heads, n_kv_heads},
-               head_dim,
-               eps,
-               dtype};
+int forward(const char *who, const Call &c, void *stream) {
   bool work;
-  const int rc = check("qk_norm_rope_forward", c, false, &work);
+  const int rc = check(who, c, false, &work);
   if (rc != PRICHS_OK || !work) return rc;
-  if (dtype == PRICHS_DTYPE_BF16)
+  if (c.dtype == PRICHS_DTYPE_BF16)
     launch_forward<bf16_t>(c, as_stream(stream));
   else
     launch_forward<float>(c, as_stream(stream));
   PRICHS_LAUNCH_CHECK("qk_norm_rope_forward launch");
   return PRICHS_OK;
+}
+
+}  // namespace
+}  // namespace prichs
+
+using namespace prichs;
+
+extern "C" int prichs_qk_norm_rope_forward(
+    const void *q, size_t ldq, const void *k, size_t ldk, const float *w_q, const float *w_k,
+    const float *cos_cache, const float *sin_cache, size_t cache_rows, const int32_t *positions,
+    size_t seq_len, size_t pos_offset, void *q_out, size_t ldqo, void *k_out, size_t ldko,
+    size_t rows, size_t n_heads, size_t n_kv_heads, size_t head_dim, float eps, int dtype,
+    void *stream) {
+  return forward("qk_norm_rope_forward",
+                 {{q, k},
+                  {nullptr, nullptr},
+                  {q_out, k_out},
+                  {ldq, ldk},
+                  {0, 0},
+                  {ldqo, ldko},
+                  {w_q, w_k},
+                  cos_cache,
+                  sin_cache,
+                  cache_rows,
+                  positions,
+                  seq_len,
+                  pos_offset,
+                  rows,
+                  {n_heads, n_kv_heads},
+                  head_dim,
+                  eps,
+                  dtype,
+                  false},
+                 stream);
+}
+
+extern "C" int prichs_qk_norm_rope_forward_zeros(
+    const void *q, size_t ldq, const void *k, size_t ldk, const float *w_q, const float *w_k,
+    const float *cos_cache, const float *sin_cache, size_t cache_rows, const int32_t *positions,
+    size_t seq_len, size_t pos_offset, void *q_out, size_t ldqo, void *k_out, size_t ldko,
+    size_t rows, size_t n_heads, size_t n_kv_heads, size_t head_dim, float eps, int dtype,
+    void *stream) {
+  return forward("qk_norm_rope_forward_zeros",
+                 {{q, k},
+                  {nullptr, nullptr},
+                  {q_out, k_out},
+                  {ldq, ldk},
+                  {0, 0},
+                  {ldqo, ldko},
+                  {w_q, w_k},
+                  cos_cache,
+                  sin_cache,
+                  cache_rows,
+                  positions,
+                  seq_len,
+                  pos_offset,
+                  rows,
+                  {n_heads, n_kv_heads},
+                  head_dim,
+                  eps,
+                  dtype,
+                  true},
+                 stream);
 }
 
 extern "C" size_t prichs_qk_norm_rope_backward_workspace(size_t rows, size_t n_heads,
@@ -461,7 +519,8 @@ extern "C" int prichs_qk_norm_rope_backward(
                {n_heads, n_kv_heads},
                head_dim,
                eps,
-               dtype};
+               dtype,
+               false};
   bool work;
   const int rc = check(who, c, true, &work);
   if (rc != PRICHS_OK) return rc;

@@ -710,11 +710,13 @@ def _norm_rope_args(w_q, w_k, cos, sin, n_heads, n_kv_heads, head_dim, positions
 
 def qk_norm_rope(q, k, w_q, w_k, cos, sin, n_heads, n_kv_heads, head_dim=128, eps=1e-5,
                  positions=None, seq_len=None, pos_offset=0, q_out=None, k_out=None, stream=None):
-    """prichs_qk_norm_rope_forward: each head of q and k (2-D row views, bf16 or f32)
-    normed with w_q / w_k (f32 [head_dim]) and rotated to its row's position: positions[r]
-    (int32 device [rows]), or r % seq_len + pos_offset (seq_len None: the rows are one
-    sequence).  cos, sin: f32 [positions, head_dim / 2].  q_out / k_out may be q / k.  With
-    n_heads or n_kv_heads 0 that operand is None.  -> (q_out, k_out)."""
+    """prichs_qk_norm_rope_forward (_zeros): each head of q and k (2-D row views, bf16 or
+    f32) normed with w_q / w_k (f32 [head_dim]) and rotated to its row's position:
+    positions[r] (int32 device [rows]), or r % seq_len + pos_offset (seq_len None: the rows
+    are one sequence).  cos, sin: f32 [positions, head_dim / 2].  q_out / k_out may be q / k.
+    With n_heads or n_kv_heads 0 that operand is None.  -> (q_out, k_out).  Rows at positions
+    outside the tables keep what q_out and k_out held (zeros where this call allocates
+    them)."""
     rows, ldq, ldk, dtype = _qk(q, k, n_heads, n_kv_heads, head_dim, ("q", "k"))
     n_pos, seq_len = _norm_rope_args(w_q, w_k, cos, sin, n_heads, n_kv_heads, head_dim, positions,
                                      seq_len, pos_offset, rows)
@@ -725,19 +727,22 @@ def qk_norm_rope(q, k, w_q, w_k, cos, sin, n_heads, n_kv_heads, head_dim=128, ep
     ctx, s = _launch_on(stream, cos, q, k, w_q, w_k, sin, positions, q_out, k_out)
     with ctx:
         ldqo, ldko = n_heads * head_dim, n_kv_heads * head_dim
+        lib = L.load()
+        forward = lib.prichs_qk_norm_rope_forward
         if q_out is None and k_out is None:  # of q's and k's rows and dtype, without gaps
             q_out = q.new_empty((rows, ldqo)) if n_heads else None
             k_out = k.new_empty((rows, ldko)) if n_kv_heads else None
+            forward = lib.prichs_qk_norm_rope_forward_zeros
         else:
             if q_out is None and n_heads:
-                q_out = q.new_empty((rows, ldqo))
+                q_out = q.new_zeros((rows, ldqo))
             if k_out is None and n_kv_heads:
-                k_out = k.new_empty((rows, ldko))
+                k_out = k.new_zeros((rows, ldko))
             r2, ldqo, ldko, d2 = _qk(q_out, k_out, n_heads, n_kv_heads, head_dim,
                                      ("q_out", "k_out"))
             if r2 != rows or d2 != dtype:
                 raise ValueError("q_out, k_out: expected the rows and the dtype of q and k")
-        L.check(L.load().prichs_qk_norm_rope_forward(
+        L.check(forward(
             _a(q), ldq, _a(k), ldk, _a(w_q), _a(w_k), cos.data_ptr(), sin.data_ptr(), n_pos,
             _a(positions), seq_len, pos_offset, _a(q_out), ldqo, _a(k_out), ldko, rows, n_heads,
             n_kv_heads, head_dim, eps, _TORCH_DTYPES[dtype], s))

@@ -1,0 +1,47 @@
+"""What the tests at the edges of the norms with rotation and of the attention over shared
+pages reach, on the CPU (tests/launch_log.py), and the refusals of the norms whose padding
+rows become zeros."""
+import pytest
+
+from prichs_amd import _lib as L
+from tests import launch_log as ll
+from tests import test_shared_prompt_abi as abi
+
+ZEROS = [(c, s) for n, _, c, s in abi.BAD if n == "prichs_qk_norm_rope_forward"]
+
+
+@pytest.mark.parametrize("change,status", ZEROS,
+                         ids=[f"{'-'.join(map(str, c))}-{i}" for i, (c, _) in enumerate(ZEROS)])
+def test_norms_with_zeros_refuse_what_those_without_do(change, status):
+    lib = L.load()
+    lib.prichs_clear_error()
+    assert abi.call(lib, "prichs_qk_norm_rope_forward_zeros", {**abi.NORM, **change}) == status
+    assert L.last_error().startswith("qk_norm_rope_forward_zeros")
+    assert abi.call(lib, "prichs_qk_norm_rope_forward_zeros", {**abi.NORM, "rows": 0}) == L.PRICHS_OK
+
+
+def test_zeros_are_written_where_rows_can_lie_outside_the_tables():
+    """A kernel of its own for positions from memory; without them the host has checked that
+    every row has one."""
+    from tests.test_gpu_qk_norm_rope_edges import PADDED
+
+    shapes = PADDED + [(9, 2, 1, 256)]
+    got = ll.run(f"""
+result = []
+for r, h, k, d in {shapes!r}:
+    for dt in (0, 1):
+        H, K = d * h, d * k
+        for pos, seq in ((P, 0), (None, 9)):
+            L.check(lib.prichs_qk_norm_rope_forward_zeros(
+                P, H, P, K, P, P, P, P, 9, pos, seq, 0, P, H, P, K, r, h, k, d, 1e-5, dt, None))
+            result.append(launches())
+""")
+    at, names = iter(got), set()
+    for _, _, _, d in shapes:
+        lanes = 4 if d <= 32 else 8 if d <= 64 else 16 if d <= 128 else 32
+        for t in ("float", "unsigned short"):
+            for kind in ("_zeros", ""):
+                (x,) = ll.as_launches(next(at))
+                assert x.kernel == f"qk_norm_rope{kind}_kernel<{t}, {lanes}>"
+                names.add(x.kernel)
+    assert len(names) == 16
