@@ -1,12 +1,12 @@
 """Norms of queries and keys with rotation: the rows without a position in outputs that the
-call allocates."""
+call allocates, and backwards whose workgroups take several blocks of rows."""
 import numpy as np
 import pytest
 import torch
 
 import norm_rope_ref as R
 from prichs_amd import ops
-from tests.test_gpu_qk_norm_rope import BF, EPS, F32, case, close, i32, tensors
+from tests.test_gpu_qk_norm_rope import BF, EPS, F32, case, close, i32, tensors, wide
 
 pytestmark = pytest.mark.gpu
 
@@ -96,3 +96,38 @@ def test_rows_that_lose_their_position_between_replays(cuda):
         for a, b in zip(got, want):
             assert torch.equal(a, b) and not a[~live].any()
 
+
+# Backwards of more than the 1024 workgroups that there are at most, and of one more: some
+# take one block of rows more than others.  Every number of lanes a head can have.
+LONG = [(3277, 12, 3, 128), (8195, 12, 3, 128), (9001, 3, 1, 256), (12001, 7, 2, 64),
+        (20001, 12, 3, 32)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows,Hq,Hk,hd", LONG)
+def test_backward_of_more_blocks_than_workgroups(cuda, rows, Hq, Hk, hd, dtype):
+    """Rows without a position among them, in the later blocks too."""
+    print("case:", rows, Hq, Hk, hd, dtype, flush=True)
+    rng = np.random.default_rng(rows + hd)
+    pos = rng.integers(0, 50, rows)
+    pad = rng.random(rows) < 0.1
+    pad[rows - 40:rows - 20] = True
+    c = case(rows, Hq, Hk, hd, dtype, rows + hd, pos, 50)
+    for a in c["x"] + c["d"]:
+        a[pad] = np.nan
+    args, at = tensors(c, positions=i32(np.where(pad, -1, pos).tolist()))
+    d = [wide(a, dtype) for a in c["d"]]
+    got = ops.qk_norm_rope_backward(*d, *args, **at)
+    keep = torch.from_numpy(~pad).cuda()
+    for i in range(2):
+        r = R.norm_rope(c["x"][i][~pad], c["w"][i], c["cos"][pos[~pad]], c["sin"][pos[~pad]], EPS,
+                        dtype, c["d"][i][~pad])
+        close(got[i][keep], r["dx"], r["e_dx"], "dx")
+        close(got[2 + i], r["dw"], r["e_dw"], "dw")
+        assert (got[i][~keep] == 0).all()
+    # The same bits again, in place, and added to what there is.
+    dw = [torch.full((hd,), 2.0, device="cuda") for _ in range(2)]
+    again = ops.qk_norm_rope_backward(*d, *args, **at, d_q=d[0], d_k=d[1], d_wq=dw[0], d_wk=dw[1],
+                                      accumulate=True)
+    for i in range(2):
+        assert torch.equal(again[i], got[i]) and torch.equal(dw[i], got[2 + i] + 2.0)

@@ -45,3 +45,19 @@ for r, h, k, d in {shapes!r}:
                 assert x.kernel == f"qk_norm_rope{kind}_kernel<{t}, {lanes}>"
                 names.add(x.kernel)
     assert len(names) == 16
+
+
+def test_long_backwards_take_more_blocks_than_workgroups():
+    from tests.test_gpu_qk_norm_rope_edges import LONG
+    from tests.test_shared_prompt_launches import rotate
+
+    cases = [(*s, dt) for s in LONG for dt in (0, 1)]
+    turns, lanes_seen = [], set()
+    for (rows, h, k, d, _), (_, bwd, dw) in zip(cases, rotate(cases)):
+        lanes = 4 if d <= 32 else 8 if d <= 64 else 16 if d <= 128 else 32
+        blocks = -(-rows * -(-(h + k) // 3) // (256 // lanes))
+        assert bwd.grid[0] == min(1024, blocks) and blocks > 1024 and blocks % 1024
+        assert bwd.kernel.endswith(f", {lanes}>")
+        turns.append(-(-blocks // 1024))
+        lanes_seen.add(lanes)
+    assert lanes_seen == {4, 8, 16, 32} and min(turns) == 2 and max(turns) >= 3
