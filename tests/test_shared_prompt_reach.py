@@ -61,3 +61,38 @@ def test_long_backwards_take_more_blocks_than_workgroups():
         turns.append(-(-blocks // 1024))
         lanes_seen.add(lanes)
     assert lanes_seen == {4, 8, 16, 32} and min(turns) == 2 and max(turns) >= 3
+
+
+def attend(batch, n_q, pages, heads, kv, groups, window=0):
+    from tests.test_shared_prompt_launches import attend as launches
+
+    ((need, got),) = launches([(batch, n_q, pages, heads, kv, groups, 1, window, 0)])
+    return need, got[0].kernel
+
+
+def test_attention_over_long_tables_is_taken_in_parts():
+    from tests import test_gpu_kv_shared_edges as t
+
+    # Parts without a softmax: every form of a call, with a window too.
+    for size, pages, window, form in t.TABLES:
+        _, name = attend(size, 1, pages or -(-t.TOP // 64), 8, 2, 1, window)
+        assert name == ("kv_shared_rows_kernel<true>" if form == "rows" else
+                        f"kv_shared_kernel<{form}, true>")
+    # Tables full of shared pages.
+    got = [attend(size, n_q, pages, 8, 2, 1) for size, pages, n_q in t.FULL]
+    assert [x for _, x in got] == ["kv_shared_kernel<1, true>", "kv_shared_kernel<2, true>"]
+    # Both of two graphs at once have a workspace, in both heights of a tile.
+    got = [attend(len(lens), n_q, p or -(-max(lens) // 64), h, k, len(groups))
+           for groups, lens, n_q, h, k, p in t.PAIR]
+    assert all(need > 0 for need, _ in got)
+    assert [x for _, x in got] == ["kv_shared_kernel<1, true>", "kv_shared_kernel<2, true>"]
+    # The captured step.
+    need, name = attend(len(t.PROMPTS) * t.EACH, 1, t.STEP_COLUMNS, *t.STEP_HEADS, len(t.PROMPTS))
+    assert need > 0 and name == "kv_shared_kernel<1, true>"
+    # lse in every kernel that gives it.
+    names = set()
+    for groups, lens, n_q, heads, kv, window, _, form in t.FORMS[::2]:
+        pages = t.pages_of(lens, n_q, heads, kv, form)
+        names.add(attend(len(lens), n_q, pages, heads, kv, len(groups), window)[1])
+    assert names == {"kv_shared_rows_kernel<true>", "kv_shared_kernel<1, true>",
+                     "kv_shared_kernel<2, true>"}
