@@ -25,7 +25,10 @@
 // windowed 17.5 -> 16 us, 2 x 256 over 4352 26 -> 24, with what follows); a second set of
 // registers cost the third workgroup a CU and was no faster.  Masks are bit fields: as
 // comparisons their results took so many scalar registers that some 80 others were held
-// in lanes of vector registers, which 80 of a page's 650 instructions moved.
+// in lanes of vector registers, which 80 of a page's 650 instructions moved.  19 to 27 are
+// held so now, none of which is read back among a page's products.  The kernels of two kinds of
+// workgroup (kv_shared_kernel) hold 48 to 54 with tiles of 16 rows, whose loop over shared pages
+// reads some 24 back a page, and 79 to 90 with tiles of 32, whose loop reads hardly any.
 //
 // The visible pages of a tile are dealt evenly to the waves of n_split workgroups in
 // contiguous runs; the waves of a workgroup join in LDS, workgroups through the
@@ -458,7 +461,9 @@ __device__ __forceinline__ void kv_attend(
             p[4 * h2 + r] = fast_exp2(fmaf(s[2 * ks2 + h2][nb][r], sh.scale_log2, neg_m));
         if constexpr (LSE)
           psum[nb] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-        // P rounded to bf16 for the product; its sum is that of the rounded values.
+        // P rounded to bf16 for the product, whose other operand is exact in bf16; its sum is
+        // that of the rounded values.  With the output's rounding (0.0017 of the norm) outputs
+        // are off by 0.0021 to 0.0023.  P in two parts would take half as many products again.
         pf[nb][ks2] = u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]),
                             pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])};
       }

@@ -42,10 +42,10 @@ __global__ __launch_bounds__(256) void kv_join_lse_kernel(
 
 // Pages up to which one workgroup of 8 waves takes a tile without a second kernel:
 // a page costs a wave some 2 us, the second kernel 2.5 on the device and 4 on the
-// host.  Captured, us (from Python in brackets), one kernel and two: one token over 8
-// pages 6.5, 7.3 (9.6, 13.3), over 16 pages 8.1, 7.5 (9.6, 13.4), over 32 pages 11.2, 7.7
-// (10.6, 13.5); 32 and 80 sequences over 16 pages 8.5, 9.3 and 9.6, 13.8, over 32 pages
-// 12.2, 11.1 and 15.6, 19.9.
+// host.  Captured, us (from Python in brackets), one kernel and two, in turn: one token over
+// 8 pages 5.7, 6.7 (9.6, 13.3), over 16 pages 7.3, 6.7 (9.6, 13.4), over 32 pages 10.5, 7.0
+// (10.6, 13.5); 32 and 80 sequences over 8 pages 5.9, 7.0 and 6.1, 8.4, over 16 pages 7.6,
+// 8.4 and 8.6, 12.9, over 32 pages 11.6, 10.4 and 14.9, 18.9.
 constexpr size_t kShortPages = 16;
 
 // How a call is cut: n_split workgroups of `waves` waves over a tile's pages.  For 256

@@ -10,7 +10,8 @@
 // launch; beyond, workgroups count them in blocks of kBlockPages and a second launch ranks
 // them behind the blocks before.  MI355X: the kernels that plan and write tables take 3 to
 // 9 us each; fork_apply 4.4 us for 7 items and 6.0 for 224; compact_apply 39 us where 3661
-// pages of three heads move (191 MB read and written, 4.9 TB/s).
+// pages of three heads move (191 MB read and written, 4.9 TB/s); kv_cache_copy of 600 pages of
+// three heads 5.8 us in a graph (7.0 a call from Python), of 16384 174 (856 MB, 4.9 TB/s).
 #include "kv_cache.hpp"
 
 #include <climits>

@@ -9,6 +9,19 @@
 // MI355X, 12 + 3 heads, us from Python (kernels): 8 sequences of one prompt of 1000
 // positions 11 (10 captured), 16 prompts of 2048 with 4 sequences each 15, 24 x 6 tokens
 // behind 8000 shared positions 25, 256 sequences behind 32768 80: 52 GFLOP, 650 TFLOP/s.
+//
+// Where little is saved, attention of each sequence by itself (kv_attention.hip) is the faster
+// call for rows of the table that name their shared pages, as those of a fork do: it deals all
+// of a sequence's pages to as many workgroups as the chip holds, this one its own pages to at
+// most eight.  One token each, us captured, this call and that one, by sequences:
+//   positions shared + own   1           4           8           16          64
+//   1000 + 200               9.2, 7.2    9.3, 7.3    9.4, 7.5    9.5, 7.7    10.0, 11.8
+//   1000 + 8000              11.4, 7.8   12.0, 9.5   14.7, 12.2  19.2, 17.7  55.6, 38.3
+//   1000 + 30000             24.8, 10.4  31.1, 16.8  31.6, 23.6  44.6, 37.0  233, 144
+//   8000 + 1000              9.4, 7.7    10.2, 9.5   11.2, 12.2  14.2, 14.4  19.8, 30.8
+//   8000 + 8000              12.4, 7.9   14.6, 11.3  17.7, 13.7  19.5, 19.4  57.5, 49.6
+//   30000 + 1000             12.6, 10.4  14.5, 13.5  15.8, 18.5  17.7, 27.9  32.1, 82.3
+//   30000 + 8000             15.1, 11.0  17.2, 15.7  19.7, 21.3  23.0, 33.0  63.8, 100
 #include "kv_attend.hpp"
 
 namespace prichs {
@@ -76,11 +89,13 @@ struct Plan {
   bool rows;                // few pages: tiles_s tiles over all of a sequence's pages, one launch
 };
 // Up to so many pages, and a CU for each tile of a sequence, one launch takes each sequence by
-// itself.  Captured, us (from Python in brackets), so and apart with a join: 8 sequences of 8
-// pages 7.1, 9.4 (10.7, 14.5), 16 pages 8.8, 9.6 (10.6, 14.4), 24 pages 10.4, 10.2 (10.7, 14.5), 32
-// pages 12.0, 10.2 (11.4, 14.5); one of 24 pages 10.2, 9.5; 80 of 24 10.9, 13.3; 20 of 24 with
-// eight tokens each 10.9, 16.0.  100 sequences, more tiles than CUs: 8 pages 11.8, 10.7 (11.3,
-// 14.9), 24 pages 18.6, 13.7.
+// itself.  Captured, us (from Python in brackets), so and apart with a join, in turn: 8 sequences
+// of 8 pages 6.4, 8.7 (10.7, 14.5), 16 pages 8.1, 8.9 (10.6, 14.4), 20 pages 9.6, 9.3, 24 pages 9.6,
+// 9.4 (10.7, 14.5), 32 pages 11.2, 9.4 (11.4, 14.5); one of 16 pages 7.8, 8.2, of 24 9.5, 8.6; 80 of
+// 24 10.5, 14.4; 20 of 24 with eight tokens each 10.2, 14.7.  So a few sequences of 20 to 24 pages
+// lose up to 0.9 us in a graph; the bound is where calls from Python, which gain 4, still do, and
+// batches do either way.  100 sequences, more tiles than CUs, in graphs of ten calls: 8 pages
+// 11.8, 10.7 (11.3, 14.9), 24 pages 18.6, 13.7.
 constexpr size_t kFewPages = 24;
 constexpr size_t kHalfRound = 384;
 constexpr size_t kManySteps = 4096, kMoreSteps = 32768;  // pages of all tiles of 16 rows

@@ -11,10 +11,10 @@
 // head are a few lane exchanges.  Such a group of lanes takes kHeads heads of its row, whose
 // loads are all in flight, with one load of the position's cos and sin (32 bytes a lane
 // against 16 of a bf16 head).  Bound by HBM where there are many rows: 4 x 2048 of 12 + 3
-// heads in bf16 (64 MB; MI355X) 13.3 us forward, 4.8 TB/s, and 19.6 backward (98 MB, 5.0);
-// by the launch where there are few (32 rows 4.0 us).  Heads a group, us of a captured
-// forward, and of a forward and backward: 1 15.0 and 38.2, 2 13.7 and 35.9, 3 13.3 and 35.0,
-// 4 13.1 and 37.9, 5 13.7 and 47.4 (registers).
+// heads in bf16 (64 MB; MI355X) 12.6 us forward, 5.1 TB/s, and 18.4 backward (98 MB, 5.3);
+// by the launch where there are few (32 rows 3.7 us).  Heads a group, us of a captured
+// forward, and of a forward and backward: 1 13.6 and 35.6, 2 12.6 and 34.1, 3 12.2 and 33.3,
+// 4 12.2 and 36.2, 5 12.6 and 44.8 (registers).
 #include "common.hpp"
 
 namespace prichs {
@@ -292,8 +292,8 @@ __global__ __launch_bounds__(1024) void qk_norm_dw_kernel(const float *__restric
 }
 
 // Workgroups of the backward: the sums of the weights' gradients end in one row of `part`
-// each.  1024 are all resident (four a CU); 512 and 2048 take 36.9 and 38.4 us where these
-// take 35.9 (4 x 2048 rows, forward and backward, at two heads a group).
+// each.  1024 are all resident (four a CU); 256, 512 and 2048 take 40.4, 34.1 and 35.7 us where
+// these take 33.3 (4 x 2048 rows, a captured forward and backward).
 constexpr size_t kBwdBlocks = 1024;
 int lanes_of(size_t hd) { return hd <= 32 ? 4 : hd <= 64 ? 8 : hd <= 128 ? 16 : 32; }
 size_t per_row_of(size_t heads) { return cdiv(heads, (size_t)kHeads); }

@@ -513,7 +513,8 @@ def kv_cache_shared_attention(q, cache, page_table, lens, group_start, shared, b
     """prichs_kv_cache_shared_attention: kv_cache_attention of a batch whose sequences
     group_start[g] .. group_start[g + 1] - 1 hold their first shared[g] positions in the
     same pages (group_start int32 device [n_groups + 1], shared [n_groups]), which are
-    read once for the group.  -> (out, lse f32 [batch, n_heads, n_q], or None)."""
+    read once for the group.  -> (out, lse f32 [batch, n_heads, n_q], or None).  Behind
+    short prompts, or with long text of each sequence's own, kv_cache_attention is faster."""
     lib = L.load()
     _kv_cache(cache, page_table, batch, n_kv_heads)
     rows, H = batch * n_q, n_heads * head_dim
