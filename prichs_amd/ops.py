@@ -735,10 +735,11 @@ def qk_norm_rope(q, k, w_q, w_k, cos, sin, n_heads, n_kv_heads, head_dim=128, ep
             k_out = k.new_empty((rows, ldko)) if n_kv_heads else None
             forward = lib.prichs_qk_norm_rope_forward_zeros
         else:
+            make = torch.empty if positions is None else torch.zeros  # all rows have one, or not
             if q_out is None and n_heads:
-                q_out = q.new_zeros((rows, ldqo))
+                q_out = make((rows, ldqo), dtype=dtype, device=q.device)
             if k_out is None and n_kv_heads:
-                k_out = k.new_zeros((rows, ldko))
+                k_out = make((rows, ldko), dtype=dtype, device=k.device)
             r2, ldqo, ldko, d2 = _qk(q_out, k_out, n_heads, n_kv_heads, head_dim,
                                      ("q_out", "k_out"))
             if r2 != rows or d2 != dtype:
